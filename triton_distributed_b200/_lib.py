@@ -177,6 +177,23 @@ class DecodeArgs(C.Structure):
         ("stream", C.c_void_p),
         ("epoch_ptr", C.c_void_p), ("epoch_done", C.c_void_p), ("ll_peer_alt", C.c_void_p * MAX_RANKS),
         ("ll_mc", C.c_void_p), ("ll_mc_alt", C.c_void_p),
+        ("window", C.c_int), ("sinks", C.c_int), ("priors", C.c_int), ("prior_o", C.c_void_p), ("prior_lse", C.c_void_p),
+    ]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("block_table", C.c_void_p), ("q_starts", C.c_void_p),
+        ("kv_lens", C.c_void_p), ("out", C.c_void_p), ("part_o", C.c_void_p), ("part_lse", C.c_void_p),
+        ("q_token", C.c_longlong), ("q_head", C.c_longlong),
+        ("stride_block", C.c_longlong), ("stride_token", C.c_longlong), ("stride_head", C.c_longlong),
+        ("tokens", C.c_int), ("B", C.c_int), ("Hq", C.c_int), ("Hkv", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int),
+        ("max_blocks", C.c_int), ("blocks", C.c_int), ("splits", C.c_int), ("row_tiles", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
+        ("shared", C.c_int), ("dtype", C.c_int),
+        ("scale", C.c_float), ("soft_cap", C.c_float),
+        ("status", C.c_void_p),
+        ("timeout_ns", C.c_uint64),
+        ("stream", C.c_void_p),
     ]
 
 
@@ -248,6 +265,7 @@ def _declare(lib):
     lib.tdist_primitive.argtypes = [C.POINTER(PrimArgs)]
     lib.tdist_bounds_checked.argtypes = []
     lib.tdist_flash_decode.argtypes = [C.POINTER(DecodeArgs)]
+    lib.tdist_attention.argtypes = [C.POINTER(AttentionArgs)]
     lib.tdist_lse_combine.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p]
     lib.tdist_dequant_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
     lib.tdist_moe_route.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -408,9 +408,39 @@ typedef struct TdistDecodeArgs {
      * ll_mc_alt = the odd-call parity, needed with epoch_ptr. */
     void* ll_mc;
     void* ll_mc_alt;
+    /* mode 0, optional: window > 0 lets every query see the last `window` keys and the first `sinks` of its sequence only
+     * (pages that hold no such key are not read, nor are their table entries). With window > 0 (0x7fffffff: no limit) the
+     * result may also take in partial results over other keys: prior_o fp32 [priors][B * Hq][D] (normalised) and
+     * prior_lse fp32 [priors][B * Hq] (natural log, -inf: no keys). */
+    int window, sinks, priors;
+    const void* prior_o;
+    const void* prior_lse;
 } TdistDecodeArgs;
 
 int tdist_flash_decode(const TdistDecodeArgs* args);
+/* Attention of many query rows over a paged cache (csrc/kernels/attention_sm100.cu). */
+typedef struct TdistAttentionArgs {
+    const void* q;            /* [tokens, Hq, D] bf16/fp16, strides q_token and q_head */
+    const void* k_cache;      /* [blocks, page, Hkv, D] */
+    const void* v_cache;
+    const void* block_table;  /* int32 [B, max_blocks]; shared: [max_blocks] */
+    const void* q_starts;     /* int32 [B + 1]: first query token of every sequence; they are its last positions. Unused if shared */
+    const void* kv_lens;      /* int32 [B]; shared: [1] */
+    void* out;                /* [tokens, Hq, D]; NULL: leave the partial results */
+    void* part_o;             /* fp32 [splits][tokens * Hq][D], with splits > 1 or without out */
+    void* part_lse;           /* fp32 [splits][tokens * Hq] */
+    long long q_token, q_head, stride_block, stride_token, stride_head;  /* in elements, multiples of 8 */
+    int tokens, B, Hq, Hkv, head_dim, page_size, max_blocks, blocks;     /* blocks: pages of the cache */
+    int splits, row_tiles;    /* row_tiles: 1 or 2 tiles of 128 rows per CTA (1 with head_dim 256) */
+    int window, sinks;        /* position p sees j <= p with j > p - window or j < sinks; 0x7fffffff = no limit */
+    int shared, dtype;        /* shared: every query token sees the same kv_lens[0] keys */
+    float scale, soft_cap;
+    void* status;
+    uint64_t timeout_ns;
+    void* stream;
+} TdistAttentionArgs;
+
+int tdist_attention(const TdistAttentionArgs* args);
 /* parts fp32 [ranks, heads, D + 1] -> out [heads, D] */
 int tdist_lse_combine(const void* parts, int ranks, int heads, int head_dim, void* out, int dtype, void* stream);
 

@@ -1,0 +1,737 @@
+// Attention of many query rows over a paged KV cache on the tcgen05 tensor cores: prefill of a ragged batch (causal, with an
+// optional sliding window and first tokens that stay visible), and the keys that all sequences of a decode batch share.
+//
+//   out[r] = sum_j p[r, j] v[j],  p[r, j] = exp(s[r, j] - lse[r]),  s = cap(scale q k^T),  lse[r] = log sum_j exp(s[r, j])
+//   over the keys j that row r sees: j <= pos(r) and (j > pos(r) - window or j < sinks)
+//
+// A tile is 128 rows of one kv head: the G query heads that share it for 128 / G tokens, so that a key is read once for all of
+// them. A CTA goes over its keys 128 at a time (64 with head_dim 256) with the running maximum and sum of a softmax:
+//   S = Q K^T in TMEM (128 x 128 fp32), a thread per row turns it into P = exp2(S - m) in 16 bits, in place of S in TMEM, and
+//   O += P V takes P from TMEM and V as it lies in the cache (its N dimension contiguous).
+// Two such chains ("streams") run in one CTA, so that the tensor cores work on one while the other is in its softmax: two row tiles
+// over the same keys where there are enough rows, else one row tile over every other block of keys, joined at the end.
+// Warps: 4 per stream for the softmax, one that issues MMAs, kLoaders that copy K and V (16-byte cp.async: pages of any
+// size and stride; rows that nobody sees are not read and become zeros) into a ring of tiles in the 128-byte-swizzled
+// layout the MMAs read.
+// Few rows over many keys are split along the keys; the partial results meet in attention_merge_kernel, or in the decode kernel.
+//
+// P is rounded to the inputs' 16 bits (relative 2^-8 or 2^-11), S, O, maximum and sum are fp32. The maximum that is subtracted
+// is raised only when it has grown by more than 2^8 (kRaise): P then lies below 2^8, whose relative rounding is the same, and O
+// is read, scaled and written back a few times per row instead of once per block.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <cstring>
+#include <mutex>
+#include <string>
+
+#include "../device/ptx.cuh"
+#include "../device/signal.cuh"
+#include "../include/tdist.h"
+#include "../runtime/host_common.h"
+
+namespace tdist {
+namespace attention {
+
+constexpr int kKernelAttention = 9;
+constexpr int kRows = 128;      // rows of a tile: the MMA's M
+constexpr int kLoaders = 2;     // warps that copy K and V
+constexpr int kLag = 2;         // tiles that a loader leaves in flight before it hands the oldest over
+constexpr float kRaise = 8.f;   // log2 of how far scores may exceed the maximum that is subtracted
+
+struct Params {
+    const void* q;           // rows of D values, strides below
+    const void* k_cache;     // [blocks, page, Hkv, D]
+    const void* v_cache;
+    const int* block_table;  // [B, max_blocks]; shared: [max_blocks]
+    const int* q_starts;     // [B + 1]; shared: nullptr
+    const int* kv_lens;      // [B]; shared: [1]
+    void* out;               // T [tokens, Hq, D], where one part holds the result
+    float* part_o;           // fp32 [splits][tokens * Hq][D], normalised
+    float* part_lse;         // fp32 [splits][tokens * Hq], natural log
+    long long q_token, q_head, stride_block, stride_token, stride_head;   // in elements
+    int tokens, B, Hq, Hkv, G, page_size, page_shift, max_blocks, blocks, splits;
+    int tile_tokens;         // tokens of a row tile: 128 / G
+    int shared;              // 1: every query token sees all kv_lens[0] keys
+    int window, sinks;       // window 0x7fffffff: none
+    float scale_log2, soft_cap;   // |scale| x log2 e
+    uint32_t q_and, q_xor;   // sign of the scale, applied to q (0 / 0: scale 0)
+    WaitCtx wctx;
+};
+
+template <int D>
+struct Shape {
+    static constexpr int KT = D <= 128 ? 128 : 64;        // keys of a block
+    static constexpr int STREAMS = D <= 128 ? 2 : 1;      // TMEM holds O of one stream only with head_dim 256
+    static constexpr int TILE = KT * D * 2;               // bytes of a K or V block
+    static constexpr int QTILE = kRows * D * 2;
+    static constexpr int CHUNKS = D / 64;                 // 128-byte columns of a tile
+    static constexpr int AREA = D == 64 ? 160 * 1024 : 224 * 1024;
+    static constexpr int SOFT = 128 * STREAMS;            // softmax threads
+    static constexpr int THREADS = SOFT + 32 + 32 * kLoaders;
+    static constexpr uint32_t O_COL = 256;                // TMEM columns: S / P of stream s at s * 128, O at O_COL + s * D
+};
+template <int D, int QT>
+constexpr int stages() {
+    return (Shape<D>::AREA - QT * Shape<D>::QTILE) / Shape<D>::TILE;
+}
+constexpr int kMaxStages = 10;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// D (TMEM) (+)= A (TMEM: a row per lane, two 16-bit values per column) x B (shared memory)
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 lanes x 32 columns: thread t of the warp writes columns [col, col + 32) of TMEM lane (lane_base + t)
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+        "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+
+// What a CTA works on: sequence b, its query tokens [i0, i0 + QT * tile_tokens) of n, the split and the blocks of keys.
+struct Work {
+    int b, i0, n, q0, kvh, split;
+    int first;      // position of token i0
+    int hi, lo;     // keys [lo, hi) and [0, s_end) are seen by some row
+    int s_end;
+    int n_sink, m0; // blocks 0 .. n_sink - 1, then m0 ..
+    int c0, nt;     // of these, the split's
+};
+
+template <int D, int QT>
+__device__ __forceinline__ bool find_work(const Params& p, Work& w) {
+    constexpr int KT = Shape<D>::KT;
+    const int lane = static_cast<int>(threadIdx.x) & 31;
+    w.split = static_cast<int>(blockIdx.x) % p.splits;
+    w.kvh = static_cast<int>(blockIdx.x) / p.splits % p.Hkv;
+    int tile = static_cast<int>(blockIdx.x) / p.splits / p.Hkv;
+    const int per = QT * p.tile_tokens;
+    const long long table_keys = static_cast<long long>(p.max_blocks) * p.page_size;
+    int kv;
+    if (p.shared) {
+        w.b = 0;
+        w.q0 = 0;
+        w.n = p.tokens;
+        w.i0 = tile * per;
+        kv = p.kv_lens[0];
+    } else {
+        // 32 sequences at a time: the one whose tiles hold number `tile`
+        int b = -1;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+            int start = 0, n = 0;
+            if (b0 + lane < p.B) {
+                start = min(max(p.q_starts[b0 + lane], 0), p.tokens);
+                n = max(min(p.q_starts[b0 + lane + 1], p.tokens) - start, 0);
+            }
+            const int mine = (n + per - 1) / per;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, tile < upto);
+            if (hit != 0) {
+                const int src = __ffs(hit) - 1;
+                b = b0 + src;
+                w.q0 = __shfl_sync(0xffffffffu, start, src);
+                w.n = __shfl_sync(0xffffffffu, n, src);
+                // the last tokens, which see the most keys, first
+                w.i0 = (__shfl_sync(0xffffffffu, upto, src) - 1 - tile) * per;
+                break;
+            }
+            tile -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (b < 0) return false;
+        w.b = b;
+        kv = p.kv_lens[b];
+    }
+    kv = kv < 0 ? 0 : (kv > table_keys ? static_cast<int>(table_keys) : kv);
+    const int rows_end = min(w.n, w.i0 + per);
+    if (p.shared) {
+        w.first = kv - 1;
+        w.lo = w.s_end = 0;
+        w.hi = kv;
+    } else {
+        w.first = kv - w.n + w.i0;
+        w.hi = max(0, kv - w.n + rows_end);
+        w.lo = min(max(0, w.first - p.window + 1), w.hi);
+        w.s_end = min(p.sinks, w.lo);
+    }
+    w.n_sink = (w.s_end + KT - 1) / KT;
+    w.m0 = max(w.lo / KT, w.n_sink);
+    const int total = w.hi > 0 ? w.n_sink + max(0, (w.hi + KT - 1) / KT - w.m0) : 0;
+    const int each = (total + p.splits - 1) / p.splits;
+    w.c0 = min(total, w.split * each);
+    w.nt = min(total, w.c0 + each) - w.c0;
+    return true;
+}
+
+// QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks.
+template <typename T, int D, int QT>
+__global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const Params p) {
+    using S = Shape<D>;
+    constexpr int KT = S::KT, NSTR = S::STREAMS, NST = stages<D, QT>(), CH = D / 8;
+    static_assert(NST >= kLag + 2 && NST <= kMaxStages, "a tile is released only once the one after it has been handed over");
+    static_assert(QT == 1 || NSTR == 2, "two row tiles need two streams");
+    constexpr int LOOK = QT == 2 ? 1 : NSTR;   // K blocks loaded ahead of the first V block
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::AREA);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 8);
+    const uint32_t q_smem = smem_u32(smem), ring = q_smem + QT * S::QTILE;
+    const uint32_t bars_u32 = smem_u32(bars);
+    auto bar_full = [&](int s) { return bars_u32 + 8u * s; };
+    auto bar_empty = [&](int s) { return bars_u32 + 8u * (kMaxStages + s); };
+    auto bar_s = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + s); };        // S is complete
+    auto bar_p = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 2 + s); };    // P is in its place
+    auto bar_o = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 4 + s); };    // O has taken it in
+    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 6);
+    const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int s = 0; s < NST; ++s) {
+            mbar_init(bar_full(s), kLoaders);
+            mbar_init(bar_empty(s), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(bar_s(s), 1);
+            mbar_init(bar_p(s), 128);
+            mbar_init(bar_o(s), 1);
+        }
+        mbar_init(bar_q, S::SOFT);
+        fence_mbar_init();
+    }
+    if (warp == S::SOFT / 32) {
+        tmem_alloc<1>(smem_u32(tmem_slot), 512);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    pdl_wait_and_release();
+
+    Work w = {};
+    const bool live = find_work<D, QT>(p, w);
+    const int nt = live ? w.nt : 0;
+    auto block_start = [&](int j) {   // first key of the split's j-th block
+        const int i = w.c0 + j;
+        return (i < w.n_sink ? i : w.m0 + i - w.n_sink) * KT;
+    };
+    // The ring's items in the order in which the MMAs take them: LOOK blocks of K, then V and K in turn, the last V.
+    const int look = min(LOOK, nt);
+    auto item_v = [&](int j) { return j < nt - look ? look + 2 * j : nt + j; };
+    auto item_k = [&](int j) { return j < look ? j : look + 2 * (j - look) + 1; };
+
+    if (warp > S::SOFT / 32) {
+        // ---------------------------------------------------------------- loaders: rows [r0, r0 + RW) of every tile
+        constexpr int RW = KT / kLoaders, RL = RW / 32, RPI = 32 / CH;   // rows of a warp, of a lane's lookups, of an instruction
+        const int r0 = (warp - S::SOFT / 32 - 1) * RW;
+        const int* table = p.block_table + static_cast<size_t>(live ? w.b : 0) * p.max_blocks;
+        const int lrow = lane / CH, lch = lane % CH;
+        const T* kl = static_cast<const T*>(p.k_cache) + static_cast<size_t>(w.kvh) * p.stride_head + lch * 8;
+        const T* vl = static_cast<const T*>(p.v_cache) + static_cast<size_t>(w.kvh) * p.stride_head + lch * 8;
+        const uint32_t lane_dst = static_cast<uint32_t>((lch >> 3) * (KT * 128));
+        const int items = 2 * nt;
+        auto block_of = [&](int n, bool& is_k) {
+            const int m = n - look, pairs = 2 * (nt - look);
+            is_k = n < look || (m < pairs && (m & 1));
+            return n < look ? n : (m < pairs ? (m >> 1) + (is_k ? look : 0) : m - (nt - look));
+        };
+        // offset of the lane's rows of item n in the cache, -1: nobody sees the key
+        auto lookup = [&](int n, long long (&off)[RL]) {
+#pragma unroll
+            for (int r = 0; r < RL; ++r) off[r] = -1;
+            if (n >= items) return;
+            bool is_k;
+            const int t0 = block_start(block_of(n, is_k)) + r0 + lane;
+#pragma unroll
+            for (int r = 0; r < RL; ++r) {
+                const int t = t0 + 32 * r;
+                if (t < w.s_end || (t >= w.lo && t < w.hi)) {
+                    const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+                    const int page = table[in_table];
+                    if (static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks))
+                        off[r] = static_cast<long long>(page) * p.stride_block + static_cast<long long>(t - in_table * p.page_size) * p.stride_token;
+                }
+            }
+        };
+        int done = 0;   // items handed over
+        auto hand_over = [&](int upto) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            for (; done < upto; ++done)
+                if (lane == 0) mbar_arrive(bar_full(done % NST));
+        };
+        long long next[RL];
+        lookup(0, next);
+        for (int n = 0; n < items; ++n) {
+            long long off[RL];
+#pragma unroll
+            for (int r = 0; r < RL; ++r) off[r] = next[r];
+            lookup(n + 1, next);
+            const int slot = n % NST;
+            const uint32_t parity = ((n / NST) & 1u) ^ 1u;
+            if (__any_sync(0xffffffffu, !mbar_test_wait(bar_empty(slot), parity))) {
+                cp_async_wait<0>();
+                hand_over(n);
+                mbar_wait(bar_empty(slot), parity, p.wctx, 1);
+            }
+            bool is_k;
+            block_of(n, is_k);
+            const T* src = is_k ? kl : vl;
+            const uint32_t dst = ring + static_cast<uint32_t>(slot) * S::TILE + lane_dst;
+#pragma unroll
+            for (int j = 0; j < RW / RPI; ++j) {
+                const int row = j * RPI + lrow;
+                const long long o = __shfl_sync(0xffffffffu, off[j * RPI / 32], row & 31);
+                const int at = r0 + row;
+                cp_async16(dst + static_cast<uint32_t>(at * 128 + (((lch & 7) ^ (at & 7)) << 4)), src + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
+            }
+            cp_async_commit();
+            if (n - kLag >= done) {
+                cp_async_wait<kLag>();
+                hand_over(n - kLag + 1);
+            }
+        }
+        cp_async_wait<0>();
+        hand_over(items);
+    } else if (warp == S::SOFT / 32) {
+        // ---------------------------------------------------------------- MMA issue
+        if (lane == 0 && nt > 0) {
+            const uint32_t fmt = sizeof(T) == 2 && __is_same(T, __half) ? 0u : 1u;
+            const uint32_t idesc_s = umma_idesc(fmt, fmt, kRows, KT);
+            const uint32_t idesc_o = umma_idesc(fmt, fmt, kRows, D) | kIdescBNMajor;
+            auto qk = [&](int tile, int stream, int item) {
+                const uint32_t kb = ring + static_cast<uint32_t>(item % NST) * S::TILE, qb = q_smem + tile * S::QTILE;
+#pragma unroll
+                for (int c = 0; c < S::CHUNKS; ++c) {
+                    const uint64_t a = umma_desc_k_sw128(qb + c * (kRows * 128)), b = umma_desc_k_sw128(kb + c * (KT * 128));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_bf16<1>(tmem + stream * 128, a + 2 * k, b + 2 * k, idesc_s, (c | k) != 0 ? 1u : 0u);
+                }
+                umma_commit(bar_s(stream));
+            };
+            auto pv = [&](int stream, int item, bool first) {
+                const uint64_t b = umma_desc_mn_sw128(ring + static_cast<uint32_t>(item % NST) * S::TILE, KT * 128);
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    umma_ts(tmem + S::O_COL + stream * D, tmem + stream * 128 + 8 * k, b + 128 * k, idesc_o, !first || k != 0 ? 1u : 0u);
+                umma_commit(bar_o(stream));
+            };
+            auto full = [&](int item) {
+                mbar_wait(bar_full(item % NST), (item / NST) & 1u, p.wctx, 2);
+                tc_fence_after();
+            };
+            mbar_wait(bar_q, 0, p.wctx, 3);
+            if constexpr (QT == 2) {
+                full(0);
+                qk(0, 0, 0);
+                qk(1, 1, 0);
+                umma_commit(bar_empty(0));
+                for (int j = 0; j < nt; ++j) {
+                    const int v = item_v(j), k = item_k(j + 1);
+                    const uint32_t parity = j & 1u;
+                    full(v);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        mbar_wait(bar_p(s), parity, p.wctx, 4);
+                        tc_fence_after();
+                        pv(s, v, j == 0);
+                        if (s == 1) umma_commit(bar_empty(v % NST));
+                        if (j + 1 < nt) {
+                            if (s == 0) full(k);
+                            // S takes the columns of the P that this product reads
+                            mbar_wait(bar_o(s), parity, p.wctx, 5);
+                            tc_fence_after();
+                            qk(s, s, k);
+                            if (s == 1) umma_commit(bar_empty(k % NST));
+                        }
+                    }
+                }
+            } else {
+                for (int j = 0; j < look; ++j) {
+                    full(j);
+                    qk(0, j, j);
+                    umma_commit(bar_empty(j % NST));
+                }
+                for (int j = 0; j < nt; ++j) {
+                    const int s = j % NSTR, v = item_v(j), k = item_k(j + LOOK);
+                    const uint32_t parity = (j / NSTR) & 1u;
+                    full(v);
+                    mbar_wait(bar_p(s), parity, p.wctx, 4);
+                    tc_fence_after();
+                    pv(s, v, j < NSTR);
+                    umma_commit(bar_empty(v % NST));
+                    if (j + LOOK < nt) {
+                        full(k);
+                        mbar_wait(bar_o(s), parity, p.wctx, 5);
+                        tc_fence_after();
+                        qk(0, s, k);
+                        umma_commit(bar_empty(k % NST));
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- softmax: a thread per row
+        const int stream = warp >> 2, row = tid & 127;
+        const int q_tile = QT == 2 ? stream : 0;
+        if (live) {
+            // Q into shared memory, zeros for rows without a token
+            for (int u = tid; u < QT * kRows * CH; u += S::SOFT) {
+                const int r = u / CH, c = u % CH, rt = r & (kRows - 1), tile = r / kRows;
+                const int t = rt / p.G, tok = w.i0 + tile * p.tile_tokens + t;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (t < p.tile_tokens && tok < w.n) {
+                    v = ld_v4(static_cast<const T*>(p.q) + static_cast<long long>(w.q0 + tok) * p.q_token +
+                              static_cast<long long>(w.kvh * p.G + rt - t * p.G) * p.q_head + c * 8);
+                    v.x = (v.x & p.q_and) ^ p.q_xor;
+                    v.y = (v.y & p.q_and) ^ p.q_xor;
+                    v.z = (v.z & p.q_and) ^ p.q_xor;
+                    v.w = (v.w & p.q_and) ^ p.q_xor;
+                }
+                *reinterpret_cast<uint4*>(smem + tile * S::QTILE + (c >> 3) * (kRows * 128) + rt * 128 + (((c & 7) ^ (rt & 7)) << 4)) = v;
+            }
+            fence_proxy_async_smem();
+        }
+        mbar_arrive(bar_q);
+
+        const int t_in = row / p.G;
+        const int tok = w.i0 + q_tile * p.tile_tokens + t_in;
+        const bool mine = live && t_in < p.tile_tokens && tok < w.n;
+        // rows of a tile see up to first .. last, and from first - window + 1 .. last - window + 1 on
+        const int tile_first = p.shared ? w.first : w.first + q_tile * p.tile_tokens;
+        const int tile_last = p.shared ? w.first : min(tile_first + p.tile_tokens - 1, w.first - w.i0 + w.n - 1);
+        const int pos = p.shared ? w.first : tile_first + t_in;
+        const float sl2 = p.soft_cap > 0.f ? 1.f : p.scale_log2;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + S::O_COL + stream * D;
+        const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
+        float m_ref = -CUDART_INF_F, l_run = 0.f;
+
+        for (int it = 0; it < my_blocks; ++it) {
+            const int t0 = block_start(QT == 2 ? it : it * NSTR + stream);
+            mbar_wait(bar_s(stream), it & 1u, p.wctx, 6);
+            tc_fence_after();
+            uint32_t s[KT / 32][32];
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
+            tmem_ld_wait();
+            if (p.soft_cap > 0.f) {
+                // cap tanh(x / cap), in the exponent's domain: 1 - 2 / (1 + exp(2 x / cap))
+                const float cap = p.soft_cap * 1.4426950408889634f, in = 2.f * p.scale_log2 / p.soft_cap;
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        s[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[c][i]) * in)));
+            }
+            const bool all = t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks);
+            if (!all) {
+                const int hi = pos - t0, lo = pos - p.window - t0, sink = p.sinks - t0;
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int j = 32 * c + i;
+                        if (!(j <= hi && (j > lo || j < sink))) s[c][i] = 0xff800000u;
+                    }
+            }
+            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[c][i]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+            if (it == 0) {
+                m_ref = top;
+            } else if (__any_sync(0xffffffffu, top > m_ref + kRaise)) {
+                const float m_new = fmaxf(m_ref, top);
+                const float alpha = m_new == m_ref ? 1.f : exp2f(m_ref - m_new);
+                m_ref = m_new;
+                l_run *= alpha;
+                mbar_wait(bar_o(stream), (it - 1) & 1u, p.wctx, 7);
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32x32(o_at + c, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tmem_st_32x32(o_at + c, o);
+                }
+            }
+            const float m_use = m_ref == -CUDART_INF_F ? 0.f : m_ref;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < KT / 64; ++h) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float a = exp2f(fmaf(__uint_as_float(s[2 * h + i / 16][(2 * i) & 31]), sl2, -m_use));
+                    const float b = exp2f(fmaf(__uint_as_float(s[2 * h + i / 16][(2 * i + 1) & 31]), sl2, -m_use));
+                    sum[i & 1] += a;
+                    sum[2 + (i & 1)] += b;
+                    pk[i] = pack2<T>(a, b);
+                }
+                tmem_st_32x32(s_at + 32 * h, pk);
+            }
+            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar_p(stream));
+        }
+        if (my_blocks > 0) {
+            mbar_wait(bar_o(stream), (my_blocks - 1) & 1u, p.wctx, 8);
+            tc_fence_after();
+        }
+
+        // ---- one row tile, two streams: the second's result to the first through shared memory (every MMA is done with it)
+        float* ex = reinterpret_cast<float*>(smem);   // [D + 2][128]
+        float f0 = 1.f, f1 = 0.f;
+        if constexpr (QT == 1 && NSTR == 2) {
+            named_barrier(1, S::SOFT);
+            if (stream == 1) {
+                ex[D * 128 + row] = m_ref;
+                ex[(D + 1) * 128 + row] = l_run;
+#pragma unroll 1
+                for (int c = 0; c < D && my_blocks > 0; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32x32(o_at + c, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) ex[(c + i) * 128 + row] = __uint_as_float(o[i]);
+                }
+            }
+            named_barrier(1, S::SOFT);
+            const float m1 = ex[D * 128 + row], l1 = ex[(D + 1) * 128 + row];
+            const float m = fmaxf(m_ref, m1), mu = m == -CUDART_INF_F ? 0.f : m;
+            f0 = exp2f(m_ref - mu);
+            f1 = exp2f(m1 - mu);
+            l_run = l_run * f0 + l1 * f1;
+            m_ref = m;
+        }
+        if (QT == 2 || stream == 0) {
+            const float inv = l_run > 0.f ? 1.f / l_run : (l_run == l_run ? 0.f : l_run);   // NaN stays NaN
+            const size_t out_row = static_cast<size_t>(w.q0 + tok) * p.Hq + static_cast<size_t>(w.kvh) * p.G + (row - t_in * p.G);
+            const size_t rows = static_cast<size_t>(p.tokens) * p.Hq;
+            const bool other = QT == 1 && NSTR == 2 && nt > 1;
+            if (p.part_o != nullptr && mine)
+                p.part_lse[w.split * rows + out_row] = l_run > 0.f ? m_ref * 0.6931471805599453f + logf(l_run) : (l_run == l_run ? -CUDART_INF_F : l_run);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (my_blocks > 0) {   // alike in the whole warp
+                    tmem_ld_32x32(o_at + c, o);
+                    tmem_ld_wait();
+                }
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    v[i] = my_blocks > 0 ? __uint_as_float(o[i]) * f0 : 0.f;
+                    if (other) v[i] += ex[(c + i) * 128 + row] * f1;
+                    v[i] *= inv;
+                }
+                if (!mine) continue;
+                if (p.part_o != nullptr) {
+                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + out_row) * D + c);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        dst[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                                            pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == S::SOFT / 32) {
+        tc_fence_after();
+        tmem_dealloc<1>(tmem, 512);
+    }
+}
+
+// out[row] = sum over the parts of exp(lse[part, row] - lse[row]) o[part, row]: D / 4 threads per row
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attention_merge_kernel(const float* part_o, const float* part_lse, int parts, int rows, T* out) {
+    pdl_wait_and_release();
+    const int per = 128 / (D / 4);
+    const long long row = static_cast<long long>(blockIdx.x) * per + threadIdx.x / (D / 4);
+    const int c = static_cast<int>(threadIdx.x) % (D / 4) * 4;
+    if (row >= rows) return;
+    float mm = -CUDART_INF_F;
+    for (int i = 0; i < parts; ++i) mm = fmaxf(mm, part_lse[static_cast<size_t>(i) * rows + row]);
+    const float mu = mm == -CUDART_INF_F ? 0.f : mm;
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        const float f = __expf(part_lse[static_cast<size_t>(i) * rows + row] - mu);
+        const float4 v = *reinterpret_cast<const float4*>(part_o + (static_cast<size_t>(i) * rows + row) * D + c);
+        sum += f;
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+    *reinterpret_cast<uint2*>(out + row * D + c) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+}
+
+}  // namespace attention
+}  // namespace tdist
+
+using namespace tdist;
+using tdist_host::fail;
+
+namespace {
+
+template <typename T, int D, int QT>
+int launch_attention(const attention::Params& p, long long grid, cudaStream_t stream) {
+    using S = attention::Shape<D>;
+    constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 8) * 8 + 16;
+    static bool done[64] = {};
+    static std::mutex setup_lock;
+    int dev = 0;
+    TDIST_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return fail(TDIST_EINVAL, "attention: device ordinal out of range");
+    {
+        std::lock_guard<std::mutex> guard(setup_lock);
+        if (!done[dev]) {
+            TDIST_CUDA_OK(cudaFuncSetAttribute(attention::attention_kernel<T, D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            done[dev] = true;
+        }
+    }
+    TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_kernel<T, D, QT>, dim3(static_cast<unsigned>(grid)), S::THREADS, smem, stream, p));
+    return 0;
+}
+
+template <typename T, int D>
+int run_attention(const TdistAttentionArgs* a, attention::Params& p) {
+    cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+    const long long per = static_cast<long long>(a->row_tiles) * p.tile_tokens;
+    // a sequence's last tile may be short: at most one more per sequence than the tokens fill
+    const long long tiles = p.shared ? (p.tokens + per - 1) / per : p.tokens / per + (p.B < p.tokens ? p.B : p.tokens);
+    const long long grid = tiles * p.Hkv * p.splits;
+    if (grid > 0x7fffffffLL) return fail(TDIST_ELIMIT, "attention: tiles * Hkv * splits exceeds the grid limit");
+    int rc;
+    if constexpr (D <= 128)
+        rc = a->row_tiles == 2 ? launch_attention<T, D, 2>(p, grid, stream) : launch_attention<T, D, 1>(p, grid, stream);
+    else
+        rc = launch_attention<T, D, 1>(p, grid, stream);
+    if (rc != 0 || p.splits == 1 || a->out == nullptr) return rc;
+    const long long rows = static_cast<long long>(p.tokens) * p.Hq, per_cta = 128 / (D / 4);
+    TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)), 128, 0,
+                                         stream, p.part_o, p.part_lse, p.splits, static_cast<int>(rows), static_cast<T*>(a->out)));
+    return 0;
+}
+
+int attention_impl(const TdistAttentionArgs* a) {
+    if (a == nullptr) return fail(TDIST_EINVAL, "attention: null args");
+    if (a->tokens < 1 || a->B < 1 || a->Hq < 1 || a->Hkv < 1 || a->Hq % a->Hkv) return fail(TDIST_EINVAL, "attention: bad token or head counts");
+    if (a->Hq / a->Hkv > attention::kRows) return fail(TDIST_ELIMIT, "attention: at most 128 query heads per kv head");
+    if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return fail(TDIST_EINVAL, "attention: head_dim must be 64, 128 or 256");
+    if (a->page_size < 1 || a->max_blocks < 1 || a->blocks < 1) return fail(TDIST_EINVAL, "attention: page_size, max_blocks and blocks must be at least 1");
+    if ((a->stride_token | a->stride_block | a->stride_head | a->q_token | a->q_head) % 8) return fail(TDIST_EINVAL, "attention: strides must be multiples of 8 elements");
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) |
+         reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->part_o)) % 16)
+        return fail(TDIST_EINVAL, "attention: q, caches, output and partials must be 16-byte aligned");
+    if (a->splits < 1 || a->splits > 256) return fail(TDIST_EINVAL, "attention: splits must be in [1, 256]");
+    if (a->row_tiles < 1 || a->row_tiles > 2 || (a->row_tiles == 2 && a->head_dim > 128)) return fail(TDIST_EINVAL, "attention: bad row_tiles");
+    if (a->window < 1 || a->sinks < 0) return fail(TDIST_EINVAL, "attention: the window must be at least 1, sinks not negative");
+    if (static_cast<long long>(a->tokens) * a->Hq > 0x7fffffffLL) return fail(TDIST_ELIMIT, "attention: tokens * Hq exceeds 2^31 - 1");
+    const bool parts = a->splits > 1 || a->out == nullptr;
+    if (!a->q || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_lens || (!a->shared && !a->q_starts) || (parts && (!a->part_o || !a->part_lse)))
+        return fail(TDIST_EINVAL, "attention: null pointer");
+    if (!(a->soft_cap >= 0.f)) return fail(TDIST_EINVAL, "attention: soft_cap must not be negative");
+    attention::Params p;
+    memset(&p, 0, sizeof(p));
+    p.q = a->q;
+    p.k_cache = a->k_cache;
+    p.v_cache = a->v_cache;
+    p.block_table = static_cast<const int*>(a->block_table);
+    p.q_starts = static_cast<const int*>(a->q_starts);
+    p.kv_lens = static_cast<const int*>(a->kv_lens);
+    p.out = a->out;
+    p.part_o = parts ? static_cast<float*>(a->part_o) : nullptr;
+    p.part_lse = static_cast<float*>(a->part_lse);
+    p.q_token = a->q_token;
+    p.q_head = a->q_head;
+    p.stride_block = a->stride_block;
+    p.stride_token = a->stride_token;
+    p.stride_head = a->stride_head;
+    p.tokens = a->tokens;
+    p.B = a->B;
+    p.Hq = a->Hq;
+    p.Hkv = a->Hkv;
+    p.G = a->Hq / a->Hkv;
+    p.page_size = a->page_size;
+    p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(a->page_size)) : -1;
+    p.max_blocks = a->max_blocks;
+    p.blocks = a->blocks;
+    p.splits = a->splits;
+    p.tile_tokens = attention::kRows / p.G;
+    p.shared = a->shared;
+    p.window = a->shared ? 0x7fffffff : a->window;
+    p.sinks = a->shared ? 0 : a->sinks;
+    p.scale_log2 = (a->scale < 0.f ? -a->scale : a->scale) * 1.4426950408889634f;
+    p.soft_cap = a->soft_cap;
+    // a scale of zero: scores of zero, through q (the kernel's factor stays positive, so that masked scores stay -inf)
+    p.q_and = a->scale == 0.f ? 0u : 0xffffffffu;
+    p.q_xor = a->scale < 0.f ? 0x80008000u : 0u;
+    if (a->scale == 0.f) p.scale_log2 = 1.f;
+    p.wctx.status = static_cast<Status*>(a->status);
+    p.wctx.timeout_ns = a->timeout_ns;
+    p.wctx.kernel_id = attention::kKernelAttention;
+    if (a->dtype == TDIST_BF16) {
+        if (a->head_dim == 64) return run_attention<__nv_bfloat16, 64>(a, p);
+        if (a->head_dim == 128) return run_attention<__nv_bfloat16, 128>(a, p);
+        return run_attention<__nv_bfloat16, 256>(a, p);
+    }
+    if (a->dtype == TDIST_F16) {
+        if (a->head_dim == 64) return run_attention<__half, 64>(a, p);
+        if (a->head_dim == 128) return run_attention<__half, 128>(a, p);
+        return run_attention<__half, 256>(a, p);
+    }
+    return fail(TDIST_EINVAL, "attention: dtype must be bf16 or fp16");
+}
+
+}  // namespace
+
+extern "C" int tdist_attention(const TdistAttentionArgs* a) { return attention_impl(a); }

@@ -72,6 +72,12 @@ struct DecodeParams {
     char* ll_peer_alt[kMaxRanks];
     char* ll_mc;            // SP, optional: multicast alias of this call's parity of the gather buffer: one
     char* ll_mc_alt;        // multimem.st per packet reaches every rank (alt = odd call numbers, device-resident epoch)
+    // windows and earlier partials (kernels with EXT only)
+    int window, sinks;      // a sequence's query sees its last `window` keys and its first `sinks`
+    int max_keys;           // most keys a sequence can have to read
+    int priors;             // partial results of other keys that the merge takes in: O [priors][B * Hq][D], LSE [priors][B * Hq]
+    const float* prior_o;
+    const float* prior_lse;
     WaitCtx wctx;
 };
 
@@ -169,7 +175,10 @@ __device__ __forceinline__ int2 sequence_by_length(const int* kv_lens, int B, in
     return pick_s;
 }
 
-template <typename T, int D, int NH>
+// EXT: the query sees a window and the first keys only (logical key i is token i below `first`, token i + gap from there on), the
+// merge takes in partial results of keys that another kernel read, and the soft cap's tanh is taken from an exponential and a division (good to
+// 2^-23 of the cap, where the hardware's is to 2^-11). A template argument, so that the plain decode keeps its registers.
+template <typename T, int D, int NH, bool EXT>
 __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_decode_kernel(const DecodeParams p) {
     constexpr int CH = D / 8;                      // 16-byte chunks per row
     constexpr int TILE = kTok * D * 2;             // bytes of one K or V block
@@ -198,6 +207,13 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
     } else {
         kv_len = p.kv_lens[b];
     }
+    int first = 0x7fffffff, gap = 0;
+    if constexpr (EXT) {
+        const int lo = max(0, kv_len - p.window);   // first key of the window
+        first = min(p.sinks, lo);
+        gap = lo - first;
+        kv_len -= gap;                              // from here on: keys to read
+    }
     const int G = p.Hq / p.Hkv;
     const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.Hq + static_cast<size_t>(kvh) * G) * D;
     const T* kc = static_cast<const T*>(p.k_cache) + static_cast<size_t>(kvh) * p.stride_head;
@@ -220,12 +236,13 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
     // exchange (head_dim 256, 32 heads on 8: 8 x 32768 keys 348 us, by token 333; 16 x 8192 in pages of one 265 and 198; head_dim
     // 128: 169.4 and 168.2, 101 and 95).
     constexpr bool BY_BLOCK = D == 64;
-    const bool whole = BY_BLOCK && (p.page_size & (kTok - 1)) == 0;
+    const bool whole = BY_BLOCK && (p.page_size & (kTok - 1)) == 0 && (!EXT || gap == 0);
     auto lookup = [&](int i) -> long long {
         long long base = -1;
         if (i < my_blocks && (whole || lane < kTok)) {
-            const int t = (blk0 + warp + i * kDecodeWarps) * kTok + (whole ? 0 : lane);
+            int t = (blk0 + warp + i * kDecodeWarps) * kTok + (whole ? 0 : lane);
             if (t < kv_len) {
+                if constexpr (EXT) t += t < first ? 0 : gap;
                 const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
                 const int page = table[in_table];
                 base = static_cast<long long>(page) * p.stride_block + static_cast<long long>(t - in_table * p.page_size) * p.stride_token;
@@ -329,7 +346,9 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float v = s[h][e];
-                if (p.soft_cap > 0.f) v = p.soft_cap * tanhf(v * p.scale / p.soft_cap) * 1.4426950408889634f;
+                if (EXT && p.soft_cap > 0.f)
+                    v = p.soft_cap * 1.4426950408889634f * (1.f - __fdividef(2.f, 1.f + exp2f(v * (2.f * sl2 / p.soft_cap))));
+                else if (p.soft_cap > 0.f) v = p.soft_cap * tanhf(v * p.scale / p.soft_cap) * 1.4426950408889634f;
                 else v *= sl2;
                 if (tok0 + kTok > kv_len) v = tok0 + (lane >> 2) + (e >> 1) * 8 < kv_len ? v : -CUDART_INF_F;
                 s[h][e] = v;
@@ -482,6 +501,9 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
         const float* src = p.cluster_merge ? part_s + static_cast<size_t>(g) * p.splits * W2 : p.partial + head * p.splits * W2;
         float mm = -CUDART_INF_F;
         for (int sidx = lane; sidx < p.splits; sidx += 32) mm = fmaxf(mm, src[sidx * W2 + D]);
+        const size_t heads = static_cast<size_t>(p.B) * p.Hq;
+        if constexpr (EXT)
+            for (int i = lane; i < p.priors; i += 32) mm = fmaxf(mm, p.prior_lse[i * heads + head]);
 #pragma unroll
         for (int o2 = 16; o2; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
         const float mu = mm == -CUDART_INF_F ? 0.f : mm;
@@ -491,6 +513,12 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
             w_s[warp * 256 + sidx] = f;
             wsum += f;
         }
+        if constexpr (EXT)
+            for (int i = lane; i < p.priors; i += 32) {
+                const float f = __expf(p.prior_lse[i * heads + head] - mu);
+                w_s[warp * 256 + p.splits + i] = f;
+                wsum += f;
+            }
 #pragma unroll
         for (int o2 = 16; o2; o2 >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o2);
         __syncwarp();
@@ -508,6 +536,17 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
                 acc.y += f * lo.y;
                 acc.z += f * hi.x;
                 acc.w += f * hi.y;
+            }
+            if constexpr (EXT) {
+#pragma unroll 8
+                for (int i = 0; i < p.priors; ++i) {
+                    const float4 v = *reinterpret_cast<const float4*>(p.prior_o + (i * heads + head) * D + c);
+                    const float f = w_s[warp * 256 + p.splits + i];
+                    acc.x += f * v.x;
+                    acc.y += f * v.y;
+                    acc.z += f * v.z;
+                    acc.w += f * v.w;
+                }
             }
             acc.x *= inv;
             acc.y *= inv;
@@ -659,7 +698,7 @@ constexpr long long kOverlapKeys = 2560;
 // Whether the CTAs may take their places while the launch before still runs (programmatic dependent launch).
 static bool overlaps_previous(const DecodeParams& p) {
     const long long ctas = static_cast<long long>(p.B) * p.Hkv * p.splits;
-    const long long keys = static_cast<long long>(p.max_blocks) * p.page_size / p.splits;
+    const long long keys = static_cast<long long>(p.max_keys) / p.splits;
     return p.B == 1 || keys <= kOverlapKeys || ctas > 2LL * tdist_host::sm_count();
 }
 
@@ -677,10 +716,10 @@ static int order_from(const DecodeParams& p, int head_dim, int per_sm) {
     if (p.B < 2 || p.B > kMaxOrdered || (p.mode == 2 && p.world > 1) || rounds <= 1.0) return 0;
     const double more = 5.0 * (rounds - 1.5);
     const double keys = kOrderValues * (more > 1.0 ? more : 1.0) / head_dim * p.splits;
-    return keys <= static_cast<double>(p.max_blocks) * p.page_size && keys < 0x7fffffff ? static_cast<int>(keys) : 0;
+    return keys <= static_cast<double>(p.max_keys) && keys < 0x7fffffff ? static_cast<int>(keys) : 0;
 }
 
-template <typename T, int D, int NH>
+template <typename T, int D, int NH, bool EXT>
 static int launch_decode(DecodeParams& p, cudaStream_t stream) {
     constexpr int ring = kDecodeWarps * decode_stages(D) * 2 * kTok * D * 2;
     constexpr int smem = ring + D * 2;   // and its alignment
@@ -699,7 +738,7 @@ static int launch_decode(DecodeParams& p, cudaStream_t stream) {
     {
         std::lock_guard<std::mutex> guard(setup_lock);
         if (!done[dev]) {
-            TDIST_CUDA_OK(cudaFuncSetAttribute(flash_decode_kernel<T, D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            TDIST_CUDA_OK(cudaFuncSetAttribute(flash_decode_kernel<T, D, NH, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             done[dev] = true;
         }
     }
@@ -724,7 +763,7 @@ static int launch_decode(DecodeParams& p, cudaStream_t stream) {
     }
     p.cluster_merge = cluster ? 1 : 0;
     p.order_from = order_from(p, D, decode_ctas_per_sm(D));
-    TDIST_CUDA_OK(cudaLaunchKernelEx(&cfg, flash_decode_kernel<T, D, NH>, p));
+    TDIST_CUDA_OK(cudaLaunchKernelEx(&cfg, flash_decode_kernel<T, D, NH, EXT>, p));
     return 0;
 }
 
@@ -759,6 +798,22 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
     p.stride_head = a->stride_head;
     p.scale = a->scale;
     p.soft_cap = a->soft_cap;
+    const bool ext = a->window > 0;
+    const long long table_keys = static_cast<long long>(a->max_blocks) * a->page_size;
+    long long max_keys = table_keys < 0x7fffffff ? table_keys : 0x7fffffff;
+    if (ext) {
+        if (a->mode != 0) return fail(TDIST_EINVAL, "decode: windows and earlier partials need mode 0");
+        if (a->sinks < 0 || a->priors < 0 || a->priors + a->splits > 256) return fail(TDIST_EINVAL, "decode: sinks must not be negative, splits and priors at most 256 in all");
+        if (a->priors > 0 && (!a->prior_o || !a->prior_lse)) return fail(TDIST_EINVAL, "decode: null pointer");
+        const long long seen = static_cast<long long>(a->window) + a->sinks;
+        if (seen < max_keys) max_keys = seen;
+    }
+    p.max_keys = static_cast<int>(max_keys);
+    p.window = a->window;
+    p.sinks = a->sinks;
+    p.priors = a->priors;
+    p.prior_o = static_cast<const float*>(a->prior_o);
+    p.prior_lse = static_cast<const float*>(a->prior_lse);
     p.mode = a->mode;
     p.world = a->world;
     p.rank = a->rank;
@@ -790,7 +845,9 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
         }
     }
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
-#define TDIST_DECODE_CASE(TT, DD) return G <= 8 ? launch_decode<TT, DD, 1>(p, stream) : launch_decode<TT, DD, 2>(p, stream)
+#define TDIST_DECODE_CASE(TT, DD)                                                                                     \
+    return ext ? (G <= 8 ? launch_decode<TT, DD, 1, true>(p, stream) : launch_decode<TT, DD, 2, true>(p, stream))     \
+               : (G <= 8 ? launch_decode<TT, DD, 1, false>(p, stream) : launch_decode<TT, DD, 2, false>(p, stream))
     const int G = p.Hq / p.Hkv;
     if (a->dtype == TDIST_BF16) {
         if (a->head_dim == 64) TDIST_DECODE_CASE(__nv_bfloat16, 64);

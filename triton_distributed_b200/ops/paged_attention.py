@@ -1,0 +1,243 @@
+"""Attention over the paged KV cache beyond plain decode: sliding windows with first tokens that stay visible (sinks), prefill of
+a ragged batch, and decode of a batch whose sequences share a prefix.
+
+* ``gqa_fwd_window_decode(q[B,Hq,D], k_cache[blocks,page,Hkv,D], v_cache, kv_lens[B], block_table[B,max_blocks], window, sinks,
+  scale, soft_cap) -> [B,Hq,D]``: the query of a sequence of n keys sees key j if j >= n - window or j < sinks
+* ``gqa_fwd_window_prefill(q[T,Hq,D], k_cache, v_cache, q_starts[B+1], kv_lens[B], block_table, window, sinks, scale,
+  soft_cap) -> [T,Hq,D]``: tokens ``q_starts[b]:q_starts[b+1]`` are the last positions of sequence b, whose keys (theirs among
+  them) are in the cache already; position p sees key j if j <= p and (j > p - window or j < sinks)
+* ``gqa_fwd_shared_prefix_decode(q[B,Hq,D], k_cache, v_cache, prefix_len[1], prefix_table[max_blocks], kv_lens[B],
+  block_table, scale, soft_cap) -> [B,Hq,D]``: the softmax runs over the keys of the prefix, read once for all, and the sequence's own
+
+``window=None`` is no limit: plain causal attention. A query that sees no key gives zeros. Pages without a visible key are not
+read, nor are their table entries (a server may have given them back). What lies in a page behind a sequence's last key may be
+anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum.
+
+Decode runs the split decode kernel (``csrc/kernels/flash_decode.cu``), prefill and the shared prefix the tcgen05 kernel
+(``csrc/kernels/attention_sm100.cu``). CPU tensors run ``ref_window_attn`` / ``ref_shared_prefix_attn``, the plain statements.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import torch
+
+from .. import _lib
+from ..runtime import default_timeout_ns, global_status, stream_ptr
+from ..utils.profile import nvtx_range
+from . import flash_decode as FD
+
+launch_count = 0
+_DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+NO_WINDOW = 0x7FFFFFFF
+
+
+def _attend(q, k, v, seen, scale, soft_cap):
+    """fp32 attention of q [n, Hq, D] over k, v [keys, Hkv, D] with a mask [n, keys]; zeros where a row sees nothing."""
+    n, Hq, D = q.shape
+    Hkv = k.shape[1]
+    s = torch.einsum("nhgd,khd->hgnk", q.float().view(n, Hkv, Hq // Hkv, D), k.float()) * scale
+    if soft_cap > 0:
+        s = soft_cap * torch.tanh(s / soft_cap)
+    s = s.masked_fill(~seen, float("-inf"))
+    p = torch.nan_to_num(torch.softmax(s, dim=-1)) if not bool(seen.any(-1).all()) else torch.softmax(s, dim=-1)
+    return torch.einsum("hgnk,khd->nhgd", p, v.float()).reshape(n, Hq, D)
+
+
+def ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window=None, sinks: int = 0, scale=None, soft_cap: float = 0.0):
+    """fp32 reference, sequence by sequence: keys gathered from their pages, an explicit mask."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    page = k_cache.shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float32, device=q.device)
+    for b in range(kv_lens.shape[0]):
+        q0, q1, kv = int(q_starts[b]), int(q_starts[b + 1]), int(kv_lens[b])
+        if q1 <= q0 or kv <= 0:
+            continue
+        pos = torch.arange(kv - (q1 - q0), kv, device=q.device).unsqueeze(1)
+        j = torch.arange(kv, device=q.device)
+        seen = j <= pos
+        if window is not None:
+            seen = seen & ((j > pos - window) | (j < sinks))
+        at = j[seen.any(0)]
+        pages = block_table[b][at // page].long()
+        out[q0:q1] = _attend(q[q0:q1], k_cache[pages, at % page], v_cache[pages, at % page], seen[:, at], scale, soft_cap)
+    return out
+
+
+def ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, scale=None, soft_cap: float = 0.0):
+    """fp32 reference: every sequence's keys are the prefix' and its own, one after the other."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    page, P = k_cache.shape[1], int(prefix_len)
+    at = torch.arange(P, device=q.device)
+    pages, rows = prefix_table[at // page].long(), at % page
+    out = torch.zeros(q.shape, dtype=torch.float32, device=q.device)
+    for b in range(q.shape[0]):
+        own = torch.arange(int(kv_lens[b]), device=q.device)
+        pg, rw = torch.cat([pages, block_table[b][own // page].long()]), torch.cat([rows, own % page])
+        if pg.numel():
+            seen = torch.ones((1, pg.numel()), dtype=torch.bool, device=q.device)
+            out[b:b + 1] = _attend(q[b:b + 1], k_cache[pg, rw], v_cache[pg, rw], seen, scale, soft_cap)
+    return out
+
+
+def _check(q, k_cache, v_cache, window, sinks, soft_cap, ints):
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError("q must be [tokens, Hq, D], the caches [blocks, page, Hkv, D]")
+    if k_cache.shape != v_cache.shape or k_cache.shape[3] != q.shape[2]:
+        raise ValueError("k and v caches need the same shape, with head_dim == q's")
+    if q.shape[1] % k_cache.shape[2]:
+        raise ValueError("the query heads must be a multiple of the kv heads")
+    if window is not None and window < 1:
+        raise ValueError("the window must be at least 1 (None: no limit)")
+    if sinks < 0 or not soft_cap >= 0:
+        raise ValueError("sinks and soft_cap must not be negative")
+    for name, t, shape in ints:
+        if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {['any' if s is None else s for s in shape]}")
+        if t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name} must hold integers (int32 or int64)")
+        if t.device != q.device:
+            raise ValueError(f"{name} must be on q's device")
+    if k_cache.device != q.device or v_cache.device != q.device:
+        raise ValueError("q and the caches must be on one device")
+    if q.device.type != "cuda":
+        return
+    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q, k_cache and v_cache must share one of bf16 / fp16")
+    if q.shape[2] not in (64, 128, 256):
+        raise ValueError("head_dim must be 64, 128 or 256")
+    if k_cache.stride(3) != 1 or v_cache.stride() != k_cache.stride() or q.stride(2) != 1:
+        raise ValueError("q and the caches must have a contiguous head dimension, the caches equal strides")
+
+
+def _check_out(out, q):
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape, dtype and device")
+    return out
+
+
+def _int32(t):
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def _splits(ctas: int, keys: int, head_dim: int, sms: int) -> int:
+    """Parts that the keys of a row tile are cut into: as many CTAs as the machine has SMs (one fits an SM), but at least four
+    blocks of keys each."""
+    block = 128 if head_dim <= 128 else 64
+    return max(1, min(sms // max(1, ctas), -(-keys // (4 * block)), 200))
+
+
+def _run(q, k_cache, v_cache, block_table, q_starts, kv_lens, out, parts, splits, row_tiles, window, sinks, scale, soft_cap, shared):
+    global launch_count
+    T, Hq, D = q.shape
+    a = _lib.AttentionArgs()
+    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    a.block_table, a.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
+    a.q_starts = None if q_starts is None else q_starts.data_ptr()
+    a.out = None if out is None else out.data_ptr()
+    a.part_o, a.part_lse = (None, None) if parts is None else (parts[0].data_ptr(), parts[1].data_ptr())
+    a.q_token, a.q_head = q.stride(0), q.stride(1)
+    a.stride_block, a.stride_token, a.stride_head = k_cache.stride(0), k_cache.stride(1), k_cache.stride(2)
+    a.tokens, a.B, a.Hq, a.Hkv, a.head_dim = T, kv_lens.shape[0], Hq, k_cache.shape[2], D
+    a.page_size, a.max_blocks, a.blocks = k_cache.shape[1], block_table.shape[-1], k_cache.shape[0]
+    a.splits, a.row_tiles, a.window, a.sinks = splits, row_tiles, window, sinks
+    a.shared, a.dtype, a.scale, a.soft_cap = int(shared), _DTYPES[q.dtype], float(scale), float(soft_cap)
+    st = global_status()
+    a.status = st.device_ptr if st is not None else None
+    a.timeout_ns = default_timeout_ns()
+    a.stream = stream_ptr(q.device)
+    _lib.check(_lib.lib().tdist_attention(C.byref(a)), "tdist_attention")
+    launch_count += 1
+
+
+def _parts(splits, rows, D, device):
+    """Partial results of the splits, from the allocator of the current stream."""
+    return (torch.empty((splits, rows, D), dtype=torch.float32, device=device), torch.empty((splits, rows), dtype=torch.float32, device=device))
+
+
+@nvtx_range("tdist.gqa_fwd_window_decode")
+def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Optional[int] = None, sinks: int = 0, scale=None,
+                          soft_cap: float = 0.0, out: Optional[torch.Tensor] = None, kv_split: int = -1):
+    """Decode attention of one query token per sequence over its last ``window`` keys and its first ``sinks``. Returns
+    ``[B, Hq, D]`` in q's dtype; at most 16 query heads per kv head, q contiguous."""
+    B = q.shape[0]
+    _check(q, k_cache, v_cache, window, sinks, soft_cap, (("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if q.device.type != "cuda":
+        starts = torch.arange(B + 1)
+        return ref_window_attn(q, k_cache, v_cache, starts, kv_lens, block_table, window, sinks, scale, soft_cap).to(q.dtype)
+    out = _check_out(out, q)
+    if B == 0:
+        return out
+    return FD._launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, 0, kv_split,
+                      window=min(window, NO_WINDOW) if window is not None else NO_WINDOW, sinks=sinks)
+
+
+@nvtx_range("tdist.gqa_fwd_window_prefill")
+def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, window: Optional[int] = None, sinks: int = 0,
+                           scale=None, soft_cap: float = 0.0, out: Optional[torch.Tensor] = None, kv_split: int = -1):
+    """Attention of a ragged batch of query tokens, the last ones of their sequences. Returns ``[T, Hq, D]`` in q's dtype. q may
+    be a view (part of a fused projection) with strides that are multiples of 8 elements; nothing is read back to the host."""
+    B = kv_lens.shape[0]
+    _check(q, k_cache, v_cache, window, sinks, soft_cap,
+           (("kv_lens", kv_lens, (B,)), ("q_starts", q_starts, (B + 1,)), ("block_table", block_table, (B, None))))
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if q.device.type != "cuda":
+        return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, scale, soft_cap).to(q.dtype)
+    T, Hq, D = q.shape
+    out = _check_out(out, q)
+    if T == 0 or B == 0:
+        return out
+    window = min(window, NO_WINDOW) if window is not None else NO_WINDOW
+    Hkv, page = k_cache.shape[2], k_cache.shape[1]
+    tile = 128 // (Hq // Hkv)
+    each = -(-T // B)                                   # tokens of a sequence, where all have as many
+    row_tiles = 2 if D <= 128 and each > tile else 1
+    if kv_split <= 0:
+        ctas = B * -(-each // (tile * row_tiles)) * Hkv
+        keys = min(block_table.shape[1] * page, window + sinks + tile * row_tiles)
+        kv_split = _splits(ctas, keys, D, FD._sm_count(q.device))
+    parts = _parts(kv_split, T * Hq, D, q.device) if kv_split > 1 else None
+    _run(q, k_cache, v_cache, _int32(block_table), _int32(q_starts), _int32(kv_lens), out, parts, kv_split, row_tiles, window, sinks, scale,
+         soft_cap, False)
+    return out
+
+
+@nvtx_range("tdist.gqa_fwd_shared_prefix_decode")
+def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, scale=None, soft_cap: float = 0.0,
+                                 out: Optional[torch.Tensor] = None, kv_split: int = -1):
+    """Decode attention of one query token per sequence over a prefix that all share and the sequence's own keys. The prefix is in
+    the pages ``prefix_table`` (``prefix_len`` keys; an integer tensor of one element on the device, or a number), the own keys in those of
+    ``block_table`` (``kv_lens`` keys, which may be zero). Returns ``[B, Hq, D]`` in q's dtype; at most 16 query heads per kv head,
+    q contiguous. ``kv_split``: parts of the prefix."""
+    B = q.shape[0]
+    if not isinstance(prefix_len, torch.Tensor):
+        prefix_len = torch.full((1,), int(prefix_len), dtype=torch.int32, device=q.device)
+    _check(q, k_cache, v_cache, None, 0, soft_cap,
+           (("prefix_len", prefix_len, (1,)), ("prefix_table", prefix_table, (None,)), ("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if q.device.type != "cuda":
+        return ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, scale, soft_cap).to(q.dtype)
+    _, Hq, D = q.shape
+    if not q.is_contiguous():
+        raise ValueError("q must be contiguous")
+    out = _check_out(out, q)
+    if B == 0:
+        return out
+    if prefix_table.shape[0] == 0:
+        return FD._launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, 0, -1, window=NO_WINDOW)
+    Hkv, page = k_cache.shape[2], k_cache.shape[1]
+    tile = 128 // (Hq // Hkv)
+    row_tiles = 2 if D <= 128 and B > tile else 1
+    if kv_split <= 0:
+        kv_split = _splits(-(-B // (tile * row_tiles)) * Hkv, prefix_table.shape[0] * page, D, FD._sm_count(q.device))
+    parts = _parts(kv_split, B * Hq, D, q.device)
+    _run(q, k_cache, v_cache, _int32(prefix_table), None, _int32(prefix_len), None, parts, kv_split, row_tiles, NO_WINDOW, 0, scale, soft_cap, True)
+    return FD._launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, 0, -1, window=NO_WINDOW, priors=parts)
