@@ -502,8 +502,9 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
         float mm = -CUDART_INF_F;
         for (int sidx = lane; sidx < p.splits; sidx += 32) mm = fmaxf(mm, src[sidx * W2 + D]);
         const size_t heads = static_cast<size_t>(p.B) * p.Hq;
-        if constexpr (EXT)
+        if constexpr (EXT) {
             for (int i = lane; i < p.priors; i += 32) mm = fmaxf(mm, p.prior_lse[i * heads + head]);
+        }
 #pragma unroll
         for (int o2 = 16; o2; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
         const float mu = mm == -CUDART_INF_F ? 0.f : mm;
@@ -513,12 +514,13 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
             w_s[warp * 256 + sidx] = f;
             wsum += f;
         }
-        if constexpr (EXT)
+        if constexpr (EXT) {
             for (int i = lane; i < p.priors; i += 32) {
                 const float f = __expf(p.prior_lse[i * heads + head] - mu);
                 w_s[warp * 256 + p.splits + i] = f;
                 wsum += f;
             }
+        }
 #pragma unroll
         for (int o2 = 16; o2; o2 >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o2);
         __syncwarp();
