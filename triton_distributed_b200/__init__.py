@@ -32,6 +32,7 @@ from .ops.moe_tp import (ag_group_gemm_inter_node, ag_group_gemm_intra_node, cre
 from .ops.moe_utils import bincount  # noqa: F401
 from .ops.nvls import create_nvls_context, nvls_allgather, nvls_allreduce, nvls_reduce_scatter  # noqa: F401
 from .ops.paged_attention import gqa_fwd_shared_prefix_decode, gqa_fwd_window_decode, gqa_fwd_window_prefill  # noqa: F401
+from .ops.sampling import SampledTokens, sample_tokens  # noqa: F401
 from .runtime import TP_GROUP, check_status, finalize_distributed, initialize_distributed, symm_heap  # noqa: F401
 from .runtime.dist import init_seed  # noqa: F401
 from .runtime.shmem_host import (nvshmem_barrier_all, nvshmem_create_tensor, nvshmem_create_tensor_list_intra_node,  # noqa: F401

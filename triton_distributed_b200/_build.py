@@ -36,6 +36,14 @@ NVCC_FLAGS = [
 ]
 
 
+# Sources whose results are defined bit by bit: IEEE division, CUDA's expf and logf, no flush of subnormals.
+PRECISE = {"sampling.cu"}
+
+
+def _flags(src: Path) -> list[str]:
+    return [f for f in NVCC_FLAGS if not (src.name in PRECISE and f == "--use_fast_math")]
+
+
 def _nvcc() -> str:
     for cand in (os.environ.get("TDIST_NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
         if cand and os.path.exists(cand):
@@ -63,10 +71,10 @@ def _headers_digest(extra_flags=()) -> str:
 def _compile_one(nvcc: str, src: Path, hdr_digest: str, verbose: bool, obj_dir: Path = OBJ_DIR, extra_flags=()) -> tuple[Path, bool, str]:
     obj = obj_dir / (src.stem + ".o")
     stamp = obj_dir / (src.stem + ".sha")
-    digest = hashlib.sha256(src.read_bytes() + hdr_digest.encode()).hexdigest()
+    digest = hashlib.sha256(src.read_bytes() + hdr_digest.encode() + " ".join(_flags(src)).encode()).hexdigest()
     if obj.exists() and stamp.exists() and stamp.read_text() == digest:
         return obj, False, ""
-    cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, *extra_flags, "-x", "cu", "-c", str(src), "-o", str(obj)]
+    cmd = [nvcc, *ARCH_FLAGS, *_flags(src), *extra_flags, "-x", "cu", "-c", str(src), "-o", str(obj)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     log = proc.stdout + proc.stderr
     if proc.returncode != 0:

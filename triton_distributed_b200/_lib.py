@@ -197,6 +197,16 @@ class AttentionArgs(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p), ("tokens", C.c_void_p), ("logprobs", C.c_void_p), ("log_norm", C.c_void_p),
+        ("stride", C.c_longlong), ("B", C.c_int), ("V", C.c_int), ("dtype", C.c_int),
+        ("one_temperature", C.c_float), ("one_top_k", C.c_int), ("one_top_p", C.c_float), ("one_min_p", C.c_float),
+        ("stream", C.c_void_p),
+    ]
+
+
 class PrimArgs(C.Structure):
     _fields_ = [
         ("data_peer", C.c_void_p * MAX_RANKS), ("sig_peer", C.c_void_p * MAX_RANKS),
@@ -266,6 +276,7 @@ def _declare(lib):
     lib.tdist_bounds_checked.argtypes = []
     lib.tdist_flash_decode.argtypes = [C.POINTER(DecodeArgs)]
     lib.tdist_attention.argtypes = [C.POINTER(AttentionArgs)]
+    lib.tdist_sample.argtypes = [C.POINTER(SampleArgs)]
     lib.tdist_lse_combine.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p]
     lib.tdist_dequant_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
     lib.tdist_moe_route.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -444,6 +444,27 @@ int tdist_attention(const TdistAttentionArgs* args);
 /* parts fp32 [ranks, heads, D + 1] -> out [heads, D] */
 int tdist_lse_combine(const void* parts, int ranks, int heads, int head_dim, void* out, int dtype, void* stream);
 
+/* ------------------------------------------------------------------ sampling (csrc/kernels/sampling.cu) */
+typedef struct TdistSampleArgs {
+    const void* logits;       /* [B, V] bf16 / fp16 / fp32, `stride` elements between rows */
+    const void* u;            /* fp32 [B] in [0, 1) */
+    const void* temperature;  /* fp32 [B], or NULL: one_temperature for all; the same for the three below */
+    const void* top_k;        /* int32 [B] */
+    const void* top_p;        /* fp32 [B] */
+    const void* min_p;        /* fp32 [B] */
+    void* tokens;             /* int32 [B], -1: no logit above -inf */
+    void* logprobs;           /* fp32 [B]: log of the token's share of the kept weights */
+    void* log_norm;           /* fp32 [B]: log of the sum of exp(logit / temperature) over the kept tokens */
+    long long stride;
+    int B, V, dtype;
+    float one_temperature;
+    int one_top_k;
+    float one_top_p, one_min_p;
+    void* stream;
+} TdistSampleArgs;
+
+int tdist_sample(const TdistSampleArgs* args);
+
 /* ------------------------------------------------------------------ device primitives, one test op each */
 enum {
     TDIST_PRIM_RING_PUT = 0, TDIST_PRIM_NOTIFY_WAIT = 1, TDIST_PRIM_NOTIFY_ADD = 2, TDIST_PRIM_PUT_SIGNAL = 3,
