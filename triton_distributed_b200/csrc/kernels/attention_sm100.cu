@@ -10,9 +10,9 @@
 //   O += P V takes P from TMEM and V as it lies in the cache (its N dimension contiguous).
 // Two such chains ("streams") run in one CTA, so that the tensor cores work on one while the other is in its softmax: two row tiles
 // over the same keys where there are enough rows, else one row tile over every other block of keys, joined at the end.
-// Warps: 4 per stream for the softmax, one that issues MMAs, kLoaders that copy K and V (16-byte cp.async: pages of any
-// size and stride; rows that nobody sees are not read and become zeros) into a ring of tiles in the 128-byte-swizzled
-// layout the MMAs read.
+// Warps: 4 per stream for the softmax, one that issues MMAs, kLoaders that copy K and V into a ring of tiles in the 128-byte-swizzled
+// layout the MMAs read: by TMA, a box per page (or 128 rows of it) and 64 head dimensions, where the page is a multiple of 8 rows and the
+// whole block is seen; by 16-byte cp.async else (pages of any size; rows that nobody sees are not read and become zeros).
 // Few rows over many keys are split along the keys; the partial results meet in attention_merge_kernel, or in the decode kernel.
 //
 // P is rounded to the inputs' 16 bits (relative 2^-8 or 2^-11), S, O, maximum and sum are fp32. The maximum that is subtracted
@@ -38,10 +38,11 @@ namespace attention {
 constexpr int kKernelAttention = 9;
 constexpr int kRows = 128;      // rows of a tile: the MMA's M
 constexpr int kLoaders = 2;     // warps that copy K and V
-constexpr int kLag = 2;         // tiles that a loader leaves in flight before it hands the oldest over
+constexpr int kPolyEvery = 4;  // every how manieth pair of exponentials is a polynomial
 constexpr float kRaise = 8.f;   // log2 of how far scores may exceed the maximum that is subtracted
 
-struct Params {
+struct alignas(64) Params {
+    CUtensorMap tm_k, tm_v;  // 64 x 1 x box_rows x 1 of (head_dim, Hkv, page, blocks); box_rows > 0
     const void* q;           // rows of D values, strides below
     const void* k_cache;     // [blocks, page, Hkv, D]
     const void* v_cache;
@@ -51,7 +52,9 @@ struct Params {
     void* out;               // T [tokens, Hq, D], where one part holds the result
     float* part_o;           // fp32 [splits][tokens * Hq][D], normalised
     float* part_lse;         // fp32 [splits][tokens * Hq], natural log
-    long long q_token, q_head, stride_block, stride_token, stride_head;   // in elements
+    long long q_token, q_head, stride_head;   // in elements
+    uint32_t unit_block, unit_token;          // strides of the cache in units of 2^unit_shift elements
+    int unit_shift, box_rows;                 // box_rows 0: no TMA
     int tokens, B, Hq, Hkv, G, page_size, page_shift, max_blocks, blocks, splits;
     int tile_tokens;         // tokens of a row tile: 128 / G
     int shared;              // 1: every query token sees all kv_lens[0] keys
@@ -82,10 +85,9 @@ constexpr int kMaxStages = 10;
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// arrives on `bar` once all cp.async that this thread has issued are complete
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 // D (TMEM) (+)= A (TMEM: a row per lane, two 16-bit values per column) x B (shared memory)
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -107,6 +109,15 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r)
         "r"(taddr)
         : "memory");
 }
+// the same, 16 columns
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename T>
@@ -115,6 +126,53 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
 template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+
+// ---- two fp32 values at a time
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^y without the special-function unit: y = n + f, |f| <= 1/2, by adding and taking away 1.5 x 2^23 (+ 127, so that the sum's low
+// bits are the exponent of 2^n); 2^f as a polynomial, p(0) = 1, fitted to the least largest relative error, 2.9e-6. Below -127 it
+// is 0, NaN stays NaN; y < 128.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t y) {
+    float lo, hi;
+    unpair(y, lo, hi);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
+    y = pair(lo, hi);
+    const float magic = 12582912.f + 127.f;
+    const uint64_t t = add2(y, pair(magic, magic));
+    const uint64_t f = fma2(add2(t, pair(-magic, -magic)), pair(-1.f, -1.f), y);
+    uint64_t p = fma2(f, pair(0.009582852944731712f, 0.009582852944731712f), pair(0.055906426161527634f, 0.055906426161527634f));
+    p = fma2(p, f, pair(0.24024099111557007f, 0.24024099111557007f));
+    p = fma2(p, f, pair(0.6931241750717163f, 0.6931241750717163f));
+    p = fma2(p, f, pair(1.f, 1.f));
+    unpair(t, lo, hi);
+    return mul2(p, pair(__uint_as_float(__float_as_uint(lo) << 23), __uint_as_float(__float_as_uint(hi) << 23)));
+}
 
 // What a CTA works on: sequence b, its query tokens [i0, i0 + QT * tile_tokens) of n, the split and the blocks of keys.
 struct Work {
@@ -197,34 +255,35 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
 
 // QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks.
 template <typename T, int D, int QT>
-__global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const Params p) {
+__global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const __grid_constant__ Params p) {
     using S = Shape<D>;
     constexpr int KT = S::KT, NSTR = S::STREAMS, NST = stages<D, QT>(), CH = D / 8;
-    static_assert(NST >= kLag + 2 && NST <= kMaxStages, "a tile is released only once the one after it has been handed over");
+    static_assert(NST >= 2 && NST <= kMaxStages, "a tile is released only once the one after it has arrived");
     static_assert(QT == 1 || NSTR == 2, "two row tiles need two streams");
     constexpr int LOOK = QT == 2 ? 1 : NSTR;   // K blocks loaded ahead of the first V block
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::AREA);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 8);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 10);
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + QT * S::QTILE;
     const uint32_t bars_u32 = smem_u32(bars);
     auto bar_full = [&](int s) { return bars_u32 + 8u * s; };
     auto bar_empty = [&](int s) { return bars_u32 + 8u * (kMaxStages + s); };
     auto bar_s = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + s); };        // S is complete
-    auto bar_p = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 2 + s); };    // P is in its place
-    auto bar_o = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 4 + s); };    // O has taken it in
-    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 6);
+    auto bar_p = [&](int s, int h) { return bars_u32 + 8u * (2 * kMaxStages + 2 + 2 * s + h); };    // a half of P is in its place
+    auto bar_o = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 6 + s); };    // O has taken it in
+    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 8);
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         for (int s = 0; s < NST; ++s) {
-            mbar_init(bar_full(s), kLoaders);
+            mbar_init(bar_full(s), 32 * kLoaders);
             mbar_init(bar_empty(s), 1);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(bar_s(s), 1);
-            mbar_init(bar_p(s), 128);
+            mbar_init(bar_p(s, 0), 128);
+            mbar_init(bar_p(s, 1), 128);
             mbar_init(bar_o(s), 1);
         }
         mbar_init(bar_q, S::SOFT);
@@ -247,157 +306,195 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const P
         const int i = w.c0 + j;
         return (i < w.n_sink ? i : w.m0 + i - w.n_sink) * KT;
     };
+    // every key of the block from t0 on is seen by some row: by TMA
+    auto whole_block = [&](int t0) { return p.box_rows > 0 && ((t0 >= w.lo && t0 + KT <= w.hi) || t0 + KT <= w.s_end); };
     // The ring's items in the order in which the MMAs take them: LOOK blocks of K, then V and K in turn, the last V.
     const int look = min(LOOK, nt);
-    auto item_v = [&](int j) { return j < nt - look ? look + 2 * j : nt + j; };
-    auto item_k = [&](int j) { return j < look ? j : look + 2 * (j - look) + 1; };
 
     if (warp > S::SOFT / 32) {
-        // ---------------------------------------------------------------- loaders: rows [r0, r0 + RW) of every tile
-        constexpr int RW = KT / kLoaders, RL = RW / 32, RPI = 32 / CH;   // rows of a warp, of a lane's lookups, of an instruction
-        const int r0 = (warp - S::SOFT / 32 - 1) * RW;
+        // ---------------------------------------------------------------- loaders
+        constexpr int RW = KT / kLoaders, RL = RW / 32, RPI = 32 / CH;   // cp.async: rows of a warp, of a lane's lookups, of an instruction
+        const int loader = warp - S::SOFT / 32 - 1, r0 = loader * RW;
         const int* table = p.block_table + static_cast<size_t>(live ? w.b : 0) * p.max_blocks;
         const int lrow = lane / CH, lch = lane % CH;
         const T* kl = static_cast<const T*>(p.k_cache) + static_cast<size_t>(w.kvh) * p.stride_head + lch * 8;
         const T* vl = static_cast<const T*>(p.v_cache) + static_cast<size_t>(w.kvh) * p.stride_head + lch * 8;
         const uint32_t lane_dst = static_cast<uint32_t>((lch >> 3) * (KT * 128));
         const int items = 2 * nt;
+        // TMA: box i of a block is 64-column i % CHUNKS of its rows [i / CHUNKS * box_rows, + box_rows); the loaders take them in turn
+        const int box_rows = p.box_rows, boxes = box_rows > 0 ? KT / box_rows * S::CHUNKS : 0;
         auto block_of = [&](int n, bool& is_k) {
             const int m = n - look, pairs = 2 * (nt - look);
             is_k = n < look || (m < pairs && (m & 1));
             return n < look ? n : (m < pairs ? (m >> 1) + (is_k ? look : 0) : m - (nt - look));
         };
-        // offset of the lane's rows of item n in the cache, -1: nobody sees the key
-        auto lookup = [&](int n, long long (&off)[RL]) {
-#pragma unroll
-            for (int r = 0; r < RL; ++r) off[r] = -1;
+        auto page_of = [&](int t, int& in_page) {
+            const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+            in_page = t - in_table * p.page_size;
+            return table[in_table];
+        };
+        constexpr uint32_t kUnseen = 0xffffffffu;
+        struct Item {
+            int t0, page, in_page;   // TMA: of the lane's group of box_rows rows
+            bool is_k, whole;
+            uint32_t off[RL];        // cp.async: the lane's rows in the cache, in units; kUnseen: nobody sees the key
+        };
+        auto lookup = [&](int n, Item& x) {
             if (n >= items) return;
-            bool is_k;
-            const int t0 = block_start(block_of(n, is_k)) + r0 + lane;
+            x.t0 = block_start(block_of(n, x.is_k));
+            x.whole = whole_block(x.t0);
+            if (x.whole) {
+                if (lane * box_rows < KT) x.page = page_of(x.t0 + lane * box_rows, x.in_page);
+            } else {
 #pragma unroll
-            for (int r = 0; r < RL; ++r) {
-                const int t = t0 + 32 * r;
-                if (t < w.s_end || (t >= w.lo && t < w.hi)) {
-                    const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-                    const int page = table[in_table];
-                    if (static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks))
-                        off[r] = static_cast<long long>(page) * p.stride_block + static_cast<long long>(t - in_table * p.page_size) * p.stride_token;
+                for (int r = 0; r < RL; ++r) {
+                    const int t = x.t0 + r0 + lane + 32 * r;
+                    x.off[r] = kUnseen;
+                    if (t < w.s_end || (t >= w.lo && t < w.hi)) {
+                        int in_page;
+                        const int page = page_of(t, in_page);
+                        if (static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks)) x.off[r] = static_cast<uint32_t>(page) * p.unit_block + static_cast<uint32_t>(in_page) * p.unit_token;
+                    }
                 }
             }
         };
-        int done = 0;   // items handed over
-        auto hand_over = [&](int upto) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            for (; done < upto; ++done)
-                if (lane == 0) mbar_arrive(bar_full(done % NST));
-        };
-        long long next[RL];
+        Item next;
         lookup(0, next);
         for (int n = 0; n < items; ++n) {
-            long long off[RL];
-#pragma unroll
-            for (int r = 0; r < RL; ++r) off[r] = next[r];
+            const Item x = next;
             lookup(n + 1, next);
             const int slot = n % NST;
-            const uint32_t parity = ((n / NST) & 1u) ^ 1u;
-            if (__any_sync(0xffffffffu, !mbar_test_wait(bar_empty(slot), parity))) {
-                cp_async_wait<0>();
-                hand_over(n);
-                mbar_wait(bar_empty(slot), parity, p.wctx, 1);
-            }
-            bool is_k;
-            block_of(n, is_k);
-            const T* src = is_k ? kl : vl;
-            const uint32_t dst = ring + static_cast<uint32_t>(slot) * S::TILE + lane_dst;
+            mbar_wait(bar_empty(slot), ((n / NST) & 1u) ^ 1u, p.wctx, 1);
+            const uint32_t dst = ring + static_cast<uint32_t>(slot) * S::TILE;
+            if (x.whole) {
+                if (loader == 0 && lane == 0) mbar_expect_tx(bar_full(slot), S::TILE);
+                else mbar_arrive(bar_full(slot));
+                const CUtensorMap* map = x.is_k ? &p.tm_k : &p.tm_v;
+                for (int r = loader; r * box_rows < KT; r += kLoaders) {
+                    const int page = __shfl_sync(0xffffffffu, x.page, r), in_page = __shfl_sync(0xffffffffu, x.in_page, r);
+                    if (elect_one()) {
 #pragma unroll
-            for (int j = 0; j < RW / RPI; ++j) {
-                const int row = j * RPI + lrow;
-                const long long o = __shfl_sync(0xffffffffu, off[j * RPI / 32], row & 31);
-                const int at = r0 + row;
-                cp_async16(dst + static_cast<uint32_t>(at * 128 + (((lch & 7) ^ (at & 7)) << 4)), src + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
-            }
-            cp_async_commit();
-            if (n - kLag >= done) {
-                cp_async_wait<kLag>();
-                hand_over(n - kLag + 1);
+                        for (int c = 0; c < S::CHUNKS; ++c)
+                            tma_load_4d(dst + c * (KT * 128) + r * box_rows * 128, map, bar_full(slot), c * 64, w.kvh, in_page, page);
+                    }
+                }
+                __syncwarp();
+            } else {
+                const T* src = x.is_k ? kl : vl;
+#pragma unroll
+                for (int j = 0; j < RW / RPI; ++j) {
+                    const int row = j * RPI + lrow, at = r0 + row;
+                    const uint32_t o = __shfl_sync(0xffffffffu, x.off[j * RPI / 32], row & 31);
+                    const bool seen = o != kUnseen;
+                    cp_async16(dst + lane_dst + static_cast<uint32_t>(at * 128 + (((lch & 7) ^ (at & 7)) << 4)),
+                               src + (seen ? static_cast<size_t>(o) << p.unit_shift : 0), seen ? 16 : 0);
+                }
+                cp_async_arrive(bar_full(slot));
             }
         }
-        cp_async_wait<0>();
-        hand_over(items);
     } else if (warp == S::SOFT / 32) {
         // ---------------------------------------------------------------- MMA issue
-        if (lane == 0 && nt > 0) {
+        if (nt > 0) {
+            const bool leader = elect_one();   // the whole warp goes along, so that descriptors stay in uniform registers
             const uint32_t fmt = sizeof(T) == 2 && __is_same(T, __half) ? 0u : 1u;
             const uint32_t idesc_s = umma_idesc(fmt, fmt, kRows, KT);
             const uint32_t idesc_o = umma_idesc(fmt, fmt, kRows, D) | kIdescBNMajor;
-            auto qk = [&](int tile, int stream, int item) {
-                const uint32_t kb = ring + static_cast<uint32_t>(item % NST) * S::TILE, qb = q_smem + tile * S::QTILE;
+            auto qk = [&](int tile, int stream, int slot) {
+                const uint32_t kb = ring + static_cast<uint32_t>(slot) * S::TILE, qb = q_smem + tile * S::QTILE;
+                if (leader) {
 #pragma unroll
-                for (int c = 0; c < S::CHUNKS; ++c) {
-                    const uint64_t a = umma_desc_k_sw128(qb + c * (kRows * 128)), b = umma_desc_k_sw128(kb + c * (KT * 128));
+                    for (int c = 0; c < S::CHUNKS; ++c) {
+                        const uint64_t a = umma_desc_k_sw128(qb + c * (kRows * 128)), b = umma_desc_k_sw128(kb + c * (KT * 128));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_bf16<1>(tmem + stream * 128, a + 2 * k, b + 2 * k, idesc_s, (c | k) != 0 ? 1u : 0u);
+                        for (int k = 0; k < 4; ++k) umma_bf16<1>(tmem + stream * 128, a + 2 * k, b + 2 * k, idesc_s, (c | k) != 0 ? 1u : 0u);
+                    }
+                    umma_commit(bar_s(stream));
                 }
-                umma_commit(bar_s(stream));
+                __syncwarp();
             };
-            auto pv = [&](int stream, int item, bool first) {
-                const uint64_t b = umma_desc_mn_sw128(ring + static_cast<uint32_t>(item % NST) * S::TILE, KT * 128);
+            auto pv = [&](int stream, int slot, uint32_t parity, bool first) {
+                const uint64_t b = umma_desc_mn_sw128(ring + static_cast<uint32_t>(slot) * S::TILE, KT * 128);
 #pragma unroll
-                for (int k = 0; k < KT / 16; ++k)
-                    umma_ts(tmem + S::O_COL + stream * D, tmem + stream * 128 + 8 * k, b + 128 * k, idesc_o, !first || k != 0 ? 1u : 0u);
-                umma_commit(bar_o(stream));
+                for (int h = 0; h < 2; ++h) {
+                    mbar_wait(bar_p(stream, h), parity, p.wctx, 4);
+                    tc_fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int k = h * (KT / 32); k < (h + 1) * (KT / 32); ++k)
+                            umma_ts(tmem + S::O_COL + stream * D, tmem + stream * 128 + 8 * k, b + 128 * k, idesc_o, !first || k != 0 ? 1u : 0u);
+                        if (h == 1) umma_commit(bar_o(stream));
+                    }
+                    __syncwarp();
+                }
             };
-            auto full = [&](int item) {
-                mbar_wait(bar_full(item % NST), (item / NST) & 1u, p.wctx, 2);
+            auto release = [&](int slot) {
+                if (leader) umma_commit(bar_empty(slot));
+                __syncwarp();
+            };
+            // the ring's next item: its slot, and the parity of its arrival
+            int slot = 0;
+            uint32_t phase = 0;
+            auto next_slot = [&]() {
+                const int at = slot;
+                if (++slot == NST) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+                return at;
+            };
+            auto full = [&](int at, uint32_t parity, int block) {
+                mbar_wait(bar_full(at), parity, p.wctx, 2);
+                if (!whole_block(block_start(block))) fence_proxy_async_smem();   // what cp.async wrote, to the MMAs' proxy
                 tc_fence_after();
             };
             mbar_wait(bar_q, 0, p.wctx, 3);
             if constexpr (QT == 2) {
-                full(0);
+                full(0, 0, 0);
+                next_slot();
                 qk(0, 0, 0);
                 qk(1, 1, 0);
-                umma_commit(bar_empty(0));
+                release(0);
                 for (int j = 0; j < nt; ++j) {
-                    const int v = item_v(j), k = item_k(j + 1);
-                    const uint32_t parity = j & 1u;
-                    full(v);
+                    const uint32_t parity = j & 1u, v_phase = phase;
+                    const int v = next_slot();
+                    const uint32_t k_phase = phase;
+                    const int k = next_slot();
+                    full(v, v_phase, j);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        mbar_wait(bar_p(s), parity, p.wctx, 4);
-                        tc_fence_after();
-                        pv(s, v, j == 0);
-                        if (s == 1) umma_commit(bar_empty(v % NST));
+                        pv(s, v, parity, j == 0);
+                        if (s == 1) release(v);
                         if (j + 1 < nt) {
-                            if (s == 0) full(k);
+                            if (s == 0) full(k, k_phase, j + 1);
                             // S takes the columns of the P that this product reads
                             mbar_wait(bar_o(s), parity, p.wctx, 5);
                             tc_fence_after();
                             qk(s, s, k);
-                            if (s == 1) umma_commit(bar_empty(k % NST));
+                            if (s == 1) release(k);
                         }
                     }
                 }
             } else {
                 for (int j = 0; j < look; ++j) {
-                    full(j);
+                    full(j, 0, j);
                     qk(0, j, j);
-                    umma_commit(bar_empty(j % NST));
+                    release(next_slot());
                 }
                 for (int j = 0; j < nt; ++j) {
-                    const int s = j % NSTR, v = item_v(j), k = item_k(j + LOOK);
-                    const uint32_t parity = (j / NSTR) & 1u;
-                    full(v);
-                    mbar_wait(bar_p(s), parity, p.wctx, 4);
-                    tc_fence_after();
-                    pv(s, v, j < NSTR);
-                    umma_commit(bar_empty(v % NST));
+                    const int s = j % NSTR;
+                    const uint32_t parity = (j / NSTR) & 1u, v_phase = phase;
+                    const int v = next_slot();
+                    full(v, v_phase, j);
+                    pv(s, v, parity, j < NSTR);
+                    release(v);
                     if (j + LOOK < nt) {
-                        full(k);
+                        const uint32_t k_phase = phase;
+                        const int k = next_slot();
+                        full(k, k_phase, j + LOOK);
                         mbar_wait(bar_o(s), parity, p.wctx, 5);
                         tc_fence_after();
                         qk(0, s, k);
-                        umma_commit(bar_empty(k % NST));
+                        release(k);
                     }
                 }
             }
@@ -444,36 +541,46 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const P
             const int t0 = block_start(QT == 2 ? it : it * NSTR + stream);
             mbar_wait(bar_s(stream), it & 1u, p.wctx, 6);
             tc_fence_after();
-            uint32_t s[KT / 32][32];
+            // ---- the row's maximum, 32 columns at a time; capped and masked scores go back to TMEM
+            const bool all = t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks);
+            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+            if (all && p.soft_cap <= 0.f) {
+                uint32_t s[2][32];
+                tmem_ld_32x32(s_at, s[0]);
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
-            tmem_ld_wait();
-            if (p.soft_cap > 0.f) {
+                for (int c = 0; c < KT / 32; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < KT / 32) tmem_ld_32x32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
+                }
+            } else {
                 // cap tanh(x / cap), in the exponent's domain: 1 - 2 / (1 + exp(2 x / cap))
                 const float cap = p.soft_cap * 1.4426950408889634f, in = 2.f * p.scale_log2 / p.soft_cap;
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        s[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[c][i]) * in)));
-            }
-            const bool all = t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks);
-            if (!all) {
                 const int hi = pos - t0, lo = pos - p.window - t0, sink = p.sinks - t0;
+#pragma unroll 1
+                for (int c = 0; c < KT; c += 32) {
+                    uint32_t s[32];
+                    tmem_ld_32x32(s_at + c, s);
+                    tmem_ld_wait();
+                    if (p.soft_cap > 0.f) {
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int j = 32 * c + i;
-                        if (!(j <= hi && (j > lo || j < sink))) s[c][i] = 0xff800000u;
+                        for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[i]) * in)));
                     }
+                    if (!all) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int j = c + i;
+                            if (!(j <= hi && (j > lo || j < sink))) s[i] = 0xff800000u;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    tmem_st_32x32(s_at + c, s);
+                }
+                tmem_st_wait();
             }
-            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-            for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[c][i]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
             if (it == 0) {
                 m_ref = top;
             } else if (__any_sync(0xffffffffu, top > m_ref + kRaise)) {
@@ -494,24 +601,46 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const P
                 }
             }
             const float m_use = m_ref == -CUDART_INF_F ? 0.f : m_ref;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            // ---- P, 32 columns at a time, over S columns that have been read
+            const uint64_t scale2 = pair(sl2, sl2), minus2 = pair(-m_use, -m_use);
+            uint64_t sum2[2] = {0ull, 0ull};
+            {
+                uint32_t s[2][32];
+                tmem_ld_32x32(s_at, s[0]);
 #pragma unroll
-            for (int h = 0; h < KT / 64; ++h) {
-                uint32_t pk[32];
+                for (int c = 0; c < KT / 32; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < KT / 32) tmem_ld_32x32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                    uint32_t pk[16];
+                    float a[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float a = exp2f(fmaf(__uint_as_float(s[2 * h + i / 16][(2 * i) & 31]), sl2, -m_use));
-                    const float b = exp2f(fmaf(__uint_as_float(s[2 * h + i / 16][(2 * i + 1) & 31]), sl2, -m_use));
-                    sum[i & 1] += a;
-                    sum[2 + (i & 1)] += b;
-                    pk[i] = pack2<T>(a, b);
+                    for (int i = 0; i < 16; ++i) {
+                        uint64_t y = fma2(pair(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), scale2, minus2);
+                        if (i % kPolyEvery == kPolyEvery - 1) y = exp2_poly(y);
+                        unpair(y, a[2 * i], a[2 * i + 1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i % kPolyEvery != kPolyEvery - 1) {
+                            a[2 * i] = exp2f(a[2 * i]);
+                            a[2 * i + 1] = exp2f(a[2 * i + 1]);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        sum2[i & 1] = add2(sum2[i & 1], pair(a[2 * i], a[2 * i + 1]));
+                        pk[i] = pack2<T>(a[2 * i], a[2 * i + 1]);
+                    }
+                    tmem_st_32x16(s_at + 16 * c, pk);
+                    if ((c + 1) % (KT / 64) == 0) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(bar_p(stream, c / (KT / 64)));
+                    }
                 }
-                tmem_st_32x32(s_at + 32 * h, pk);
             }
-            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(bar_p(stream));
+            float sum_lo, sum_hi;
+            unpair(add2(sum2[0], sum2[1]), sum_lo, sum_hi);
+            l_run += sum_lo + sum_hi;
         }
         if (my_blocks > 0) {
             mbar_wait(bar_o(stream), (my_blocks - 1) & 1u, p.wctx, 8);
@@ -625,7 +754,7 @@ namespace {
 template <typename T, int D, int QT>
 int launch_attention(const attention::Params& p, long long grid, cudaStream_t stream) {
     using S = attention::Shape<D>;
-    constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 8) * 8 + 16;
+    constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 10) * 8 + 16;
     static bool done[64] = {};
     static std::mutex setup_lock;
     int dev = 0;
@@ -693,9 +822,15 @@ int attention_impl(const TdistAttentionArgs* a) {
     p.part_lse = static_cast<float*>(a->part_lse);
     p.q_token = a->q_token;
     p.q_head = a->q_head;
-    p.stride_block = a->stride_block;
-    p.stride_token = a->stride_token;
     p.stride_head = a->stride_head;
+    // offsets of a key in the cache as 32-bit numbers of the largest unit that divides both strides (at least 16 bytes: 64 GB per cache)
+    const long long strides = a->stride_block | a->stride_token;
+    p.unit_shift = strides == 0 ? 3 : __builtin_ctzll(static_cast<unsigned long long>(strides));
+    if (p.unit_shift > 16) p.unit_shift = 16;
+    const long long units = (a->stride_block >> p.unit_shift) * (a->blocks - 1LL) + (a->stride_token >> p.unit_shift) * (a->page_size - 1LL);
+    if (a->stride_block < 0 || a->stride_token < 0 || a->stride_head < 0 || units >= 0xffffffffLL) return fail(TDIST_ELIMIT, "attention: cache strides negative or beyond 2^32 units");
+    p.unit_block = static_cast<uint32_t>(a->stride_block >> p.unit_shift);
+    p.unit_token = static_cast<uint32_t>(a->stride_token >> p.unit_shift);
     p.tokens = a->tokens;
     p.B = a->B;
     p.Hq = a->Hq;
@@ -716,6 +851,20 @@ int attention_impl(const TdistAttentionArgs* a) {
     p.q_and = a->scale == 0.f ? 0u : 0xffffffffu;
     p.q_xor = a->scale < 0.f ? 0x80008000u : 0u;
     if (a->scale == 0.f) p.scale_log2 = 1.f;
+    // TMA: boxes of as many rows as divide both a page and a block of keys, at least the swizzle's eight
+    const int block = a->head_dim <= 128 ? 128 : 64;
+    int rows = a->page_size & -a->page_size;
+    if (rows > block) rows = block;
+    if (rows >= 8 && a->stride_token > 0 && a->stride_block > 0 && a->stride_head > 0) {
+        const uint64_t dims[4] = {static_cast<uint64_t>(a->head_dim), static_cast<uint64_t>(a->Hkv), static_cast<uint64_t>(a->page_size), static_cast<uint64_t>(a->blocks)};
+        const uint64_t bytes[3] = {static_cast<uint64_t>(a->stride_head) * 2, static_cast<uint64_t>(a->stride_token) * 2, static_cast<uint64_t>(a->stride_block) * 2};
+        const uint32_t box[4] = {64, 1, static_cast<uint32_t>(rows), 1};
+        const CUtensorMapDataType type = a->dtype == TDIST_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+        int rc = tdist_host::encode_tmap(&p.tm_k, type, 2, 4, a->k_cache, dims, bytes, box, tdist_host::Swizzle::B128, false);
+        if (rc == 0) rc = tdist_host::encode_tmap(&p.tm_v, type, 2, 4, a->v_cache, dims, bytes, box, tdist_host::Swizzle::B128, false);
+        if (rc != 0) return rc;
+        p.box_rows = rows;
+    }
     p.wctx.status = static_cast<Status*>(a->status);
     p.wctx.timeout_ns = a->timeout_ns;
     p.wctx.kernel_id = attention::kKernelAttention;

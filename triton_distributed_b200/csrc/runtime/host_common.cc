@@ -49,8 +49,8 @@ std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> g_tmap_cache;
 }  // namespace
 
 int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int rank_, const void* base,
-                const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, Swizzle sw) {
-    if (rank_ < 2 || rank_ > 3) return fail(TDIST_EINVAL, "encode_tmap: rank must be 2 or 3");
+                const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, Swizzle sw, bool keep) {
+    if (rank_ < 2 || rank_ > 4) return fail(TDIST_EINVAL, "encode_tmap: rank must be 2, 3 or 4");
     if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
         return fail(TDIST_EINVAL, "tensor map base address is not 16-byte aligned");
     for (int i = 0; i + 1 < rank_; ++i)
@@ -66,10 +66,10 @@ int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int
                    static_cast<uint64_t>(sw == Swizzle::B128);
     for (int i = 0; i < rank_; ++i) {
         key.words[2 + i] = dims[i];
-        key.words[8 + i] = box[i];
+        key.words[9 + i] = box[i];
     }
-    for (int i = 0; i + 1 < rank_; ++i) key.words[5 + i] = strides_bytes[i];
-    {
+    for (int i = 0; i + 1 < rank_; ++i) key.words[6 + i] = strides_bytes[i];
+    if (keep) {
         std::lock_guard<std::mutex> lk(g_tmap_mu);
         auto it = g_tmap_cache.find(key);
         if (it != g_tmap_cache.end()) {
@@ -83,10 +83,10 @@ int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int
                                   CUtensorMapFloatOOBfill);
     static EncodeFn encode = reinterpret_cast<EncodeFn>(driver_fn("cuTensorMapEncodeTiled"));
     if (encode == nullptr) return TDIST_EDRIVER;
-    cuuint64_t gdims[3];
-    cuuint64_t gstrides[2];
-    cuuint32_t gbox[3];
-    cuuint32_t estr[3] = {1, 1, 1};
+    cuuint64_t gdims[4];
+    cuuint64_t gstrides[3];
+    cuuint32_t gbox[4];
+    cuuint32_t estr[4] = {1, 1, 1, 1};
     for (int i = 0; i < rank_; ++i) {
         gdims[i] = dims[i];
         gbox[i] = box[i];
@@ -98,7 +98,7 @@ int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(TDIST_EINVAL, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(static_cast<int>(r)));
-    {
+    if (keep) {
         std::lock_guard<std::mutex> lk(g_tmap_mu);
         if (g_tmap_cache.size() > 4096) g_tmap_cache.clear();
         g_tmap_cache.emplace(key, *out);

@@ -25,11 +25,11 @@ void* driver_fn(const char* name);
 
 enum class Swizzle { None, B128 };
 
-// Encodes (or fetches from the cache) a tiled tensor map of rank 2 or 3. dims/box are in
-// elements, innermost first; strides_bytes[i] is the byte stride of dimension i+1.
+// Encodes (or fetches from the cache; `keep` false: neither looks there nor leaves it there) a tiled tensor map of rank 2 to 4. dims/box
+// are in elements, innermost first; strides_bytes[i] is the byte stride of dimension i+1.
 // Returns 0 or a TDIST_E* code.
 int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int rank_, const void* base,
-                const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, Swizzle sw);
+                const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, Swizzle sw, bool keep = true);
 
 int sm_count();
 
