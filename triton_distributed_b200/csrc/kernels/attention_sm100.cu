@@ -6,11 +6,11 @@
 //
 // A tile is 128 rows of one kv head: the G query heads that share it for 128 / G tokens, so that a key is read once for all of
 // them. A CTA goes over its keys 128 at a time (64 with head_dim 256) with the running maximum and sum of a softmax:
-//   S = Q K^T in TMEM (128 x 128 fp32), a thread per row turns it into P = exp2(S - m) in 16 bits, in place of S in TMEM, and
+//   S = Q K^T in TMEM (128 x 128 fp32), two threads per row turn it into P = exp2(S - m) in 16 bits, in place of S in TMEM, and
 //   O += P V takes P from TMEM and V as it lies in the cache (its N dimension contiguous).
 // Two such chains ("streams") run in one CTA, so that the tensor cores work on one while the other is in its softmax: two row tiles
 // over the same keys where there are enough rows, else one row tile over every other block of keys, joined at the end.
-// Warps: 4 per stream for the softmax, one that issues MMAs, kLoaders that copy K and V into a ring of tiles in the 128-byte-swizzled
+// Warps: 8 per stream for the softmax (two threads per row), one that issues MMAs, kLoaders that copy K and V into a ring of tiles in the 128-byte-swizzled
 // layout the MMAs read: by TMA, a box per page (or 128 rows of it) and 64 head dimensions, where the page is a multiple of 8 rows and the
 // whole block is seen; by 16-byte cp.async else (pages of any size; rows that nobody sees are not read and become zeros).
 // Few rows over many keys are split along the keys; the partial results meet in attention_merge_kernel, or in the decode kernel.
@@ -72,7 +72,8 @@ struct Shape {
     static constexpr int QTILE = kRows * D * 2;
     static constexpr int CHUNKS = D / 64;                 // 128-byte columns of a tile
     static constexpr int AREA = D == 64 ? 160 * 1024 : 224 * 1024;
-    static constexpr int SOFT = 128 * STREAMS;            // softmax threads
+    static constexpr int HALF = KT / 2;                   // keys of a softmax thread
+    static constexpr int SOFT = 256 * STREAMS;            // softmax threads: two per row
     static constexpr int THREADS = SOFT + 32 + 32 * kLoaders;
     static constexpr uint32_t O_COL = 256;                // TMEM columns: S / P of stream s at s * 128, O at O_COL + s * D
 };
@@ -97,19 +98,25 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
         "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 32 lanes x 32 columns: thread t of the warp writes columns [col, col + 32) of TMEM lane (lane_base + t)
-__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-        "r"(taddr)
-        : "memory");
+// one column
+__device__ __forceinline__ void tmem_st_32x1(uint32_t taddr, float v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%1], {%0};" ::"f"(v), "r"(taddr) : "memory");
 }
-// the same, 16 columns
+__device__ __forceinline__ float tmem_ld_32x1(uint32_t taddr) {
+    float v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(v) : "r"(taddr) : "memory");
+    return v;
+}
+// Barrier of `n` threads that tells all whether one of them had `v`.
+__device__ __forceinline__ bool barrier_or(uint32_t id, uint32_t n, bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\tbar.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r)
+                 : "r"(id), "r"(n), "r"(static_cast<uint32_t>(v))
+                 : "memory");
+    return r != 0;
+}
+// 32 lanes x 16 columns: thread t of the warp writes columns [col, col + 16) of TMEM lane (lane_base + t)
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
@@ -421,7 +428,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                     if (leader) {
 #pragma unroll
                         for (int k = h * (KT / 32); k < (h + 1) * (KT / 32); ++k)
-                            umma_ts(tmem + S::O_COL + stream * D, tmem + stream * 128 + 8 * k, b + 128 * k, idesc_o, !first || k != 0 ? 1u : 0u);
+                            umma_ts(tmem + S::O_COL + stream * D, tmem + stream * 128 + h * S::HALF + 8 * (k - h * (KT / 32)), b + 128 * k, idesc_o, !first || k != 0 ? 1u : 0u);
                         if (h == 1) umma_commit(bar_o(stream));
                     }
                     __syncwarp();
@@ -501,8 +508,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         }
         __syncwarp();
     } else {
-        // ---------------------------------------------------------------- softmax: a thread per row
-        const int stream = warp >> 2, row = tid & 127;
+        // ---------------------------------------------------------------- softmax: two threads per row, half of the block's keys each
+        const int stream = warp >> 3, half = (warp >> 2) & 1, row = tid & 127;
         const int q_tile = QT == 2 ? stream : 0;
         if (live) {
             // Q into shared memory, zeros for rows without a token
@@ -533,57 +540,59 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int pos = p.shared ? w.first : tile_first + t_in;
         const float sl2 = p.soft_cap > 0.f ? 1.f : p.scale_log2;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + S::O_COL + stream * D;
+        // this half's columns of S, which begin with those of its P, and of O
+        const uint32_t s_at = tmem + lanes + stream * 128 + half * S::HALF, o_at = tmem + lanes + S::O_COL + stream * D + half * (D / 2);
         const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
         float m_ref = -CUDART_INF_F, l_run = 0.f;
+        // The other half's value, through a column of S that both have read and that P leaves alone.
+        auto exchange = [&](float v) {
+            tmem_st_32x1(s_at + S::HALF - 1, v);
+            tmem_st_wait();
+            tc_fence_before();
+            named_barrier(1 + stream, 256);
+            tc_fence_after();
+            const float got = tmem_ld_32x1(half == 0 ? s_at + 2 * S::HALF - 1 : s_at - 1);
+            tmem_ld_wait();
+            return got;
+        };
 
         for (int it = 0; it < my_blocks; ++it) {
             const int t0 = block_start(QT == 2 ? it : it * NSTR + stream);
             mbar_wait(bar_s(stream), it & 1u, p.wctx, 6);
             tc_fence_after();
-            // ---- the row's maximum, 32 columns at a time; capped and masked scores go back to TMEM
-            const bool all = t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks);
-            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-            if (all && p.soft_cap <= 0.f) {
-                uint32_t s[2][32];
-                tmem_ld_32x32(s_at, s[0]);
+            constexpr int NC = S::HALF / 32;
+            uint32_t s[NC][32];
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    tmem_ld_wait();
-                    if (c + 1 < KT / 32) tmem_ld_32x32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
-                }
-            } else {
+            for (int c = 0; c < NC; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
+            tmem_ld_wait();
+            if (p.soft_cap > 0.f) {
                 // cap tanh(x / cap), in the exponent's domain: 1 - 2 / (1 + exp(2 x / cap))
                 const float cap = p.soft_cap * 1.4426950408889634f, in = 2.f * p.scale_log2 / p.soft_cap;
-                const int hi = pos - t0, lo = pos - p.window - t0, sink = p.sinks - t0;
-#pragma unroll 1
-                for (int c = 0; c < KT; c += 32) {
-                    uint32_t s[32];
-                    tmem_ld_32x32(s_at + c, s);
-                    tmem_ld_wait();
-                    if (p.soft_cap > 0.f) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[i]) * in)));
-                    }
-                    if (!all) {
+                for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int j = c + i;
-                            if (!(j <= hi && (j > lo || j < sink))) s[i] = 0xff800000u;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                    tmem_st_32x32(s_at + c, s);
-                }
-                tmem_st_wait();
+                    for (int i = 0; i < 32; ++i) s[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[c][i]) * in)));
             }
-            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
+            if (!(t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks))) {
+                const int k0 = t0 + half * S::HALF, hi = pos - k0, lo = pos - p.window - k0, sink = p.sinks - k0;
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int j = 32 * c + i;
+                        if (!(j <= hi && (j > lo || j < sink))) s[c][i] = 0xff800000u;
+                    }
+            }
+            float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+            float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
             if (it == 0) {
-                m_ref = top;
-            } else if (__any_sync(0xffffffffu, top > m_ref + kRaise)) {
+                m_ref = fmaxf(top, exchange(top));
+            } else if (barrier_or(1 + stream, 256, top > m_ref + kRaise)) {
+                top = fmaxf(top, exchange(top));
                 const float m_new = fmaxf(m_ref, top);
                 const float alpha = m_new == m_ref ? 1.f : exp2f(m_ref - m_new);
                 m_ref = m_new;
@@ -591,53 +600,46 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                 mbar_wait(bar_o(stream), (it - 1) & 1u, p.wctx, 7);
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld_32x32(o_at + c, o);
+                for (int c = 0; c < D / 2; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld_32x16(o_at + c, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                    tmem_st_32x32(o_at + c, o);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tmem_st_32x16(o_at + c, o);
                 }
+                // O is whole before either half lets the next product begin
+                tmem_st_wait();
+                tc_fence_before();
+                named_barrier(1 + stream, 256);
             }
             const float m_use = m_ref == -CUDART_INF_F ? 0.f : m_ref;
-            // ---- P, 32 columns at a time, over S columns that have been read
             const uint64_t scale2 = pair(sl2, sl2), minus2 = pair(-m_use, -m_use);
             uint64_t sum2[2] = {0ull, 0ull};
-            {
-                uint32_t s[2][32];
-                tmem_ld_32x32(s_at, s[0]);
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    tmem_ld_wait();
-                    if (c + 1 < KT / 32) tmem_ld_32x32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t pk[16];
-                    float a[32];
+            for (int c = 0; c < NC; ++c) {
+                uint32_t pk[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        uint64_t y = fma2(pair(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), scale2, minus2);
-                        if (i % kPolyEvery == kPolyEvery - 1) y = exp2_poly(y);
-                        unpair(y, a[2 * i], a[2 * i + 1]);
+                for (int i = 0; i < 16; ++i) {
+                    uint64_t y = fma2(pair(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, minus2);
+                    float a, b;
+                    if (i % kPolyEvery == kPolyEvery - 1) {
+                        y = exp2_poly(y);
+                        unpair(y, a, b);
+                    } else {
+                        unpair(y, a, b);
+                        a = exp2f(a);
+                        b = exp2f(b);
+                        y = pair(a, b);
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (i % kPolyEvery != kPolyEvery - 1) {
-                            a[2 * i] = exp2f(a[2 * i]);
-                            a[2 * i + 1] = exp2f(a[2 * i + 1]);
-                        }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        sum2[i & 1] = add2(sum2[i & 1], pair(a[2 * i], a[2 * i + 1]));
-                        pk[i] = pack2<T>(a[2 * i], a[2 * i + 1]);
-                    }
-                    tmem_st_32x16(s_at + 16 * c, pk);
-                    if ((c + 1) % (KT / 64) == 0) {
-                        tmem_st_wait();
-                        tc_fence_before();
-                        mbar_arrive(bar_p(stream, c / (KT / 64)));
-                    }
+                    sum2[i & 1] = add2(sum2[i & 1], y);
+                    pk[i] = pack2<T>(a, b);
                 }
+                tmem_st_32x16(s_at + 16 * c, pk);
             }
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar_p(stream, half));
             float sum_lo, sum_hi;
             unpair(add2(sum2[0], sum2[1]), sum_lo, sum_hi);
             l_run += sum_lo + sum_hi;
@@ -645,26 +647,29 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         if (my_blocks > 0) {
             mbar_wait(bar_o(stream), (my_blocks - 1) & 1u, p.wctx, 8);
             tc_fence_after();
+            l_run += exchange(l_run);
         }
 
         // ---- one row tile, two streams: the second's result to the first through shared memory (every MMA is done with it)
         float* ex = reinterpret_cast<float*>(smem);   // [D + 2][128]
         float f0 = 1.f, f1 = 0.f;
         if constexpr (QT == 1 && NSTR == 2) {
-            named_barrier(1, S::SOFT);
+            named_barrier(3, S::SOFT);
             if (stream == 1) {
-                ex[D * 128 + row] = m_ref;
-                ex[(D + 1) * 128 + row] = l_run;
+                if (half == 0) {
+                    ex[D * 128 + row] = m_ref;
+                    ex[(D + 1) * 128 + row] = l_run;
+                }
 #pragma unroll 1
-                for (int c = 0; c < D && my_blocks > 0; c += 32) {
+                for (int c = 0; c < D / 2 && my_blocks > 0; c += 32) {
                     uint32_t o[32];
                     tmem_ld_32x32(o_at + c, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) ex[(c + i) * 128 + row] = __uint_as_float(o[i]);
+                    for (int i = 0; i < 32; ++i) ex[(half * (D / 2) + c + i) * 128 + row] = __uint_as_float(o[i]);
                 }
             }
-            named_barrier(1, S::SOFT);
+            named_barrier(3, S::SOFT);
             const float m1 = ex[D * 128 + row], l1 = ex[(D + 1) * 128 + row];
             const float m = fmaxf(m_ref, m1), mu = m == -CUDART_INF_F ? 0.f : m;
             f0 = exp2f(m_ref - mu);
@@ -677,10 +682,10 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             const size_t out_row = static_cast<size_t>(w.q0 + tok) * p.Hq + static_cast<size_t>(w.kvh) * p.G + (row - t_in * p.G);
             const size_t rows = static_cast<size_t>(p.tokens) * p.Hq;
             const bool other = QT == 1 && NSTR == 2 && nt > 1;
-            if (p.part_o != nullptr && mine)
+            if (p.part_o != nullptr && mine && half == 0)
                 p.part_lse[w.split * rows + out_row] = l_run > 0.f ? m_ref * 0.6931471805599453f + logf(l_run) : (l_run == l_run ? -CUDART_INF_F : l_run);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = 0; c < D / 2; c += 32) {
                 uint32_t o[32];
                 if (my_blocks > 0) {   // alike in the whole warp
                     tmem_ld_32x32(o_at + c, o);
@@ -690,16 +695,16 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     v[i] = my_blocks > 0 ? __uint_as_float(o[i]) * f0 : 0.f;
-                    if (other) v[i] += ex[(c + i) * 128 + row] * f1;
+                    if (other) v[i] += ex[(half * (D / 2) + c + i) * 128 + row] * f1;
                     v[i] *= inv;
                 }
                 if (!mine) continue;
                 if (p.part_o != nullptr) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + out_row) * D + c);
+                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + out_row) * D + half * (D / 2) + c);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 } else {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + c);
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + half * (D / 2) + c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         dst[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
