@@ -131,6 +131,18 @@ def _batch_splits(pairs: int, max_kv: int, head_dim: int, sms: int, one_wave: in
     return best
 
 
+def choose_splits(B: int, Hq: int, Hkv: int, D: int, max_kv: int, held: int, device) -> int:
+    """Splits of a decode over at most ``max_kv`` keys per sequence; the cache has room for ``held`` keys in all."""
+    splits = default_splits(B, Hkv, max_kv, device, D)
+    if B > 1:
+        # a table is often as wide as the longest sequence a server admits; lengths spread evenly over (0, n] take half of it
+        more = _batch_splits(B * Hkv, min(max_kv, max(1, 2 * held // B)), D, _sm_count(device), splits, held < B * max_kv)
+        # only where the partials meet in shared memory: the shared workspace is not for calls that did without it
+        if (Hq // Hkv) * more * (D + 2) * 4 <= 48 * 1024:
+            splits = more
+    return splits
+
+
 class _Workspace:
     """Split-merge scratch, cached per (device, stream, shape): the launches of one stream follow one another, those of two
     need not. Never given back: a captured launch keeps its addresses. (Launches captured on one stream share theirs, so
@@ -152,7 +164,7 @@ class _Workspace:
 
 def _launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, mode, splits, max_kv=None,
             ll_ptrs=None, world=1, rank=0, epoch=0, workspace=None, stream=None, push_only=False,
-            ll_ptrs_odd=None, epoch_dev=None, ll_mc=None, ll_mc_odd=None, window=0, sinks=0, priors=None):
+            ll_ptrs_odd=None, epoch_dev=None, ll_mc=None, ll_mc_odd=None):
     global launch_count
     B, Hq, D = q.shape
     blocks, page, Hkv, Dk = k_cache.shape
@@ -165,18 +177,7 @@ def _launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, mod
     if splits <= 0:
         if max_kv is None:
             max_kv = page * block_table.shape[1]
-        if window > 0:
-            max_kv = min(max_kv, window + sinks)
-        splits = default_splits(B, Hkv, max_kv, q.device, D)
-        if B > 1:
-            # a table is often as wide as the longest sequence a server admits; lengths spread evenly over (0, n] take half of it
-            held = blocks * page
-            more = _batch_splits(B * Hkv, min(max_kv, max(1, 2 * held // B)), D, _sm_count(q.device), splits, held < B * max_kv)
-            # only where the partials meet in shared memory: the shared workspace is not for calls that did without it
-            if (Hq // Hkv) * more * (D + 2) * 4 <= 48 * 1024:
-                splits = more
-    if priors is not None:
-        splits = min(splits, 256 - priors[0].shape[0])   # the merge takes 256 parts in all
+        splits = choose_splits(B, Hq, Hkv, D, max_kv, blocks * page, q.device)
     handle = stream_ptr(q.device, stream)
     partial, counters = workspace if workspace is not None else _Workspace.get(q.device, stream, handle, B, Hq, Hkv, D, splits)
     a = _lib.DecodeArgs()
@@ -193,9 +194,6 @@ def _launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, mod
     a.scale, a.soft_cap = float(scale), float(soft_cap)
     a.mode, a.dtype, a.world, a.rank, a.epoch = mode, _DTYPES[q.dtype], world, rank, epoch
     a.push_only = int(push_only)
-    a.window, a.sinks = window, sinks
-    if priors is not None:
-        a.priors, a.prior_o, a.prior_lse = priors[0].shape[0], priors[0].data_ptr(), priors[1].data_ptr()
     if ll_ptrs is not None:
         a.ll_peer = ll_ptrs
     if ll_mc is not None:

@@ -112,9 +112,9 @@ def _check(q, k_cache, v_cache, window, sinks, soft_cap, ints):
         raise ValueError("q and the caches must have a contiguous head dimension, the caches equal strides")
 
 
-def _check_out(out, q):
+def _output(out, q):
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape, dtype and device")
     return out
@@ -131,32 +131,94 @@ def _splits(ctas: int, keys: int, head_dim: int, sms: int) -> int:
     return max(1, min(sms // max(1, ctas), -(-keys // (4 * block)), 200))
 
 
-def _run(q, k_cache, v_cache, block_table, q_starts, kv_lens, out, parts, splits, row_tiles, window, sinks, scale, soft_cap, shared):
-    global launch_count
-    T, Hq, D = q.shape
+# What a call works out from its tensors' shapes, strides and types and its settings (never from their addresses or contents): checks,
+# splits, and the native arguments but for the pointers. Bounded, as a ragged batch has a new number of tokens every step.
+_PLANS: dict = {}
+
+
+def _layout(*tensors):
+    return tuple((t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors)
+
+
+def _settings(window, sinks, scale, soft_cap):
+    """The settings as plain numbers (a plan is found by their values)."""
+    return None if window is None else int(window), int(sinks), None if scale is None else float(scale), float(soft_cap)
+
+
+def _remember(key, plan):
+    if len(_PLANS) >= 4096:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
+def _attention_args(q, k_cache, block_table, batch, splits, row_tiles, window, sinks, scale, soft_cap, shared):
     a = _lib.AttentionArgs()
-    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    a.block_table, a.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
-    a.q_starts = None if q_starts is None else q_starts.data_ptr()
-    a.out = None if out is None else out.data_ptr()
-    a.part_o, a.part_lse = (None, None) if parts is None else (parts[0].data_ptr(), parts[1].data_ptr())
     a.q_token, a.q_head = q.stride(0), q.stride(1)
     a.stride_block, a.stride_token, a.stride_head = k_cache.stride(0), k_cache.stride(1), k_cache.stride(2)
-    a.tokens, a.B, a.Hq, a.Hkv, a.head_dim = T, kv_lens.shape[0], Hq, k_cache.shape[2], D
+    a.tokens, a.B, a.Hq, a.Hkv, a.head_dim = q.shape[0], batch, q.shape[1], k_cache.shape[2], q.shape[2]
     a.page_size, a.max_blocks, a.blocks = k_cache.shape[1], block_table.shape[-1], k_cache.shape[0]
     a.splits, a.row_tiles, a.window, a.sinks = splits, row_tiles, window, sinks
     a.shared, a.dtype, a.scale, a.soft_cap = int(shared), _DTYPES[q.dtype], float(scale), float(soft_cap)
-    st = global_status()
-    a.status = st.device_ptr if st is not None else None
-    a.timeout_ns = default_timeout_ns()
-    a.stream = stream_ptr(q.device)
-    _lib.check(_lib.lib().tdist_attention(C.byref(a)), "tdist_attention")
+    return a
+
+
+def _run_attention(template, q, k_cache, v_cache, table, starts, lens, out, parts, rows, status, handle):
+    """``parts``: fp32 ``[splits * rows * (D + 1)]``, the partial results and behind them their LSE; None: none needed."""
+    global launch_count
+    a = _lib.AttentionArgs.from_buffer_copy(template)
+    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    a.block_table, a.kv_lens = table.data_ptr(), lens.data_ptr()
+    if starts is not None:
+        a.q_starts = starts.data_ptr()
+    if out is not None:
+        a.out = out.data_ptr()
+    if parts is not None:
+        a.part_o = parts.data_ptr()
+        a.part_lse = a.part_o + 4 * a.splits * rows * a.head_dim
+    a.status, a.timeout_ns, a.stream = status, default_timeout_ns(), handle
+    code = _lib.lib().tdist_attention(C.byref(a))
+    if code:
+        _lib.check(code, "tdist_attention")
     launch_count += 1
+    return a
 
 
-def _parts(splits, rows, D, device):
-    """Partial results of the splits, from the allocator of the current stream."""
-    return (torch.empty((splits, rows, D), dtype=torch.float32, device=device), torch.empty((splits, rows), dtype=torch.float32, device=device))
+def _run_decode(template, q, k_cache, v_cache, table, lens, out, status, handle, priors=None):
+    """The split decode kernel over windows, or with the partial results of another kernel (its arguments)."""
+    a = _lib.DecodeArgs.from_buffer_copy(template)
+    partial, counters = FD._Workspace.get(q.device, None, handle, a.B, a.Hq, a.Hkv, a.head_dim, a.splits)
+    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    a.block_table, a.kv_lens, a.out = table.data_ptr(), lens.data_ptr(), out.data_ptr()
+    a.partial, a.counters = partial.data_ptr(), counters.data_ptr()
+    if priors is not None:
+        a.prior_o, a.prior_lse = priors.part_o, priors.part_lse
+    a.status, a.timeout_ns, a.stream = status, default_timeout_ns(), handle
+    code = _lib.lib().tdist_flash_decode(C.byref(a))
+    if code:
+        _lib.check(code, "tdist_flash_decode")
+    FD.launch_count += 1
+
+
+def _decode_args(q, k_cache, block_table, window, sinks, scale, soft_cap, kv_split, priors=0):
+    if not q.is_contiguous():
+        raise ValueError("q must be contiguous")
+    B, Hq, D = q.shape
+    blocks, page, Hkv, _ = k_cache.shape
+    a = _lib.DecodeArgs()
+    a.B, a.Hq, a.Hkv, a.head_dim, a.page_size = B, Hq, Hkv, D, page
+    a.max_blocks = block_table.shape[1]
+    most = min(page * block_table.shape[1], window + sinks)
+    a.splits = min(FD.choose_splits(B, Hq, Hkv, D, most, blocks * page, q.device) if kv_split <= 0 else kv_split, 256 - priors)
+    a.stride_block, a.stride_token, a.stride_head = k_cache.stride(0), k_cache.stride(1), k_cache.stride(2)
+    a.scale, a.soft_cap, a.dtype, a.world = float(scale), float(soft_cap), _DTYPES[q.dtype], 1
+    a.window, a.sinks, a.priors = window, sinks, priors
+    return a
+
+
+def _status_ptr():
+    st = global_status()
+    return st.device_ptr if st is not None else None
 
 
 @nvtx_range("tdist.gqa_fwd_window_decode")
@@ -164,18 +226,22 @@ def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Opt
                           soft_cap: float = 0.0, out: Optional[torch.Tensor] = None, kv_split: int = -1):
     """Decode attention of one query token per sequence over its last ``window`` keys and its first ``sinks``. Returns
     ``[B, Hq, D]`` in q's dtype; at most 16 query heads per kv head, q contiguous."""
-    B = q.shape[0]
-    _check(q, k_cache, v_cache, window, sinks, soft_cap, (("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1])
-    if q.device.type != "cuda":
-        starts = torch.arange(B + 1)
-        return ref_window_attn(q, k_cache, v_cache, starts, kv_lens, block_table, window, sinks, scale, soft_cap).to(q.dtype)
-    out = _check_out(out, q)
-    if B == 0:
-        return out
-    return FD._launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, 0, kv_split,
-                      window=min(window, NO_WINDOW) if window is not None else NO_WINDOW, sinks=sinks)
+    window, sinks, scale, soft_cap = _settings(window, sinks, scale, soft_cap)
+    key = (gqa_fwd_window_decode, _layout(q, k_cache, v_cache, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
+    args = _PLANS.get(key)
+    if args is None:
+        B = q.shape[0]
+        _check(q, k_cache, v_cache, window, sinks, soft_cap, (("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
+        factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        if q.device.type != "cuda":
+            return ref_window_attn(q, k_cache, v_cache, torch.arange(B + 1), kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
+        if B == 0:
+            return _output(out, q)
+        args = _remember(key, _decode_args(q, k_cache, block_table, min(window, NO_WINDOW) if window is not None else NO_WINDOW, sinks, factor,
+                                           soft_cap, kv_split))
+    out = _output(out, q)
+    _run_decode(args, q, k_cache, v_cache, _int32(block_table), _int32(kv_lens), out, _status_ptr(), stream_ptr(q.device))
+    return out
 
 
 @nvtx_range("tdist.gqa_fwd_window_prefill")
@@ -183,29 +249,34 @@ def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, 
                            scale=None, soft_cap: float = 0.0, out: Optional[torch.Tensor] = None, kv_split: int = -1):
     """Attention of a ragged batch of query tokens, the last ones of their sequences. Returns ``[T, Hq, D]`` in q's dtype. q may
     be a view (part of a fused projection) with strides that are multiples of 8 elements; nothing is read back to the host."""
-    B = kv_lens.shape[0]
-    _check(q, k_cache, v_cache, window, sinks, soft_cap,
-           (("kv_lens", kv_lens, (B,)), ("q_starts", q_starts, (B + 1,)), ("block_table", block_table, (B, None))))
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1])
-    if q.device.type != "cuda":
-        return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, scale, soft_cap).to(q.dtype)
-    T, Hq, D = q.shape
-    out = _check_out(out, q)
-    if T == 0 or B == 0:
-        return out
-    window = min(window, NO_WINDOW) if window is not None else NO_WINDOW
-    Hkv, page = k_cache.shape[2], k_cache.shape[1]
-    tile = 128 // (Hq // Hkv)
-    each = -(-T // B)                                   # tokens of a sequence, where all have as many
-    row_tiles = 2 if D <= 128 and each > tile else 1
-    if kv_split <= 0:
-        ctas = B * -(-each // (tile * row_tiles)) * Hkv
-        keys = min(block_table.shape[1] * page, window + sinks + tile * row_tiles)
-        kv_split = _splits(ctas, keys, D, FD._sm_count(q.device))
-    parts = _parts(kv_split, T * Hq, D, q.device) if kv_split > 1 else None
-    _run(q, k_cache, v_cache, _int32(block_table), _int32(q_starts), _int32(kv_lens), out, parts, kv_split, row_tiles, window, sinks, scale,
-         soft_cap, False)
+    window, sinks, scale, soft_cap = _settings(window, sinks, scale, soft_cap)
+    key = (gqa_fwd_window_prefill, _layout(q, k_cache, v_cache, q_starts, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
+    args = _PLANS.get(key)
+    if args is None:
+        B = kv_lens.shape[0]
+        _check(q, k_cache, v_cache, window, sinks, soft_cap,
+               (("kv_lens", kv_lens, (B,)), ("q_starts", q_starts, (B + 1,)), ("block_table", block_table, (B, None))))
+        factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        if q.device.type != "cuda":
+            return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
+        T, Hq, D = q.shape
+        if T == 0 or B == 0:
+            return _output(out, q)
+        most = min(window, NO_WINDOW) if window is not None else NO_WINDOW
+        tile = 128 // (Hq // k_cache.shape[2])
+        each = -(-T // B)                                   # tokens of a sequence, where all have as many
+        row_tiles = 2 if D <= 128 and each > tile else 1
+        splits = kv_split
+        if splits <= 0:
+            ctas = B * -(-each // (tile * row_tiles)) * k_cache.shape[2]
+            keys = min(block_table.shape[1] * k_cache.shape[1], most + sinks + tile * row_tiles)
+            splits = _splits(ctas, keys, D, FD._sm_count(q.device))
+        args = _remember(key, _attention_args(q, k_cache, block_table, B, splits, row_tiles, most, sinks, factor, soft_cap, False))
+    out = _output(out, q)
+    rows = args.tokens * args.Hq
+    parts = torch.empty(args.splits * rows * (args.head_dim + 1), dtype=torch.float32, device=q.device) if args.splits > 1 else None
+    _run_attention(args, q, k_cache, v_cache, _int32(block_table), _int32(q_starts), _int32(kv_lens), out, parts, rows, _status_ptr(),
+                   stream_ptr(q.device))
     return out
 
 
@@ -216,28 +287,36 @@ def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, 
     the pages ``prefix_table`` (``prefix_len`` keys; an integer tensor of one element on the device, or a number), the own keys in those of
     ``block_table`` (``kv_lens`` keys, which may be zero). Returns ``[B, Hq, D]`` in q's dtype; at most 16 query heads per kv head,
     q contiguous. ``kv_split``: parts of the prefix."""
-    B = q.shape[0]
     if not isinstance(prefix_len, torch.Tensor):
         prefix_len = torch.full((1,), int(prefix_len), dtype=torch.int32, device=q.device)
-    _check(q, k_cache, v_cache, None, 0, soft_cap,
-           (("prefix_len", prefix_len, (1,)), ("prefix_table", prefix_table, (None,)), ("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1])
-    if q.device.type != "cuda":
-        return ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, scale, soft_cap).to(q.dtype)
-    _, Hq, D = q.shape
-    if not q.is_contiguous():
-        raise ValueError("q must be contiguous")
-    out = _check_out(out, q)
-    if B == 0:
-        return out
-    if prefix_table.shape[0] == 0:
-        return FD._launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, 0, -1, window=NO_WINDOW)
-    Hkv, page = k_cache.shape[2], k_cache.shape[1]
-    tile = 128 // (Hq // Hkv)
-    row_tiles = 2 if D <= 128 and B > tile else 1
-    if kv_split <= 0:
-        kv_split = _splits(-(-B // (tile * row_tiles)) * Hkv, prefix_table.shape[0] * page, D, FD._sm_count(q.device))
-    parts = _parts(kv_split, B * Hq, D, q.device)
-    _run(q, k_cache, v_cache, _int32(prefix_table), None, _int32(prefix_len), None, parts, kv_split, row_tiles, NO_WINDOW, 0, scale, soft_cap, True)
-    return FD._launch(q, k_cache, v_cache, kv_lens, block_table, scale, soft_cap, out, 0, -1, window=NO_WINDOW, priors=parts)
+    _, _, scale, soft_cap = _settings(None, 0, scale, soft_cap)
+    key = (gqa_fwd_shared_prefix_decode, _layout(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table), scale, soft_cap, kv_split)
+    plan = _PLANS.get(key)
+    if plan is None:
+        B = q.shape[0]
+        _check(q, k_cache, v_cache, None, 0, soft_cap,
+               (("prefix_len", prefix_len, (1,)), ("prefix_table", prefix_table, (None,)), ("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
+        factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        if q.device.type != "cuda":
+            return ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, factor, soft_cap).to(q.dtype)
+        _, Hq, D = q.shape
+        if B == 0:
+            return _output(out, q)
+        first, splits = None, 0
+        if prefix_table.shape[0] > 0:
+            tile = 128 // (Hq // k_cache.shape[2])
+            row_tiles = 2 if D <= 128 and B > tile else 1
+            splits = kv_split
+            if splits <= 0:
+                splits = _splits(-(-B // (tile * row_tiles)) * k_cache.shape[2], prefix_table.shape[0] * k_cache.shape[1], D, FD._sm_count(q.device))
+            first = _attention_args(q, k_cache, prefix_table, 1, splits, row_tiles, NO_WINDOW, 0, factor, soft_cap, True)
+        plan = _remember(key, (first, _decode_args(q, k_cache, block_table, NO_WINDOW, 0, factor, soft_cap, -1, splits)))
+    first, second = plan
+    out = _output(out, q)
+    status, handle, priors = _status_ptr(), stream_ptr(q.device), None
+    if first is not None:
+        rows = first.tokens * first.Hq
+        parts = torch.empty(first.splits * rows * (first.head_dim + 1), dtype=torch.float32, device=q.device)
+        priors = _run_attention(first, q, k_cache, v_cache, _int32(prefix_table), None, _int32(prefix_len), None, parts, rows, status, handle)
+    _run_decode(second, q, k_cache, v_cache, _int32(block_table), _int32(kv_lens), out, status, handle, priors)
+    return out
