@@ -66,6 +66,27 @@ def ref_sample_tokens(logits, u, temperature: Setting = 1.0, top_k: Setting = 0,
                          torch.where(none, float("-inf"), top * inv + norm).view(B))
 
 
+_CHECKED: set = set()
+
+
+def _check(logits, u, settings):
+    if logits.dim() != 2 or u.shape != logits.shape[:1]:
+        raise ValueError("logits must be [B, V] and u [B]")
+    if logits.shape[1] < 1:
+        raise ValueError("sampling needs at least one logit per row")
+    if u.dtype != torch.float32 or logits.dtype not in _DTYPES:
+        raise TypeError("u must be fp32, logits bf16, fp16 or fp32")
+    if u.device != logits.device:
+        raise ValueError("u must be on the logits' device")
+    for name, v in zip(("temperature", "top_k", "top_p", "min_p"), settings):
+        if isinstance(v, torch.Tensor):
+            if v.shape != logits.shape[:1] or v.device != logits.device:
+                raise ValueError(f"{name} must be a number or a tensor [B] on the logits' device")
+            dtypes = (torch.int32, torch.int64) if name == "top_k" else (torch.float32,)
+            if v.dtype not in dtypes:
+                raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}")
+
+
 @nvtx_range("tdist.sample_tokens")
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0, top_p: Setting = 1.0,
                   min_p: Setting = 0.0) -> SampledTokens:
@@ -73,52 +94,55 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     all rows or a tensor ``[B]`` (fp32; ``top_k`` int32 or int64). Off: ``top_k <= 0``, ``top_p >= 1``, ``min_p <= 0``; ``temperature <= 0``
     takes the largest logit, the lowest index of equal ones. Logits of -inf or NaN are never drawn."""
     global launch_count
-    if logits.dim() != 2 or u.shape != logits.shape[:1]:
-        raise ValueError("logits must be [B, V] and u [B]")
-    B, V = logits.shape
-    if V < 1:
-        raise ValueError("sampling needs at least one logit per row")
-    if u.dtype != torch.float32 or logits.dtype not in _DTYPES:
-        raise TypeError("u must be fp32, logits bf16, fp16 or fp32")
-    for name, v, dtypes in (("temperature", temperature, (torch.float32,)), ("top_k", top_k, (torch.int32, torch.int64)),
-                            ("top_p", top_p, (torch.float32,)), ("min_p", min_p, (torch.float32,))):
-        if isinstance(v, torch.Tensor):
-            if v.shape != (B,) or v.device != logits.device:
-                raise ValueError(f"{name} must be a number or a tensor [B] on the logits' device")
-            if v.dtype not in dtypes:
-                raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}")
-    if u.device != logits.device:
-        raise ValueError("u must be on the logits' device")
+    given = (temperature, top_k, top_p, min_p)
+    # the checks' outcome depends on shapes, types and devices only, and is kept by them
+    key = (logits.shape, logits.dtype, logits.get_device(), u.shape, u.dtype, u.get_device(),
+           tuple([(v.shape, v.dtype, v.get_device()) if isinstance(v, torch.Tensor) else None for v in given]))
+    if key not in _CHECKED:
+        _check(logits, u, given)
+        if len(_CHECKED) >= 1024:
+            _CHECKED.clear()
+        _CHECKED.add(key)
     if logits.device.type != "cuda":
         return ref_sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    B, V = logits.shape
     if logits.stride(1) != 1:
         logits = logits.contiguous()
-    out = SampledTokens(torch.empty(B, dtype=torch.int32, device=logits.device), torch.empty(B, dtype=torch.float32, device=logits.device),
-                        torch.empty(B, dtype=torch.float32, device=logits.device))
+    # one allocation, the tokens' bits among the floats
+    tokens, logprobs, log_norm = torch.empty((3, B), dtype=torch.float32, device=logits.device).unbind()
+    out = SampledTokens(tokens.view(torch.int32), logprobs, log_norm)
     if B == 0:
         return out
     a = _lib.SampleArgs()
-    held = []   # copies that have to outlive the launch call
-
-    def per_row(v, dtype):
-        if not isinstance(v, torch.Tensor):
-            return None
-        if dtype == torch.int32 and v.dtype == torch.int64:
-            v = v.clamp(0, V)
-        v = v.to(dtype).contiguous()
-        held.append(v)
-        return v.data_ptr()
-
-    a.logits, a.u = logits.data_ptr(), per_row(u, torch.float32)
-    a.temperature, a.top_k = per_row(temperature, torch.float32), per_row(top_k, torch.int32)
-    a.top_p, a.min_p = per_row(top_p, torch.float32), per_row(min_p, torch.float32)
-    a.one_temperature = 0.0 if a.temperature is not None else float(temperature)
-    a.one_top_k = 0 if a.top_k is not None else max(0, min(int(top_k), V))
-    a.one_top_p = 0.0 if a.top_p is not None else float(top_p)
-    a.one_min_p = 0.0 if a.min_p is not None else float(min_p)
-    a.tokens, a.logprobs, a.log_norm = out.tokens.data_ptr(), out.logprobs.data_ptr(), out.log_norm.data_ptr()
-    a.stride, a.B, a.V, a.dtype = logits.stride(0), B, V, _DTYPES[logits.dtype]
+    a.logits, a.stride, a.B, a.V, a.dtype = logits.data_ptr(), logits.stride(0), B, V, _DTYPES[logits.dtype]
+    if not u.is_contiguous():
+        u = u.contiguous()
+    a.u = u.data_ptr()
+    # tensors are read by the row, numbers serve all rows; copies outlive the launch call in these names
+    if isinstance(temperature, torch.Tensor):
+        temperature = temperature.contiguous()
+        a.temperature = temperature.data_ptr()
+    else:
+        a.one_temperature = temperature
+    if isinstance(top_k, torch.Tensor):
+        top_k = (top_k if top_k.dtype == torch.int32 else top_k.clamp(0, V).to(torch.int32)).contiguous()
+        a.top_k = top_k.data_ptr()
+    else:
+        a.one_top_k = max(0, min(int(top_k), V))
+    if isinstance(top_p, torch.Tensor):
+        top_p = top_p.contiguous()
+        a.top_p = top_p.data_ptr()
+    else:
+        a.one_top_p = top_p
+    if isinstance(min_p, torch.Tensor):
+        min_p = min_p.contiguous()
+        a.min_p = min_p.data_ptr()
+    else:
+        a.one_min_p = min_p
+    a.tokens, a.logprobs, a.log_norm = out.tokens.data_ptr(), logprobs.data_ptr(), log_norm.data_ptr()
     a.stream = stream_ptr(logits.device)
-    _lib.check(_lib.lib().tdist_sample(C.byref(a)), "tdist_sample")
+    code = _lib.lib().tdist_sample(C.byref(a))
+    if code:
+        _lib.check(code, "tdist_sample")
     launch_count += 1
     return out
