@@ -5,13 +5,14 @@
 //   over the keys j that row r sees: j <= pos(r) and (j > pos(r) - window or j < sinks)
 //
 // A tile is 128 rows of one kv head: the G query heads that share it for 128 / G tokens, so that a key is read once for all of
-// them. A CTA goes over its keys 128 at a time (64 with head_dim 256) with the running maximum and sum of a softmax:
-//   S = Q K^T in TMEM (128 x 128 fp32), two threads per row turn it into P = exp2(S - m) in 16 bits, in place of S in TMEM, and
+// them. A CTA goes over its keys 64 at a time with the running maximum and sum of a softmax:
+//   S = Q K^T in TMEM (128 x 64 fp32), a thread per row turns it into P = exp2(S - m) in 16 bits, in place of S in TMEM, and
 //   O += P V takes P from TMEM and V as it lies in the cache (its N dimension contiguous).
-// Two such chains ("streams") run in one CTA, so that the tensor cores work on one while the other is in its softmax: two row tiles
-// over the same keys where there are enough rows, else one row tile over every other block of keys, joined at the end.
-// Warps: 8 per stream for the softmax (two threads per row), one that issues MMAs, kLoaders that copy K and V into a ring of tiles in the 128-byte-swizzled
-// layout the MMAs read: by TMA, a box per page (or 128 rows of it) and 64 head dimensions, where the page is a multiple of 8 rows and the
+// Two such chains ("streams") run in one CTA: two row tiles over the same keys where there are enough rows, else one row tile over every
+// other block of keys, joined at the end (one stream with head_dim 256, whose O fills TMEM). Each stream has two S, so that the
+// tensor cores work on the next block's S and the last one's O while its threads are in a softmax.
+// Warps: 4 per stream for the softmax, one per stream that issues MMAs, kLoaders that copy K and V into a ring of tiles in the 128-byte-swizzled
+// layout the MMAs read: by TMA, a box per page (or 64 rows of it) and 64 head dimensions, where the page is a multiple of 8 rows and the
 // whole block is seen; by 16-byte cp.async else (pages of any size; rows that nobody sees are not read and become zeros).
 // Few rows over many keys are split along the keys; the partial results meet in attention_merge_kernel, or in the decode kernel.
 //
@@ -37,8 +38,8 @@ namespace attention {
 
 constexpr int kKernelAttention = 9;
 constexpr int kRows = 128;      // rows of a tile: the MMA's M
+constexpr int kKeys = 64;       // keys of a block
 constexpr int kLoaders = 2;     // warps that copy K and V
-constexpr int kPolyEvery = 4;  // every how manieth pair of exponentials is a polynomial
 constexpr float kRaise = 8.f;   // log2 of how far scores may exceed the maximum that is subtracted
 
 struct alignas(64) Params {
@@ -66,22 +67,20 @@ struct alignas(64) Params {
 
 template <int D>
 struct Shape {
-    static constexpr int KT = D <= 128 ? 128 : 64;        // keys of a block
-    static constexpr int STREAMS = D <= 128 ? 2 : 1;      // TMEM holds O of one stream only with head_dim 256
-    static constexpr int TILE = KT * D * 2;               // bytes of a K or V block
+    static constexpr int STREAMS = D <= 128 ? 2 : 1;
+    static constexpr int TILE = kKeys * D * 2;            // bytes of a K or V block
     static constexpr int QTILE = kRows * D * 2;
     static constexpr int CHUNKS = D / 64;                 // 128-byte columns of a tile
     static constexpr int AREA = D == 64 ? 160 * 1024 : 224 * 1024;
-    static constexpr int HALF = KT / 2;                   // keys of a softmax thread
-    static constexpr int SOFT = 256 * STREAMS;            // softmax threads: two per row
-    static constexpr int THREADS = SOFT + 32 + 32 * kLoaders;
-    static constexpr uint32_t O_COL = 256;                // TMEM columns: S / P of stream s at s * 128, O at O_COL + s * D
+    static constexpr int SOFT = 128 * STREAMS;            // softmax threads
+    static constexpr int THREADS = SOFT + 32 * STREAMS + 32 * kLoaders;
+    static constexpr uint32_t O_COL = 256;                // TMEM columns: S / P of stream s at s * 128 (+ 64), O at O_COL + s * D
 };
 template <int D, int QT>
 constexpr int stages() {
     return (Shape<D>::AREA - QT * Shape<D>::QTILE) / Shape<D>::TILE;
 }
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 18;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
@@ -97,24 +96,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
         "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
-}
-// one column
-__device__ __forceinline__ void tmem_st_32x1(uint32_t taddr, float v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%1], {%0};" ::"f"(v), "r"(taddr) : "memory");
-}
-__device__ __forceinline__ float tmem_ld_32x1(uint32_t taddr) {
-    float v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(v) : "r"(taddr) : "memory");
-    return v;
-}
-// Barrier of `n` threads that tells all whether one of them had `v`.
-__device__ __forceinline__ bool barrier_or(uint32_t id, uint32_t n, bool v) {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\tbar.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(r)
-                 : "r"(id), "r"(n), "r"(static_cast<uint32_t>(v))
-                 : "memory");
-    return r != 0;
 }
 // 32 lanes x 16 columns: thread t of the warp writes columns [col, col + 16) of TMEM lane (lane_base + t)
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
@@ -151,34 +132,25 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^y without the special-function unit: y = n + f, |f| <= 1/2, by adding and taking away 1.5 x 2^23 (+ 127, so that the sum's low
-// bits are the exponent of 2^n); 2^f as a polynomial, p(0) = 1, fitted to the least largest relative error, 2.9e-6. Below -127 it
-// is 0, NaN stays NaN; y < 128.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t y) {
-    float lo, hi;
-    unpair(y, lo, hi);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
-    y = pair(lo, hi);
-    const float magic = 12582912.f + 127.f;
-    const uint64_t t = add2(y, pair(magic, magic));
-    const uint64_t f = fma2(add2(t, pair(-magic, -magic)), pair(-1.f, -1.f), y);
-    uint64_t p = fma2(f, pair(0.009582852944731712f, 0.009582852944731712f), pair(0.055906426161527634f, 0.055906426161527634f));
-    p = fma2(p, f, pair(0.24024099111557007f, 0.24024099111557007f));
-    p = fma2(p, f, pair(0.6931241750717163f, 0.6931241750717163f));
-    p = fma2(p, f, pair(1.f, 1.f));
-    unpair(t, lo, hi);
-    return mul2(p, pair(__uint_as_float(__float_as_uint(lo) << 23), __uint_as_float(__float_as_uint(hi) << 23)));
+// P = 2^(s scale - m) for 32 scores, packed, and their sum. (Some of the exponentials as a polynomial on the FMA pipe, to relieve the
+// special-function unit with its 8 clocks per warp: of 16 pairs 2 to 6, in stages between the others or not: no faster, 16384 tokens 1864 us
+// without, 1897 to 1974 with them.)
+template <typename T>
+__device__ __forceinline__ void exponentials(const uint32_t (&s)[32], uint64_t scale2, uint64_t minus2, uint32_t (&pk)[16], uint64_t (&sum2)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float a, b;
+        unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, minus2), a, b);
+        a = exp2f(a);
+        b = exp2f(b);
+        sum2[i & 1] = add2(sum2[i & 1], pair(a, b));
+        pk[i] = pack2<T>(a, b);
+    }
 }
 
 // What a CTA works on: sequence b, its query tokens [i0, i0 + QT * tile_tokens) of n, the split and the blocks of keys.
@@ -193,7 +165,7 @@ struct Work {
 
 template <int D, int QT>
 __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
-    constexpr int KT = Shape<D>::KT;
+    constexpr int KT = kKeys;
     const int lane = static_cast<int>(threadIdx.x) & 31;
     w.split = static_cast<int>(blockIdx.x) % p.splits;
     w.kvh = static_cast<int>(blockIdx.x) / p.splits % p.Hkv;
@@ -264,33 +236,34 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
 template <typename T, int D, int QT>
 __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const __grid_constant__ Params p) {
     using S = Shape<D>;
-    constexpr int KT = S::KT, NSTR = S::STREAMS, NST = stages<D, QT>(), CH = D / 8;
+    constexpr int KT = kKeys, NSTR = S::STREAMS, NST = stages<D, QT>(), CH = D / 8;
     static_assert(NST >= 2 && NST <= kMaxStages, "a tile is released only once the one after it has arrived");
     static_assert(QT == 1 || NSTR == 2, "two row tiles need two streams");
-    constexpr int LOOK = QT == 2 ? 1 : NSTR;   // K blocks loaded ahead of the first V block
+    constexpr int LOOK = QT == 2 ? 2 : 2 * NSTR;   // K blocks ahead of the first V block: two S per stream
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::AREA);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 10);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 12);
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + QT * S::QTILE;
     const uint32_t bars_u32 = smem_u32(bars);
     auto bar_full = [&](int s) { return bars_u32 + 8u * s; };
     auto bar_empty = [&](int s) { return bars_u32 + 8u * (kMaxStages + s); };
-    auto bar_s = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + s); };        // S is complete
-    auto bar_p = [&](int s, int h) { return bars_u32 + 8u * (2 * kMaxStages + 2 + 2 * s + h); };    // a half of P is in its place
-    auto bar_o = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 6 + s); };    // O has taken it in
-    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 8);
+    auto bar_s = [&](int s, int b) { return bars_u32 + 8u * (2 * kMaxStages + 2 * s + b); };        // S is complete
+    auto bar_p = [&](int s, int b) { return bars_u32 + 8u * (2 * kMaxStages + 4 + 2 * s + b); };    // P is in its place
+    auto bar_o = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 8 + s); };                   // O has taken it in
+    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 10);
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         for (int s = 0; s < NST; ++s) {
             mbar_init(bar_full(s), 32 * kLoaders);
-            mbar_init(bar_empty(s), 1);
+            mbar_init(bar_empty(s), QT);   // streams that take it in
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(bar_s(s), 1);
-            mbar_init(bar_p(s, 0), 128);
-            mbar_init(bar_p(s, 1), 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(bar_s(s, b), 1);
+                mbar_init(bar_p(s, b), 128);
+            }
             mbar_init(bar_o(s), 1);
         }
         mbar_init(bar_q, S::SOFT);
@@ -313,15 +286,22 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int i = w.c0 + j;
         return (i < w.n_sink ? i : w.m0 + i - w.n_sink) * KT;
     };
-    // every key of the block from t0 on is seen by some row: by TMA
-    auto whole_block = [&](int t0) { return p.box_rows > 0 && ((t0 >= w.lo && t0 + KT <= w.hi) || t0 + KT <= w.s_end); };
-    // The ring's items in the order in which the MMAs take them: LOOK blocks of K, then V and K in turn, the last V.
+    // Blocks of which every key is seen by some row come by TMA: the split's [tma0, tma1)
+    int tma0 = 0, tma1 = 0;
+    if (p.box_rows > 0 && nt > 0) {
+        tma0 = max(0, w.n_sink + max(w.m0, (w.lo + KT - 1) / KT) - w.m0 - w.c0);
+        tma1 = min(nt, w.n_sink + w.hi / KT - w.m0 - w.c0);
+    }
+    auto by_tma = [&](int j) { return j >= tma0 && j < tma1; };
+    // The ring's items in the order in which the loaders bring them: LOOK blocks of K, then V and K in turn, the last of V.
     const int look = min(LOOK, nt);
+    auto item_v = [&](int j) { return j < nt - look ? look + 2 * j : nt + j; };
+    auto item_k = [&](int j) { return j < look ? j : look + 2 * (j - look) + 1; };
 
-    if (warp > S::SOFT / 32) {
+    if (warp >= S::SOFT / 32 + NSTR) {
         // ---------------------------------------------------------------- loaders
         constexpr int RW = KT / kLoaders, RL = RW / 32, RPI = 32 / CH;   // cp.async: rows of a warp, of a lane's lookups, of an instruction
-        const int loader = warp - S::SOFT / 32 - 1, r0 = loader * RW;
+        const int loader = warp - S::SOFT / 32 - NSTR, r0 = loader * RW;
         const int* table = p.block_table + static_cast<size_t>(live ? w.b : 0) * p.max_blocks;
         const int lrow = lane / CH, lch = lane % CH;
         const T* kl = static_cast<const T*>(p.k_cache) + static_cast<size_t>(w.kvh) * p.stride_head + lch * 8;
@@ -348,8 +328,9 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         };
         auto lookup = [&](int n, Item& x) {
             if (n >= items) return;
-            x.t0 = block_start(block_of(n, x.is_k));
-            x.whole = whole_block(x.t0);
+            const int j = block_of(n, x.is_k);
+            x.t0 = block_start(j);
+            x.whole = by_tma(j);
             if (x.whole) {
                 if (lane * box_rows < KT) x.page = page_of(x.t0 + lane * box_rows, x.in_page);
             } else {
@@ -399,117 +380,66 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                 cp_async_arrive(bar_full(slot));
             }
         }
-    } else if (warp == S::SOFT / 32) {
-        // ---------------------------------------------------------------- MMA issue
-        if (nt > 0) {
-            const bool leader = elect_one();   // the whole warp goes along, so that descriptors stay in uniform registers
-            const uint32_t fmt = sizeof(T) == 2 && __is_same(T, __half) ? 0u : 1u;
-            const uint32_t idesc_s = umma_idesc(fmt, fmt, kRows, KT);
-            const uint32_t idesc_o = umma_idesc(fmt, fmt, kRows, D) | kIdescBNMajor;
-            auto qk = [&](int tile, int stream, int slot) {
-                const uint32_t kb = ring + static_cast<uint32_t>(slot) * S::TILE, qb = q_smem + tile * S::QTILE;
+    } else if (warp >= S::SOFT / 32) {
+        // ---------------------------------------------------------------- MMA issue, a warp per stream: one's waits under the other's products
+        const int stream = warp - S::SOFT / 32;
+        const bool leader = elect_one();   // the whole warp goes along, so that descriptors stay in uniform registers
+        const uint32_t fmt = sizeof(T) == 2 && __is_same(T, __half) ? 0u : 1u;
+        const uint32_t idesc_s = umma_idesc(fmt, fmt, kRows, KT);
+        const uint32_t idesc_o = umma_idesc(fmt, fmt, kRows, D) | kIdescBNMajor;
+        const uint32_t qb = q_smem + (QT == 2 ? stream : 0) * S::QTILE, s_col = tmem + stream * 128, o_col = tmem + S::O_COL + stream * D;
+        const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
+        auto block = [&](int it) { return QT == 2 ? it : it * NSTR + stream; };   // number of the stream's `it`-th block
+        auto arrived = [&](int item, int j) {
+            mbar_wait(bar_full(item % NST), (item / NST) & 1u, p.wctx, 2);
+            if (!by_tma(j)) fence_proxy_async_smem();   // what cp.async wrote, to the MMAs' proxy
+            tc_fence_after();
+        };
+        auto qk = [&](int it) {
+            const int j = block(it), item = item_k(j), slot = item % NST, buf = it & 1;
+            arrived(item, j);
+            const uint32_t kb = ring + static_cast<uint32_t>(slot) * S::TILE;
+            if (leader) {
+#pragma unroll
+                for (int c = 0; c < S::CHUNKS; ++c) {
+                    const uint64_t a = umma_desc_k_sw128(qb + c * (kRows * 128)), b = umma_desc_k_sw128(kb + c * (KT * 128));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_bf16<1>(s_col + buf * 64, a + 2 * k, b + 2 * k, idesc_s, (c | k) != 0 ? 1u : 0u);
+                }
+                umma_commit(bar_s(stream, buf));
+                umma_commit(bar_empty(slot));
+            }
+            __syncwarp();
+        };
+        if (my_blocks > 0) {
+            mbar_wait(bar_q, 0, p.wctx, 3);
+            // half a block behind the other stream, so that one's exponentials run beside the other's loads and maxima
+            if (stream == 1) mbar_wait(bar_p(0, 0), 0, p.wctx, 9);
+            for (int it = 0; it < min(2, my_blocks); ++it) qk(it);
+            for (int it = 0; it < my_blocks; ++it) {
+                const int j = block(it), item = item_v(j), slot = item % NST, buf = it & 1;
+                arrived(item, j);
+                const uint64_t b = umma_desc_mn_sw128(ring + static_cast<uint32_t>(slot) * S::TILE, KT * 128);
+                mbar_wait(bar_p(stream, buf), (it >> 1) & 1u, p.wctx, 4);
+                tc_fence_after();
                 if (leader) {
 #pragma unroll
-                    for (int c = 0; c < S::CHUNKS; ++c) {
-                        const uint64_t a = umma_desc_k_sw128(qb + c * (kRows * 128)), b = umma_desc_k_sw128(kb + c * (KT * 128));
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) umma_bf16<1>(tmem + stream * 128, a + 2 * k, b + 2 * k, idesc_s, (c | k) != 0 ? 1u : 0u);
-                    }
-                    umma_commit(bar_s(stream));
+                    for (int k = 0; k < KT / 16; ++k) umma_ts(o_col, s_col + buf * 64 + 8 * k, b + 128 * k, idesc_o, it > 0 || k != 0 ? 1u : 0u);
+                    umma_commit(bar_o(stream));
+                    umma_commit(bar_empty(slot));
                 }
                 __syncwarp();
-            };
-            auto pv = [&](int stream, int slot, uint32_t parity, bool first) {
-                const uint64_t b = umma_desc_mn_sw128(ring + static_cast<uint32_t>(slot) * S::TILE, KT * 128);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    mbar_wait(bar_p(stream, h), parity, p.wctx, 4);
+                if (it + 2 < my_blocks) {
+                    // this P has been taken in: the next S but one takes its columns
+                    mbar_wait(bar_o(stream), it & 1u, p.wctx, 5);
                     tc_fence_after();
-                    if (leader) {
-#pragma unroll
-                        for (int k = h * (KT / 32); k < (h + 1) * (KT / 32); ++k)
-                            umma_ts(tmem + S::O_COL + stream * D, tmem + stream * 128 + h * S::HALF + 8 * (k - h * (KT / 32)), b + 128 * k, idesc_o, !first || k != 0 ? 1u : 0u);
-                        if (h == 1) umma_commit(bar_o(stream));
-                    }
-                    __syncwarp();
-                }
-            };
-            auto release = [&](int slot) {
-                if (leader) umma_commit(bar_empty(slot));
-                __syncwarp();
-            };
-            // the ring's next item: its slot, and the parity of its arrival
-            int slot = 0;
-            uint32_t phase = 0;
-            auto next_slot = [&]() {
-                const int at = slot;
-                if (++slot == NST) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-                return at;
-            };
-            auto full = [&](int at, uint32_t parity, int block) {
-                mbar_wait(bar_full(at), parity, p.wctx, 2);
-                if (!whole_block(block_start(block))) fence_proxy_async_smem();   // what cp.async wrote, to the MMAs' proxy
-                tc_fence_after();
-            };
-            mbar_wait(bar_q, 0, p.wctx, 3);
-            if constexpr (QT == 2) {
-                full(0, 0, 0);
-                next_slot();
-                qk(0, 0, 0);
-                qk(1, 1, 0);
-                release(0);
-                for (int j = 0; j < nt; ++j) {
-                    const uint32_t parity = j & 1u, v_phase = phase;
-                    const int v = next_slot();
-                    const uint32_t k_phase = phase;
-                    const int k = next_slot();
-                    full(v, v_phase, j);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        pv(s, v, parity, j == 0);
-                        if (s == 1) release(v);
-                        if (j + 1 < nt) {
-                            if (s == 0) full(k, k_phase, j + 1);
-                            // S takes the columns of the P that this product reads
-                            mbar_wait(bar_o(s), parity, p.wctx, 5);
-                            tc_fence_after();
-                            qk(s, s, k);
-                            if (s == 1) release(k);
-                        }
-                    }
-                }
-            } else {
-                for (int j = 0; j < look; ++j) {
-                    full(j, 0, j);
-                    qk(0, j, j);
-                    release(next_slot());
-                }
-                for (int j = 0; j < nt; ++j) {
-                    const int s = j % NSTR;
-                    const uint32_t parity = (j / NSTR) & 1u, v_phase = phase;
-                    const int v = next_slot();
-                    full(v, v_phase, j);
-                    pv(s, v, parity, j < NSTR);
-                    release(v);
-                    if (j + LOOK < nt) {
-                        const uint32_t k_phase = phase;
-                        const int k = next_slot();
-                        full(k, k_phase, j + LOOK);
-                        mbar_wait(bar_o(s), parity, p.wctx, 5);
-                        tc_fence_after();
-                        qk(0, s, k);
-                        release(k);
-                    }
+                    qk(it + 2);
                 }
             }
         }
-        __syncwarp();
     } else {
-        // ---------------------------------------------------------------- softmax: two threads per row, half of the block's keys each
-        const int stream = warp >> 3, half = (warp >> 2) & 1, row = tid & 127;
+        // ---------------------------------------------------------------- softmax: a thread per row
+        const int stream = warp >> 2, row = tid & 127;
         const int q_tile = QT == 2 ? stream : 0;
         if (live) {
             // Q into shared memory, zeros for rows without a token
@@ -538,45 +468,35 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int tile_first = p.shared ? w.first : w.first + q_tile * p.tile_tokens;
         const int tile_last = p.shared ? w.first : min(tile_first + p.tile_tokens - 1, w.first - w.i0 + w.n - 1);
         const int pos = p.shared ? w.first : tile_first + t_in;
-        const float sl2 = p.soft_cap > 0.f ? 1.f : p.scale_log2;
+        const bool capped = p.soft_cap > 0.f;
+        const float sl2 = capped ? 1.f : p.scale_log2;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        // this half's columns of S, which begin with those of its P, and of O
-        const uint32_t s_at = tmem + lanes + stream * 128 + half * S::HALF, o_at = tmem + lanes + S::O_COL + stream * D + half * (D / 2);
+        const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + S::O_COL + stream * D;
         const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
         float m_ref = -CUDART_INF_F, l_run = 0.f;
-        // The other half's value, through a column of S that both have read and that P leaves alone.
-        auto exchange = [&](float v) {
-            tmem_st_32x1(s_at + S::HALF - 1, v);
-            tmem_st_wait();
-            tc_fence_before();
-            named_barrier(1 + stream, 256);
-            tc_fence_after();
-            const float got = tmem_ld_32x1(half == 0 ? s_at + 2 * S::HALF - 1 : s_at - 1);
-            tmem_ld_wait();
-            return got;
-        };
-
         for (int it = 0; it < my_blocks; ++it) {
             const int t0 = block_start(QT == 2 ? it : it * NSTR + stream);
-            mbar_wait(bar_s(stream), it & 1u, p.wctx, 6);
+            const int buf = it & 1;
+            const uint32_t at = s_at + buf * 64;
+            const bool edge = !(t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks));   // some row does not see all
+            mbar_wait(bar_s(stream, buf), (it >> 1) & 1u, p.wctx, 6);
             tc_fence_after();
-            constexpr int NC = S::HALF / 32;
-            uint32_t s[NC][32];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
+            uint32_t s[2][32];
+            tmem_ld_32x32(at, s[0]);
+            tmem_ld_32x32(at + 32, s[1]);
             tmem_ld_wait();
-            if (p.soft_cap > 0.f) {
+            if (capped) {
                 // cap tanh(x / cap), in the exponent's domain: 1 - 2 / (1 + exp(2 x / cap))
                 const float cap = p.soft_cap * 1.4426950408889634f, in = 2.f * p.scale_log2 / p.soft_cap;
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[c][i]) * in)));
             }
-            if (!(t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks))) {
-                const int k0 = t0 + half * S::HALF, hi = pos - k0, lo = pos - p.window - k0, sink = p.sinks - k0;
+            if (edge) {
+                const int hi = pos - t0, lo = pos - p.window - t0, sink = p.sinks - t0;
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int j = 32 * c + i;
@@ -585,14 +505,13 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             }
             float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-            float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
+            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
             if (it == 0) {
-                m_ref = fmaxf(top, exchange(top));
-            } else if (barrier_or(1 + stream, 256, top > m_ref + kRaise)) {
-                top = fmaxf(top, exchange(top));
+                m_ref = top;
+            } else if (__any_sync(0xffffffffu, top > m_ref + kRaise)) {
                 const float m_new = fmaxf(m_ref, top);
                 const float alpha = m_new == m_ref ? 1.f : exp2f(m_ref - m_new);
                 m_ref = m_new;
@@ -600,7 +519,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                 mbar_wait(bar_o(stream), (it - 1) & 1u, p.wctx, 7);
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D / 2; c += 16) {
+                for (int c = 0; c < D; c += 16) {
                     uint32_t o[16];
                     tmem_ld_32x16(o_at + c, o);
                     tmem_ld_wait();
@@ -608,68 +527,48 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                     tmem_st_32x16(o_at + c, o);
                 }
-                // O is whole before either half lets the next product begin
-                tmem_st_wait();
-                tc_fence_before();
-                named_barrier(1 + stream, 256);
             }
             const float m_use = m_ref == -CUDART_INF_F ? 0.f : m_ref;
             const uint64_t scale2 = pair(sl2, sl2), minus2 = pair(-m_use, -m_use);
             uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    uint64_t y = fma2(pair(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, minus2);
-                    float a, b;
-                    if (i % kPolyEvery == kPolyEvery - 1) {
-                        y = exp2_poly(y);
-                        unpair(y, a, b);
-                    } else {
-                        unpair(y, a, b);
-                        a = exp2f(a);
-                        b = exp2f(b);
-                        y = pair(a, b);
-                    }
-                    sum2[i & 1] = add2(sum2[i & 1], y);
-                    pk[i] = pack2<T>(a, b);
-                }
-                tmem_st_32x16(s_at + 16 * c, pk);
+                exponentials<T>(s[c], scale2, minus2, pk, sum2);
+                tmem_st_32x16(at + 16 * c, pk);
             }
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(bar_p(stream, half));
+            mbar_arrive(bar_p(stream, buf));
             float sum_lo, sum_hi;
             unpair(add2(sum2[0], sum2[1]), sum_lo, sum_hi);
             l_run += sum_lo + sum_hi;
         }
         if (my_blocks > 0) {
+            // the last two products may both be under way: one after the other, as a barrier only tells its phases' parity
+            if (my_blocks > 1) mbar_wait(bar_o(stream), (my_blocks - 2) & 1u, p.wctx, 8);
             mbar_wait(bar_o(stream), (my_blocks - 1) & 1u, p.wctx, 8);
             tc_fence_after();
-            l_run += exchange(l_run);
         }
 
         // ---- one row tile, two streams: the second's result to the first through shared memory (every MMA is done with it)
         float* ex = reinterpret_cast<float*>(smem);   // [D + 2][128]
         float f0 = 1.f, f1 = 0.f;
         if constexpr (QT == 1 && NSTR == 2) {
-            named_barrier(3, S::SOFT);
+            named_barrier(1, S::SOFT);
             if (stream == 1) {
-                if (half == 0) {
-                    ex[D * 128 + row] = m_ref;
-                    ex[(D + 1) * 128 + row] = l_run;
-                }
+                ex[D * 128 + row] = m_ref;
+                ex[(D + 1) * 128 + row] = l_run;
 #pragma unroll 1
-                for (int c = 0; c < D / 2 && my_blocks > 0; c += 32) {
+                for (int c = 0; c < D && my_blocks > 0; c += 32) {
                     uint32_t o[32];
                     tmem_ld_32x32(o_at + c, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) ex[(half * (D / 2) + c + i) * 128 + row] = __uint_as_float(o[i]);
+                    for (int i = 0; i < 32; ++i) ex[(c + i) * 128 + row] = __uint_as_float(o[i]);
                 }
             }
-            named_barrier(3, S::SOFT);
+            named_barrier(1, S::SOFT);
             const float m1 = ex[D * 128 + row], l1 = ex[(D + 1) * 128 + row];
             const float m = fmaxf(m_ref, m1), mu = m == -CUDART_INF_F ? 0.f : m;
             f0 = exp2f(m_ref - mu);
@@ -682,10 +581,10 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             const size_t out_row = static_cast<size_t>(w.q0 + tok) * p.Hq + static_cast<size_t>(w.kvh) * p.G + (row - t_in * p.G);
             const size_t rows = static_cast<size_t>(p.tokens) * p.Hq;
             const bool other = QT == 1 && NSTR == 2 && nt > 1;
-            if (p.part_o != nullptr && mine && half == 0)
+            if (p.part_o != nullptr && mine)
                 p.part_lse[w.split * rows + out_row] = l_run > 0.f ? m_ref * 0.6931471805599453f + logf(l_run) : (l_run == l_run ? -CUDART_INF_F : l_run);
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 32) {
+            for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 if (my_blocks > 0) {   // alike in the whole warp
                     tmem_ld_32x32(o_at + c, o);
@@ -695,16 +594,16 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     v[i] = my_blocks > 0 ? __uint_as_float(o[i]) * f0 : 0.f;
-                    if (other) v[i] += ex[(half * (D / 2) + c + i) * 128 + row] * f1;
+                    if (other) v[i] += ex[(c + i) * 128 + row] * f1;
                     v[i] *= inv;
                 }
                 if (!mine) continue;
                 if (p.part_o != nullptr) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + out_row) * D + half * (D / 2) + c);
+                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + out_row) * D + c);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 } else {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + half * (D / 2) + c);
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         dst[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
@@ -759,7 +658,7 @@ namespace {
 template <typename T, int D, int QT>
 int launch_attention(const attention::Params& p, long long grid, cudaStream_t stream) {
     using S = attention::Shape<D>;
-    constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 10) * 8 + 16;
+    constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 12) * 8 + 16;
     static bool done[64] = {};
     static std::mutex setup_lock;
     int dev = 0;
@@ -857,9 +756,8 @@ int attention_impl(const TdistAttentionArgs* a) {
     p.q_xor = a->scale < 0.f ? 0x80008000u : 0u;
     if (a->scale == 0.f) p.scale_log2 = 1.f;
     // TMA: boxes of as many rows as divide both a page and a block of keys, at least the swizzle's eight
-    const int block = a->head_dim <= 128 ? 128 : 64;
     int rows = a->page_size & -a->page_size;
-    if (rows > block) rows = block;
+    if (rows > attention::kKeys) rows = attention::kKeys;
     if (rows >= 8 && a->stride_token > 0 && a->stride_block > 0 && a->stride_head > 0) {
         const uint64_t dims[4] = {static_cast<uint64_t>(a->head_dim), static_cast<uint64_t>(a->Hkv), static_cast<uint64_t>(a->page_size), static_cast<uint64_t>(a->blocks)};
         const uint64_t bytes[3] = {static_cast<uint64_t>(a->stride_head) * 2, static_cast<uint64_t>(a->stride_token) * 2, static_cast<uint64_t>(a->stride_block) * 2};

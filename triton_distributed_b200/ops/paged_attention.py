@@ -125,10 +125,9 @@ def _int32(t):
 
 
 def _splits(ctas: int, keys: int, head_dim: int, sms: int) -> int:
-    """Parts that the keys of a row tile are cut into: as many CTAs as the machine has SMs (one fits an SM), but at least four
-    blocks of keys each."""
-    block = 128 if head_dim <= 128 else 64
-    return max(1, min(sms // max(1, ctas), -(-keys // (4 * block)), 200))
+    """Parts that the keys of a row tile are cut into: as many CTAs as the machine has SMs (one fits an SM), but at least 512 keys
+    (256 with head_dim 256) each."""
+    return max(1, min(sms // max(1, ctas), -(-keys // (512 if head_dim <= 128 else 256)), 200))
 
 
 # What a call works out from its tensors' shapes, strides and types and its settings (never from their addresses or contents): checks,
