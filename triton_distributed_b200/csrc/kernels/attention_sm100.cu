@@ -132,6 +132,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -150,6 +155,26 @@ __device__ __forceinline__ void exponentials(const uint32_t (&s)[32], uint64_t s
         b = exp2f(b);
         sum2[i & 1] = add2(sum2[i & 1], pair(a, b));
         pk[i] = pack2<T>(a, b);
+    }
+}
+
+// s = out tanh(in s) where |in s| <= kCapSmall: tanh(z) / z as a polynomial in z^2, fitted to the least largest relative error, 7.3e-8. (The
+// exponential and the quotient it does without cost 16 clocks of the special-function unit per warp, twice what the softmax's own exponential
+// does.)
+constexpr float kCapSmall = 0.6f;
+__device__ __forceinline__ void cap_scores(uint32_t (&s)[32], float in, float out) {
+    const uint64_t in2 = pair(in, in), out2 = pair(out, out);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint64_t z = mul2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), in2), u = mul2(z, z);
+        uint64_t q = fma2(u, pair(0.01547542680054903f, 0.01547542680054903f), pair(-0.05210148170590401f, -0.05210148170590401f));
+        q = fma2(q, u, pair(0.13310173153877258f, 0.13310173153877258f));
+        q = fma2(q, u, pair(-0.33332309126853943f, -0.33332309126853943f));
+        q = fma2(q, u, pair(0.9999999403953552f, 0.9999999403953552f));
+        float lo, hi;
+        unpair(mul2(mul2(q, z), out2), lo, hi);
+        s[2 * i] = __float_as_uint(lo);
+        s[2 * i + 1] = __float_as_uint(hi);
     }
 }
 
@@ -443,19 +468,28 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int q_tile = QT == 2 ? stream : 0;
         if (live) {
             // Q into shared memory, zeros for rows without a token
-            for (int u = tid; u < QT * kRows * CH; u += S::SOFT) {
-                const int r = u / CH, c = u % CH, rt = r & (kRows - 1), tile = r / kRows;
-                const int t = rt / p.G, tok = w.i0 + tile * p.tile_tokens + t;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (t < p.tile_tokens && tok < w.n) {
-                    v = ld_v4(static_cast<const T*>(p.q) + static_cast<long long>(w.q0 + tok) * p.q_token +
-                              static_cast<long long>(w.kvh * p.G + rt - t * p.G) * p.q_head + c * 8);
-                    v.x = (v.x & p.q_and) ^ p.q_xor;
-                    v.y = (v.y & p.q_and) ^ p.q_xor;
-                    v.z = (v.z & p.q_and) ^ p.q_xor;
-                    v.w = (v.w & p.q_and) ^ p.q_xor;
+            constexpr int UNITS = QT * kRows * CH / S::SOFT, AHEAD = UNITS < 8 ? UNITS : 8;   // 16 bytes each; loads of a thread under way at once
+            static_assert(UNITS % AHEAD == 0 && S::SOFT % CH == 0, "a thread keeps its place in a row");
+            const int c = tid % CH;
+            const T* q = static_cast<const T*>(p.q) + static_cast<long long>(w.q0 + w.i0) * p.q_token + static_cast<long long>(w.kvh * p.G) * p.q_head + c * 8;
+#pragma unroll 1
+            for (int u0 = 0; u0 < UNITS; u0 += AHEAD) {
+                uint4 v[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int r = tid / CH + (u0 + u) * (S::SOFT / CH), rt = r & (kRows - 1), t = rt / p.G, tok = r / kRows * p.tile_tokens + t;
+                    v[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (t < p.tile_tokens && w.i0 + tok < w.n) v[u] = ld_v4(q + static_cast<long long>(tok) * p.q_token + static_cast<long long>(rt - t * p.G) * p.q_head);
                 }
-                *reinterpret_cast<uint4*>(smem + tile * S::QTILE + (c >> 3) * (kRows * 128) + rt * 128 + (((c & 7) ^ (rt & 7)) << 4)) = v;
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int r = tid / CH + (u0 + u) * (S::SOFT / CH), rt = r & (kRows - 1);
+                    v[u].x = (v[u].x & p.q_and) ^ p.q_xor;
+                    v[u].y = (v[u].y & p.q_and) ^ p.q_xor;
+                    v[u].z = (v[u].z & p.q_and) ^ p.q_xor;
+                    v[u].w = (v[u].w & p.q_and) ^ p.q_xor;
+                    *reinterpret_cast<uint4*>(smem + r / kRows * S::QTILE + (c >> 3) * (kRows * 128) + rt * 128 + (((c & 7) ^ (rt & 7)) << 4)) = v[u];
+                }
             }
             fence_proxy_async_smem();
         }
@@ -470,6 +504,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int pos = p.shared ? w.first : tile_first + t_in;
         const bool capped = p.soft_cap > 0.f;
         const float sl2 = capped ? 1.f : p.scale_log2;
+        // cap_out tanh(cap_in s): the cap in the exponent's domain; scores up to cap_small by a polynomial
+        const float cap_out = p.soft_cap * 1.4426950408889634f, cap_in = capped ? p.scale_log2 / cap_out : 0.f, cap_small = capped ? kCapSmall / cap_in : 0.f;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + S::O_COL + stream * D;
         const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
@@ -486,12 +522,22 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             tmem_ld_32x32(at + 32, s[1]);
             tmem_ld_wait();
             if (capped) {
-                // cap tanh(x / cap), in the exponent's domain: 1 - 2 / (1 + exp(2 x / cap))
-                const float cap = p.soft_cap * 1.4426950408889634f, in = 2.f * p.scale_log2 / p.soft_cap;
+                // cap tanh(x / cap), in the exponent's domain
+                float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(__uint_as_float(s[c][i]) * in)));
+                    for (int i = 0; i < 32; ++i) big[i & 3] = fmaxf(big[i & 3], fabsf(__uint_as_float(s[c][i])));
+                if (__all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= cap_small)) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) cap_scores(s[c], cap_in, cap_out);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)   // 1 - 2 / (1 + exp(2 x / cap)); NaN stays NaN
+                            s[c][i] = __float_as_uint(cap_out - __fdividef(2.f * cap_out, 1.f + exp2f(__uint_as_float(s[c][i]) * (2.f * 1.4426950408889634f * cap_in))));
+                }
             }
             if (edge) {
                 const int hi = pos - t0, lo = pos - p.window - t0, sink = p.sinks - t0;
@@ -599,9 +645,12 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                 }
                 if (!mine) continue;
                 if (p.part_o != nullptr) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_o + (w.split * rows + out_row) * D + c);
+                    float* dst = p.part_o + (w.split * rows + out_row) * D + c;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    for (int i = 0; i < 32; i += 8)   // a sector at a time
+                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]),
+                                     "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7])
+                                     : "memory");
                 } else {
                     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + c);
 #pragma unroll
@@ -703,8 +752,8 @@ int attention_impl(const TdistAttentionArgs* a) {
     if (a->page_size < 1 || a->max_blocks < 1 || a->blocks < 1) return fail(TDIST_EINVAL, "attention: page_size, max_blocks and blocks must be at least 1");
     if ((a->stride_token | a->stride_block | a->stride_head | a->q_token | a->q_head) % 8) return fail(TDIST_EINVAL, "attention: strides must be multiples of 8 elements");
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) |
-         reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->part_o)) % 16)
-        return fail(TDIST_EINVAL, "attention: q, caches, output and partials must be 16-byte aligned");
+         reinterpret_cast<uintptr_t>(a->out)) % 16 || reinterpret_cast<uintptr_t>(a->part_o) % 32)
+        return fail(TDIST_EINVAL, "attention: q, caches and output must be 16-byte aligned, partials 32-byte");
     if (a->splits < 1 || a->splits > 256) return fail(TDIST_EINVAL, "attention: splits must be in [1, 256]");
     if (a->row_tiles < 1 || a->row_tiles > 2 || (a->row_tiles == 2 && a->head_dim > 128)) return fail(TDIST_EINVAL, "attention: bad row_tiles");
     if (a->window < 1 || a->sinks < 0) return fail(TDIST_EINVAL, "attention: the window must be at least 1, sinks not negative");

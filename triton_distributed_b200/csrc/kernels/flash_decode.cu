@@ -540,14 +540,21 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
                 acc.w += f * hi.y;
             }
             if constexpr (EXT) {
-#pragma unroll 8
-                for (int i = 0; i < p.priors; ++i) {
-                    const float4 v = *reinterpret_cast<const float4*>(p.prior_o + (i * heads + head) * D + c);
-                    const float f = w_s[warp * 256 + p.splits + i];
-                    acc.x += f * v.x;
-                    acc.y += f * v.y;
-                    acc.z += f * v.z;
-                    acc.w += f * v.w;
+                // eight loads under way at once, the last ones too
+                for (int i0 = 0; i0 < p.priors; i0 += 8) {
+                    float4 v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (i0 + u < p.priors) v[u] = *reinterpret_cast<const float4*>(p.prior_o + ((i0 + u) * heads + head) * D + c);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (i0 + u >= p.priors) break;
+                        const float f = w_s[warp * 256 + p.splits + i0 + u];
+                        acc.x += f * v[u].x;
+                        acc.y += f * v[u].y;
+                        acc.z += f * v[u].z;
+                        acc.w += f * v[u].w;
+                    }
                 }
             }
             acc.x *= inv;

@@ -125,9 +125,10 @@ def _int32(t):
 
 
 def _splits(ctas: int, keys: int, head_dim: int, sms: int) -> int:
-    """Parts that the keys of a row tile are cut into: as many CTAs as the machine has SMs (one fits an SM), but at least 512 keys
-    (256 with head_dim 256) each."""
-    return max(1, min(sms // max(1, ctas), -(-keys // (512 if head_dim <= 128 else 256)), 200))
+    """Parts that the keys of a row tile are cut into: as many CTAs as the machine has SMs (one fits an SM), but at least 256 keys
+    (512 with head_dim 256) each: below that the parts' merge costs more (8 sequences, prefix of 2048, heads of 128, parts of 512 / 228 / 146
+    keys 20.9 / 17.6 / 19.1 us; 201 sequences, 5003, heads of 256, parts of 834 / 556 / 357 keys 62.6 / 51.4 / 58.0 us)."""
+    return max(1, min(sms // max(1, ctas), -(-keys // (256 if head_dim <= 128 else 512)), 200))
 
 
 # What a call works out from its tensors' shapes, strides and types and its settings (never from their addresses or contents): checks,
