@@ -17,7 +17,7 @@ dispatcher namespace.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -28,6 +28,8 @@ from .ops import gemm as G
 from .ops import gemm_fp8 as F8
 from .ops import moe_tp as MT
 from .ops import moe_utils as MU
+from .ops import paged_attention as PA
+from .ops import sampling as SA
 
 _CONTEXTS: Dict[int, object] = {}
 _NEXT = [1]
@@ -274,6 +276,59 @@ def _(partials):
     return partials.new_empty(tuple(partials.shape[1:-1]) + (partials.shape[-1] - 1,), dtype=torch.bfloat16)
 
 
+# ---------------------------------------------------------------------------- paged attention, sampling
+@_op("tdist::gqa_fwd_window_decode", mutates_args=())
+def gqa_fwd_window_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
+                          window: Optional[int], sinks: int, scale: float, soft_cap: float) -> torch.Tensor:
+    """decode attention over the last `window` keys and the first `sinks`"""
+    return PA.gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window, sinks, scale, soft_cap)
+
+
+@gqa_fwd_window_decode.register_fake
+def _(q, k_cache, v_cache, kv_lens, block_table, window, sinks, scale, soft_cap):
+    return q.new_empty(q.shape)
+
+
+@_op("tdist::gqa_fwd_window_prefill", mutates_args=())
+def gqa_fwd_window_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor,
+                           block_table: torch.Tensor, window: Optional[int], sinks: int, scale: float, soft_cap: float) -> torch.Tensor:
+    """attention of a ragged batch of query tokens, the last ones of their sequences"""
+    return PA.gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, scale, soft_cap)
+
+
+@gqa_fwd_window_prefill.register_fake
+def _(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, scale, soft_cap):
+    return q.new_empty(q.shape)
+
+
+@_op("tdist::gqa_fwd_shared_prefix_decode", mutates_args=())
+def gqa_fwd_shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_len: torch.Tensor,
+                                 prefix_table: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor, scale: float,
+                                 soft_cap: float) -> torch.Tensor:
+    """decode attention over a prefix that all sequences share and each one's own keys"""
+    return PA.gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, scale, soft_cap)
+
+
+@gqa_fwd_shared_prefix_decode.register_fake
+def _(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, scale, soft_cap):
+    return q.new_empty(q.shape)
+
+
+@_op("tdist::sample_tokens", mutates_args=())
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
+                  min_p: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(tokens int32, logprobs fp32, log_norm fp32), settings per row"""
+    out = SA.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    return out.tokens.clone(), out.logprobs.clone(), out.log_norm.clone()
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p):
+    B = logits.shape[0]
+    return (logits.new_empty((B,), dtype=torch.int32), logits.new_empty((B,), dtype=torch.float32), logits.new_empty((B,), dtype=torch.float32))
+
+
 OP_NAMES = ["gemm", "ag_gemm", "gemm_rs", "gemm_fp8", "ag_gemm_fp8", "group_gemm", "reduce_scatter", "barrier_all", "moe_topk_softmax",
             "moe_ag_scatter_align_block_size", "moe_dispatch", "moe_combine", "ep_dispatch", "ep_combine", "gqa_fwd_batch_decode",
-            "gqa_fwd_batch_decode_intra_rank", "sp_gqa_fwd_batch_decode", "lse_combine"]
+            "gqa_fwd_batch_decode_intra_rank", "sp_gqa_fwd_batch_decode", "lse_combine",
+            "gqa_fwd_window_decode", "gqa_fwd_window_prefill", "gqa_fwd_shared_prefix_decode", "sample_tokens"]
