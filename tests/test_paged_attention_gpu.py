@@ -345,3 +345,60 @@ def test_refusals(cuda_device):
     with pytest.raises(_lib.TdistError):
         P(odd, k, v, starts, lens, table)
     assert P(q[:0], k, v, torch.zeros(3, dtype=torch.int32, device=dev), lens, table).shape == (0, 8, 128)
+
+
+def test_more_tokens_than_keys_without_a_window(cuda_device):
+    """The first query positions lie before the first key: they see nothing, the later ones what is there."""
+    for lens in ([(40, 7)], [(300, 200), (5, 1), (70, 64)]):
+        out = _prefill_case(cuda_device, "bf16", 8, 2, 128, 16, lens, None, 0)
+        assert (out[:lens[0][0] - lens[0][1]] == 0).all() and (out[lens[0][0] - lens[0][1]:lens[0][0]] != 0).any()
+        _prefill_case(cuda_device, "fp16", 8, 2, 64, 16, lens, None, 3)
+
+
+@pytest.mark.parametrize("page", [16, 1])
+def test_caches_with_heads_before_tokens(cuda_device, page):
+    """[blocks, Hkv, page, D] in memory, seen as [blocks, page, Hkv, D]; a cache of more heads than are used."""
+    dev = cuda_device
+    torch.manual_seed(page)
+    for D in (64, 128, 256):
+        base = torch.randn(2, 40 * 16 // page, 6, page, D, device=dev).to(torch.bfloat16)
+        k, v = (base[i].permute(0, 2, 1, 3)[:, :, 1:4] for i in range(2))
+        need = -(-300 // page)
+        order = torch.randperm(k.shape[0], device=dev).to(torch.int32)
+        table = order[:2 * need].view(2, need)
+        q = torch.randn(90, 12, D, device=dev).to(torch.bfloat16)
+        lens = torch.tensor([300, 77], dtype=torch.int32, device=dev)
+        out = tdist.gqa_fwd_window_prefill(q, k, v, torch.tensor([0, 60, 90], device=dev), lens, table, window=120, sinks=3)
+        dec = tdist.gqa_fwd_window_decode(q[[59, 89]].contiguous(), k, v, lens, table, window=120, sinks=3)
+        pre = tdist.gqa_fwd_shared_prefix_decode(q[:2].contiguous(), k, v, 200, table[0], torch.tensor([77, 0], device=dev), table.flip(0))
+        check_status()
+        for b, (a, e, n) in enumerate(((0, 60, 300), (60, 90, 77))):
+            r, sp = _exact(q[a:e], _keys(k, table[b], n), _keys(v, table[b], n), _mask(e - a, n, 120, 3, dev), D ** -0.5, 0.0)
+            _compare(out[a:e], r, sp, 2.0 ** -8)
+            _compare(dec[b:b + 1], r[-1:], sp[-1:], 2.0 ** -8)
+            kk = torch.cat([_keys(k, table[0], 200), _keys(k, table[1], 77)]) if b == 0 else _keys(k, table[0], 200)
+            vv = torch.cat([_keys(v, table[0], 200), _keys(v, table[1], 77)]) if b == 0 else _keys(v, table[0], 200)
+            r, sp = _exact(q[b:b + 1], kk, vv, torch.ones(1, kk.shape[0], dtype=torch.bool, device=dev), D ** -0.5, 0.0)
+            _compare(pre[b:b + 1], r, sp, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_soft_caps_on_both_sides_of_the_polynomial(cuda_device, D):
+    """Scores far below the cap, around it, and beyond it, in one batch."""
+    dev = cuda_device
+    for scale, cap in ((0.01, 30.0), (0.3, 2.0), (2.0, 5.0)):
+        _prefill_case(dev, "fp16", 8, 2, D, 16, [(40, 400), (70, 90)], 300, 2, cap=cap, scale=scale)
+
+
+def test_refusals_of_head_counts_and_parts(cuda_device):
+    dev = cuda_device
+    k, v = _cache(8, 16, 1, 128, torch.bfloat16, dev)
+    table, lens, pre = torch.zeros(2, 4, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int32, device=dev), torch.zeros(4, dtype=torch.int32, device=dev)
+    q = torch.zeros(2, 17, 128, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(ValueError):
+        tdist.gqa_fwd_window_decode(q, k, v, lens, table, window=4)
+    with pytest.raises(ValueError):
+        tdist.gqa_fwd_shared_prefix_decode(q, k, v, 5, pre, lens, table)
+    with pytest.raises(ValueError):
+        tdist.gqa_fwd_shared_prefix_decode(q[:, :8].contiguous(), k, v, 5, pre, lens, table, kv_split=201)
+    assert tdist.gqa_fwd_window_prefill(q, k, v, torch.arange(3, device=dev), lens, table, window=4).shape == q.shape   # prefill takes them

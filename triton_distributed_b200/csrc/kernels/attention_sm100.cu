@@ -106,6 +106,12 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
+// the same, 8 columns
+__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename T>
@@ -163,16 +169,15 @@ __device__ __forceinline__ void exponentials(const uint32_t (&s)[32], uint64_t s
 // does.)
 constexpr float kCapSmall = 0.6f;
 __device__ __forceinline__ void cap_scores(uint32_t (&s)[32], float in, float out) {
-    const uint64_t in2 = pair(in, in), out2 = pair(out, out);
+    const uint64_t in2 = pair(in, in);
+    auto both = [&](float c) { return pair(c * out, c * out); };
+    const uint64_t c0 = both(0.9999999403953552f), c1 = both(-0.33332309126853943f), c2 = both(0.13310173153877258f), c3 = both(-0.05210148170590401f),
+                   c4 = both(0.01547542680054903f);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const uint64_t z = mul2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), in2), u = mul2(z, z);
-        uint64_t q = fma2(u, pair(0.01547542680054903f, 0.01547542680054903f), pair(-0.05210148170590401f, -0.05210148170590401f));
-        q = fma2(q, u, pair(0.13310173153877258f, 0.13310173153877258f));
-        q = fma2(q, u, pair(-0.33332309126853943f, -0.33332309126853943f));
-        q = fma2(q, u, pair(0.9999999403953552f, 0.9999999403953552f));
         float lo, hi;
-        unpair(mul2(mul2(q, z), out2), lo, hi);
+        unpair(mul2(fma2(fma2(fma2(fma2(u, c4, c3), u, c2), u, c1), u, c0), z), lo, hi);
         s[2 * i] = __float_as_uint(lo);
         s[2 * i + 1] = __float_as_uint(hi);
     }
@@ -245,7 +250,7 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
     } else {
         w.first = kv - w.n + w.i0;
         w.hi = max(0, kv - w.n + rows_end);
-        w.lo = min(max(0, w.first - p.window + 1), w.hi);
+        w.lo = min(p.window > w.first ? 0 : w.first - p.window + 1, w.hi);   // (the first position may lie before the first key)
         w.s_end = min(p.sinks, w.lo);
     }
     w.n_sink = (w.s_end + KT - 1) / KT;
@@ -502,6 +507,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int tile_first = p.shared ? w.first : w.first + q_tile * p.tile_tokens;
         const int tile_last = p.shared ? w.first : min(tile_first + p.tile_tokens - 1, w.first - w.i0 + w.n - 1);
         const int pos = p.shared ? w.first : tile_first + t_in;
+        // the keys up to these are out of the window: of this row, of the tile's last one
+        const int below = p.window > pos ? -1 : pos - p.window, tile_below = p.window > tile_last ? -1 : tile_last - p.window;
         const bool capped = p.soft_cap > 0.f;
         const float sl2 = capped ? 1.f : p.scale_log2;
         // cap_out tanh(cap_in s): the cap in the exponent's domain; scores up to cap_small by a polynomial
@@ -514,7 +521,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             const int t0 = block_start(QT == 2 ? it : it * NSTR + stream);
             const int buf = it & 1;
             const uint32_t at = s_at + buf * 64;
-            const bool edge = !(t0 + KT - 1 <= tile_first && (t0 > tile_last - p.window || t0 + KT <= p.sinks));   // some row does not see all
+            const bool edge = !(t0 + KT - 1 <= tile_first && (t0 > tile_below || t0 + KT <= p.sinks));   // some row does not see all
             mbar_wait(bar_s(stream, buf), (it >> 1) & 1u, p.wctx, 6);
             tc_fence_after();
             uint32_t s[2][32];
@@ -532,15 +539,26 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
 #pragma unroll
                     for (int c = 0; c < 2; ++c) cap_scores(s[c], cap_in, cap_out);
                 } else {
+                    // 1 - 2 / (1 + exp(2 x / cap)); NaN stays NaN. Eight columns at a time through TMEM: unrolled, it would crowd the loop out of
+                    // the instruction cache.
+#pragma unroll 1
+                    for (int c = 0; c < 64; c += 8) {
+                        uint32_t e[8];
+                        tmem_ld_32x8(at + c, e);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)   // 1 - 2 / (1 + exp(2 x / cap)); NaN stays NaN
-                            s[c][i] = __float_as_uint(cap_out - __fdividef(2.f * cap_out, 1.f + exp2f(__uint_as_float(s[c][i]) * (2.f * 1.4426950408889634f * cap_in))));
+                        for (int i = 0; i < 8; ++i)
+                            e[i] = __float_as_uint(cap_out - __fdividef(2.f * cap_out, 1.f + exp2f(__uint_as_float(e[i]) * (2.f * 1.4426950408889634f * cap_in))));
+                        tmem_st_32x8(at + c, e);
+                    }
+                    tmem_st_wait();
+                    tmem_ld_32x32(at, s[0]);
+                    tmem_ld_32x32(at + 32, s[1]);
+                    tmem_ld_wait();
                 }
             }
             if (edge) {
-                const int hi = pos - t0, lo = pos - p.window - t0, sink = p.sinks - t0;
+                const int hi = pos - t0, lo = below - t0, sink = p.sinks - t0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll

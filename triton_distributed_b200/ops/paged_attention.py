@@ -205,6 +205,8 @@ def _decode_args(q, k_cache, block_table, window, sinks, scale, soft_cap, kv_spl
         raise ValueError("q must be contiguous")
     B, Hq, D = q.shape
     blocks, page, Hkv, _ = k_cache.shape
+    if Hq // Hkv > 16:
+        raise ValueError("decode takes at most 16 query heads per kv head")
     a = _lib.DecodeArgs()
     a.B, a.Hq, a.Hkv, a.head_dim, a.page_size = B, Hq, Hkv, D, page
     a.max_blocks = block_table.shape[1]
@@ -307,6 +309,8 @@ def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, 
             tile = 128 // (Hq // k_cache.shape[2])
             row_tiles = 2 if D <= 128 and B > tile else 1
             splits = kv_split
+            if splits > 200:
+                raise ValueError("kv_split must be at most 200")
             if splits <= 0:
                 splits = _splits(-(-B // (tile * row_tiles)) * k_cache.shape[2], prefix_table.shape[0] * k_cache.shape[1], D, FD._sm_count(q.device))
             first = _attention_args(q, k_cache, prefix_table, 1, splits, row_tiles, NO_WINDOW, 0, factor, soft_cap, True)
