@@ -164,22 +164,43 @@ __device__ __forceinline__ void exponentials(const uint32_t (&s)[32], uint64_t s
     }
 }
 
-// s = out tanh(in s) where |in s| <= kCapSmall: tanh(z) / z as a polynomial in z^2, fitted to the least largest relative error, 7.3e-8. (The
+// out tanh(in s) where |in s| <= kCapSmall: tanh(z) / z as a polynomial in z^2, fitted to the least largest relative error, 7.3e-8. (The
 // exponential and the quotient it does without cost 16 clocks of the special-function unit per warp, twice what the softmax's own exponential
-// does.)
-constexpr float kCapSmall = 0.6f;
-__device__ __forceinline__ void cap_scores(uint32_t (&s)[32], float in, float out) {
-    const uint64_t in2 = pair(in, in);
-    auto both = [&](float c) { return pair(c * out, c * out); };
-    const uint64_t c0 = both(0.9999999403953552f), c1 = both(-0.33332309126853943f), c2 = both(0.13310173153877258f), c3 = both(-0.05210148170590401f),
-                   c4 = both(0.01547542680054903f);
+// does.) The coefficients hold the powers of `in` up to the ninth: within fp32's range for `in` in [2^-12, 2^12], and other caps go without.
+constexpr float kCapSmall = 0.6f, kCapRange = 4096.f;
+struct Cap {
+    float c[5];
+};
+__device__ __forceinline__ Cap cap_polynomial(float in, float out) {
+    const float u = in * in;
+    Cap k;
+    float f = out * in;
+    k.c[0] = 0.9999999403953552f * f;
+    k.c[1] = -0.33332309126853943f * (f *= u);
+    k.c[2] = 0.13310173153877258f * (f *= u);
+    k.c[3] = -0.05210148170590401f * (f *= u);
+    k.c[4] = 0.01547542680054903f * (f *= u);
+    return k;
+}
+__device__ __forceinline__ float cap_score(float s, const Cap& k) {   // -inf stays -inf
+    const float u = s * s;
+    return fmaf(fmaf(fmaf(fmaf(u, k.c[4], k.c[3]), u, k.c[2]), u, k.c[1]), u, k.c[0]) * s;
+}
+// P = 2^(cap(s) - m): as above. The maximum is known before the cap is taken, as the cap keeps the order, so that one pair's polynomial runs
+// under another's exponentials.
+template <typename T>
+__device__ __forceinline__ void capped_exponentials(const uint32_t (&s)[32], const Cap& k, uint64_t minus2, uint32_t (&pk)[16], uint64_t (&sum2)[2]) {
+    auto both = [&](int i) { return pair(k.c[i], k.c[i]); };
+    const uint64_t c0 = both(0), c1 = both(1), c2 = both(2), c3 = both(3), c4 = both(4);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const uint64_t z = mul2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), in2), u = mul2(z, z);
-        float lo, hi;
-        unpair(mul2(fma2(fma2(fma2(fma2(u, c4, c3), u, c2), u, c1), u, c0), z), lo, hi);
-        s[2 * i] = __float_as_uint(lo);
-        s[2 * i + 1] = __float_as_uint(hi);
+        const uint64_t x = pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), u = mul2(x, x);
+        float a, b;
+        unpair(fma2(fma2(fma2(fma2(fma2(u, c4, c3), u, c2), u, c1), u, c0), x, minus2), a, b);
+        a = exp2f(a);
+        b = exp2f(b);
+        sum2[i & 1] = add2(sum2[i & 1], pair(a, b));
+        pk[i] = pack2<T>(a, b);
     }
 }
 
@@ -262,8 +283,9 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
     return true;
 }
 
-// QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks.
-template <typename T, int D, int QT>
+// QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks. CAPPED: with a soft cap (a kernel of
+// its own: with both in one, 16384 tokens without a cap took 1890 to 1940 us instead of @@).
+template <typename T, int D, int QT, bool CAPPED>
 __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const __grid_constant__ Params p) {
     using S = Shape<D>;
     constexpr int KT = kKeys, NSTR = S::STREAMS, NST = stages<D, QT>(), CH = D / 8;
@@ -509,10 +531,11 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const int pos = p.shared ? w.first : tile_first + t_in;
         // the keys up to these are out of the window: of this row, of the tile's last one
         const int below = p.window > pos ? -1 : pos - p.window, tile_below = p.window > tile_last ? -1 : tile_last - p.window;
-        const bool capped = p.soft_cap > 0.f;
-        const float sl2 = capped ? 1.f : p.scale_log2;
+        const float sl2 = CAPPED ? 1.f : p.scale_log2;
         // cap_out tanh(cap_in s): the cap in the exponent's domain; scores up to cap_small by a polynomial
-        const float cap_out = p.soft_cap * 1.4426950408889634f, cap_in = capped ? p.scale_log2 / cap_out : 0.f, cap_small = capped ? kCapSmall / cap_in : 0.f;
+        const float cap_out = p.soft_cap * 1.4426950408889634f, cap_in = CAPPED ? p.scale_log2 / cap_out : 0.f;
+        const float cap_small = cap_in >= 1.f / kCapRange && cap_in <= kCapRange ? kCapSmall / cap_in : -1.f;
+        const Cap cap = cap_polynomial(cap_in, cap_out);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + S::O_COL + stream * D;
         const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
@@ -528,17 +551,15 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             tmem_ld_32x32(at, s[0]);
             tmem_ld_32x32(at + 32, s[1]);
             tmem_ld_wait();
-            if (capped) {
-                // cap tanh(x / cap), in the exponent's domain
+            bool small = false;   // the cap is yet to be taken, by its polynomial
+            if constexpr (CAPPED) {
                 float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) big[i & 3] = fmaxf(big[i & 3], fabsf(__uint_as_float(s[c][i])));
-                if (__all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= cap_small)) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) cap_scores(s[c], cap_in, cap_out);
-                } else {
+                small = __all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= cap_small);
+                if (!small) {
                     // 1 - 2 / (1 + exp(2 x / cap)); NaN stays NaN. Eight columns at a time through TMEM: unrolled, it would crowd the loop out of
                     // the instruction cache.
 #pragma unroll 1
@@ -572,7 +593,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
+            const float raw = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), top = small ? cap_score(raw, cap) : raw * sl2;
             if (it == 0) {
                 m_ref = top;
             } else if (__any_sync(0xffffffffu, top > m_ref + kRaise)) {
@@ -598,7 +619,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
-                exponentials<T>(s[c], scale2, minus2, pk, sum2);
+                if (small) capped_exponentials<T>(s[c], cap, minus2, pk, sum2);
+                else exponentials<T>(s[c], scale2, minus2, pk, sum2);
                 tmem_st_32x16(at + 16 * c, pk);
             }
             tmem_st_wait();
@@ -722,7 +744,7 @@ using tdist_host::fail;
 
 namespace {
 
-template <typename T, int D, int QT>
+template <typename T, int D, int QT, bool CAPPED>
 int launch_attention(const attention::Params& p, long long grid, cudaStream_t stream) {
     using S = attention::Shape<D>;
     constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 12) * 8 + 16;
@@ -734,15 +756,15 @@ int launch_attention(const attention::Params& p, long long grid, cudaStream_t st
     {
         std::lock_guard<std::mutex> guard(setup_lock);
         if (!done[dev]) {
-            TDIST_CUDA_OK(cudaFuncSetAttribute(attention::attention_kernel<T, D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            TDIST_CUDA_OK(cudaFuncSetAttribute(attention::attention_kernel<T, D, QT, CAPPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             done[dev] = true;
         }
     }
-    TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_kernel<T, D, QT>, dim3(static_cast<unsigned>(grid)), S::THREADS, smem, stream, p));
+    TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_kernel<T, D, QT, CAPPED>, dim3(static_cast<unsigned>(grid)), S::THREADS, smem, stream, p));
     return 0;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CAPPED>
 int run_attention(const TdistAttentionArgs* a, attention::Params& p) {
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     const long long per = static_cast<long long>(a->row_tiles) * p.tile_tokens;
@@ -752,14 +774,25 @@ int run_attention(const TdistAttentionArgs* a, attention::Params& p) {
     if (grid > 0x7fffffffLL) return fail(TDIST_ELIMIT, "attention: tiles * Hkv * splits exceeds the grid limit");
     int rc;
     if constexpr (D <= 128)
-        rc = a->row_tiles == 2 ? launch_attention<T, D, 2>(p, grid, stream) : launch_attention<T, D, 1>(p, grid, stream);
+        rc = a->row_tiles == 2 ? launch_attention<T, D, 2, CAPPED>(p, grid, stream) : launch_attention<T, D, 1, CAPPED>(p, grid, stream);
     else
-        rc = launch_attention<T, D, 1>(p, grid, stream);
+        rc = launch_attention<T, D, 1, CAPPED>(p, grid, stream);
     if (rc != 0 || p.splits == 1 || a->out == nullptr) return rc;
     const long long rows = static_cast<long long>(p.tokens) * p.Hq, per_cta = 128 / (D / 4);
     TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)), 128, 0,
                                          stream, p.part_o, p.part_lse, p.splits, static_cast<int>(rows), static_cast<T*>(a->out)));
     return 0;
+}
+
+template <typename T, bool CAPPED>
+int by_head_dim(const TdistAttentionArgs* a, attention::Params& p) {
+    if (a->head_dim == 64) return run_attention<T, 64, CAPPED>(a, p);
+    if (a->head_dim == 128) return run_attention<T, 128, CAPPED>(a, p);
+    return run_attention<T, 256, CAPPED>(a, p);
+}
+template <typename T>
+int by_head_dim(const TdistAttentionArgs* a, attention::Params& p) {
+    return p.soft_cap > 0.f ? by_head_dim<T, true>(a, p) : by_head_dim<T, false>(a, p);
 }
 
 int attention_impl(const TdistAttentionArgs* a) {
@@ -838,16 +871,8 @@ int attention_impl(const TdistAttentionArgs* a) {
     p.wctx.status = static_cast<Status*>(a->status);
     p.wctx.timeout_ns = a->timeout_ns;
     p.wctx.kernel_id = attention::kKernelAttention;
-    if (a->dtype == TDIST_BF16) {
-        if (a->head_dim == 64) return run_attention<__nv_bfloat16, 64>(a, p);
-        if (a->head_dim == 128) return run_attention<__nv_bfloat16, 128>(a, p);
-        return run_attention<__nv_bfloat16, 256>(a, p);
-    }
-    if (a->dtype == TDIST_F16) {
-        if (a->head_dim == 64) return run_attention<__half, 64>(a, p);
-        if (a->head_dim == 128) return run_attention<__half, 128>(a, p);
-        return run_attention<__half, 256>(a, p);
-    }
+    if (a->dtype == TDIST_BF16) return by_head_dim<__nv_bfloat16>(a, p);
+    if (a->dtype == TDIST_F16) return by_head_dim<__half>(a, p);
     return fail(TDIST_EINVAL, "attention: dtype must be bf16 or fp16");
 }
 
