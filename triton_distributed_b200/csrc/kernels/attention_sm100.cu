@@ -81,6 +81,7 @@ constexpr int stages() {
     return (Shape<D>::AREA - QT * Shape<D>::QTILE) / Shape<D>::TILE;
 }
 constexpr int kMaxStages = 18;
+constexpr int kBars = 2 * kMaxStages + 14;   // full, empty, S, P, O, Q, go
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
@@ -284,7 +285,7 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
 }
 
 // QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks. CAPPED: with a soft cap (a kernel of
-// its own: with both in one, 16384 tokens without a cap took 1890 to 1940 us instead of @@).
+// its own: with both in one, 16384 tokens without a cap 1890 to 1940 us, by itself 1710 to 1820).
 template <typename T, int D, int QT, bool CAPPED>
 __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const __grid_constant__ Params p) {
     using S = Shape<D>;
@@ -295,15 +296,15 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::AREA);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 12);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + QT * S::QTILE;
     const uint32_t bars_u32 = smem_u32(bars);
     auto bar_full = [&](int s) { return bars_u32 + 8u * s; };
     auto bar_empty = [&](int s) { return bars_u32 + 8u * (kMaxStages + s); };
     auto bar_s = [&](int s, int b) { return bars_u32 + 8u * (2 * kMaxStages + 2 * s + b); };        // S is complete
     auto bar_p = [&](int s, int b) { return bars_u32 + 8u * (2 * kMaxStages + 4 + 2 * s + b); };    // P is in its place
-    auto bar_o = [&](int s) { return bars_u32 + 8u * (2 * kMaxStages + 8 + s); };                   // O has taken it in
-    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 10);
+    auto bar_o = [&](int s, int b) { return bars_u32 + 8u * (2 * kMaxStages + 8 + 2 * s + b); };    // O has taken it in
+    const uint32_t bar_q = bars_u32 + 8u * (2 * kMaxStages + 12), bar_go = bars_u32 + 8u * (2 * kMaxStages + 13);
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -315,10 +316,11 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             for (int b = 0; b < 2; ++b) {
                 mbar_init(bar_s(s, b), 1);
                 mbar_init(bar_p(s, b), 128);
+                mbar_init(bar_o(s, b), 1);
             }
-            mbar_init(bar_o(s), 1);
         }
         mbar_init(bar_q, S::SOFT);
+        mbar_init(bar_go, 1);
         fence_mbar_init();
     }
     if (warp == S::SOFT / 32) {
@@ -465,25 +467,27 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         };
         if (my_blocks > 0) {
             mbar_wait(bar_q, 0, p.wctx, 3);
-            // half a block behind the other stream, so that one's exponentials run beside the other's loads and maxima
-            if (stream == 1) mbar_wait(bar_p(0, 0), 0, p.wctx, 9);
+            // half a block behind the other stream, so that one's exponentials run beside the other's loads and maxima (a barrier of one phase: that
+            // of the other's P may be two phases further by the time this warp looks)
+            if (stream == 1) mbar_wait(bar_go, 0, p.wctx, 9);
             for (int it = 0; it < min(2, my_blocks); ++it) qk(it);
             for (int it = 0; it < my_blocks; ++it) {
                 const int j = block(it), item = item_v(j), slot = item % NST, buf = it & 1;
                 arrived(item, j);
                 const uint64_t b = umma_desc_mn_sw128(ring + static_cast<uint32_t>(slot) * S::TILE, KT * 128);
                 mbar_wait(bar_p(stream, buf), (it >> 1) & 1u, p.wctx, 4);
+                if (NSTR == 2 && stream == 0 && it == 0 && lane == 0) mbar_arrive(bar_go);
                 tc_fence_after();
                 if (leader) {
 #pragma unroll
                     for (int k = 0; k < KT / 16; ++k) umma_ts(o_col, s_col + buf * 64 + 8 * k, b + 128 * k, idesc_o, it > 0 || k != 0 ? 1u : 0u);
-                    umma_commit(bar_o(stream));
+                    umma_commit(bar_o(stream, buf));
                     umma_commit(bar_empty(slot));
                 }
                 __syncwarp();
                 if (it + 2 < my_blocks) {
                     // this P has been taken in: the next S but one takes its columns
-                    mbar_wait(bar_o(stream), it & 1u, p.wctx, 5);
+                    mbar_wait(bar_o(stream, buf), (it >> 1) & 1u, p.wctx, 5);
                     tc_fence_after();
                     qk(it + 2);
                 }
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                 const float alpha = m_new == m_ref ? 1.f : exp2f(m_ref - m_new);
                 m_ref = m_new;
                 l_run *= alpha;
-                mbar_wait(bar_o(stream), (it - 1) & 1u, p.wctx, 7);
+                mbar_wait(bar_o(stream, buf ^ 1), ((it - 1) >> 1) & 1u, p.wctx, 7);
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
@@ -631,9 +635,9 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             l_run += sum_lo + sum_hi;
         }
         if (my_blocks > 0) {
-            // the last two products may both be under way: one after the other, as a barrier only tells its phases' parity
-            if (my_blocks > 1) mbar_wait(bar_o(stream), (my_blocks - 2) & 1u, p.wctx, 8);
-            mbar_wait(bar_o(stream), (my_blocks - 1) & 1u, p.wctx, 8);
+            // The last two products may both be under way or both be done. A barrier only tells its phases' parity, hence one for each S: the phase
+            // before the last product's is over, as the last S came after it.
+            mbar_wait(bar_o(stream, (my_blocks - 1) & 1), ((my_blocks - 1) >> 1) & 1u, p.wctx, 8);
             tc_fence_after();
         }
 
@@ -747,7 +751,7 @@ namespace {
 template <typename T, int D, int QT, bool CAPPED>
 int launch_attention(const attention::Params& p, long long grid, cudaStream_t stream) {
     using S = attention::Shape<D>;
-    constexpr int smem = S::AREA + 1024 + (2 * attention::kMaxStages + 12) * 8 + 16;
+    constexpr int smem = S::AREA + 1024 + attention::kBars * 8 + 16;
     static bool done[64] = {};
     static std::mutex setup_lock;
     int dev = 0;
