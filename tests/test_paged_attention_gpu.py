@@ -402,3 +402,53 @@ def test_refusals_of_head_counts_and_parts(cuda_device):
     with pytest.raises(ValueError):
         tdist.gqa_fwd_shared_prefix_decode(q[:, :8].contiguous(), k, v, 5, pre, lens, table, kv_split=201)
     assert tdist.gqa_fwd_window_prefill(q, k, v, torch.arange(3, device=dev), lens, table, window=4).shape == q.shape   # prefill takes them
+
+
+@pytest.mark.parametrize("indices", [torch.int32, torch.int64])
+def test_shared_prefix_behind_writes_of_its_inputs(cuda_device, indices):
+    """Calls one after the other without a wait between them, each behind kernels that write its queries, caches, table and lengths: the own
+    keys' kernel starts while the prefix' one runs, but not before what both read is there. Integers in 64 bits are converted on the way."""
+    dev, B, P, page = cuda_device, 70, 4096, 16
+    torch.manual_seed(8)
+    pages, most = P // page + B * 8, 8
+    rounds = []
+    for _ in range(4):
+        k, v = _cache(pages, page, 2, 128, torch.bfloat16, dev)
+        order = torch.randperm(pages, device=dev)
+        rounds.append((torch.randn(B, 8, 128, device=dev).to(torch.bfloat16), k, v, torch.tensor([P - 7], device=dev).to(indices),
+                       order[:P // page].to(indices), torch.randint(0, most * page + 1, (B,), device=dev).to(indices),
+                       order[P // page:].view(B, most).to(indices)))
+    now = [torch.zeros_like(t) for t in rounds[0]]
+    outs = []
+    for given in rounds * 3:
+        for dst, src in zip(now, given):
+            dst.copy_(src)
+        outs.append(tdist.gqa_fwd_shared_prefix_decode(*now))
+    check_status()
+    for i, (q, k, v, n, first, lens, table) in enumerate(rounds):
+        for out in outs[i + 4::4]:
+            assert torch.equal(out, outs[i])
+        for b in range(0, B, 9):
+            own = int(lens[b])
+            keys = [torch.cat([_keys(c, first, int(n)), _keys(c, table[b], own)]) for c in (k, v)]
+            r, s = _exact(q[b:b + 1], keys[0], keys[1], torch.ones(1, int(n) + own, dtype=torch.bool, device=dev), 128 ** -0.5, 0.0)
+            _compare(outs[i][b:b + 1], r, s, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_short_rows(cuda_device, D):
+    """Tiles of one to four blocks of keys, thousands of them one after the other: every wait ends, every call gives the same."""
+    dev, n = cuda_device, 6000
+    torch.manual_seed(9)
+    k, v = _cache(n // 16 + 1, 16, 4, D, torch.bfloat16, dev)
+    q = torch.randn(n, 8, D, device=dev).to(torch.bfloat16)
+    table = torch.randperm(n // 16 + 1, device=dev).view(1, -1).to(torch.int32)
+    starts, lens = torch.tensor([0, n], dtype=torch.int32, device=dev), torch.tensor([n], dtype=torch.int32, device=dev)
+    for window in (1, 40, 130):
+        outs = [tdist.gqa_fwd_window_prefill(q, k, v, starts, lens, table, window=window) for _ in range(20)]
+        check_status()
+        for out in outs[1:]:
+            assert torch.equal(out, outs[0])
+        last = 300
+        r, s = _exact(q[-last:], _keys(k, table[0], n), _keys(v, table[0], n), _mask(last, n, window, 0, dev), D ** -0.5, 0.0)
+        _compare(outs[0][-last:], r, s, 2.0 ** -8)

@@ -224,7 +224,7 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
     int tile = static_cast<int>(blockIdx.x) / p.splits / p.Hkv;
     const int per = QT * p.tile_tokens;
     const long long table_keys = static_cast<long long>(p.max_blocks) * p.page_size;
-    int kv;
+    int kv = 0;
     if (p.shared) {
         w.b = 0;
         w.q0 = 0;
@@ -235,8 +235,9 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
         // 32 sequences at a time: the one whose tiles hold number `tile`
         int b = -1;
         for (int b0 = 0; b0 < p.B; b0 += 32) {
-            int start = 0, n = 0;
+            int start = 0, n = 0, keys = 0;
             if (b0 + lane < p.B) {
+                keys = p.kv_lens[b0 + lane];
                 start = min(max(p.q_starts[b0 + lane], 0), p.tokens);
                 n = max(min(p.q_starts[b0 + lane + 1], p.tokens) - start, 0);
             }
@@ -253,6 +254,7 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
                 b = b0 + src;
                 w.q0 = __shfl_sync(0xffffffffu, start, src);
                 w.n = __shfl_sync(0xffffffffu, n, src);
+                kv = __shfl_sync(0xffffffffu, keys, src);
                 // the last tokens, which see the most keys, first
                 w.i0 = (__shfl_sync(0xffffffffu, upto, src) - 1 - tile) * per;
                 break;
@@ -261,7 +263,6 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
         }
         if (b < 0) return false;
         w.b = b;
-        kv = p.kv_lens[b];
     }
     kv = kv < 0 ? 0 : (kv > table_keys ? static_cast<int>(table_keys) : kv);
     const int rows_end = min(w.n, w.i0 + per);
@@ -327,14 +328,13 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         tmem_alloc<1>(smem_u32(tmem_slot), 512);
         tmem_relinquish<1>();
     }
+    pdl_wait_and_release();
+    Work w = {};
+    const bool live = find_work<D, QT>(p, w);   // its loads under the others' set-up
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-    pdl_wait_and_release();
-
-    Work w = {};
-    const bool live = find_work<D, QT>(p, w);
     const int nt = live ? w.nt : 0;
     auto block_start = [&](int j) {   // first key of the split's j-th block
         const int i = w.c0 + j;

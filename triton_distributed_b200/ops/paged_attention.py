@@ -184,16 +184,18 @@ def _run_attention(template, q, k_cache, v_cache, table, starts, lens, out, part
     return a
 
 
-def _run_decode(template, q, k_cache, v_cache, table, lens, out, status, handle, priors=None):
-    """The split decode kernel over windows, or with the partial results of another kernel (its arguments)."""
+def _decode_call(template, q, k_cache, v_cache, table, lens, out, status, handle):
+    """Arguments of the split decode kernel over windows, or with the partial results of another kernel."""
     a = _lib.DecodeArgs.from_buffer_copy(template)
     partial, counters = FD._Workspace.get(q.device, None, handle, a.B, a.Hq, a.Hkv, a.head_dim, a.splits)
     a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     a.block_table, a.kv_lens, a.out = table.data_ptr(), lens.data_ptr(), out.data_ptr()
     a.partial, a.counters = partial.data_ptr(), counters.data_ptr()
-    if priors is not None:
-        a.prior_o, a.prior_lse = priors.part_o, priors.part_lse
     a.status, a.timeout_ns, a.stream = status, default_timeout_ns(), handle
+    return a
+
+
+def _run_decode(a):
     code = _lib.lib().tdist_flash_decode(C.byref(a))
     if code:
         _lib.check(code, "tdist_flash_decode")
@@ -242,7 +244,8 @@ def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Opt
         args = _remember(key, _decode_args(q, k_cache, block_table, min(window, NO_WINDOW) if window is not None else NO_WINDOW, sinks, factor,
                                            soft_cap, kv_split))
     out = _output(out, q)
-    _run_decode(args, q, k_cache, v_cache, _int32(block_table), _int32(kv_lens), out, _status_ptr(), stream_ptr(q.device))
+    table, lens = _int32(block_table), _int32(kv_lens)
+    _run_decode(_decode_call(args, q, k_cache, v_cache, table, lens, out, _status_ptr(), stream_ptr(q.device)))
     return out
 
 
@@ -317,10 +320,14 @@ def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, 
         plan = _remember(key, (first, _decode_args(q, k_cache, block_table, NO_WINDOW, 0, factor, soft_cap, -1, splits)))
     first, second = plan
     out = _output(out, q)
-    status, handle, priors = _status_ptr(), stream_ptr(q.device), None
+    status, handle = _status_ptr(), stream_ptr(q.device)
+    own_table, own_lens = _int32(block_table), _int32(kv_lens)
+    own = _decode_call(second, q, k_cache, v_cache, own_table, own_lens, out, status, handle)
     if first is not None:
+        # the decode kernel starts while the prefix' one runs: nothing is launched between the two
         rows = first.tokens * first.Hq
         parts = torch.empty(first.splits * rows * (first.head_dim + 1), dtype=torch.float32, device=q.device)
-        priors = _run_attention(first, q, k_cache, v_cache, _int32(prefix_table), None, _int32(prefix_len), None, parts, rows, status, handle)
-    _run_decode(second, q, k_cache, v_cache, _int32(block_table), _int32(kv_lens), out, status, handle, priors)
+        prefix = _run_attention(first, q, k_cache, v_cache, _int32(prefix_table), None, _int32(prefix_len), None, parts, rows, status, handle)
+        own.prior_o, own.prior_lse, own.early = prefix.part_o, prefix.part_lse, 1
+    _run_decode(own)
     return out
