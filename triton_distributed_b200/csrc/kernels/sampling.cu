@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     uint4* part = reinterpret_cast<uint4*>(smem_raw + sizeof(Shared));   // this CTA's part of the row
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
     const int rank = static_cast<int>(blockIdx.x) % p.cl, row_no = static_cast<int>(blockIdx.x) / p.cl;
+    cluster_arrive();   // its counterpart stands before the first store into another CTA
     if (tid == 0) s.found = -1;
     auto clear = [&]() {
         for (int i = tid; i < 2 * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(s.lo)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -202,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         float* tops = reinterpret_cast<float*>(s.scan);
         if (lane == 0) tops[warp] = m;
         __syncthreads();
+        cluster_wait();   // every CTA of the cluster runs
         if (warp == 0) {
             m = lane < kWarps ? tops[lane] : -CUDART_INF_F;
 #pragma unroll
