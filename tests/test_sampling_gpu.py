@@ -212,3 +212,18 @@ def test_refusals(cuda_device):
     with pytest.raises(_lib.TdistError):
         tdist.sample_tokens(torch.zeros(1, 1, device=cuda_device).expand(1, 600000).contiguous(), u[:1])
     assert tdist.sample_tokens(x[:0], u[:0]).tokens.shape == (0,)
+
+
+@pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (0, 0.5, 0.0), (5, 0.5, 0.1), (0, 1.0, 0.2)])
+def test_a_temperature_that_is_no_number(cuda_device, k, p, m):
+    """NaN among the rows' temperatures: the largest logit, whatever the filters, as for 0."""
+    torch.manual_seed(8)
+    logits, u = torch.randn(3, 9001, device=cuda_device), torch.rand(3, device=cuda_device)
+    t = torch.tensor([float("nan"), 0.7, -1.0], device=cuda_device)
+    got, ref = tdist.sample_tokens(logits, u, t, k, p, m), ref_sample_tokens(logits, u, t, k, p, m)
+    check_status()
+    assert torch.equal(got.tokens, ref.tokens)
+    assert torch.equal(got.tokens[::2].long(), logits[::2].argmax(1))
+    assert torch.equal(got.log_norm[::2], logits[::2].amax(1)) and got.logprobs[::2].tolist() == [0.0, 0.0]
+    one = tdist.sample_tokens(logits, u, float("nan"), k, p, m)
+    assert torch.equal(one.tokens.long(), logits.argmax(1))

@@ -172,3 +172,10 @@ def test_the_example_on_a_gpu(cuda_device):
     drawn = _example().run(cuda_device)
     check_status()
     assert drawn.shape == (6, 20) and (drawn >= 0).all()
+
+
+def test_a_temperature_that_is_no_number():
+    torch.manual_seed(6)
+    x, u = torch.randn(3, 30), torch.rand(3)
+    got = tdist.sample_tokens(x, u, torch.tensor([math.nan, 0.0, math.nan]), 5, 0.9, 0.1)
+    assert torch.equal(got.tokens.long(), x.argmax(1)) and torch.equal(got.log_norm, x.amax(1)) and not got.logprobs.any()

@@ -8,7 +8,7 @@
 //   token = the first index (by index) at which the sum of the kept w passes floor(u W), W = sum of the kept w
 //   logprob = (x[token] - max) / temperature - log(W / 2^31),  log_norm = max / temperature + log(W / 2^31)
 //
-// Temperature 0: the largest logit (lowest index). NaN counts as -inf; a row without anything above -inf gives token -1.
+// Temperature 0, below or NaN: the largest logit (lowest index). A NaN logit counts as -inf; a row without anything above -inf gives token -1.
 // Weights below 2^-32 of the largest are zero: tokens that no 24-bit random number could have drawn.
 //
 // A row belongs to a cluster of 1 to 8 CTAs. Each reads its part from HBM once, into shared memory, and goes over it there: the maximum;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     const float top_p = p.top_p ? p.top_p[row_no] : p.one_top_p;
     const float min_p = p.min_p ? p.min_p[row_no] : p.one_min_p;
     const int top_k = p.top_k ? p.top_k[row_no] : p.one_top_k;
-    const bool greedy = temperature <= 0.f;
+    const bool greedy = !(temperature > 0.f);   // NaN too
     const bool by_k = top_k > 0 && top_k < p.V && !greedy, by_p = top_p < 1.f && !greedy;
     const uint32_t least = min_p > 0.f && !greedy ? static_cast<uint32_t>(ceil(static_cast<double>(fminf(min_p, 1.f)) * kOne)) : 0u;
 

@@ -44,7 +44,7 @@ def ref_sample_tokens(logits, u, temperature: Setting = 1.0, top_k: Setting = 0,
     t, k, p, m = per_row(temperature, torch.float32), per_row(top_k, torch.int64), per_row(top_p, torch.float32), per_row(min_p, torch.float32)
     x = logits.float()
     x = torch.where(torch.isnan(x), float("-inf"), x) + 0.0
-    greedy = t <= 0
+    greedy = ~(t > 0)
     inv = 1.0 / torch.where(greedy, 1.0, t)
     top = x.amax(1, keepdim=True)
     y = torch.where(x == top, 0.0, (x - top) * inv)
@@ -92,7 +92,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
                   min_p: Setting = 0.0) -> SampledTokens:
     """``logits [B, V]`` (bf16, fp16 or fp32, any distance between rows), ``u`` fp32 ``[B]`` in [0, 1). Each setting is a number for
     all rows or a tensor ``[B]`` (fp32; ``top_k`` int32 or int64). Off: ``top_k <= 0``, ``top_p >= 1``, ``min_p <= 0``; ``temperature <= 0``
-    takes the largest logit, the lowest index of equal ones. Logits of -inf or NaN are never drawn."""
+    (or NaN) takes the largest logit, the lowest index of equal ones. Logits of -inf or NaN are never drawn."""
     global launch_count
     given = (temperature, top_k, top_p, min_p)
     # the checks' outcome depends on shapes, types and devices only, and is kept by them
