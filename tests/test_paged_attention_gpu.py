@@ -452,3 +452,15 @@ def test_many_short_rows(cuda_device, D):
         last = 300
         r, s = _exact(q[-last:], _keys(k, table[0], n), _keys(v, table[0], n), _mask(last, n, window, 0, dev), D ** -0.5, 0.0)
         _compare(outs[0][-last:], r, s, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("window,sinks", [(5, 2 ** 31), (5, 2 ** 32 + 1), (2 ** 32 + 1, 0)])
+def test_settings_beyond_32_bits(cuda_device, window, sinks):
+    """More first tokens, or a wider window, than any sequence is long: every key up to the query's position."""
+    _prefill_case(cuda_device, "bf16", 8, 2, 128, 16, [(9, 50), (30, 200)], window, sinks)
+    torch.manual_seed(1)
+    k, v = _cache(20, 16, 2, 64, torch.bfloat16, cuda_device)
+    q = torch.randn(2, 8, 64, device=cuda_device).to(torch.bfloat16)
+    table, lens = torch.arange(20, dtype=torch.int32, device=cuda_device).view(2, 10), torch.tensor([160, 33], dtype=torch.int32, device=cuda_device)
+    out = tdist.gqa_fwd_window_decode(q, k, v, lens, table, window=window, sinks=sinks)
+    assert torch.equal(out, tdist.gqa_fwd_window_decode(q, k, v, lens, table))

@@ -142,7 +142,8 @@ def _layout(*tensors):
 
 def _settings(window, sinks, scale, soft_cap):
     """The settings as plain numbers (a plan is found by their values)."""
-    return None if window is None else int(window), int(sinks), None if scale is None else float(scale), float(soft_cap)
+    # (no sequence has more than 2^31 - 1 keys: the native arguments are 32 bits wide)
+    return None if window is None else min(int(window), NO_WINDOW), min(int(sinks), NO_WINDOW), None if scale is None else float(scale), float(soft_cap)
 
 
 def _remember(key, plan):
@@ -241,7 +242,7 @@ def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Opt
             return ref_window_attn(q, k_cache, v_cache, torch.arange(B + 1), kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
         if B == 0:
             return _output(out, q)
-        args = _remember(key, _decode_args(q, k_cache, block_table, min(window, NO_WINDOW) if window is not None else NO_WINDOW, sinks, factor,
+        args = _remember(key, _decode_args(q, k_cache, block_table, NO_WINDOW if window is None else window, sinks, factor,
                                            soft_cap, kv_split))
     out = _output(out, q)
     table, lens = _int32(block_table), _int32(kv_lens)
@@ -267,7 +268,7 @@ def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, 
         T, Hq, D = q.shape
         if T == 0 or B == 0:
             return _output(out, q)
-        most = min(window, NO_WINDOW) if window is not None else NO_WINDOW
+        most = NO_WINDOW if window is None else window
         tile = 128 // (Hq // k_cache.shape[2])
         each = -(-T // B)                                   # tokens of a sequence, where all have as many
         row_tiles = 2 if D <= 128 and each > tile else 1
