@@ -1,0 +1,36 @@
+"""What the serving operators refuse before any launch, and their CPU statements on infinities, NaN and empty batches."""
+import ctypes as C
+
+import pytest
+
+from triton_distributed_b200 import _lib
+
+
+def _decode_args(**changed):
+    """A call that nothing is wrong with but ``changed``. The addresses are numbers: nothing may come of the call but its refusal."""
+    a = _lib.DecodeArgs()
+    base = 1 << 20
+    a.q, a.k_cache, a.v_cache, a.block_table, a.kv_lens, a.partial, a.counters, a.out = (base * (i + 1) for i in range(8))
+    a.B, a.Hq, a.Hkv, a.head_dim, a.page_size, a.max_blocks, a.splits, a.world = 2, 8, 2, 128, 16, 4, 1, 1
+    a.stride_block, a.stride_token, a.stride_head, a.scale, a.dtype = 16 * 256, 256, 128, 1.0, _lib.DT_BF16
+    for name, value in changed.items():
+        setattr(a, name, value)
+    return a
+
+
+WINDOW = dict(window=64, sinks=4)
+
+
+@pytest.mark.parametrize("ext", [{}, WINDOW])
+@pytest.mark.parametrize("field,address", [("k_cache", (2 << 20) + 8), ("v_cache", (3 << 20) + 8), ("k_cache", (2 << 20) + 2), ("q", (1 << 20) + 2),
+                                           ("out", (8 << 20) + 4), ("partial", (6 << 20) + 4)])
+def test_decode_refuses_misaligned_addresses(ext, field, address):
+    """Every copy and store of the kernel needs its width's alignment; a slice of a cache has it in its strides but not in its base."""
+    code = _lib.lib().tdist_flash_decode(C.byref(_decode_args(**ext, **{field: address})))
+    assert code != 0 and b"aligned" in _lib.lib().tdist_last_error()
+
+
+def test_decode_refuses_misaligned_earlier_partials():
+    a = _decode_args(**WINDOW, priors=2, prior_o=(9 << 20) + 4, prior_lse=10 << 20)
+    code = _lib.lib().tdist_flash_decode(C.byref(a))
+    assert code != 0 and b"aligned" in _lib.lib().tdist_last_error()

@@ -840,6 +840,11 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
     p.wctx.rank = a->rank;
     if (!p.q || !p.k_cache || !p.v_cache || !p.block_table || !p.kv_lens || !p.partial || !p.counters || !p.out)
         return fail(TDIST_EINVAL, "decode: null pointer");
+    // the widths the kernel loads and stores with: K and V by 16 bytes, q by 4, the result by 8 (O || LSE and the exchange's by 4)
+    auto misaligned = [](const void* ptr, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes != 0; };
+    if (misaligned(a->k_cache, 16) || misaligned(a->v_cache, 16) || misaligned(a->q, 4) || misaligned(a->out, a->mode == 0 ? 8 : 4) ||
+        misaligned(a->partial, 8) || misaligned(p.prior_o, 16))
+        return fail(TDIST_EINVAL, "decode: the caches must be 16-byte aligned, q 4-byte, the output 8-byte, earlier partials 16-byte");
     if (a->mode == 2) {
         if (a->world < 1 || a->world > TDIST_MAX_RANKS || a->rank < 0 || a->rank >= a->world) return fail(TDIST_EINVAL, "decode: world/rank out of range");
         if (a->epoch == 0 && a->epoch_ptr == nullptr) return fail(TDIST_EINVAL, "decode: the epoch of a sequence-parallel call must be non-zero");
