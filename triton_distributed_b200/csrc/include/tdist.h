@@ -411,9 +411,8 @@ typedef struct TdistDecodeArgs {
     /* mode 0, optional: window > 0 lets every query see the last `window` keys and the first `sinks` of its sequence only
      * (pages that hold no such key are not read, nor are their table entries). With window > 0 (0x7fffffff: no limit) the
      * result may also take in partial results over other keys: prior_o fp32 [priors][B * Hq][D] (normalised) and
-     * prior_lse fp32 [priors][B * Hq] (natural log, -inf: no keys). early: 1 if the launch before this one in the stream is the
-     * tdist_attention that makes them, and what else this call reads was launched before that one: own keys are then read while it runs. */
-    int window, sinks, priors, early;
+     * prior_lse fp32 [priors][B * Hq] (natural log, -inf: no keys). */
+    int window, sinks, priors;
     const void* prior_o;
     const void* prior_lse;
 } TdistDecodeArgs;

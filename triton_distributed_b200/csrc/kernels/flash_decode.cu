@@ -75,7 +75,6 @@ struct DecodeParams {
     // windows and earlier partials (kernels with EXT only)
     int window, sinks;      // a sequence's query sees its last `window` keys and its first `sinks`
     int max_keys;           // most keys a sequence can have to read
-    int early;              // the launch before makes the priors, and all else is complete before that one lets this one in
     int priors;             // partial results of other keys that the merge takes in: O [priors][B * Hq][D], LSE [priors][B * Hq]
     const float* prior_o;
     const float* prior_lse;
@@ -196,7 +195,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
 
     const int tid = static_cast<int>(threadIdx.x);
     const int warp = tid >> 5, lane = tid & 31;
-    if (!EXT || !p.early) pdl_wait_and_release(p.mode != 2 || p.world == 1);
+    pdl_wait_and_release(p.mode != 2 || p.world == 1);
     const int split = static_cast<int>(blockIdx.x) % p.splits;
     const int kvh = (static_cast<int>(blockIdx.x) / p.splits) % p.Hkv;
     int b = static_cast<int>(blockIdx.x) / (p.splits * p.Hkv);
@@ -493,10 +492,6 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
         __threadfence();
     }
 
-    if constexpr (EXT) {
-        // 64 sequences, prefix of 32768 keys, 1024 own: 81.7 us, with the wait in front 85.0
-        if (p.early) pdl_wait_and_release();
-    }
     // A warp per query head: lanes first turn the per-split LSEs into normalised weights (kept in
     // shared memory), then every lane merges 4 output columns with independent 16-byte loads.
     float* merged = o_s;                       // [G][W2] merged O || LSE of this rank (SP mode)
@@ -826,7 +821,6 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
     p.window = a->window;
     p.sinks = a->sinks;
     p.priors = a->priors;
-    p.early = a->priors > 0 ? a->early : 0;
     p.prior_o = static_cast<const float*>(a->prior_o);
     p.prior_lse = static_cast<const float*>(a->prior_lse);
     p.mode = a->mode;

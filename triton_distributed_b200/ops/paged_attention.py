@@ -325,10 +325,9 @@ def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, 
     own_table, own_lens = _int32(block_table), _int32(kv_lens)
     own = _decode_call(second, q, k_cache, v_cache, own_table, own_lens, out, status, handle)
     if first is not None:
-        # the decode kernel starts while the prefix' one runs: nothing is launched between the two
         rows = first.tokens * first.Hq
         parts = torch.empty(first.splits * rows * (first.head_dim + 1), dtype=torch.float32, device=q.device)
         prefix = _run_attention(first, q, k_cache, v_cache, _int32(prefix_table), None, _int32(prefix_len), None, parts, rows, status, handle)
-        own.prior_o, own.prior_lse, own.early = prefix.part_o, prefix.part_lse, 1
+        own.prior_o, own.prior_lse = prefix.part_o, prefix.part_lse
     _run_decode(own)
     return out
