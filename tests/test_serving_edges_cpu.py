@@ -18,7 +18,7 @@ def _decode_args(**changed):
     return a
 
 
-WINDOW = dict(window=64, sinks=4)
+WINDOW = dict(window=64, sinks=4, blocks=9)
 
 
 @pytest.mark.parametrize("ext", [{}, WINDOW])
@@ -34,3 +34,8 @@ def test_decode_refuses_misaligned_earlier_partials():
     a = _decode_args(**WINDOW, priors=2, prior_o=(9 << 20) + 4, prior_lse=10 << 20)
     code = _lib.lib().tdist_flash_decode(C.byref(a))
     assert code != 0 and b"aligned" in _lib.lib().tdist_last_error()
+
+
+def test_windowed_decode_needs_the_number_of_pages():
+    code = _lib.lib().tdist_flash_decode(C.byref(_decode_args(window=64, sinks=4, blocks=0)))
+    assert code != 0 and b"blocks" in _lib.lib().tdist_last_error()

@@ -1,4 +1,4 @@
-"""Serving operators where they can go wrong: calls interleaved on one stream."""
+"""Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors."""
 import pytest
 import torch
 
@@ -47,3 +47,50 @@ def test_interleaved_shared_prefix_calls_on_one_stream(cuda_device, monkeypatch)
     check_status()
     for pair in got:
         assert all(torch.equal(a, b) for a, b in zip(pair, want))
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (64, 1), (128, 16), (256, 64)])
+@pytest.mark.parametrize("splits", [-1, 1, 16])
+def test_lengths_beyond_the_table_are_cut(cuda_device, D, page, splits):
+    """As many keys as the table has room for, whatever the length says; lengths below zero are none."""
+    dev = cuda_device
+    torch.manual_seed(D + page)
+    room = 320 // page
+    k, v = _pool(3 * room, page, 2, D, torch.bfloat16, dev)
+    table = torch.randperm(3 * room, device=dev).view(3, room).to(torch.int32)
+    q = torch.randn(3, 8, D, device=dev).to(torch.bfloat16)
+    for window, sinks in ((None, 0), (100, 3)):
+        args = dict(window=window, sinks=sinks, kv_split=splits)
+        got = tdist.gqa_fwd_window_decode(q, k, v, _ints([321, 2 ** 31 - 1, -5], dev), table, **args)
+        want = tdist.gqa_fwd_window_decode(q, k, v, _ints([320, 320, 0], dev), table, **args)
+        check_status()
+        assert torch.equal(got, want) and not got[2].any()
+    pre = torch.randperm(3 * room, device=dev)[:room].to(torch.int32)
+    got = tdist.gqa_fwd_shared_prefix_decode(q, k, v, 77, pre, _ints([1000, 320, -1], dev), table)
+    want = tdist.gqa_fwd_shared_prefix_decode(q, k, v, 77, pre, _ints([320, 320, 0], dev), table)
+    check_status()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (64, 1), (128, 16), (256, 64), (128, 3)])
+@pytest.mark.parametrize("bad", [-1, 10 ** 9])
+def test_pages_that_the_cache_does_not_have_read_as_zeros(cuda_device, D, page, bad):
+    dev = cuda_device
+    torch.manual_seed(D + page)
+    room = -(-320 // page)
+    k, v = _pool(2 * room + 1, page, 2, D, torch.bfloat16, dev)
+    k[-1], v[-1] = 0, 0
+    order = torch.randperm(2 * room, device=dev).view(2, room).to(torch.int32)
+    wrong, zeros = order.clone(), order.clone()
+    for i in (0, room // 2, room - 1):
+        wrong[0, i], zeros[0, i] = bad, 2 * room
+    q = torch.randn(2, 8, D, device=dev).to(torch.bfloat16)
+    lens = _ints([315, 320], dev)
+    for window, sinks in ((None, 0), (200, 3)):
+        for splits in (-1, 1, 16):
+            a, b = (tdist.gqa_fwd_window_decode(q, k, v, lens, t, window=window, sinks=sinks, kv_split=splits) for t in (wrong, zeros))
+            check_status()
+            assert torch.equal(a, b)
+        a, b = (tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 1, 2], dev), lens, t, window=window, sinks=sinks) for t in (wrong, zeros))
+        check_status()
+        assert torch.equal(a, b)

@@ -177,7 +177,7 @@ class DecodeArgs(C.Structure):
         ("stream", C.c_void_p),
         ("epoch_ptr", C.c_void_p), ("epoch_done", C.c_void_p), ("ll_peer_alt", C.c_void_p * MAX_RANKS),
         ("ll_mc", C.c_void_p), ("ll_mc_alt", C.c_void_p),
-        ("window", C.c_int), ("sinks", C.c_int), ("priors", C.c_int), ("prior_o", C.c_void_p), ("prior_lse", C.c_void_p),
+        ("window", C.c_int), ("sinks", C.c_int), ("priors", C.c_int), ("blocks", C.c_int), ("prior_o", C.c_void_p), ("prior_lse", C.c_void_p),
     ]
 
 

@@ -75,6 +75,7 @@ struct DecodeParams {
     // windows and earlier partials (kernels with EXT only)
     int window, sinks;      // a sequence's query sees its last `window` keys and its first `sinks`
     int max_keys;           // most keys a sequence can have to read
+    int table_keys, blocks; // EXT: keys that a row of the table has room for, pages of the cache
     int priors;             // partial results of other keys that the merge takes in: O [priors][B * Hq][D], LSE [priors][B * Hq]
     const float* prior_o;
     const float* prior_lse;
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
     }
     int first = 0x7fffffff, gap = 0;
     if constexpr (EXT) {
+        kv_len = min(max(kv_len, 0), p.table_keys);
         const int lo = max(0, kv_len - p.window);   // first key of the window
         first = min(p.sinks, lo);
         gap = lo - first;
@@ -245,6 +247,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
                 if constexpr (EXT) t += t < first ? 0 : gap;
                 const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
                 const int page = table[in_table];
+                if (EXT && static_cast<unsigned>(page) >= static_cast<unsigned>(p.blocks)) return -1;   // reads as zeros, like a row past the end
                 base = static_cast<long long>(page) * p.stride_block + static_cast<long long>(t - in_table * p.page_size) * p.stride_token;
             }
         }
@@ -266,7 +269,9 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
             if (BY_BLOCK) off = base + row_off + static_cast<long long>(j * ROWS) * p.stride_token;
             if (!whole) off = __shfl_sync(0xffffffffu, base, row);
             // rows past the end are zero-filled
-            const int nbytes = (BY_BLOCK ? row < left : off >= 0) ? 16 : 0;
+            bool seen = BY_BLOCK ? row < left : off >= 0;
+            if (BY_BLOCK && EXT) seen = seen && (whole ? base : off) >= 0;
+            const int nbytes = seen ? 16 : 0;
             if (nbytes == 0) off = 0;
             cp_async16(ks + tile_off<D>(row, lch), kl + off, nbytes);
             cp_async16(ks + TILE + tile_off<D>(row, lch), vl + off, nbytes);
@@ -816,6 +821,9 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
         if (a->priors > 0 && (!a->prior_o || !a->prior_lse)) return fail(TDIST_EINVAL, "decode: null pointer");
         const long long seen = static_cast<long long>(a->window) + a->sinks;
         if (seen < max_keys) max_keys = seen;
+        if (a->blocks < 1) return fail(TDIST_EINVAL, "decode: blocks must be at least 1");
+        p.table_keys = static_cast<int>(table_keys < 0x7fffffff ? table_keys : 0x7fffffff);
+        p.blocks = a->blocks;
     }
     p.max_keys = static_cast<int>(max_keys);
     p.window = a->window;

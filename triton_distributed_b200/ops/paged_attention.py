@@ -11,7 +11,8 @@ a ragged batch, and decode of a batch whose sequences share a prefix.
 
 ``window=None`` is no limit: plain causal attention. A query that sees no key gives zeros. Pages without a visible key are not
 read, nor are their table entries (a server may have given them back). What lies in a page behind a sequence's last key may be
-anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum.
+anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum. On a GPU lengths are
+cut to what the table has room for, and a page that the cache does not have reads as zeros: nothing outside the tensors is touched.
 
 Decode runs the split decode kernel (``csrc/kernels/flash_decode.cu``), prefill and the shared prefix the tcgen05 kernel
 (``csrc/kernels/attention_sm100.cu``). CPU tensors run ``ref_window_attn`` / ``ref_shared_prefix_attn``, the plain statements.
@@ -217,7 +218,7 @@ def _decode_args(q, k_cache, block_table, window, sinks, scale, soft_cap, kv_spl
     a.splits = min(FD.choose_splits(B, Hq, Hkv, D, most, blocks * page, q.device) if kv_split <= 0 else kv_split, 256 - priors)
     a.stride_block, a.stride_token, a.stride_head = k_cache.stride(0), k_cache.stride(1), k_cache.stride(2)
     a.scale, a.soft_cap, a.dtype, a.world = float(scale), float(soft_cap), _DTYPES[q.dtype], 1
-    a.window, a.sinks, a.priors = window, sinks, priors
+    a.window, a.sinks, a.priors, a.blocks = window, sinks, priors, blocks
     return a
 
 
