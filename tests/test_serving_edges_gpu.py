@@ -1,12 +1,14 @@
-"""Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors."""
+"""Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities."""
 import pytest
 import torch
 
 import triton_distributed_b200 as tdist
+from triton_distributed_b200.ops import flash_decode as FD
 from triton_distributed_b200.ops import paged_attention as PA
-from triton_distributed_b200.runtime import check_status
+from triton_distributed_b200.runtime import LocalWorld, check_status
 
 pytestmark = pytest.mark.gpu
+DTYPES = {"bf16": (torch.bfloat16, 2.0 ** -8), "fp16": (torch.float16, 2.0 ** -11)}
 
 
 def _pool(pages, page, Hkv, D, dt, dev):
@@ -15,6 +17,32 @@ def _pool(pages, page, Hkv, D, dt, dev):
 
 def _ints(values, dev):
     return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def _exact(q, k, v, scale, cap=0.0, seen=None):
+    """float64: q [n, Hq, D], k, v [keys, Hkv, D], seen [n, keys] (None: all) -> out, sum p |v|. NaN where the formula gives it."""
+    n, Hq, D = q.shape
+    Hkv = k.shape[1]
+    s = torch.einsum("nhgd,khd->hgnk", q.double().view(n, Hkv, Hq // Hkv, D), k.double()) * scale
+    if cap > 0:
+        s = cap * torch.tanh(s / cap)
+    if seen is not None:
+        s = s.masked_fill(~seen, float("-inf"))
+    p = torch.softmax(s, -1)
+    both = [torch.einsum("hgnk,khd->nhgd", p, x).reshape(n, Hq, D) for x in (v.double(), v.double().abs())]
+    return both[0], both[1]
+
+
+def _keys(cache, table, n):
+    return cache[table.long()].flatten(0, 1)[:n]
+
+
+def _compare(out, ref, spread, u):
+    """Within the bounds of test_paged_attention_gpu.py, and NaN exactly where the formula is."""
+    assert torch.equal(out.isnan(), ref.isnan())
+    bound = u * (spread + ref.abs()) + 1e-4 * spread + 1e-6
+    worst = ((out.double() - ref).abs() - bound).nan_to_num(0.0).max()
+    assert worst <= 0, float(worst)
 
 
 def test_interleaved_shared_prefix_calls_on_one_stream(cuda_device, monkeypatch):
@@ -94,3 +122,66 @@ def test_pages_that_the_cache_does_not_have_read_as_zeros(cuda_device, D, page, 
         a, b = (tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 1, 2], dev), lens, t, window=window, sinks=sinks) for t in (wrong, zeros))
         check_status()
         assert torch.equal(a, b)
+
+
+def _spoil(what, q, k, v, at):
+    """One value of sequence 1 that is no number, or infinite (scores of both infinities, and -inf alone, which weighs nothing)."""
+    page, row = at
+    if what == "q":
+        q[1, 2, 5] = float("nan")
+    elif what == "k":
+        k[page, row, 0, 3] = float("nan")
+    elif what == "v":
+        v[page, row, 0, 3] = float("nan")
+    elif what == "k inf":
+        k[page, row, 0, 3] = float("inf")
+
+
+@pytest.mark.parametrize("what", ["q", "k", "v", "k inf"])
+@pytest.mark.parametrize("splits", [-1, 1, 3, 16])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16"), (256, "bf16")])
+def test_what_is_no_number_shows(cuda_device, what, splits, D, dtype):
+    """A NaN, or an infinite score, in what a query sees makes its result NaN as the formula says, never a result over the other keys."""
+    dev, (dt, u), page, n = cuda_device, DTYPES[dtype], 16, 700
+    torch.manual_seed(D + splits)
+    k, v = _pool(3 * 44 + 20, page, 2, D, dt, dev)
+    order = torch.randperm(3 * 44 + 20, device=dev).to(torch.int32)
+    table, pre = order[:132].view(3, 44), order[132:]
+    q = torch.randn(3, 8, D, device=dev).to(dt)
+    _spoil(what, q, k, v, (int(table[1, 40]), 7))   # key 647
+    lens, scale = _ints([n, n, n], dev), D ** -0.5
+    refs = [_exact(q[b:b + 1], _keys(k, table[b], n), _keys(v, table[b], n), scale) for b in range(3)]
+    ref, spread = (torch.cat(t) for t in zip(*refs))
+    assert ref[1].isnan().any() and not ref[0].isnan().any()
+    for out in (tdist.gqa_fwd_window_decode(q, k, v, lens, table, kv_split=splits),
+                tdist.gqa_fwd_batch_decode(q, k, v, None, None, lens, table, scale, kv_split=splits)):
+        check_status()
+        _compare(out, ref, spread, u)
+    part = tdist.gqa_fwd_batch_decode_intra_rank(q, k, v, None, None, lens, table, scale, kv_split=splits)
+    assert torch.equal(part[..., :D].isnan(), ref.isnan()) and torch.equal(part[..., D].isnan(), ref.isnan().all(-1))
+    merged = FD.inter_rank_combine(torch.stack([part, part]), dt)
+    check_status()
+    assert torch.equal(merged.isnan(), ref.isnan())
+    refs = [_exact(q[b:b + 1], torch.cat([_keys(k, pre, 300), _keys(k, table[b], n)]), torch.cat([_keys(v, pre, 300), _keys(v, table[b], n)]), scale)
+            for b in range(3)]
+    out = tdist.gqa_fwd_shared_prefix_decode(q, k, v, 300, pre, lens, table)
+    check_status()
+    _compare(out, *(torch.cat(t) for t in zip(*refs)), u)
+
+
+def test_what_is_no_number_shows_on_every_rank(cuda_device):
+    """The exchange of a sequence-parallel decode takes it along."""
+    dev, world, B, Hq, Hkv, D = cuda_device, 2, 2, 8, 2, 128
+    torch.manual_seed(2)
+    lw = LocalWorld(world, dev)
+    ctxs = [FD.create_sp_decode_context(r, world, B, Hq, D, heap=lw.heap(r), device=dev) for r in range(world)]
+    q = torch.randn(B, Hq, D, device=dev).to(torch.bfloat16)
+    lens = torch.full((world, B), 100, dtype=torch.int32, device=dev)
+    shards = [(*_pool(14, 16, Hkv, D, torch.bfloat16, dev), torch.arange(14, dtype=torch.int32, device=dev).view(2, 7)) for _ in range(world)]
+    shards[1][0][9, 0, 0, 0] = float("nan")   # rank 1, sequence 1, kv head 0
+    for r in range(world):
+        FD.sp_gqa_fwd_batch_decode(ctxs[r], q, shards[r][0], shards[r][1], lens, shards[r][2], phase=1)
+    outs = [FD.sp_gqa_fwd_batch_decode(ctxs[r], q, shards[r][0], shards[r][1], lens, shards[r][2], phase=2) for r in range(world)]
+    check_status()
+    for out in outs:
+        assert out[1, :4].isnan().all() and not out[1, 4:].isnan().any() and not out[0].isnan().any()

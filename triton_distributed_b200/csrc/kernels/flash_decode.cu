@@ -127,6 +127,9 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// What a sum of weights gives where it is not positive: 0 without keys, NaN where a score was NaN (which the comparisons pass over)
+__device__ __forceinline__ float without_weight(float sum, float value) { return sum == sum ? value : sum; }
+
 // Shared-memory tiles hold rows of D elements; the 16-byte chunk index is XOR-ed with the row
 // so that ldmatrix (8 rows x 16 bytes) and cp.async (one row per half-warp) are conflict-free.
 template <int D>
@@ -462,8 +465,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
             l += l_s[w][g] * f;
             acc += o_s[(static_cast<size_t>(w) * HEADS + g) * OP + c] * f;
         }
-        const float val = l > 0.f ? acc / l : 0.f;
-        const float lse = l > 0.f ? mm * 0.6931471805599453f + logf(l) : -CUDART_INF_F;
+        const float val = l > 0.f ? acc / l : without_weight(l, 0.f);
+        const float lse = l > 0.f ? mm * 0.6931471805599453f + logf(l) : without_weight(l, -CUDART_INF_F);
         if (p.cluster_merge) {
             // straight into the leader CTA's shared memory: [G][splits][W2], the layout the merge below reads
             const uint32_t at = part_leader + static_cast<uint32_t>(((g * p.splits + split) * W2 + c) * 4);
@@ -529,8 +532,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
 #pragma unroll
         for (int o2 = 16; o2; o2 >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o2);
         __syncwarp();
-        const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
-        const float lse = wsum > 0.f ? mm + logf(wsum) : -CUDART_INF_F;
+        const float inv = wsum > 0.f ? 1.f / wsum : without_weight(wsum, 0.f);
+        const float lse = wsum > 0.f ? mm + logf(wsum) : without_weight(wsum, -CUDART_INF_F);
         for (int c = lane * 4; c < D; c += 128) {
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
@@ -644,7 +647,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
             a0 += f * __uint_as_float(static_cast<uint32_t>(v));
             a1 += f * __uint_as_float(static_cast<uint32_t>(v >> 32));
         }
-        const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+        const float inv = wsum > 0.f ? 1.f / wsum : without_weight(wsum, 0.f);
         T* dst = static_cast<T*>(p.out) + (static_cast<size_t>(b) * p.Hq + kvh * G + g) * D + c;
         *reinterpret_cast<uint32_t*>(dst) = pack2<T>(a0 * inv, a1 * inv);
     }
@@ -679,7 +682,7 @@ __global__ void lse_combine_kernel(const float* parts, int R, int heads, int D, 
             wsum += f;
             acc += f * src[c];
         }
-        out[static_cast<size_t>(h) * D + c] = from_float<T>(wsum > 0.f ? acc / wsum : 0.f);
+        out[static_cast<size_t>(h) * D + c] = from_float<T>(wsum > 0.f ? acc / wsum : without_weight(wsum, 0.f));
     }
 }
 
