@@ -1,4 +1,5 @@
-"""Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities."""
+"""Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities,
+tokens of no sequence."""
 import pytest
 import torch
 
@@ -185,3 +186,35 @@ def test_what_is_no_number_shows_on_every_rank(cuda_device):
     check_status()
     for out in outs:
         assert out[1, :4].isnan().all() and not out[1, 4:].isnan().any() and not out[0].isnan().any()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kv_split", [-1, 1, 4])
+@pytest.mark.parametrize("T,starts", [(300, [40, 100, 100, 250]), (34, [0, 33]), (34, [1, 34]), (65, [0, 64]), (500, [0, 1]), (90, [45, 45]), (40, [0, 0, 40])])
+def test_tokens_of_no_sequence_give_zeros(cuda_device, D, kv_split, T, starts):
+    """q padded to a fixed number of tokens, as for a captured graph: before the first sequence's and behind the last one's."""
+    dev = cuda_device
+    torch.manual_seed(T + D)
+    B = len(starts) - 1
+    k, v = _pool(B * 30, 16, 2, D, torch.bfloat16, dev)
+    table = torch.randperm(B * 30, device=dev).view(B, 30).to(torch.int32)
+    lens = _ints([450 - 50 * b for b in range(B)], dev)
+    q = torch.randn(T, 8, D, device=dev).to(torch.bfloat16)
+    first, last = starts[0], starts[-1]
+    for window in (None, 60):
+        out = torch.full_like(q, float("nan"))
+        tdist.gqa_fwd_window_prefill(q, k, v, _ints(starts, dev), lens, table, window=window, out=out, kv_split=kv_split)
+        check_status()
+        assert not out[:first].any() and not out[last:].any()
+        if last > first:
+            alone = tdist.gqa_fwd_window_prefill(q[first:last], k, v, _ints([s - first for s in starts], dev), lens, table, window=window, kv_split=kv_split if kv_split > 0 else 2)
+            torch.testing.assert_close(out[first:last].float(), alone.float(), atol=2.0 ** -6, rtol=2.0 ** -6)
+
+
+def test_tokens_without_any_sequence_give_zeros(cuda_device):
+    dev = cuda_device
+    k, v = _pool(4, 16, 2, 64, torch.bfloat16, dev)
+    q = torch.randn(5, 8, 64, device=dev).to(torch.bfloat16)
+    out = torch.full_like(q, float("nan"))
+    tdist.gqa_fwd_window_prefill(q, k, v, _ints([0], dev), _ints([], dev), torch.zeros((0, 4), dtype=torch.int32, device=dev), out=out)
+    assert not out.any()

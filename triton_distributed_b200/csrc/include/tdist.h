@@ -426,7 +426,8 @@ typedef struct TdistAttentionArgs {
     const void* k_cache;      /* [blocks, page, Hkv, D] */
     const void* v_cache;
     const void* block_table;  /* int32 [B, max_blocks]; shared: [max_blocks] */
-    const void* q_starts;     /* int32 [B + 1]: first query token of every sequence; they are its last positions. Unused if shared */
+    const void* q_starts;     /* int32 [B + 1]: first query token of every sequence; they are its last positions. Tokens before the
+                               * first and from the last one on belong to none: zeros. Unused if shared */
     const void* kv_lens;      /* int32 [B]; shared: [1] */
     void* out;                /* [tokens, Hq, D]; NULL: leave the partial results */
     void* part_o;             /* fp32 [splits][tokens * Hq][D], with splits > 1 or without out */

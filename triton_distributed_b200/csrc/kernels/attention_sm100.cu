@@ -525,6 +525,20 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             fence_proxy_async_smem();
         }
         mbar_arrive(bar_q);
+        if (!p.shared) {
+            // tokens of no sequence, before the first one's and behind the last one's: zeros (LSE -inf), spread over the CTAs of a kv head and split
+            const int lead = min(max(p.q_starts[0], 0), p.tokens), tail = max(min(p.q_starts[p.B], p.tokens), lead);
+            const int per_tile = p.splits * p.Hkv, n = lead + p.tokens - tail;
+            for (int i = static_cast<int>(blockIdx.x) / per_tile; i < n; i += static_cast<int>(gridDim.x) / per_tile) {
+                const size_t first = static_cast<size_t>(i < lead ? i : tail + i - lead) * p.Hq + static_cast<size_t>(w.kvh) * p.G;
+                const size_t rows = static_cast<size_t>(p.tokens) * p.Hq;
+                uint4* dst = p.part_o != nullptr ? reinterpret_cast<uint4*>(p.part_o + (w.split * rows + first) * D)
+                                                 : reinterpret_cast<uint4*>(static_cast<T*>(p.out) + first * D);
+                const int units = p.G * D / (p.part_o != nullptr ? 4 : 8);
+                for (int u = tid; u < units; u += S::SOFT) dst[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (p.part_o != nullptr && tid < p.G) p.part_lse[w.split * rows + first + tid] = -CUDART_INF_F;
+            }
+        }
 
         const int t_in = row / p.G;
         const int tok = w.i0 + q_tile * p.tile_tokens + t_in;

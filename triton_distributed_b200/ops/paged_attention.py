@@ -9,7 +9,8 @@ a ragged batch, and decode of a batch whose sequences share a prefix.
 * ``gqa_fwd_shared_prefix_decode(q[B,Hq,D], k_cache, v_cache, prefix_len[1], prefix_table[max_blocks], kv_lens[B],
   block_table, scale, soft_cap) -> [B,Hq,D]``: the softmax runs over the keys of the prefix, read once for all, and the sequence's own
 
-``window=None`` is no limit: plain causal attention. A query that sees no key gives zeros. Pages without a visible key are not
+``window=None`` is no limit: plain causal attention. A query that sees no key gives zeros, and so does a token that ``q_starts`` (which must
+not decrease) gives to no sequence, as in a batch padded for a captured graph. Pages without a visible key are not
 read, nor are their table entries (a server may have given them back). What lies in a page behind a sequence's last key may be
 anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum. On a GPU lengths are
 cut to what the table has room for, and a page that the cache does not have reads as zeros: nothing outside the tensors is touched.
@@ -268,7 +269,7 @@ def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, 
             return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
         T, Hq, D = q.shape
         if T == 0 or B == 0:
-            return _output(out, q)
+            return _output(out, q).zero_()
         most = NO_WINDOW if window is None else window
         tile = 128 // (Hq // k_cache.shape[2])
         each = -(-T // B)                                   # tokens of a sequence, where all have as many
