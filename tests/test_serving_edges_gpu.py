@@ -1,5 +1,5 @@
 """Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities,
-tokens of no sequence."""
+tokens of no sequence, large soft caps."""
 import pytest
 import torch
 
@@ -218,3 +218,63 @@ def test_tokens_without_any_sequence_give_zeros(cuda_device):
     out = torch.full_like(q, float("nan"))
     tdist.gqa_fwd_window_prefill(q, k, v, _ints([0], dev), _ints([], dev), torch.zeros((0, 4), dtype=torch.int32, device=dev), out=out)
     assert not out.any()
+
+
+@pytest.mark.parametrize("cap", [65.0, 300.0, 1e3, 1e5, 1e8, 1e30, 3e38])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_large_soft_caps_change_little(cuda_device, cap, D):
+    """The cap's error goes with the score, not with the cap: the bound is that of a call without one."""
+    dev, page, n = cuda_device, 16, 900
+    torch.manual_seed(D)
+    k, v = _pool(3 * 57, page, 2, D, torch.float16, dev)
+    order = torch.randperm(3 * 57, device=dev).to(torch.int32)
+    table, pre = order[:114].view(2, 57), order[114:]
+    scale = 3.5 * D ** -0.5   # scores of some 3.5
+    q = torch.randn(140, 8, D, device=dev).to(torch.float16)
+    seen = torch.arange(n, device=dev).view(1, -1) <= torch.arange(n - 70, n, device=dev).view(-1, 1)
+    for loud in (False, True):
+        if loud:
+            q[3] *= 8000.0    # one token whose scores reach caps of 1e3 and more, in the tiles of the others
+        refs = [_exact(q[70 * b:70 * b + 70], _keys(k, table[b], n), _keys(v, table[b], n), scale, cap, seen) for b in range(2)]
+        ref, spread = (torch.cat(t) for t in zip(*refs))
+        quiet = torch.arange(140, device=dev) != 3
+        for split in (-1, 1, 3):
+            out = tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 70, 140], dev), _ints([n, n], dev), table, scale=scale, soft_cap=cap, kv_split=split)
+            check_status()
+            assert out.isfinite().all()
+            _compare(out[quiet], ref[quiet], spread[quiet], 2.0 ** -11)
+    q = torch.randn(2, 8, D, device=dev).to(torch.float16)
+    for loud in (False, True):
+        if loud:
+            q[0, 1] *= 8000.0   # a head beside the others of its MMA
+        refs = [_exact(q[b:b + 1], _keys(k, table[b], n), _keys(v, table[b], n), scale, cap) for b in range(2)]
+        both = [_exact(q[b:b + 1], torch.cat([_keys(k, pre, 500), _keys(k, table[b], n)]), torch.cat([_keys(v, pre, 500), _keys(v, table[b], n)]), scale, cap)
+                for b in range(2)]
+        quiet = torch.ones(2, 8, dtype=torch.bool, device=dev)
+        quiet[0, 1] = not loud
+        for split in (-1, 1, 16):
+            out = tdist.gqa_fwd_window_decode(q, k, v, _ints([n, n], dev), table, scale=scale, soft_cap=cap, kv_split=split)
+            pfx = tdist.gqa_fwd_shared_prefix_decode(q, k, v, 500, pre, _ints([n, n], dev), table, scale=scale, soft_cap=cap, kv_split=split)
+            check_status()
+            for got, want in ((out, refs), (pfx, both)):
+                ref, spread = (torch.cat(t) for t in zip(*want))
+                assert got.isfinite().all()
+                _compare(got[quiet], ref[quiet], spread[quiet], 2.0 ** -11)
+
+
+@pytest.mark.parametrize("scale,cap", [(1e-5, 1e-6), (1e-5, 30.0), (1e-9, 1e-9), (30.0, 1e-3), (2e4, 50.0), (1e-12, 1e3), (0.0, 1e4)])
+def test_soft_caps_and_scales_of_any_size(cuda_device, scale, cap):
+    """Also where the polynomial's coefficients leave fp32's range; masked scores on both sides of the window stay out."""
+    dev, page, n, D = cuda_device, 16, 500, 64
+    torch.manual_seed(7)
+    k, v = _pool(32, page, 2, D, torch.float16, dev)
+    table = torch.randperm(32, device=dev).view(1, 32).to(torch.int32)
+    q = torch.randn(150, 8, D, device=dev).to(torch.float16)
+    pos, j = torch.arange(n - 150, n, device=dev).view(-1, 1), torch.arange(n, device=dev).view(1, -1)
+    seen = (j <= pos) & ((j > pos - 100) | (j < 3))
+    ref, spread = _exact(q, _keys(k, table[0], n), _keys(v, table[0], n), scale, cap, seen)
+    out = tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 150], dev), _ints([n], dev), table, window=100, sinks=3, scale=scale, soft_cap=cap)
+    dec = tdist.gqa_fwd_window_decode(q[149:], k, v, _ints([n], dev), table, window=100, sinks=3, scale=scale, soft_cap=cap)
+    check_status()
+    _compare(out, ref, spread, 2.0 ** -11)
+    _compare(dec, ref[149:], spread[149:], 2.0 ** -11)

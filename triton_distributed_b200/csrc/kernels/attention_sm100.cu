@@ -30,6 +30,7 @@
 
 #include "../device/ptx.cuh"
 #include "../device/signal.cuh"
+#include "../device/soft_cap.cuh"
 #include "../include/tdist.h"
 #include "../runtime/host_common.h"
 
@@ -165,37 +166,44 @@ __device__ __forceinline__ void exponentials(const uint32_t (&s)[32], uint64_t s
     }
 }
 
-// out tanh(in s) where |in s| <= kCapSmall: tanh(z) / z as a polynomial in z^2, fitted to the least largest relative error, 7.3e-8. (The
-// exponential and the quotient it does without cost 16 clocks of the special-function unit per warp, twice what the softmax's own exponential
-// does.) The coefficients hold the powers of `in` up to the ninth: within fp32's range for `in` in [2^-12, 2^12], and other caps go without.
-constexpr float kCapSmall = 0.6f, kCapRange = 4096.f;
+// out tanh(in s) where |in s| <= kCapSmall, by the polynomial. (The exponential and the quotient it does without cost 16 clocks of the
+// special-function unit per warp, twice what the softmax's own exponential does.) The coefficients hold the powers of `in` up to the ninth (FOLDED):
+// within fp32's range for `in` in [2^-12, 2^12] and their product with `out` in [2^-23, 2^23]. Other caps multiply the score by `in` first, in a kernel of its own (for all caps: 7 ragged
+// prompts with heads of 64 284 us instead of 271; 2 x 1024 tokens, cap 1000, 170 us, by the way of large scores 475).
+__host__ __device__ inline bool foldable(float in, float scale) {
+    return in >= 1.f / 4096.f && in <= 4096.f && scale >= 1.f / 8388608.f && scale <= 8388608.f;
+}
+enum Capped { kUncapped, kFolded, kUnfolded };
 struct Cap {
-    float c[5];
+    float c[5], in;
 };
-__device__ __forceinline__ Cap cap_polynomial(float in, float out) {
-    const float u = in * in;
+template <bool FOLDED>
+__device__ __forceinline__ Cap cap_polynomial(float in, float scale) {   // scale: out * in
+    const float u = FOLDED ? in * in : 1.f;
     Cap k;
-    float f = out * in;
-    k.c[0] = 0.9999999403953552f * f;
-    k.c[1] = -0.33332309126853943f * (f *= u);
-    k.c[2] = 0.13310173153877258f * (f *= u);
-    k.c[3] = -0.05210148170590401f * (f *= u);
-    k.c[4] = 0.01547542680054903f * (f *= u);
+    k.in = FOLDED ? 1.f : fmaxf(in, 1e-37f);   // above zero for masked scores, which are -inf
+    float f = scale;
+    k.c[0] = kCapC0 * f;
+    k.c[1] = kCapC1 * (f *= u);
+    k.c[2] = kCapC2 * (f *= u);
+    k.c[3] = kCapC3 * (f *= u);
+    k.c[4] = kCapC4 * (f *= u);
     return k;
 }
+template <bool FOLDED>
 __device__ __forceinline__ float cap_score(float s, const Cap& k) {   // -inf stays -inf
-    const float u = s * s;
+    const float z = FOLDED ? s : s * k.in, u = z * z;
     return fmaf(fmaf(fmaf(fmaf(u, k.c[4], k.c[3]), u, k.c[2]), u, k.c[1]), u, k.c[0]) * s;
 }
 // P = 2^(cap(s) - m): as above. The maximum is known before the cap is taken, as the cap keeps the order, so that one pair's polynomial runs
 // under another's exponentials.
-template <typename T>
+template <typename T, bool FOLDED>
 __device__ __forceinline__ void capped_exponentials(const uint32_t (&s)[32], const Cap& k, uint64_t minus2, uint32_t (&pk)[16], uint64_t (&sum2)[2]) {
     auto both = [&](int i) { return pair(k.c[i], k.c[i]); };
-    const uint64_t c0 = both(0), c1 = both(1), c2 = both(2), c3 = both(3), c4 = both(4);
+    const uint64_t c0 = both(0), c1 = both(1), c2 = both(2), c3 = both(3), c4 = both(4), in2 = pair(k.in, k.in);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const uint64_t x = pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), u = mul2(x, x);
+        const uint64_t x = pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), z = FOLDED ? x : mul2(x, in2), u = mul2(z, z);
         float a, b;
         unpair(fma2(fma2(fma2(fma2(fma2(u, c4, c3), u, c2), u, c1), u, c0), x, minus2), a, b);
         a = exp2f(a);
@@ -285,11 +293,12 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
     return true;
 }
 
-// QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks. CAPPED: with a soft cap (a kernel of
+// QT: row tiles of the CTA. Two: a stream each, all blocks of keys. One: the streams take turns at the blocks. CAP: with a soft cap (a kernel of
 // its own: with both in one, 16384 tokens without a cap 1890 to 1940 us, by itself 1710 to 1820).
-template <typename T, int D, int QT, bool CAPPED>
+template <typename T, int D, int QT, Capped CAP>
 __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const __grid_constant__ Params p) {
     using S = Shape<D>;
+    constexpr bool CAPPED = CAP != kUncapped, FOLDED = CAP == kFolded;
     constexpr int KT = kKeys, NSTR = S::STREAMS, NST = stages<D, QT>(), CH = D / 8;
     static_assert(NST >= 2 && NST <= kMaxStages, "a tile is released only once the one after it has arrived");
     static_assert(QT == 1 || NSTR == 2, "two row tiles need two streams");
@@ -552,8 +561,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const float sl2 = CAPPED ? 1.f : p.scale_log2;
         // cap_out tanh(cap_in s): the cap in the exponent's domain; scores up to cap_small by a polynomial
         const float cap_out = p.soft_cap * 1.4426950408889634f, cap_in = CAPPED ? p.scale_log2 / cap_out : 0.f;
-        const float cap_small = cap_in >= 1.f / kCapRange && cap_in <= kCapRange ? kCapSmall / cap_in : -1.f;
-        const Cap cap = cap_polynomial(cap_in, cap_out);
+        const float cap_small = p.scale_log2 >= 1e-30f ? kCapSmall / cap_in : -1.f;   // (the coefficients must not be zero either)
+        const Cap cap = cap_polynomial<FOLDED>(cap_in, p.scale_log2);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + S::O_COL + stream * D;
         const int my_blocks = QT == 2 ? nt : (nt - stream + NSTR - 1) / NSTR;
@@ -578,8 +587,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                     for (int i = 0; i < 32; ++i) big[i & 3] = fmaxf(big[i & 3], fabsf(__uint_as_float(s[c][i])));
                 small = __all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= cap_small);
                 if (!small) {
-                    // 1 - 2 / (1 + exp(2 x / cap)); NaN stays NaN. Eight columns at a time through TMEM: unrolled, it would crowd the loop out of
-                    // the instruction cache.
+                    // Score by score, the small ones beside large ones too. Eight columns at a time through TMEM: unrolled, it would crowd the
+                    // loop out of the instruction cache.
 #pragma unroll 1
                     for (int c = 0; c < 64; c += 8) {
                         uint32_t e[8];
@@ -587,7 +596,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            e[i] = __float_as_uint(cap_out - __fdividef(2.f * cap_out, 1.f + exp2f(__uint_as_float(e[i]) * (2.f * 1.4426950408889634f * cap_in))));
+                            e[i] = __float_as_uint(p.soft_cap > kCapNear ? soft_cap(__uint_as_float(e[i]) * p.scale_log2, __uint_as_float(e[i]) * cap_in, cap_out)
+                                                                         : soft_cap_far(__uint_as_float(e[i]) * cap_in, cap_out));
                         tmem_st_32x8(at + c, e);
                     }
                     tmem_st_wait();
@@ -611,7 +621,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-            const float raw = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), top = small ? cap_score(raw, cap) : raw * sl2;
+            const float raw = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), top = small ? cap_score<FOLDED>(raw, cap) : raw * sl2;
             if (it == 0) {
                 m_ref = top;
             } else if (__any_sync(0xffffffffu, top > m_ref + kRaise)) {
@@ -637,7 +647,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
-                if (small) capped_exponentials<T>(s[c], cap, minus2, pk, sum2);
+                if (small) capped_exponentials<T, FOLDED>(s[c], cap, minus2, pk, sum2);
                 else exponentials<T>(s[c], scale2, minus2, pk, sum2);
                 tmem_st_32x16(at + 16 * c, pk);
             }
@@ -762,7 +772,7 @@ using tdist_host::fail;
 
 namespace {
 
-template <typename T, int D, int QT, bool CAPPED>
+template <typename T, int D, int QT, attention::Capped CAP>
 int launch_attention(const attention::Params& p, long long grid, cudaStream_t stream) {
     using S = attention::Shape<D>;
     constexpr int smem = S::AREA + 1024 + attention::kBars * 8 + 16;
@@ -774,15 +784,15 @@ int launch_attention(const attention::Params& p, long long grid, cudaStream_t st
     {
         std::lock_guard<std::mutex> guard(setup_lock);
         if (!done[dev]) {
-            TDIST_CUDA_OK(cudaFuncSetAttribute(attention::attention_kernel<T, D, QT, CAPPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            TDIST_CUDA_OK(cudaFuncSetAttribute(attention::attention_kernel<T, D, QT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             done[dev] = true;
         }
     }
-    TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_kernel<T, D, QT, CAPPED>, dim3(static_cast<unsigned>(grid)), S::THREADS, smem, stream, p));
+    TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_kernel<T, D, QT, CAP>, dim3(static_cast<unsigned>(grid)), S::THREADS, smem, stream, p));
     return 0;
 }
 
-template <typename T, int D, bool CAPPED>
+template <typename T, int D, attention::Capped CAP>
 int run_attention(const TdistAttentionArgs* a, attention::Params& p) {
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     const long long per = static_cast<long long>(a->row_tiles) * p.tile_tokens;
@@ -792,9 +802,9 @@ int run_attention(const TdistAttentionArgs* a, attention::Params& p) {
     if (grid > 0x7fffffffLL) return fail(TDIST_ELIMIT, "attention: tiles * Hkv * splits exceeds the grid limit");
     int rc;
     if constexpr (D <= 128)
-        rc = a->row_tiles == 2 ? launch_attention<T, D, 2, CAPPED>(p, grid, stream) : launch_attention<T, D, 1, CAPPED>(p, grid, stream);
+        rc = a->row_tiles == 2 ? launch_attention<T, D, 2, CAP>(p, grid, stream) : launch_attention<T, D, 1, CAP>(p, grid, stream);
     else
-        rc = launch_attention<T, D, 1, CAPPED>(p, grid, stream);
+        rc = launch_attention<T, D, 1, CAP>(p, grid, stream);
     if (rc != 0 || p.splits == 1 || a->out == nullptr) return rc;
     const long long rows = static_cast<long long>(p.tokens) * p.Hq, per_cta = 128 / (D / 4);
     TDIST_CUDA_OK(tdist_host::launch_pdl(attention::attention_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)), 128, 0,
@@ -802,15 +812,17 @@ int run_attention(const TdistAttentionArgs* a, attention::Params& p) {
     return 0;
 }
 
-template <typename T, bool CAPPED>
+template <typename T, attention::Capped CAP>
 int by_head_dim(const TdistAttentionArgs* a, attention::Params& p) {
-    if (a->head_dim == 64) return run_attention<T, 64, CAPPED>(a, p);
-    if (a->head_dim == 128) return run_attention<T, 128, CAPPED>(a, p);
-    return run_attention<T, 256, CAPPED>(a, p);
+    if (a->head_dim == 64) return run_attention<T, 64, CAP>(a, p);
+    if (a->head_dim == 128) return run_attention<T, 128, CAP>(a, p);
+    return run_attention<T, 256, CAP>(a, p);
 }
 template <typename T>
 int by_head_dim(const TdistAttentionArgs* a, attention::Params& p) {
-    return p.soft_cap > 0.f ? by_head_dim<T, true>(a, p) : by_head_dim<T, false>(a, p);
+    using namespace attention;
+    if (!(p.soft_cap > 0.f)) return by_head_dim<T, kUncapped>(a, p);
+    return foldable(p.scale_log2 / (p.soft_cap * 1.4426950408889634f), p.scale_log2) ? by_head_dim<T, kFolded>(a, p) : by_head_dim<T, kUnfolded>(a, p);
 }
 
 int attention_impl(const TdistAttentionArgs* a) {

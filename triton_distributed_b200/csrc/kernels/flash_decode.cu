@@ -36,6 +36,7 @@
 #include "../device/ll.cuh"
 #include "../device/ptx.cuh"
 #include "../device/signal.cuh"
+#include "../device/soft_cap.cuh"
 #include "../include/tdist.h"
 #include "../include/tdist_noalloc.h"
 #include "../runtime/host_common.h"
@@ -180,8 +181,8 @@ __device__ __forceinline__ int2 sequence_by_length(const int* kv_lens, int B, in
 }
 
 // EXT: the query sees a window and the first keys only (logical key i is token i below `first`, token i + gap from there on), the
-// merge takes in partial results of keys that another kernel read, and the soft cap's tanh is taken from an exponential and a division (good to
-// 2^-23 of the cap, where the hardware's is to 2^-11). A template argument, so that the plain decode keeps its registers.
+// merge takes in partial results of keys that another kernel read, and the soft cap is good to 2^-22 of the cap, or of the score where the cap is
+// large (the plain decode takes the hardware's tanh, good to 2^-11 of the score). A template argument, so that the plain decode keeps its registers.
 template <typename T, int D, int NH, bool EXT>
 __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_decode_kernel(const DecodeParams p) {
     constexpr int CH = D / 8;                      // 16-byte chunks per row
@@ -317,6 +318,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
             m_use[h][r] = l_run[h][r] = 0.f;
         }
     const float sl2 = p.scale * 1.4426950408889634f;
+    const bool near_cap = p.soft_cap > 0.f && p.soft_cap <= kCapNear, far_cap = p.soft_cap > kCapNear;   // EXT
+    const float cap_in = far_cap ? p.scale / p.soft_cap : 0.f, unit = far_cap ? 1.f : sl2;
     // ldmatrix addresses inside a block: row, and the swizzled chunk with the lane's part of its number
     const int krow = (lane & 7) + ((lane >> 3) & 1) * 8;
     const uint32_t k_at = static_cast<uint32_t>(krow * (D * 2)) + static_cast<uint32_t>(((lane >> 4) ^ (krow & 7)) << 4);
@@ -349,15 +352,21 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(D)) flash_d
         }
         // scale, soft cap, mask, online softmax
         bool higher = false;
+        if (EXT && far_cap) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[h][e] = soft_cap(s[h][e] * sl2, s[h][e] * cap_in, p.soft_cap * 1.4426950408889634f);
+        }
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float v = s[h][e];
-                if (EXT && p.soft_cap > 0.f)
+                if (EXT && near_cap)
                     v = p.soft_cap * 1.4426950408889634f * (1.f - __fdividef(2.f, 1.f + exp2f(v * (2.f * sl2 / p.soft_cap))));
-                else if (p.soft_cap > 0.f) v = p.soft_cap * tanhf(v * p.scale / p.soft_cap) * 1.4426950408889634f;
-                else v *= sl2;
+                else if (!EXT && p.soft_cap > 0.f) v = p.soft_cap * tanhf(v * p.scale / p.soft_cap) * 1.4426950408889634f;
+                else v *= EXT ? unit : sl2;
                 if (tok0 + kTok > kv_len) v = tok0 + (lane >> 2) + (e >> 1) * 8 < kv_len ? v : -CUDART_INF_F;
                 s[h][e] = v;
                 higher |= v > m_run[h][e & 1];
