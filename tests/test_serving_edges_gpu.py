@@ -1,5 +1,5 @@
 """Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities,
-tokens of no sequence, large soft caps."""
+tokens of no sequence, large soft caps, tables without a column."""
 import pytest
 import torch
 
@@ -278,3 +278,22 @@ def test_soft_caps_and_scales_of_any_size(cuda_device, scale, cap):
     check_status()
     _compare(out, ref, spread, 2.0 ** -11)
     _compare(dec, ref[149:], spread[149:], 2.0 ** -11)
+
+
+def test_tables_without_a_column(cuda_device):
+    """No own keys yet: the prefix alone. No keys at all: zeros."""
+    dev = cuda_device
+    torch.manual_seed(1)
+    k, v = _pool(20, 16, 2, 128, torch.bfloat16, dev)
+    q = torch.randn(3, 8, 128, device=dev).to(torch.bfloat16)
+    pre, none, lens = torch.randperm(20, device=dev).to(torch.int32), torch.zeros((3, 0), dtype=torch.int32, device=dev), _ints([0, 0, 0], dev)
+    got = tdist.gqa_fwd_shared_prefix_decode(q, k, v, 300, pre, lens, none)
+    want = tdist.gqa_fwd_shared_prefix_decode(q, k, v, 300, pre, lens, pre[:3].view(3, 1))
+    check_status()
+    ref, spread = _exact(q, _keys(k, pre, 300), _keys(v, pre, 300), 128 ** -0.5)
+    _compare(got, ref, spread, 2.0 ** -8)
+    torch.testing.assert_close(got.float(), want.float(), atol=2.0 ** -8, rtol=2.0 ** -8)
+    for out in (tdist.gqa_fwd_shared_prefix_decode(q, k, v, 0, pre[:0], lens, none), tdist.gqa_fwd_window_decode(q, k, v, lens, none, window=9),
+                tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 1, 2, 3], dev), lens, none)):
+        check_status()
+        assert out.shape == q.shape and not out.any()

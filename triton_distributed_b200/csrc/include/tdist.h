@@ -412,8 +412,8 @@ typedef struct TdistDecodeArgs {
      * (pages that hold no such key are not read, nor are their table entries). With window > 0 (0x7fffffff: no limit) the
      * result may also take in partial results over other keys: prior_o fp32 [priors][B * Hq][D] (normalised) and
      * prior_lse fp32 [priors][B * Hq] (natural log, -inf: no keys).
-     * blocks: pages of the cache, needed with window > 0. Lengths are then cut to what the table has room for, and keys of a page that the cache
-     * does not have read as zeros. */
+     * blocks: pages of the cache, needed with window > 0. Lengths are then cut to what the table has room for (max_blocks may be 0, block_table
+     * NULL: no keys), and keys of a page that the cache does not have read as zeros. */
     int window, sinks, priors, blocks;
     const void* prior_o;
     const void* prior_lse;

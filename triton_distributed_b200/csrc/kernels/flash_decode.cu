@@ -800,7 +800,9 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
     if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return fail(TDIST_EINVAL, "decode: head_dim must be 64, 128 or 256");
     if (a->stride_token % 8 || a->stride_block % 8 || a->stride_head % 8) return fail(TDIST_EINVAL, "decode: cache strides must be multiples of 8 elements");
     if (a->mode < 0 || a->mode > 2) return fail(TDIST_EINVAL, "decode: bad mode");
-    if (a->page_size < 1 || a->max_blocks < 1) return fail(TDIST_EINVAL, "decode: page_size and max_blocks must be at least 1");
+    // with a window a table without columns is one without keys: the result is the earlier partials', or zeros
+    const bool no_table = a->window > 0 && a->max_blocks == 0;
+    if (a->page_size < 1 || (a->max_blocks < 1 && !no_table)) return fail(TDIST_EINVAL, "decode: page_size and max_blocks must be at least 1");
     if (static_cast<long long>(a->B) * a->Hkv * a->splits > 0x7fffffffLL) return fail(TDIST_ELIMIT, "decode: B * Hkv * splits exceeds the grid limit");
     DecodeParams p;
     memset(&p, 0, sizeof(p));
@@ -852,7 +854,7 @@ static int flash_decode_impl(const TdistDecodeArgs* a) {
     p.wctx.timeout_ns = a->timeout_ns;
     p.wctx.kernel_id = kKernelDecode;
     p.wctx.rank = a->rank;
-    if (!p.q || !p.k_cache || !p.v_cache || !p.block_table || !p.kv_lens || !p.partial || !p.counters || !p.out)
+    if (!p.q || !p.k_cache || !p.v_cache || (!p.block_table && !no_table) || !p.kv_lens || !p.partial || !p.counters || !p.out)
         return fail(TDIST_EINVAL, "decode: null pointer");
     // the widths the kernel loads and stores with: K and V by 16 bytes, q by 4, the result by 8 (O || LSE and the exchange's by 4)
     auto misaligned = [](const void* ptr, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes != 0; };

@@ -268,7 +268,7 @@ def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, 
         if q.device.type != "cuda":
             return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
         T, Hq, D = q.shape
-        if T == 0 or B == 0:
+        if T == 0 or B == 0 or block_table.shape[1] == 0:
             return _output(out, q).zero_()
         most = NO_WINDOW if window is None else window
         tile = 128 // (Hq // k_cache.shape[2])
