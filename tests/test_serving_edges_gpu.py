@@ -1,5 +1,5 @@
 """Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities,
-tokens of no sequence, large soft caps, tables without a column."""
+tokens of no sequence, large soft caps, tables without a column, too many heads."""
 import pytest
 import torch
 
@@ -297,3 +297,21 @@ def test_tables_without_a_column(cuda_device):
                 tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 1, 2, 3], dev), lens, none)):
         check_status()
         assert out.shape == q.shape and not out.any()
+
+
+def test_refusals_of_many_heads_per_kv_head(cuda_device):
+    dev = cuda_device
+    k, v = _pool(8, 16, 1, 128, torch.bfloat16, dev)
+    table, lens = torch.zeros(2, 4, dtype=torch.int32, device=dev), _ints([1, 1], dev)
+    q = torch.zeros(2, 129, 128, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(ValueError, match="128 query heads"):
+        tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 1, 2], dev), lens, table)
+    with pytest.raises(ValueError, match="16 query heads"):
+        tdist.gqa_fwd_shared_prefix_decode(q, k, v, 5, table[0], lens, table)
+    with pytest.raises(ValueError, match="16 query heads"):
+        tdist.gqa_fwd_window_decode(q, k, v, lens, table)
+    with pytest.raises(ValueError, match="multiple of the kv heads"):
+        tdist.gqa_fwd_window_decode(q, k[:, :, :0], v[:, :, :0], lens, table)
+    with pytest.raises(ValueError, match="multiple of the kv heads"):
+        tdist.gqa_fwd_window_decode(q[:, :0], k, v, lens, table)
+    assert tdist.gqa_fwd_window_prefill(q[:, :128], k, v, _ints([0, 1, 2], dev), lens, table).shape == (2, 128, 128)

@@ -84,12 +84,13 @@ def ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_len
     return out
 
 
-def _check(q, k_cache, v_cache, window, sinks, soft_cap, ints):
+def _check(q, k_cache, v_cache, window, sinks, soft_cap, ints, most_heads):
+    """``most_heads``: query heads per kv head that the operator's kernels take."""
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError("q must be [tokens, Hq, D], the caches [blocks, page, Hkv, D]")
     if k_cache.shape != v_cache.shape or k_cache.shape[3] != q.shape[2]:
         raise ValueError("k and v caches need the same shape, with head_dim == q's")
-    if q.shape[1] % k_cache.shape[2]:
+    if k_cache.shape[2] < 1 or q.shape[1] < 1 or q.shape[1] % k_cache.shape[2]:
         raise ValueError("the query heads must be a multiple of the kv heads")
     if window is not None and window < 1:
         raise ValueError("the window must be at least 1 (None: no limit)")
@@ -108,6 +109,8 @@ def _check(q, k_cache, v_cache, window, sinks, soft_cap, ints):
         return
     if q.dtype not in _DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise TypeError("q, k_cache and v_cache must share one of bf16 / fp16")
+    if q.shape[1] > most_heads * k_cache.shape[2]:
+        raise ValueError(f"at most {most_heads} query heads per kv head")
     if q.shape[2] not in (64, 128, 256):
         raise ValueError("head_dim must be 64, 128 or 256")
     if k_cache.stride(3) != 1 or v_cache.stride() != k_cache.stride() or q.stride(2) != 1:
@@ -210,8 +213,6 @@ def _decode_args(q, k_cache, block_table, window, sinks, scale, soft_cap, kv_spl
         raise ValueError("q must be contiguous")
     B, Hq, D = q.shape
     blocks, page, Hkv, _ = k_cache.shape
-    if Hq // Hkv > 16:
-        raise ValueError("decode takes at most 16 query heads per kv head")
     a = _lib.DecodeArgs()
     a.B, a.Hq, a.Hkv, a.head_dim, a.page_size = B, Hq, Hkv, D, page
     a.max_blocks = block_table.shape[1]
@@ -238,7 +239,7 @@ def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Opt
     args = _PLANS.get(key)
     if args is None:
         B = q.shape[0]
-        _check(q, k_cache, v_cache, window, sinks, soft_cap, (("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
+        _check(q, k_cache, v_cache, window, sinks, soft_cap, (("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))), 16)
         factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         if q.device.type != "cuda":
             return ref_window_attn(q, k_cache, v_cache, torch.arange(B + 1), kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
@@ -255,15 +256,16 @@ def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Opt
 @nvtx_range("tdist.gqa_fwd_window_prefill")
 def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, window: Optional[int] = None, sinks: int = 0,
                            scale=None, soft_cap: float = 0.0, out: Optional[torch.Tensor] = None, kv_split: int = -1):
-    """Attention of a ragged batch of query tokens, the last ones of their sequences. Returns ``[T, Hq, D]`` in q's dtype. q may
-    be a view (part of a fused projection) with strides that are multiples of 8 elements; nothing is read back to the host."""
+    """Attention of a ragged batch of query tokens, the last ones of their sequences. Returns ``[T, Hq, D]`` in q's dtype; at most 128
+    query heads per kv head. q may be a view (part of a fused projection) with strides that are multiples of 8 elements; nothing is read
+    back to the host."""
     window, sinks, scale, soft_cap = _settings(window, sinks, scale, soft_cap)
     key = (gqa_fwd_window_prefill, _layout(q, k_cache, v_cache, q_starts, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
     args = _PLANS.get(key)
     if args is None:
         B = kv_lens.shape[0]
         _check(q, k_cache, v_cache, window, sinks, soft_cap,
-               (("kv_lens", kv_lens, (B,)), ("q_starts", q_starts, (B + 1,)), ("block_table", block_table, (B, None))))
+               (("kv_lens", kv_lens, (B,)), ("q_starts", q_starts, (B + 1,)), ("block_table", block_table, (B, None))), 128)
         factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         if q.device.type != "cuda":
             return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
@@ -303,7 +305,8 @@ def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, 
     if plan is None:
         B = q.shape[0]
         _check(q, k_cache, v_cache, None, 0, soft_cap,
-               (("prefix_len", prefix_len, (1,)), ("prefix_table", prefix_table, (None,)), ("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))))
+               (("prefix_len", prefix_len, (1,)), ("prefix_table", prefix_table, (None,)), ("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))),
+               16)
         factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         if q.device.type != "cuda":
             return ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, factor, soft_cap).to(q.dtype)
