@@ -1,8 +1,11 @@
 """What the serving operators refuse before any launch, and their CPU statements on infinities, NaN and empty batches."""
 import ctypes as C
+import math
 
 import pytest
+import torch
 
+import triton_distributed_b200 as tdist
 from triton_distributed_b200 import _lib
 
 
@@ -39,3 +42,19 @@ def test_decode_refuses_misaligned_earlier_partials():
 def test_windowed_decode_needs_the_number_of_pages():
     code = _lib.lib().tdist_flash_decode(C.byref(_decode_args(window=64, sinks=4, blocks=0)))
     assert code != 0 and b"blocks" in _lib.lib().tdist_last_error()
+
+
+@pytest.mark.parametrize("tokens", [4, 10])   # 10: the first two lie before the first key
+def test_what_is_no_number_shows_beside_rows_that_see_nothing(tokens):
+    torch.manual_seed(1)
+    k, v, q = torch.randn(4, 4, 1, 8), torch.randn(4, 4, 1, 8), torch.randn(tokens, 2, 8)
+    k[1, 1] = math.nan   # key 5 of 8: the last three queries see it
+    out = tdist.gqa_fwd_window_prefill(q, k, v, torch.tensor([0, tokens]), torch.tensor([8]), torch.arange(4).view(1, 4))
+    assert out[-3:].isnan().all() and not out[:-3].isnan().any()
+    assert not out[:-8].any()
+
+
+def test_a_query_whose_scores_are_all_minus_infinity_gives_zeros():
+    k, v, q = torch.zeros(1, 4, 1, 8), torch.randn(1, 4, 1, 8), torch.ones(1, 2, 8)
+    k[..., 0] = -math.inf
+    assert not tdist.gqa_fwd_window_decode(q, k, v, torch.tensor([3]), torch.zeros(1, 1, dtype=torch.int32)).any()

@@ -315,3 +315,23 @@ def test_refusals_of_many_heads_per_kv_head(cuda_device):
     with pytest.raises(ValueError, match="multiple of the kv heads"):
         tdist.gqa_fwd_window_decode(q[:, :0], k, v, lens, table)
     assert tdist.gqa_fwd_window_prefill(q[:, :128], k, v, _ints([0, 1, 2], dev), lens, table).shape == (2, 128, 128)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("split", [1, 4])
+def test_prefill_passes_on_what_is_no_number_and_what_weighs_nothing(cuda_device, D, split):
+    """A NaN key shows in the rows that see it and leaves those of other sequences alone; scores that are all -inf are like no keys."""
+    dev = cuda_device
+    torch.manual_seed(D)
+    k, v = _pool(60, 16, 2, D, torch.bfloat16, dev)
+    table = torch.randperm(60, device=dev).view(3, 20).to(torch.int32)
+    q = torch.randn(300, 8, D, device=dev).to(torch.bfloat16).abs() + 0.1
+    k[int(table[1, 19]), 15, 0, 0] = float("nan")         # sequence 1, its last key, kv head 0
+    k[table[2].long(), :, 1, 0] = float("-inf")           # sequence 2, kv head 1
+    out = tdist.gqa_fwd_window_prefill(q, k, v, _ints([0, 100, 200, 300], dev), _ints([320, 320, 320], dev), table, kv_split=split)
+    check_status()
+    assert out[199, :4].isnan().all() and not out[:100].isnan().any() and not out[100:200, 4:].isnan().any()
+    assert not out[200:, 4:].any() and out[200:, :4].isfinite().all() and out[200:, :4].any()
+    dec = tdist.gqa_fwd_window_decode(q[199:300:50].contiguous(), k, v, _ints([320] * 3, dev), table, kv_split=split)
+    check_status()
+    assert dec[1, :4].isnan().all() and not dec[2, 4:].any() and not dec[0].isnan().any()

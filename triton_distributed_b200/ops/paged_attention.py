@@ -9,7 +9,7 @@ a ragged batch, and decode of a batch whose sequences share a prefix.
 * ``gqa_fwd_shared_prefix_decode(q[B,Hq,D], k_cache, v_cache, prefix_len[1], prefix_table[max_blocks], kv_lens[B],
   block_table, scale, soft_cap) -> [B,Hq,D]``: the softmax runs over the keys of the prefix, read once for all, and the sequence's own
 
-``window=None`` is no limit: plain causal attention. A query that sees no key gives zeros, and so does a token that ``q_starts`` (which must
+``window=None`` is no limit: plain causal attention. A query that sees no key (or none whose score is above -inf) gives zeros, and so does a token that ``q_starts`` (which must
 not decrease) gives to no sequence, as in a batch padded for a captured graph. Pages without a visible key are not
 read, nor are their table entries (a server may have given them back). What lies in a page behind a sequence's last key may be
 anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum. On a GPU lengths are
@@ -37,14 +37,14 @@ NO_WINDOW = 0x7FFFFFFF
 
 
 def _attend(q, k, v, seen, scale, soft_cap):
-    """fp32 attention of q [n, Hq, D] over k, v [keys, Hkv, D] with a mask [n, keys]; zeros where a row sees nothing."""
+    """fp32 attention of q [n, Hq, D] over k, v [keys, Hkv, D] with a mask [n, keys]; zeros where a row sees nothing above -inf."""
     n, Hq, D = q.shape
     Hkv = k.shape[1]
     s = torch.einsum("nhgd,khd->hgnk", q.float().view(n, Hkv, Hq // Hkv, D), k.float()) * scale
     if soft_cap > 0:
         s = soft_cap * torch.tanh(s / soft_cap)
     s = s.masked_fill(~seen, float("-inf"))
-    p = torch.nan_to_num(torch.softmax(s, dim=-1)) if not bool(seen.any(-1).all()) else torch.softmax(s, dim=-1)
+    p = torch.softmax(s, dim=-1).masked_fill((s == float("-inf")).all(-1, keepdim=True), 0.0)
     return torch.einsum("hgnk,khd->nhgd", p, v.float()).reshape(n, Hq, D)
 
 
