@@ -58,3 +58,16 @@ def test_a_query_whose_scores_are_all_minus_infinity_gives_zeros():
     k, v, q = torch.zeros(1, 4, 1, 8), torch.randn(1, 4, 1, 8), torch.ones(1, 2, 8)
     k[..., 0] = -math.inf
     assert not tdist.gqa_fwd_window_decode(q, k, v, torch.tensor([3]), torch.zeros(1, 1, dtype=torch.int32)).any()
+
+
+def test_results_go_into_a_given_tensor_on_the_cpu_too():
+    torch.manual_seed(2)
+    k, v, q = torch.randn(6, 4, 2, 8), torch.randn(6, 4, 2, 8), torch.randn(2, 4, 8)
+    table, lens, pre = torch.tensor([[0, 1], [2, 3]]), torch.tensor([7, 5]), torch.tensor([4, 5])
+    for call in (lambda **o: tdist.gqa_fwd_window_decode(q, k, v, lens, table, window=3, **o),
+                 lambda **o: tdist.gqa_fwd_window_prefill(q, k, v, torch.arange(3), lens, table, **o),
+                 lambda **o: tdist.gqa_fwd_shared_prefix_decode(q, k, v, 6, pre, lens, table, **o)):
+        out = torch.full_like(q, math.nan)
+        assert call(out=out) is out and torch.equal(out, call())
+        with pytest.raises(ValueError):
+            call(out=torch.empty(2, 4, 9))

@@ -125,6 +125,11 @@ def _output(out, q):
     return out
 
 
+def _stated(ref, q, out):
+    """What a plain statement gave, as the result of the call."""
+    return ref.to(q.dtype) if out is None else _output(out, q).copy_(ref)
+
+
 def _int32(t):
     return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
 
@@ -242,7 +247,7 @@ def gqa_fwd_window_decode(q, k_cache, v_cache, kv_lens, block_table, window: Opt
         _check(q, k_cache, v_cache, window, sinks, soft_cap, (("kv_lens", kv_lens, (B,)), ("block_table", block_table, (B, None))), 16)
         factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         if q.device.type != "cuda":
-            return ref_window_attn(q, k_cache, v_cache, torch.arange(B + 1), kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
+            return _stated(ref_window_attn(q, k_cache, v_cache, torch.arange(B + 1), kv_lens, block_table, window, sinks, factor, soft_cap), q, out)
         if B == 0:
             return _output(out, q)
         args = _remember(key, _decode_args(q, k_cache, block_table, NO_WINDOW if window is None else window, sinks, factor,
@@ -268,7 +273,7 @@ def gqa_fwd_window_prefill(q, k_cache, v_cache, q_starts, kv_lens, block_table, 
                (("kv_lens", kv_lens, (B,)), ("q_starts", q_starts, (B + 1,)), ("block_table", block_table, (B, None))), 128)
         factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         if q.device.type != "cuda":
-            return ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, factor, soft_cap).to(q.dtype)
+            return _stated(ref_window_attn(q, k_cache, v_cache, q_starts, kv_lens, block_table, window, sinks, factor, soft_cap), q, out)
         T, Hq, D = q.shape
         if T == 0 or B == 0 or block_table.shape[1] == 0:
             return _output(out, q).zero_()
@@ -309,7 +314,7 @@ def gqa_fwd_shared_prefix_decode(q, k_cache, v_cache, prefix_len, prefix_table, 
                16)
         factor = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         if q.device.type != "cuda":
-            return ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, factor, soft_cap).to(q.dtype)
+            return _stated(ref_shared_prefix_attn(q, k_cache, v_cache, prefix_len, prefix_table, kv_lens, block_table, factor, soft_cap), q, out)
         _, Hq, D = q.shape
         if B == 0:
             return _output(out, q)
