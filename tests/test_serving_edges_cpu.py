@@ -71,3 +71,18 @@ def test_results_go_into_a_given_tensor_on_the_cpu_too():
         assert call(out=out) is out and torch.equal(out, call())
         with pytest.raises(ValueError):
             call(out=torch.empty(2, 4, 9))
+
+
+@pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (0, 0.5, 0.0), (700, 0.9, 0.0), (0, 0.3, 0.5)])
+def test_an_infinite_temperature_draws_evenly_from_what_is_there(k, p, m):
+    torch.manual_seed(3)
+    x = torch.randn(9, 1001)
+    x[:, ::2] = -math.inf      # 500 of 1001 are left
+    x[:, 5::10] = math.nan     # and 400 of these
+    got = tdist.sample_tokens(x, torch.linspace(0, 0.999, 9), math.inf, k, p, m)
+    kept = math.ceil(float(torch.tensor(p)) * 400)   # top_p is fp32; top_k lets all 400 through
+    assert x.gather(1, got.tokens.long().view(-1, 1)).isfinite().all()
+    torch.testing.assert_close(got.logprobs, torch.full((9,), -math.log(kept)), atol=1e-6, rtol=1e-6)
+    order = torch.sort(x.nan_to_num(nan=-math.inf, neginf=-math.inf), dim=1, descending=True, stable=True).indices[:, :kept].sort(1).values
+    at = torch.floor(torch.linspace(0, 0.999, 9).double() * kept * 2.0 ** 31).div(2.0 ** 31).floor().long()
+    assert torch.equal(got.tokens.long(), order.gather(1, at.view(-1, 1)).view(-1))

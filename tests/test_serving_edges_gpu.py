@@ -1,5 +1,7 @@
 """Serving operators where they can go wrong: calls interleaved on one stream, lengths and pages beyond the tensors, NaN and infinities,
 tokens of no sequence, large soft caps, tables without a column, too many heads."""
+import math
+
 import pytest
 import torch
 
@@ -335,3 +337,19 @@ def test_prefill_passes_on_what_is_no_number_and_what_weighs_nothing(cuda_device
     dec = tdist.gqa_fwd_window_decode(q[199:300:50].contiguous(), k, v, _ints([320] * 3, dev), table, kv_split=split)
     check_status()
     assert dec[1, :4].isnan().all() and not dec[2, 4:].any() and not dec[0].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_infinite_temperature_on_a_gpu(cuda_device, dtype):
+    """All finite logits weigh alike, those of -inf or NaN nothing; the same tokens as the statement's."""
+    from triton_distributed_b200.ops.sampling import ref_sample_tokens
+    torch.manual_seed(3)
+    x = torch.randn(9, 30001, device=cuda_device).to(dtype)
+    x[:, ::2] = -math.inf
+    x[:, 5::10] = math.nan
+    u = torch.linspace(0, 0.999, 9, device=cuda_device)
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.5, 0.0), (700, 0.9, 0.0), (0, 0.3, 0.5)):
+        got, want = tdist.sample_tokens(x, u, math.inf, k, p, m), ref_sample_tokens(x, u, math.inf, k, p, m)
+        check_status()
+        assert torch.equal(got.tokens, want.tokens) and x.gather(1, got.tokens.long().view(-1, 1)).isfinite().all()
+        torch.testing.assert_close(got.logprobs, want.logprobs, atol=1e-5, rtol=1e-5)
