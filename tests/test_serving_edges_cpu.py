@@ -86,3 +86,15 @@ def test_an_infinite_temperature_draws_evenly_from_what_is_there(k, p, m):
     order = torch.sort(x.nan_to_num(nan=-math.inf, neginf=-math.inf), dim=1, descending=True, stable=True).indices[:, :kept].sort(1).values
     at = torch.floor(torch.linspace(0, 0.999, 9).double() * kept * 2.0 ** 31).div(2.0 ** 31).floor().long()
     assert torch.equal(got.tokens.long(), order.gather(1, at.view(-1, 1)).view(-1))
+
+
+@pytest.mark.parametrize("p", [1.0, 0.5])
+def test_infinite_logits_at_an_infinite_temperature(p):
+    """They weigh alike and the finite ones nothing, as at any temperature."""
+    x = torch.randn(4, 31)
+    x[:, 3::9] = math.inf   # 3, 12, 21, 30
+    u = torch.tensor([0.0, 0.3, 0.6, 0.99])
+    for t in (1.0, math.inf):
+        got = tdist.sample_tokens(x, u, t, top_p=p)
+        assert got.tokens.tolist() == ([3, 12, 21, 30] if p == 1.0 else [3, 3, 12, 12])
+        torch.testing.assert_close(got.logprobs, torch.full((4,), -math.log(4 * p)))

@@ -47,7 +47,8 @@ def ref_sample_tokens(logits, u, temperature: Setting = 1.0, top_k: Setting = 0,
     greedy = ~(t > 0)
     inv = 1.0 / torch.where(greedy, 1.0, t)
     top = x.amax(1, keepdim=True)
-    y = torch.where(x == top, 0.0, torch.where(x == float("-inf"), x, (x - top) * inv))   # (at an infinite temperature -inf x 0 is NaN)
+    below = x - top
+    y = torch.where(x == top, 0.0, torch.where(below == float("-inf"), below, below * inv))   # (at an infinite temperature -inf x 0 is NaN)
     w = torch.round(torch.exp(y) * ONE).long()
     order = torch.sort(x, dim=1, descending=True, stable=True).indices
     ws = w.gather(1, order)
