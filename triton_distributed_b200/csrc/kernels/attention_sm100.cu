@@ -16,9 +16,14 @@
 // whole block is seen; by 16-byte cp.async else (pages of any size; rows that nobody sees are not read and become zeros).
 // Few rows over many keys are split along the keys; the partial results meet in attention_merge_kernel, or in the decode kernel.
 //
-// P is rounded to the inputs' 16 bits (relative 2^-8 or 2^-11), S, O, maximum and sum are fp32. The maximum that is subtracted
-// is raised only when it has grown by more than 2^8 (kRaise): P then lies below 2^8, whose relative rounding is the same, and O
-// is read, scaled and written back a few times per row instead of once per block.
+// P is rounded to the inputs' 16 bits (relative 2^-8; 2^-11 in fp16, whose numbers end at 2^-24: smaller P are multiples of that), S, O,
+// maximum and sum are fp32. The maximum that is subtracted is raised only when it has grown by more than 2^8 (kRaise): O is read, scaled and
+// written back a few times per row instead of once per block, and the largest P, which is 1 otherwise, is rounded like the others. Raised at once /
+// by this rule: 2048 tokens 186 / 160 us, error against 64 bits 2.3e-3 both; 16384 tokens 2347 / 1921; ragged prompts in fp16 315 / 271, 2.5e-4 /
+// 2.6e-4; prefix of 32768 keys 95 / 88, 2.3e-3 / 2.4e-3.
+// A product that lies below the accumulator's 24 bits is cut by the tensor cores, as in any sum in fp32, and fp16's P below 2^-25 are zero: beside
+// one key that weighs 2^24 times as much as each of n others in its chain, up to n 2^-25 of the result is lost (131072 keys alike, 2^-25 each:
+// 3.9e-3; a P lifted by 2^7 to keep fp16's small ones was no better and lost more to the cut, 2.0e-3 where it is 0 without, at 2^-20).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -168,8 +173,8 @@ __device__ __forceinline__ void exponentials(const uint32_t (&s)[32], uint64_t s
 
 // out tanh(in s) where |in s| <= kCapSmall, by the polynomial. (The exponential and the quotient it does without cost 16 clocks of the
 // special-function unit per warp, twice what the softmax's own exponential does.) The coefficients hold the powers of `in` up to the ninth (FOLDED):
-// within fp32's range for `in` in [2^-12, 2^12] and their product with `out` in [2^-23, 2^23]. Other caps multiply the score by `in` first, in a kernel of its own (for all caps: 7 ragged
-// prompts with heads of 64 284 us instead of 271; 2 x 1024 tokens, cap 1000, 170 us, by the way of large scores 475).
+// within fp32's range for `in` in [2^-12, 2^12] and `in` x `out` in [2^-23, 2^23]. Other caps multiply the score by `in` first, in a kernel of its
+// own (for all caps: 7 ragged prompts with heads of 64 284 us instead of 271; 2 x 1024 tokens, cap 1000, 170 us, by the way of large scores 475).
 __host__ __device__ inline bool foldable(float in, float scale) {
     return in >= 1.f / 4096.f && in <= 4096.f && scale >= 1.f / 8388608.f && scale <= 8388608.f;
 }
@@ -371,8 +376,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) attention_kernel(const _
         const T* vl = static_cast<const T*>(p.v_cache) + static_cast<size_t>(w.kvh) * p.stride_head + lch * 8;
         const uint32_t lane_dst = static_cast<uint32_t>((lch >> 3) * (KT * 128));
         const int items = 2 * nt;
-        // TMA: box i of a block is 64-column i % CHUNKS of its rows [i / CHUNKS * box_rows, + box_rows); the loaders take them in turn
-        const int box_rows = p.box_rows, boxes = box_rows > 0 ? KT / box_rows * S::CHUNKS : 0;
+        // TMA: the loaders take a block's groups of box_rows rows in turn (the first one all of a block in one page), a box per 64 columns of a group
+        const int box_rows = p.box_rows;
         auto block_of = [&](int n, bool& is_k) {
             const int m = n - look, pairs = 2 * (nt - look);
             is_k = n < look || (m < pairs && (m & 1));

@@ -9,7 +9,7 @@
 //   logprob = (x[token] - max) / temperature - log(W / 2^31),  log_norm = max / temperature + log(W / 2^31)
 //
 // Temperature 0, below or NaN: the largest logit (lowest index). A NaN logit counts as -inf; a row without anything above -inf gives token -1.
-// Weights below 2^-32 of the largest are zero: tokens that no 24-bit random number could have drawn.
+// Weights below 2^-32 of the largest are zero, at most V 2^-32 of the largest in all (200000 tokens: 4.7e-5).
 //
 // A row belongs to a cluster of 1 to 8 CTAs. Each reads its part from HBM once, into shared memory, and goes over it there: the maximum;
 // for top-k a histogram of counts over bins that are linear in x (they spread logits evenly where bins of the bits would heap them on a few
@@ -47,7 +47,10 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kGroups = kBins / 16;
 constexpr int kCand = 1024;
-constexpr int kList = 256;                // elements of a warp's run that can matter; more: the whole run is gone over
+// Elements of a warp's run that can matter; more: the whole run is gone over, and the pass that looked for them is lost. Two CTAs' shared memory
+// leaves room for less than twice as many. It holds what top-k leaves, and top-p's where the runs are short or steep; 128256 logits of deviation 2.5 in 64 runs leave 732
+// at temperature 1, p 0.9. Without lists / with them: 1 x 32000 15.1 / 15.2 us, 64 x 128256 63.1 / 61.8, 256 x 100003 176 / 163.
+constexpr int kList = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSlice = 65536;          // elements of a CTA: a bin's sums of 16-bit halves of the weights stay below 2^32
 constexpr int kMaxSliceBytes = 180 * 1024;

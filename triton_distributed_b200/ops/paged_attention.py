@@ -9,11 +9,12 @@ a ragged batch, and decode of a batch whose sequences share a prefix.
 * ``gqa_fwd_shared_prefix_decode(q[B,Hq,D], k_cache, v_cache, prefix_len[1], prefix_table[max_blocks], kv_lens[B],
   block_table, scale, soft_cap) -> [B,Hq,D]``: the softmax runs over the keys of the prefix, read once for all, and the sequence's own
 
-``window=None`` is no limit: plain causal attention. A query that sees no key (or none whose score is above -inf) gives zeros, and so does a token that ``q_starts`` (which must
-not decrease) gives to no sequence, as in a batch padded for a captured graph. Pages without a visible key are not
-read, nor are their table entries (a server may have given them back). What lies in a page behind a sequence's last key may be
-anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum. On a GPU lengths are
-cut to what the table has room for, and a page that the cache does not have reads as zeros: nothing outside the tensors is touched.
+``window=None`` is no limit: plain causal attention. A query that sees no key (or none whose score is above -inf) gives zeros, and so does
+a token that ``q_starts`` (which must not decrease) gives to no sequence, as in a batch padded for a captured graph. Pages without a
+visible key are not read, nor are their table entries (a server may have given them back). What lies in a page behind a sequence's last
+key may be anything; keys that only some of a sequence's queries see have to be finite, as 0 x NaN is NaN in every query's sum. A NaN that
+a query sees makes its result NaN. On a GPU lengths are cut to what the table has room for, and a page that the cache does not have reads
+as zeros: nothing outside the tensors is touched.
 
 Decode runs the split decode kernel (``csrc/kernels/flash_decode.cu``), prefill and the shared prefix the tcgen05 kernel
 (``csrc/kernels/attention_sm100.cu``). CPU tensors run ``ref_window_attn`` / ``ref_shared_prefix_attn``, the plain statements.
@@ -136,13 +137,14 @@ def _int32(t):
 
 def _splits(ctas: int, keys: int, head_dim: int, sms: int) -> int:
     """Parts that the keys of a row tile are cut into: as many CTAs as the machine has SMs (one fits an SM), but at least 256 keys
-    (512 with head_dim 256) each: below that the parts' merge costs more (8 sequences, prefix of 2048, heads of 128, parts of 512 / 228 / 146
-    keys 20.9 / 17.6 / 19.1 us; 201 sequences, 5003, heads of 256, parts of 834 / 556 / 357 keys 62.6 / 51.4 / 58.0 us)."""
+    (512 with head_dim 256) each: below that the parts' merge costs about what it saves (8 sequences, prefix of 2048, heads of 128, parts of 512 / 256 / 114
+    keys 20.8 / 17.8 / 19.5 us; 201 sequences, 5003, heads of 256, parts of 834 / 500 / 357 keys 59.1 / 56.7 / 55.7 us)."""
     return max(1, min(sms // max(1, ctas), -(-keys // (256 if head_dim <= 128 else 512)), 200))
 
 
 # What a call works out from its tensors' shapes, strides and types and its settings (never from their addresses or contents): checks,
-# splits, and the native arguments but for the pointers. Bounded, as a ragged batch has a new number of tokens every step.
+# splits, and the native arguments but for the pointers. Bounded, as a ragged batch has a new number of tokens every step; a call of a new shape
+# works it all out (prefill 25.9 us of host time, 12.6 with a plan).
 _PLANS: dict = {}
 
 
