@@ -375,7 +375,7 @@ int tdist_moe_gate_topk(const void* x, const void* gate, int ntok, int hidden, i
 /* ------------------------------------------------------------------ GQA flash decode */
 typedef struct TdistDecodeArgs {
     const void* q;            /* [B, Hq, D] bf16/fp16 */
-    const void* k_cache;      /* [blocks, page, Hkv, D] (any strides that are multiples of 8 elements) */
+    const void* k_cache;      /* [blocks, page, Hkv, D] (any strides that are multiples of 8 elements), 16-byte aligned */
     const void* v_cache;
     const void* block_table;  /* int32 [B, max_blocks] */
     const void* kv_lens;      /* int32 [B]: keys held by THIS rank per sequence */
