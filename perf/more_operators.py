@@ -139,6 +139,12 @@ def work(case):
     return {"bytes": 2.0 * keys * hkv * _row(case) + 4.0 * case["B"] * case["hq"] * D, "flops": 4.0 * keys * case["hq"] * D}
 
 
+def _quotient(a, b):
+    """a / b, rounded once (with a number on either side torch multiplies by a rounded reciprocal)."""
+    t = a if isinstance(a, torch.Tensor) else b
+    return torch.div(a if t is a else torch.full_like(t, a), b if t is b else torch.full_like(t, b))
+
+
 def _bf16_down(x):
     """The largest bf16 that is not above x (fp32), as fp32."""
     b = x.to(torch.bfloat16)
@@ -150,11 +156,11 @@ def _quantise(x, bits):
     x = x.float()
     if bits == 8:
         most = x.abs().amax(-1, keepdim=True).clamp_min(LEAST)
-        return (torch.round(x * (127.0 / most)) + 128.0).to(torch.uint8), (most / 127.0).squeeze(-1)
+        return (torch.round(x * _quotient(127.0, most)) + 128.0).to(torch.uint8), _quotient(most, 127.0).squeeze(-1)
     g = x.unflatten(-1, (-1, 64))
     least = _bf16_down(g.amin(-1, keepdim=True))
-    step = -_bf16_down(-((g.amax(-1, keepdim=True) - least) / 15.0).clamp_min(LEAST))
-    code = torch.round((g - least) * (1.0 / step)).clamp(0.0, 15.0).to(torch.uint8).flatten(-2)
+    step = -_bf16_down(-_quotient(g.amax(-1, keepdim=True) - least, 15.0).clamp_min(LEAST))
+    code = torch.round((g - least) * _quotient(1.0, step)).clamp(0.0, 15.0).to(torch.uint8).flatten(-2)
     return code[..., 0::2] | (code[..., 1::2] << 4), torch.cat([step, least], -1).to(torch.bfloat16)
 
 
@@ -302,13 +308,13 @@ def _plain_linear(s):
     """Sums of 1024 products of 8-bit integers are exact in fp32; between them whole numbers."""
     x, w, k = s["x"].float(), s["w"], s["case"]["k"]
     most = x.abs().amax(1, keepdim=True).clamp_min(LEAST)
-    codes = torch.round(x * (127.0 / most))
+    codes = torch.round(x * _quotient(127.0, most))
     y = torch.empty((x.shape[0], w.shape[0]), dtype=s["x"].dtype, device="cuda")
     for n0 in range(0, w.shape[0], 16384):
         acc = 0
         for k0 in range(0, k, 1024):
             acc = acc + torch.matmul(codes[:, k0:k0 + 1024], w[n0:n0 + 16384, k0:k0 + 1024].float().t()).to(torch.int32)
-        y[:, n0:n0 + 16384] = acc.float() * (most / 127.0) * s["w_scale"][n0:n0 + 16384]
+        y[:, n0:n0 + 16384] = acc.float() * _quotient(most, 127.0) * s["w_scale"][n0:n0 + 16384]
     return y
 
 
