@@ -207,6 +207,31 @@ class SampleArgs(C.Structure):
     ]
 
 
+class QuantCacheArgs(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("code_block", C.c_longlong), ("code_token", C.c_longlong), ("code_head", C.c_longlong),
+        ("scale_block", C.c_longlong), ("scale_head", C.c_longlong), ("scale_token", C.c_longlong),
+        ("blocks", C.c_int), ("page_size", C.c_int), ("Hkv", C.c_int), ("head_dim", C.c_int), ("bits", C.c_int), ("dtype", C.c_int),
+        ("rows", C.c_longlong),
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_token", C.c_longlong), ("k_head", C.c_longlong), ("v_token", C.c_longlong), ("v_head", C.c_longlong),
+        ("slots", C.c_void_p),
+        ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("starts", C.c_void_p), ("lens", C.c_void_p), ("table", C.c_void_p),
+        ("B", C.c_int), ("max_blocks", C.c_int),
+        ("stream", C.c_void_p),
+    ]
+
+
+class QuantDecodeArgs(C.Structure):
+    _fields_ = [
+        ("cache", QuantCacheArgs),
+        ("q", C.c_void_p), ("out", C.c_void_p), ("part", C.c_void_p),
+        ("Hq", C.c_int), ("splits", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
+        ("scale", C.c_float), ("soft_cap", C.c_float),
+    ]
+
+
 class PrimArgs(C.Structure):
     _fields_ = [
         ("data_peer", C.c_void_p * MAX_RANKS), ("sig_peer", C.c_void_p * MAX_RANKS),
@@ -277,6 +302,9 @@ def _declare(lib):
     lib.tdist_flash_decode.argtypes = [C.POINTER(DecodeArgs)]
     lib.tdist_attention.argtypes = [C.POINTER(AttentionArgs)]
     lib.tdist_sample.argtypes = [C.POINTER(SampleArgs)]
+    lib.tdist_quant_cache_write.argtypes = [C.POINTER(QuantCacheArgs)]
+    lib.tdist_quant_cache_read.argtypes = [C.POINTER(QuantCacheArgs)]
+    lib.tdist_quant_decode.argtypes = [C.POINTER(QuantDecodeArgs)]
     lib.tdist_lse_combine.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p]
     lib.tdist_dequant_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
     lib.tdist_moe_route.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

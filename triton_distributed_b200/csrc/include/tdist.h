@@ -468,6 +468,40 @@ typedef struct TdistSampleArgs {
 
 int tdist_sample(const TdistSampleArgs* args);
 
+/* ------------------------------------------------------------------ KV cache in 8 or 4 bits (csrc/kernels/quantized_cache.cu, quantized_decode.cu) */
+typedef struct TdistQuantCacheArgs {
+    void *k_codes, *v_codes;     /* uint8 [blocks, page, Hkv, D] (8 bits) or [.., D / 2] (4 bits), the last dimension contiguous */
+    void *k_scales, *v_scales;   /* fp32 [blocks, Hkv, page] or pairs of bf16 (step, least) [blocks, Hkv, page, D / 64, 2] */
+    long long code_block, code_token, code_head;      /* strides in bytes, multiples of 16 */
+    long long scale_block, scale_head, scale_token;   /* in bytes, multiples of a row's scales (4 or D / 16) */
+    int blocks, page_size, Hkv, head_dim, bits;
+    int dtype;                   /* of rows outside the cache: TDIST_BF16 / TDIST_F16 */
+    long long rows;              /* write: tokens; read: rows of the outputs */
+    /* write: k, v [rows, Hkv, D], strides in bytes, multiples of 16; slots int32 [rows]: page x page_size + place in it, others are left out */
+    const void *k, *v;
+    long long k_token, k_head, v_token, v_head;
+    const void* slots;
+    /* read: sequence b's keys are rows starts[b] .. starts[b] + lens[b] - 1 of k_out, v_out [rows, Hkv, D]; rows of no sequence are zeros */
+    void *k_out, *v_out;
+    const void *starts, *lens, *table;   /* int32 [B + 1], [B], [B, max_blocks] (decode: lens and table) */
+    int B, max_blocks;
+    void* stream;
+} TdistQuantCacheArgs;
+
+#define TDIST_QUANT_DECODE_SPLITS 512
+typedef struct TdistQuantDecodeArgs {
+    TdistQuantCacheArgs cache;
+    const void* q;               /* [B, Hq, D] */
+    void* out;                   /* [B, Hq, D] */
+    void* part;                  /* fp32 [B, Hq, splits, D + 2] where splits > 8 */
+    int Hq, splits, window, sinks;
+    float scale, soft_cap;
+} TdistQuantDecodeArgs;
+
+int tdist_quant_cache_write(const TdistQuantCacheArgs* args);
+int tdist_quant_cache_read(const TdistQuantCacheArgs* args);
+int tdist_quant_decode(const TdistQuantDecodeArgs* args);
+
 /* ------------------------------------------------------------------ device primitives, one test op each */
 enum {
     TDIST_PRIM_RING_PUT = 0, TDIST_PRIM_NOTIFY_WAIT = 1, TDIST_PRIM_NOTIFY_ADD = 2, TDIST_PRIM_PUT_SIGNAL = 3,

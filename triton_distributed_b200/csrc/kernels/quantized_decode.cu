@@ -1,0 +1,754 @@
+// Decode attention over a paged KV cache in 8 or 4 bits (format: quantized_cache.cu), one query token per sequence.
+//
+//   s_j = scale q . k_j, k_j = ks_j c_j             4 bits: k_j = step_jg c_j + least_jg in every group g of 64 dimensions
+//   o   = sum_j p_j vs_j c'_j / sum_j p_j           p_j = exp(s_j - max)
+//
+// The rows are never dequantised. Codes are small whole numbers, exact in fp16, so the products with them run on tensor cores
+// (mma.sync m16n8k16, fp16 operands, fp32 sums) and the scales are applied where they are one number per key: to the score (4 bits: to
+// a group's part of it, and least_jg times the sum of q over the group is added), and to the weight p_j vs_j, with the sum of p_j least_jg
+// kept beside the product. A query is brought to [2^13, 2^14) by a power of two first, so that bf16's range fits fp16 (values 2^-28 of
+// the largest lose bits). Weights are divided by a power of two above all vs_j so far, so that p_j vs_j / S lies in [0, 1] whatever the
+// values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest.
+//
+// As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
+// S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix. What is different is the way of the codes: a byte is no MMA operand, so they go
+// through registers anyway, and they are loaded there straight from global memory, without shared memory. The sum over a row's dimensions may
+// run in any order and the output's dimensions may be dealt to the MMA's rows in any order, so both are chosen by what a wide load
+// gives: of 64 dimensions of a key, the four lanes of a quad take 16 neighbouring ones each, and of a value's each eighth lane an eighth.
+// A warp's next 16 tokens are loaded as soon as their registers are free: all 16 warps of an SM have 4 KB under way most of the time.
+//
+// A CTA is 8 warps of one (sequence, kv head, part of the keys); tiles of 16 tokens go round the warps. Warps meet in shared memory;
+// up to 8 parts are a cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); more parts go through a
+// workspace and a second kernel. No counters: nothing has to be zero before a call, and calls share nothing.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <cstring>
+#include <string>
+
+#include "../device/ptx.cuh"
+#include "../device/soft_cap.cuh"
+#include "../include/tdist.h"
+#include "../runtime/host_common.h"
+
+namespace tdist {
+namespace qdecode {
+
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int TOK = 16;          // tokens of a tile
+constexpr int MAX_CLUSTER = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+    const void* q;                 // [B, Hq, D]
+    const uint8_t *k, *v;
+    const char *ks, *vs;
+    const int *table, *lens;
+    float* part;                   // [B * Hq][splits][D + 2]: sums, maximum, sum of weights (more than MAX_CLUSTER parts)
+    void* out;
+    long long code_block, code_token, code_head, scale_block, scale_head, scale_token;   // bytes
+    int Hq, Hkv, head_tiles, page_size, page_shift, max_blocks, blocks, splits, window, sinks, table_keys, is_f16;
+    float scale, soft_cap;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// A byte or nibble n under the exponent of 1024 is the fp16 number 1024 + n; in the upper nibble of a byte, 1024 + 16 n.
+constexpr uint32_t kMagic = 0x64006400u;
+constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a 0x64
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) { return hsub2(__byte_perm(w, kMagic, sel), 0x64806480u); }   // - 1152
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return hsub2((w & 0x000f000fu) | kMagic, kMagic); }
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return hfma2((w & 0x00f000f0u) | kMagic, 0x2c002c00u, 0xd400d400u); }   // / 16 - 64
+
+__device__ __forceinline__ uint32_t ldg32(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+template <int W>
+struct Words { uint32_t w[W]; };
+// W words from p, aligned to their size (W up to 4) or to 16 bytes
+template <int W>
+__device__ __forceinline__ Words<W> load_words(const void* p) {
+    Words<W> r;
+    if constexpr (W == 1) {
+        r.w[0] = ldg32(p);
+    } else if constexpr (W == 2) {
+        asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i)
+            asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r.w[4 * i]), "=r"(r.w[4 * i + 1]), "=r"(r.w[4 * i + 2]), "=r"(r.w[4 * i + 3])
+                         : "l"(static_cast<const char*>(p) + 16 * i));
+    }
+    return r;
+}
+
+template <int BITS, int D>
+struct Shape {
+    static constexpr int NG = BITS == 8 ? 1 : D / 64;      // scales of a row
+    static constexpr int KC = D / 64;                      // 64-dimension chunks of a key
+    static constexpr int KW = BITS == 8 ? 4 : 2;           // words of a chunk and lane
+    // values: VC chunks, of each of which a lane holds an eighth of the dimensions in VW words
+    static constexpr int VC = BITS == 4 ? D / 64 : (D == 256 ? 2 : 1);
+    static constexpr int VD = D / VC / 8;                  // dimensions of a chunk and lane
+    static constexpr int VW = VD * BITS / 32;
+    static constexpr int VB = D * BITS / 8 / VC;           // bytes of a chunk
+    static constexpr int MT = D / 16;                      // MMAs of a tile
+};
+
+// O and what belongs to it, per warp, in shared memory: heads [8 NH] rows of D + 4 floats
+__host__ __device__ constexpr int o_pitch(int d) { return d + 4; }
+
+template <int BITS, int D, int NH, bool WHOLE>
+__global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode_kernel(const Params p) {
+    using S = Shape<BITS, D>;
+    constexpr int HEADS = 8 * NH, OP = o_pitch(D);
+    extern __shared__ float o_s[];                          // [WARPS][HEADS][OP], then the cluster's slices
+    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    __shared__ float part_m[MAX_CLUSTER][HEADS], part_l[MAX_CLUSTER][HEADS];
+    const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+    const int g = lane >> 2, c = lane & 3;
+    const bool in_cluster = p.splits > 1 && p.splits <= MAX_CLUSTER;
+    if (in_cluster) cluster_arrive();                       // waited for before the first store into another CTA
+    pdl_wait_and_release();
+
+    int x = static_cast<int>(blockIdx.x);
+    const int split = x % p.splits;
+    x /= p.splits;
+    const int tile_of_heads = x % p.head_tiles;
+    x /= p.head_tiles;
+    const int kvh = x % p.Hkv, b = x / p.Hkv;
+    const int G = p.Hq / p.Hkv;
+    const int heads = min(HEADS, G - tile_of_heads * HEADS);
+    const size_t head0 = static_cast<size_t>(b) * p.Hq + kvh * G + tile_of_heads * HEADS;
+
+    // ---- the keys: tiles of the first `first` tokens, then those from the window's first token on (a tile's first token is a multiple of 16)
+    const int n = min(max(p.lens[b], 0), p.table_keys);
+    const int lo = max(0, n - p.window);
+    const int first = min(p.sinks, lo);
+    const int sink_tiles = (first + TOK - 1) / TOK;
+    const int t_lo = lo / TOK;
+    const int tiles = sink_tiles + (n + TOK - 1) / TOK - t_lo;
+    const int per = (tiles + p.splits - 1) / p.splits;
+    const int i0 = min(split * per, tiles) + warp, i1 = min((split + 1) * per, tiles);
+
+    const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
+    const uint8_t* kc = p.k + kvh * p.code_head;
+    const uint8_t* vc = p.v + kvh * p.code_head;
+    const char* ksc = p.ks + kvh * p.scale_head;
+    const char* vsc = p.vs + kvh * p.scale_head;
+
+    // A tile's place: its first token and the limits of what is seen of it
+    auto first_token = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + t_lo) * TOK; };
+    // page (and row) of the tile's first token (WHOLE: pages of a multiple of 16), or of token `lane`; -1: not seen, or no page of the cache
+    auto lookup = [&](int i, int& page, int& row) {
+        page = -1;
+        row = 0;
+        if (i < i1 && (WHOLE || lane < TOK)) {
+            const int t = first_token(i) + (WHOLE ? 0 : lane);
+            const bool seen = WHOLE || (i < sink_tiles ? t < first : t >= lo && t < n);
+            if (seen) {
+                const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+                page = static_cast<int>(ldg32(table + in_table));
+                row = t - in_table * p.page_size;
+                if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.blocks)) page = -1;
+            }
+        }
+    };
+    Words<S::KW> kw[2][S::KC];     // tokens g, g + 8
+    Words<S::NG> kscale[2], vscale[2];
+    Words<S::VW> vw[4][S::VC];     // tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+    auto place = [&](int page, int row, int r, long long block, long long token) -> long long {
+        if (WHOLE) return page < 0 ? -1 : page * block + (row + r) * token;
+        const int pg = __shfl_sync(0xffffffffu, page, r), rw = __shfl_sync(0xffffffffu, row, r);
+        return pg < 0 ? -1 : pg * block + rw * token;
+    };
+    auto load_k = [&](int page, int row) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const long long at = place(page, row, g + 8 * r, p.code_block, p.code_token);
+            const long long sat = place(page, row, g + 8 * r, p.scale_block, p.scale_token);
+#pragma unroll
+            for (int j = 0; j < S::KC; ++j) {
+                if (at >= 0) kw[r][j] = load_words<S::KW>(kc + at + j * (64 * BITS / 8) + c * (16 * BITS / 8));
+                else
+#pragma unroll
+                    for (int w = 0; w < S::KW; ++w) kw[r][j].w[w] = 0;
+            }
+            if (sat >= 0) {
+                kscale[r] = load_words<S::NG>(ksc + sat);
+            } else {
+#pragma unroll
+                for (int w = 0; w < S::NG; ++w) kscale[r].w[w] = 0;
+            }
+        }
+    };
+    auto load_v = [&](int page, int row) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long long at = place(page, row, 2 * c + (r & 1) + (r >> 1) * 8, p.code_block, p.code_token);
+#pragma unroll
+            for (int j = 0; j < S::VC; ++j) {
+                if (at >= 0) vw[r][j] = load_words<S::VW>(vc + at + j * S::VB + g * (S::VB / 8));
+                else
+#pragma unroll
+                    for (int w = 0; w < S::VW; ++w) vw[r][j].w[w] = 0;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const long long sat = place(page, row, g + 8 * r, p.scale_block, p.scale_token);
+            if (sat >= 0) {
+                vscale[r] = load_words<S::NG>(vsc + sat);
+            } else {
+#pragma unroll
+                for (int w = 0; w < S::NG; ++w) vscale[r].w[w] = 0;
+            }
+        }
+    };
+
+    int page, row;
+    lookup(i0, page, row);
+    load_k(page, row);
+    load_v(page, row);
+    lookup(i0 + WARPS, page, row);
+
+    // ---- q as the second operand: column g of the MMA is head 8 h + g, its dimensions 16 c .. 16 c + 15 of every 64 are this lane's
+    uint32_t qf[NH][S::KC][4][2];
+    float factor[NH][2];           // of heads 8 h + 2 c + {0, 1}: what turns a product of codes into a score in units of log2
+    float qsum[NH][2][S::NG];      // 4 bits: the sum of the scaled q over a group
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+        const int head = 8 * h + g;
+        const char* src = static_cast<const char*>(p.q) + (head0 + (head < heads ? head : 0)) * (D * 2) + c * 32;
+        float f[S::KC][16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < S::KC; ++j) {
+            const Words<8> w = load_words<8>(src + j * 128);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (p.is_f16) {
+                    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w.w[e]));
+                    f[j][2 * e] = t.x;
+                    f[j][2 * e + 1] = t.y;
+                } else {
+                    f[j][2 * e] = __uint_as_float(w.w[e] << 16);
+                    f[j][2 * e + 1] = __uint_as_float(w.w[e] & 0xffff0000u);
+                }
+                top = max(top, max(__float_as_uint(f[j][2 * e]) & 0x7fffffffu, __float_as_uint(f[j][2 * e + 1]) & 0x7fffffffu));
+            }
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^up brings the largest to [2^13, 2^14); none for zeros, infinities and NaN. 2^up and its inverse are normal numbers
+        const int e = static_cast<int>(top >> 23);
+        const int up = e == 0 || e == 255 ? 0 : min(100, 140 - e);
+        const float mul = head < heads ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : 0.f;
+#pragma unroll
+        for (int j = 0; j < S::KC; ++j) {
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                f[j][k] = head < heads ? __half2float(__float2half_rn(f[j][k] * mul)) : 0.f;
+                sum += f[j][k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // the order in which the codes of a chunk come out of their words
+                if (BITS == 8) {
+                    qf[h][j][k][0] = pack_f16x2(f[j][4 * k], f[j][4 * k + 1]);
+                    qf[h][j][k][1] = pack_f16x2(f[j][4 * k + 2], f[j][4 * k + 3]);
+                } else {
+                    const int d = (k >> 1) * 8 + (k & 1) * 2;
+                    qf[h][j][k][0] = pack_f16x2(f[j][d], f[j][d + 4]);
+                    qf[h][j][k][1] = pack_f16x2(f[j][d + 1], f[j][d + 5]);
+                }
+            }
+            if (BITS == 4) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) qsum[h][r][j] = __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4);
+            }
+        }
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) factor[h][r] = __shfl_sync(0xffffffffu, down, (2 * c + r) * 4) * (p.soft_cap > 0.f ? 1.f : kLog2e);
+    }
+
+    // ---- sums: O^T in units of `unit` (a power of two), columns are heads 8 h + 2 c + {0, 1}
+    float o[NH][S::MT][4];
+    float m_run[NH][2], m_use[NH][2], l_run[NH][2];
+    float low[NH][2][S::NG];       // 4 bits: sum of p least, of this lane's tokens
+    float unit = 0.f, inv_unit = 0.f;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+#pragma unroll
+        for (int j = 0; j < S::MT; ++j) o[h][j][0] = o[h][j][1] = o[h][j][2] = o[h][j][3] = 0.f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            m_run[h][r] = -CUDART_INF_F;
+            m_use[h][r] = l_run[h][r] = 0.f;
+#pragma unroll
+            for (int k = 0; k < S::NG; ++k) low[h][r][k] = 0.f;
+        }
+    }
+    const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
+
+    for (int i = i0; i < i1; i += WARPS) {
+        // ---- S^T = K Q^T, a sum per group of dimensions
+        float s[NH][4];
+        float acc[NH][S::NG][4];
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int k = 0; k < S::NG; ++k) acc[h][k][0] = acc[h][k][1] = acc[h][k][2] = acc[h][k][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < S::KC; ++j) {
+            constexpr int last = S::NG - 1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t a[4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if (BITS == 8) {
+                        const uint32_t w = kw[r][j].w[k % S::KW];
+                        a[r] = bytes_to_half2(w, kLowBytes);
+                        a[2 + r] = bytes_to_half2(w, kHighBytes);
+                    } else {
+                        const uint32_t w = kw[r][j].w[k >> 1] >> ((k & 1) * 8);
+                        a[r] = low_nibbles(w);
+                        a[2 + r] = high_nibbles(w);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < NH; ++h) mma_f16(acc[h][min(j, last)], a[0], a[1], a[2], a[3], qf[h][j][k][0], qf[h][j][k][1]);
+            }
+        }
+        // ---- scales, cap, mask
+        const int t0 = first_token(i);
+        const bool sink = i < sink_tiles;
+        bool higher = false, seen[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int t = t0 + g + 8 * r;
+            seen[r] = sink ? t < first : t >= lo && t < n;
+        }
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = e >> 1;
+                float v = 0.f;
+                if (BITS == 8) {
+                    v = acc[h][0][e] * __uint_as_float(kscale[r].w[0]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < S::NG; ++k)
+                        v += __uint_as_float(kscale[r].w[k] << 16) * acc[h][k][e] + __uint_as_float(kscale[r].w[k] & 0xffff0000u) * qsum[h][e & 1][k];
+                }
+                v *= factor[h][e & 1];
+                if (p.soft_cap > 0.f) v = soft_cap(v * kLog2e, v * cap_inv, p.soft_cap * kLog2e);
+                v = seen[r] ? v : -CUDART_INF_F;
+                s[h][e] = v;
+                higher |= v > m_run[h][e & 1];
+            }
+        // ---- the values' scales, as weights in units of `unit`
+        float vmul[2][S::NG], vleast[2][S::NG];
+        float most = 0.f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int k = 0; k < S::NG; ++k) {
+                vmul[r][k] = seen[r] ? __uint_as_float(BITS == 8 ? vscale[r].w[k] : vscale[r].w[k] << 16) : 0.f;
+                if (BITS == 4) vleast[r][k] = seen[r] ? __uint_as_float(vscale[r].w[k] & 0xffff0000u) : 0.f;
+                most = fmaxf(most, vmul[r][k]);
+            }
+        higher |= most > unit;
+        // the next tile's keys: theirs are the registers that are free now
+        if (i + WARPS < i1) load_k(page, row);
+        if (__any_sync(0xffffffffu, higher)) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+            float shrink = 1.f;
+            if (most > unit) {
+                // the next power of two, whose inverse is a normal number too
+                const uint32_t e = min((__float_as_uint(most) >> 23) + 1u, 250u);
+                const float up = __uint_as_float(e << 23);
+                shrink = unit / up;
+                unit = up;
+                inv_unit = __uint_as_float((254u - e) << 23);
+            }
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float mx = fmaxf(s[h][r], s[h][2 + r]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float m_new = fmaxf(m_run[h][r], mx);
+                    m_use[h][r] = m_new == -CUDART_INF_F ? 0.f : m_new;
+                    const float alpha = exp2f(m_run[h][r] - m_use[h][r]);
+                    m_run[h][r] = m_new;
+                    l_run[h][r] *= alpha;
+#pragma unroll
+                    for (int k = 0; k < S::NG; ++k) low[h][r][k] *= alpha;
+                    const float both = alpha * shrink;
+#pragma unroll
+                    for (int j = 0; j < S::MT; ++j) {
+                        o[h][j][r] *= both;
+                        o[h][j][2 + r] *= both;
+                    }
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int k = 0; k < S::NG; ++k) vmul[r][k] *= inv_unit;
+        // ---- P^T times the scales as the second operand: tokens in pairs per lane, heads over lane / 4
+        uint32_t pb[NH][S::NG][2];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            const float p0 = exp2f(s[h][0] - m_use[h][0]), p1 = exp2f(s[h][1] - m_use[h][1]);
+            const float p2 = exp2f(s[h][2] - m_use[h][0]), p3 = exp2f(s[h][3] - m_use[h][1]);
+            l_run[h][0] += p0 + p2;
+            l_run[h][1] += p1 + p3;
+#pragma unroll
+            for (int k = 0; k < S::NG; ++k) {
+                if (BITS == 4) {
+                    low[h][0][k] += p0 * vleast[0][k] + p2 * vleast[1][k];
+                    low[h][1][k] += p1 * vleast[0][k] + p3 * vleast[1][k];
+                }
+                pb[h][k][0] = movmatrix_trans(pack_f16x2(p0 * vmul[0][k], p1 * vmul[0][k]));
+                pb[h][k][1] = movmatrix_trans(pack_f16x2(p2 * vmul[1][k], p3 * vmul[1][k]));
+            }
+        }
+        // ---- O^T += V^T P^T: row g of MMA m is dimension 2 m of the lane's, row g + 8 the one after it
+#pragma unroll
+        for (int j = 0; j < S::VC; ++j) {
+            constexpr int last = S::NG - 1;
+#pragma unroll
+            for (int w = 0; w < S::VW; ++w) {
+                const uint32_t w0 = vw[0][j].w[w], w1 = vw[1][j].w[w], w2 = vw[2][j].w[w], w3 = vw[3][j].w[w];
+                if (BITS == 8) {
+                    // bytes of two tokens side by side
+                    const uint32_t a01 = __byte_perm(w0, w1, 0x5140u), a23 = __byte_perm(w0, w1, 0x7362u);
+                    const uint32_t b01 = __byte_perm(w2, w3, 0x5140u), b23 = __byte_perm(w2, w3, 0x7362u);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const uint32_t a = m ? a23 : a01, bb = m ? b23 : b01;
+                        const uint32_t x0 = bytes_to_half2(a, kLowBytes), x1 = bytes_to_half2(a, kHighBytes);
+                        const uint32_t x2 = bytes_to_half2(bb, kLowBytes), x3 = bytes_to_half2(bb, kHighBytes);
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        // four codes of each of two tokens
+                        const uint32_t a = __byte_perm(w0, w1, half ? 0x7632u : 0x5410u), bb = __byte_perm(w2, w3, half ? 0x7632u : 0x5410u);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            const uint32_t x0 = low_nibbles(a >> (8 * m)), x1 = high_nibbles(a >> (8 * m));
+                            const uint32_t x2 = low_nibbles(bb >> (8 * m)), x3 = high_nibbles(bb >> (8 * m));
+#pragma unroll
+                            for (int h = 0; h < NH; ++h)
+                                mma_f16(o[h][j * (S::VD / 2) + w * 4 + half * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
+                        }
+                    }
+                }
+            }
+        }
+        if (i + WARPS < i1) {
+            load_v(page, row);
+            lookup(i + 2 * WARPS, page, row);
+        }
+    }
+
+    // ---- the warps meet in shared memory
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int head = 8 * h + 2 * c + r;
+            float l = l_run[h][r];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            if (g == 0) {
+                m_s[warp][head] = m_run[h][r];
+                l_s[warp][head] = l;
+            }
+            float* dst = o_s + (warp * HEADS + head) * OP;
+#pragma unroll
+            for (int j = 0; j < S::VC; ++j) {
+                float add = 0.f;
+                if (BITS == 4) {
+                    add = low[h][r][min(j, S::NG - 1)];
+                    add += __shfl_xor_sync(0xffffffffu, add, 4);
+                    add += __shfl_xor_sync(0xffffffffu, add, 8);
+                    add += __shfl_xor_sync(0xffffffffu, add, 16);
+                }
+#pragma unroll
+                for (int k = 0; k < S::VD / 2; ++k) {
+                    const int m = j * (S::VD / 2) + k;
+                    *reinterpret_cast<float2*>(dst + j * (D / S::VC) + g * S::VD + 2 * k) =
+                        make_float2(o[h][m][r] * unit + add, o[h][m][2 + r] * unit + add);
+                }
+            }
+        }
+    __syncthreads();
+    if (in_cluster) cluster_wait();   // every CTA of the cluster runs
+
+    // A part's sums go to the slice's owner (the CTA itself without a cluster), relative to the part's maximum
+    const int total = heads * D;
+    const int slices = in_cluster ? p.splits : 1;
+    const int slice = ((total + slices - 1) / slices + 3) & ~3;
+    float* slice_s = o_s + WARPS * HEADS * OP;              // [splits][slice]
+    const bool to_workspace = p.splits > MAX_CLUSTER;
+    for (int idx = static_cast<int>(threadIdx.x); idx < total; idx += THREADS) {
+        const int head = idx / D, d = idx % D;
+        float m = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w][head]);
+        const float mu = m == -CUDART_INF_F ? 0.f : m;
+        float l = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = exp2f(m_s[w][head] - mu);
+            l += l_s[w][head] * f;
+            sum += o_s[(w * HEADS + head) * OP + d] * f;
+        }
+        if (to_workspace) {
+            float* dst = p.part + ((head0 + head) * p.splits + split) * (D + 2);
+            dst[d] = sum;
+            if (d == 0) {
+                dst[D] = m;
+                dst[D + 1] = l;
+            }
+        } else {
+            const int owner = idx / slice;
+            float* at = slice_s + split * slice + (idx - owner * slice);
+            if (in_cluster) st_shared_cluster_f32(mapa_u32(smem_u32(at), static_cast<uint32_t>(owner)), sum);
+            else *at = sum;
+            if (d == 0) {
+                for (int o2 = 0; o2 < slices; ++o2) {
+                    if (in_cluster) {
+                        st_shared_cluster_f32(mapa_u32(smem_u32(&part_m[split][head]), static_cast<uint32_t>(o2)), m);
+                        st_shared_cluster_f32(mapa_u32(smem_u32(&part_l[split][head]), static_cast<uint32_t>(o2)), l);
+                    } else {
+                        part_m[0][head] = m;
+                        part_l[0][head] = l;
+                    }
+                }
+            }
+        }
+    }
+    if (to_workspace) return;
+    if (in_cluster) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    const int base = in_cluster ? split * slice : 0;
+    const int mine = min(slice, total - base);
+    for (int idx = static_cast<int>(threadIdx.x) * 2; idx < mine; idx += THREADS * 2) {   // (D and slices are even)
+        const int head = (base + idx) / D;
+        float m = -CUDART_INF_F;
+        for (int s2 = 0; s2 < slices; ++s2) m = fmaxf(m, part_m[s2][head]);
+        const float mu = m == -CUDART_INF_F ? 0.f : m;
+        float l = 0.f, a0 = 0.f, a1 = 0.f;
+        for (int s2 = 0; s2 < slices; ++s2) {
+            const float f = exp2f(part_m[s2][head] - mu);
+            l += part_l[s2][head] * f;
+            const float2 v = *reinterpret_cast<const float2*>(slice_s + s2 * slice + idx);
+            a0 += v.x * f;
+            a1 += v.y * f;
+        }
+        // a sum of weights that is not positive: no keys (zeros), or a NaN among the scores
+        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+        const uint32_t w = p.is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
+        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.out) + (head0 * D + base + idx) * 2) = w;
+    }
+}
+
+// The parts of a head, from the workspace: a CTA per head, a thread per two dimensions.
+__global__ void __launch_bounds__(128) merge_kernel(const float* part, int splits, int D, int is_f16, void* out) {
+    __shared__ float f_s[512];
+    __shared__ float l_s;
+    pdl_wait_and_release();
+    const size_t head = blockIdx.x;
+    const float* src = part + head * splits * (D + 2);
+    const int lane = static_cast<int>(threadIdx.x) & 31;
+    if (threadIdx.x < 32) {
+        float m = -CUDART_INF_F;
+        for (int s = lane; s < splits; s += 32) m = fmaxf(m, src[s * (D + 2) + D]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float mu = m == -CUDART_INF_F ? 0.f : m;
+        float l = 0.f;
+        for (int s = lane; s < splits; s += 32) {
+            const float f = exp2f(src[s * (D + 2) + D] - mu);
+            f_s[s] = f;
+            l += f * src[s * (D + 2) + D + 1];
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) l_s = l;
+    }
+    __syncthreads();
+    const float l = l_s;
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    const int d = static_cast<int>(threadIdx.x) * 2;
+    if (d >= D) return;
+    float a0 = 0.f, a1 = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) {
+        const float2 v = *reinterpret_cast<const float2*>(src + s * (D + 2) + d);
+        a0 += v.x * f_s[s];
+        a1 += v.y * f_s[s];
+    }
+    const uint32_t w = is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
+    *reinterpret_cast<uint32_t*>(static_cast<char*>(out) + (head * D + d) * 2) = w;
+}
+
+template <int BITS, int D, int NH, bool WHOLE>
+int launch(const Params& p, int grid, cudaStream_t stream) {
+    const int cluster = p.splits > 1 && p.splits <= MAX_CLUSTER ? p.splits : 1;
+    // slices: a part's share of 8 NH heads, rounded up to 4 floats
+    const int smem = (WARPS * 8 * NH * o_pitch(D) + 8 * NH * D + 4 * MAX_CLUSTER) * 4;
+    const auto fn = decode_kernel<BITS, D, NH, WHOLE>;
+    TDIST_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0] = tdist_host::pdl_attribute();
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    TDIST_CUDA_OK(cudaLaunchKernelEx(&cfg, fn, p));
+    return 0;
+}
+
+template <int BITS, int D>
+int launch_heads(const Params& p, int nh, bool whole, int grid, cudaStream_t stream) {
+    // heads of 256 take one tile of query heads: two would need more registers than there are
+    if constexpr (D != 256) {
+        if (nh == 2) return whole ? launch<BITS, D, 2, true>(p, grid, stream) : launch<BITS, D, 2, false>(p, grid, stream);
+    }
+    return whole ? launch<BITS, D, 1, true>(p, grid, stream) : launch<BITS, D, 1, false>(p, grid, stream);
+}
+
+template <int BITS>
+int launch_dim(const Params& p, int head_dim, int nh, bool whole, int grid, cudaStream_t stream) {
+    return head_dim == 64 ? launch_heads<BITS, 64>(p, nh, whole, grid, stream)
+                          : (head_dim == 128 ? launch_heads<BITS, 128>(p, nh, whole, grid, stream) : launch_heads<BITS, 256>(p, nh, whole, grid, stream));
+}
+
+}  // namespace qdecode
+}  // namespace tdist
+
+using namespace tdist;
+using tdist_host::fail;
+
+extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
+    using namespace tdist::qdecode;
+    const TdistQuantCacheArgs& c = a->cache;
+    if (c.bits != 8 && c.bits != 4) return fail(TDIST_EINVAL, "quantised decode: 8 or 4 bits");
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return fail(TDIST_EINVAL, "quantised decode: head_dim must be 64, 128 or 256");
+    if (c.Hkv < 1 || a->Hq < 1 || a->Hq % c.Hkv || c.page_size < 1 || c.B < 0 || c.blocks < 0 || c.max_blocks < 0)
+        return fail(TDIST_EINVAL, "quantised decode: bad shape");
+    if (c.dtype != TDIST_BF16 && c.dtype != TDIST_F16) return fail(TDIST_EINVAL, "quantised decode: q must be bf16 or fp16");
+    if (a->splits < 1 || a->splits > TDIST_QUANT_DECODE_SPLITS || (a->splits > MAX_CLUSTER && a->part == nullptr))
+        return fail(TDIST_EINVAL, "quantised decode: parts");
+    if (a->window < 1 || a->sinks < 0 || !(a->soft_cap >= 0.f)) return fail(TDIST_EINVAL, "quantised decode: window, sinks or soft cap");
+    const uintptr_t code_align = reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.v_codes) |
+                                 static_cast<uintptr_t>(c.code_block | c.code_token | c.code_head);
+    const uintptr_t scale_align = reinterpret_cast<uintptr_t>(c.k_scales) | reinterpret_cast<uintptr_t>(c.v_scales) |
+                                  static_cast<uintptr_t>(c.scale_block | c.scale_head | c.scale_token);
+    if ((code_align & 15) || (scale_align & (c.bits == 8 ? 3 : c.head_dim / 16 - 1)))
+        return fail(TDIST_EINVAL, "quantised decode: codes must lie on 16 bytes, a row's scales on their size");
+    if ((reinterpret_cast<uintptr_t>(a->q) & 15) || (reinterpret_cast<uintptr_t>(a->out) & 3))
+        return fail(TDIST_EINVAL, "quantised decode: q must lie on 16 bytes, out on 4");
+    if (c.B == 0) return 0;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.q = a->q;
+    p.k = static_cast<const uint8_t*>(c.k_codes);
+    p.v = static_cast<const uint8_t*>(c.v_codes);
+    p.ks = static_cast<const char*>(c.k_scales);
+    p.vs = static_cast<const char*>(c.v_scales);
+    p.table = static_cast<const int*>(c.table);
+    p.lens = static_cast<const int*>(c.lens);
+    p.part = static_cast<float*>(a->part);
+    p.out = a->out;
+    p.code_block = c.code_block;
+    p.code_token = c.code_token;
+    p.code_head = c.code_head;
+    p.scale_block = c.scale_block;
+    p.scale_head = c.scale_head;
+    p.scale_token = c.scale_token;
+    p.Hq = a->Hq;
+    p.Hkv = c.Hkv;
+    const int G = a->Hq / c.Hkv;
+    const int nh = G > 8 && c.head_dim != 256 ? 2 : 1;
+    p.head_tiles = (G + 8 * nh - 1) / (8 * nh);
+    p.page_size = c.page_size;
+    p.page_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (c.page_size == 1 << i) p.page_shift = i;
+    p.max_blocks = c.max_blocks;
+    p.blocks = c.blocks;
+    p.splits = a->splits;
+    p.window = a->window;
+    p.sinks = a->sinks;
+    const long long keys = static_cast<long long>(c.max_blocks) * c.page_size;
+    p.table_keys = static_cast<int>(keys < 0x7fffffc0ll ? keys : 0x7fffffc0ll);
+    p.is_f16 = c.dtype == TDIST_F16;
+    p.scale = a->scale;
+    p.soft_cap = a->soft_cap;
+    const long long grid = static_cast<long long>(c.B) * c.Hkv * p.head_tiles * a->splits;
+    if (grid > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many sequences");
+    const bool whole = c.page_size % TOK == 0;
+    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    const int rc = c.bits == 8 ? launch_dim<8>(p, c.head_dim, nh, whole, static_cast<int>(grid), stream)
+                               : launch_dim<4>(p, c.head_dim, nh, whole, static_cast<int>(grid), stream);
+    if (rc) return rc;
+    if (a->splits > MAX_CLUSTER)
+        TDIST_CUDA_OK(tdist_host::launch_pdl(merge_kernel, dim3(static_cast<unsigned>(c.B * a->Hq)), 128, 0, stream, p.part, a->splits, c.head_dim,
+                                             p.is_f16, a->out));
+    return 0;
+}

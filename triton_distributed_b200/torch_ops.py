@@ -29,6 +29,7 @@ from .ops import gemm_fp8 as F8
 from .ops import moe_tp as MT
 from .ops import moe_utils as MU
 from .ops import paged_attention as PA
+from .ops import quantized_cache as QC
 from .ops import sampling as SA
 
 _CONTEXTS: Dict[int, object] = {}
@@ -328,7 +329,47 @@ def _(logits, u, temperature, top_k, top_p, min_p):
     return (logits.new_empty((B,), dtype=torch.int32), logits.new_empty((B,), dtype=torch.float32), logits.new_empty((B,), dtype=torch.float32))
 
 
+# ---------------------------------------------------------------------------- KV cache in 8 or 4 bits
+@_op("tdist::kv_cache_write", mutates_args=("k_codes", "v_codes", "k_scales", "v_scales"))
+def kv_cache_write(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, k: torch.Tensor,
+                   v: torch.Tensor, slots: torch.Tensor) -> None:
+    """rows quantised into their places of the cache"""
+    QC.kv_cache_write(QC.QuantizedKVCache(k_codes, v_codes, k_scales, v_scales), k, v, slots)
+
+
+@kv_cache_write.register_fake
+def _(k_codes, v_codes, k_scales, v_scales, k, v, slots):
+    return None
+
+
+@_op("tdist::kv_cache_read", mutates_args=())
+def kv_cache_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, starts: torch.Tensor,
+                  kv_lens: torch.Tensor, block_table: torch.Tensor, rows: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [rows, Hkv, D] of a batch's sequences"""
+    return QC.kv_cache_read(QC.QuantizedKVCache(k_codes, v_codes, k_scales, v_scales), starts, kv_lens, block_table, rows, dtype)
+
+
+@kv_cache_read.register_fake
+def _(k_codes, v_codes, k_scales, v_scales, starts, kv_lens, block_table, rows, dtype):
+    shape = (rows, k_codes.shape[2], k_codes.shape[3] * (1 if k_scales.dim() == 3 else 2))
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+@_op("tdist::gqa_fwd_quantized_decode", mutates_args=())
+def gqa_fwd_quantized_decode(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                             kv_lens: torch.Tensor, block_table: torch.Tensor, window: Optional[int], sinks: int, scale: float,
+                             soft_cap: float) -> torch.Tensor:
+    """decode attention over a cache in 8 or 4 bits"""
+    return QC.gqa_fwd_quantized_decode(q, QC.QuantizedKVCache(k_codes, v_codes, k_scales, v_scales), kv_lens, block_table, window, sinks, scale, soft_cap)
+
+
+@gqa_fwd_quantized_decode.register_fake
+def _(q, k_codes, v_codes, k_scales, v_scales, kv_lens, block_table, window, sinks, scale, soft_cap):
+    return q.new_empty(q.shape)
+
+
 OP_NAMES = ["gemm", "ag_gemm", "gemm_rs", "gemm_fp8", "ag_gemm_fp8", "group_gemm", "reduce_scatter", "barrier_all", "moe_topk_softmax",
             "moe_ag_scatter_align_block_size", "moe_dispatch", "moe_combine", "ep_dispatch", "ep_combine", "gqa_fwd_batch_decode",
             "gqa_fwd_batch_decode_intra_rank", "sp_gqa_fwd_batch_decode", "lse_combine",
-            "gqa_fwd_window_decode", "gqa_fwd_window_prefill", "gqa_fwd_shared_prefix_decode", "sample_tokens"]
+            "gqa_fwd_window_decode", "gqa_fwd_window_prefill", "gqa_fwd_shared_prefix_decode", "sample_tokens",
+            "kv_cache_write", "kv_cache_read", "gqa_fwd_quantized_decode"]
