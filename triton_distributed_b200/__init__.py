@@ -25,6 +25,7 @@ from .ops.gemm import (ag_gemm_inter_node, ag_gemm_intra_node, create_ag_gemm_in
                        gemm_rs_op)
 from .ops.gemm_fp8 import (ag_gemm_fp8, create_ag_gemm_fp8_context, gemm_fp8_blockscaled, quantize_fp8_blockwise,  # noqa: F401
                            quantize_fp8_rowwise)
+from .ops.gemm_int8 import gemm_int8, quantize_int8_rowwise  # noqa: F401
 from .ops.moe_ep import create_ep_context, ep_combine, ep_dispatch, expert_out_buffer  # noqa: F401
 from .ops.moe_tp import (ag_group_gemm_inter_node, ag_group_gemm_intra_node, create_ag_group_gemm_inter_node_context,  # noqa: F401
                          create_ag_group_gemm_intra_node_context, create_moe_rs_context, group_gemm, moe_reduce_rs,

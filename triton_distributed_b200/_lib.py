@@ -232,6 +232,16 @@ class QuantDecodeArgs(C.Structure):
     ]
 
 
+class GemmInt8Args(C.Structure):
+    _fields_ = [
+        ("a", C.c_void_p), ("b", C.c_void_p), ("sa", C.c_void_p), ("sb", C.c_void_p), ("c", C.c_void_p),
+        ("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("dtype", C.c_int),
+        ("status", C.c_void_p),
+        ("timeout_ns", C.c_uint64),
+        ("stream", C.c_void_p),
+    ]
+
+
 class PrimArgs(C.Structure):
     _fields_ = [
         ("data_peer", C.c_void_p * MAX_RANKS), ("sig_peer", C.c_void_p * MAX_RANKS),
@@ -305,6 +315,9 @@ def _declare(lib):
     lib.tdist_quant_cache_write.argtypes = [C.POINTER(QuantCacheArgs)]
     lib.tdist_quant_cache_read.argtypes = [C.POINTER(QuantCacheArgs)]
     lib.tdist_quant_decode.argtypes = [C.POINTER(QuantDecodeArgs)]
+    lib.tdist_gemm_int8.argtypes = [C.POINTER(GemmInt8Args)]
+    lib.tdist_gemm_int8_schedule_check.argtypes = [C.c_int] * 4
+    lib.tdist_quant_int8_rowwise.argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p]
     lib.tdist_lse_combine.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p]
     lib.tdist_dequant_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
     lib.tdist_moe_route.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

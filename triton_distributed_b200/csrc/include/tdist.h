@@ -502,6 +502,21 @@ int tdist_quant_cache_write(const TdistQuantCacheArgs* args);
 int tdist_quant_cache_read(const TdistQuantCacheArgs* args);
 int tdist_quant_decode(const TdistQuantDecodeArgs* args);
 
+/* ------------------------------------------------------------------ GEMM of 8-bit integers (csrc/kernels/gemm_int8_sm100.cu, quantize_int8.cu) */
+typedef struct TdistGemmInt8Args {
+    const void *a, *b;       /* int8 [M, K], [N, K], contiguous; K a multiple of 16 below 131072, N of 8 */
+    const void *sa, *sb;     /* fp32 [M], [N] */
+    void* c;                 /* [M, N] bf16 / fp16 */
+    int m, n, k, dtype;
+    void* status;
+    uint64_t timeout_ns;
+    void* stream;
+} TdistGemmInt8Args;
+
+int tdist_gemm_int8(const TdistGemmInt8Args* args);
+int tdist_gemm_int8_schedule_check(int wide, int units, int m_tiles, int n_tiles);
+int tdist_quant_int8_rowwise(const void* x, long long row_stride, void* out, void* scale, long long rows, int k, int dtype, void* stream);
+
 /* ------------------------------------------------------------------ device primitives, one test op each */
 enum {
     TDIST_PRIM_RING_PUT = 0, TDIST_PRIM_NOTIFY_WAIT = 1, TDIST_PRIM_NOTIFY_ADD = 2, TDIST_PRIM_PUT_SIGNAL = 3,

@@ -1,0 +1,439 @@
+// GEMM of 8-bit integers with a scale per row of A and per row of B (tokens and output channels) for sm_100a:
+//
+//   C[m, n] = (sum_k A[m, k] B[n, k]) SA[m] SB[n]        A, B signed 8 bits, sums in 32-bit integers, C bf16 / fp16
+//
+// The sums are exact (K is limited to 131071, so that even -128 x -128 throughout stays below 2^31); a result is off by the roundings
+// of the sum to fp32, of two products and of the result's type.
+//
+// tcgen05.mma kind::i8 runs at twice the rate of kind::f16 on operands of half the size, so the bytes per K step and the time of
+// its MMAs are those of the bf16 GEMM with K / 2, and the kernel is built like that one's CTA-pair tilings (gemm_sm100.cu): a cluster of two CTAs
+// computes 256 x bn (narrow) or 256 x 2 bn (WIDE, both halves sharing the A rows through the collector), K advances 128 bytes
+// per stage, TMA fills 128-byte-swizzled stages, one thread of the leader issues the MMAs, sums lie in two TMEM slots of 256 columns.
+// What follows the product differs: an epilogue thread owns a row, so SA is one number per thread, and SB four columns per load, from L1.
+//
+// Warps (192 threads): 0 = TMA producer, 1 = MMA issuer and TMEM owner, 2..5 = epilogue (TMEM -> scale -> swizzled smem -> TMA store).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstring>
+
+#include "../device/ptx.cuh"
+#include "../device/signal.cuh"
+#include "../include/tdist.h"
+#include "../runtime/host_common.h"
+#include "gemm_int8.h"
+
+namespace tdist {
+namespace int8 {
+
+constexpr int BM = 128, BN = 256, BK = 128, UMMA_K = 32;   // BK, UMMA_K: values = bytes
+constexpr int A_BYTES = BM * BK;
+constexpr int EPI_COLS = 64, EPI_BYTES = BM * EPI_COLS * 2;
+constexpr int PIPE_BYTES = 192 * 1024;
+constexpr int SMEM_TILES = PIPE_BYTES + 2 * EPI_BYTES;
+constexpr int SMEM_BYTES = SMEM_TILES + 1024 + 256;
+constexpr int THREADS = 192, TMEM_COLS = 512, MAX_STAGES = 6, GROUP_M = 8;
+constexpr int kKernelGemmInt8 = 12;
+
+struct Params {
+    CUtensorMap tm_a;   // {K, M, 1}, box {128, 128}
+    CUtensorMap tm_b;   // {K, N, 1}, box {128, bn / 2}
+    CUtensorMap tm_c;   // {N, M, 1}, box {64, 128}
+    const float *sa, *sb;
+    int m, n, k_blocks, m_tiles, n_tiles, bn, num_items, is_f16;
+    WaitCtx wctx;
+};
+
+// One unit of work of a CTA pair: `halves` neighbouring tiles of bn columns of a row of tiles.
+struct Work {
+    int m_tile, n_tile, halves;
+};
+
+// Items in groups of GROUP_M rows of tiles that sweep all columns, dealt round-robin. Narrow: an item is one tile of bn columns. WIDE: a
+// pair of neighbouring ones (the odd last tile of a row stands alone), and where the items of a last, partial round would leave at least half
+// of the units idle they are cut into halves. Returns false when the unit has nothing left.
+template <bool WIDE>
+__host__ __device__ __forceinline__ bool get_work(int num_items, int m_tiles, int n_tiles, int unit, int units, int round, Work& w) {
+    const int across = WIDE ? (n_tiles + 1) / 2 : n_tiles;
+    int t = unit + round * units, half = -1;
+    if (WIDE) {
+        const int full = num_items / units, rest = num_items - full * units;
+        if (round == full && 2 * rest <= units) {
+            if (unit >= 2 * rest) return false;
+            t = full * units + (unit >> 1);
+            half = unit & 1;
+        }
+    }
+    if (t >= num_items) return false;
+    const int span = GROUP_M * across, g = t / span, first = g * GROUP_M;
+    const int r = t - g * span, rows = m_tiles - first < GROUP_M ? m_tiles - first : GROUP_M;
+    const int col = r / rows;
+    w.m_tile = first + (r - col * rows);
+    w.n_tile = WIDE ? 2 * col : col;
+    w.halves = WIDE && w.n_tile + 1 < n_tiles ? 2 : 1;
+    if (half >= 0) {
+        if (half >= w.halves) {
+            w.halves = 0;   // the second half of an item that has one
+        } else {
+            w.n_tile += half;
+            w.halves = 1;
+        }
+    }
+    return true;
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(THREADS, 1) gemm_int8_kernel(const __grid_constant__ Params p) {
+    constexpr int B_BYTES = BN / 2 * BK;                       // of a half, per CTA
+    constexpr int STAGE_BYTES = A_BYTES + (WIDE ? 2 : 1) * B_BYTES;
+    constexpr int STAGES = PIPE_BYTES / STAGE_BYTES;           // 4 or 6
+    static_assert(STAGES <= MAX_STAGES, "barrier area too small");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SMEM_TILES);   // full, empty, tmem full (2), tmem empty (2)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 4);
+    const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+    const int cta_rank = static_cast<int>(cluster_ctarank());
+    const int unit = static_cast<int>(blockIdx.x) >> 1, units = static_cast<int>(gridDim.x) >> 1;
+    const uint32_t bars_u32 = smem_u32(bars);
+    auto bar_full = [&](uint32_t s) { return bars_u32 + 8u * s; };
+    auto bar_empty = [&](uint32_t s) { return bars_u32 + 8u * (MAX_STAGES + s); };
+    auto bar_tfull = [&](uint32_t b) { return bars_u32 + 8u * (2 * MAX_STAGES + b); };
+    auto bar_tempty = [&](uint32_t b) { return bars_u32 + 8u * (2 * MAX_STAGES + 2 + b); };
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&p.tm_a);
+        prefetch_tensormap(&p.tm_b);
+        for (uint32_t s = 0; s < STAGES; ++s) {
+            mbar_init(bar_full(s), 1);
+            mbar_init(bar_empty(s), 1);
+        }
+        for (uint32_t b = 0; b < 2; ++b) {
+            mbar_init(bar_tfull(b), 1);
+            mbar_init(bar_tempty(b), 8);   // an arrival per epilogue warp of both CTAs
+        }
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc<2>(smem_u32(tmem_slot), TMEM_COLS);
+        tmem_relinquish<2>();
+    }
+    tc_fence_before();
+    cluster_arrive();   // the other CTA signals this one's barriers
+    cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    pdl_wait_and_release();
+
+    Work w;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, phase = 1;
+            for (int round = 0; get_work<WIDE>(p.num_items, p.m_tiles, p.n_tiles, unit, units, round, w); ++round) {
+                if (w.halves == 0) continue;
+                const int row = (w.m_tile * 2 + cta_rank) * BM;
+                const int col = w.n_tile * p.bn + cta_rank * (p.bn / 2);
+                const uint32_t tx = A_BYTES + static_cast<uint32_t>(w.halves * (p.bn / 2) * BK);
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    mbar_wait(bar_empty(s), phase, p.wctx, 2);
+                    const uint32_t sa = smem_u32(smem) + s * STAGE_BYTES;
+                    if (cta_rank == 0) mbar_expect_tx(bar_full(s), 2 * tx);   // both CTAs' bytes are counted on the leader's barrier
+                    const uint32_t full = mapa_u32(bar_full(s), 0);
+                    tma_load_3d_pair(sa, &p.tm_a, full, kb * BK, row, 0);
+                    tma_load_3d_pair(sa + A_BYTES, &p.tm_b, full, kb * BK, col, 0);
+                    if (WIDE && w.halves == 2) tma_load_3d_pair(sa + A_BYTES + B_BYTES, &p.tm_b, full, kb * BK, col + p.bn, 0);
+                    if (++s == STAGES) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && cta_rank == 0) {
+            const uint32_t idesc = umma_idesc_s8(2 * BM, static_cast<uint32_t>(p.bn));
+            uint32_t s = 0, phase = 0, uses[2] = {0, 0}, next = 0;
+            for (int round = 0; get_work<WIDE>(p.num_items, p.m_tiles, p.n_tiles, unit, units, round, w); ++round) {
+                if (w.halves == 0) continue;
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    mbar_wait(bar_full(s), phase, p.wctx, 4);
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem) + s * STAGE_BYTES;
+                    const uint64_t ad = umma_desc_k_sw128(sa), bd = umma_desc_k_sw128(sa + A_BYTES), bd1 = umma_desc_k_sw128(sa + A_BYTES + B_BYTES);
+                    if (WIDE && w.halves == 2 && kb > 0) {
+#pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; ++k) {
+                            umma_s8_pair_collect<kCollectorFill>(tmem_base, ad + 2 * k, bd + 2 * k, idesc, 1u);
+                            umma_s8_pair_collect<kCollectorLastUse>(tmem_base + BN, ad + 2 * k, bd1 + 2 * k, idesc, 1u);
+                        }
+                    } else {
+                        for (int h = 0; h < w.halves; ++h) {
+                            const uint32_t slot = w.halves == 2 ? static_cast<uint32_t>(h) : next;
+                            if (kb == 0) {
+                                mbar_wait(bar_tempty(slot), (uses[slot] & 1u) ^ 1u, p.wctx, 3);   // its previous sums have been read
+                                tc_fence_after();
+                            }
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k)
+                                umma_s8<2>(tmem_base + slot * BN, ad + 2 * k, (h ? bd1 : bd) + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+                        }
+                    }
+                    umma_commit_pair(bar_empty(s), 3);
+                    if (++s == STAGES) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+                for (int h = 0; h < w.halves; ++h) {
+                    const uint32_t slot = w.halves == 2 ? static_cast<uint32_t>(h) : next;
+                    umma_commit_pair(bar_tfull(slot), 3);
+                    ++uses[slot];
+                }
+                if (w.halves == 1) next ^= 1u;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;   // TMEM lane quadrant this warp may read
+        const int row_in_tile = q * 32 + lane;
+        const bool issuer = warp == 2 && lane == 0;
+        uint32_t uses[2] = {0, 0}, next = 0, chunk = 0;
+        for (int round = 0; get_work<WIDE>(p.num_items, p.m_tiles, p.n_tiles, unit, units, round, w); ++round) {
+            if (w.halves == 0) continue;
+            const int row = (w.m_tile * 2 + cta_rank) * BM;
+            const float sa = row + row_in_tile < p.m ? p.sa[row + row_in_tile] : 0.f;
+            for (int h = 0; h < w.halves; ++h) {
+                const uint32_t slot = w.halves == 2 ? static_cast<uint32_t>(h) : next;
+                mbar_wait(bar_tfull(slot), uses[slot] & 1u, p.wctx, 5);
+                tc_fence_after();
+                ++uses[slot];
+                const int col = (w.n_tile + h) * p.bn;
+#pragma unroll 1
+                for (int c = 0; c < p.bn / EPI_COLS; ++c) {
+                    uint32_t r[2][32];
+                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + slot * BN + c * EPI_COLS;
+                    tmem_ld_32x32(taddr, r[0]);
+                    tmem_ld_32x32(taddr + 32, r[1]);
+                    tmem_ld_wait();
+                    if (c == p.bn / EPI_COLS - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(bar_tempty(slot), 0);
+                    }
+                    uint8_t* cs = smem + PIPE_BYTES + (chunk++ & 1) * EPI_BYTES;
+                    uint4 o[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = col + c * EPI_COLS + 8 * j;
+                        uint32_t v[4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float4 sb = at < p.n ? *reinterpret_cast<const float4*>(p.sb + at + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);   // N is a multiple of 8
+                            const uint32_t* x = r[j >> 2] + 8 * (j & 3) + 4 * i;
+                            const float f0 = static_cast<float>(static_cast<int>(x[0])) * sa * sb.x, f1 = static_cast<float>(static_cast<int>(x[1])) * sa * sb.y;
+                            const float f2 = static_cast<float>(static_cast<int>(x[2])) * sa * sb.z, f3 = static_cast<float>(static_cast<int>(x[3])) * sa * sb.w;
+                            v[2 * i] = p.is_f16 ? pack_f16x2(f0, f1) : pack_bf16x2(f0, f1);
+                            v[2 * i + 1] = p.is_f16 ? pack_f16x2(f2, f3) : pack_bf16x2(f2, f3);
+                        }
+                        o[j] = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                    named_barrier(1, 128);   // the store that last read this buffer has drained
+                    uint8_t* rowp = cs + row_in_tile * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(rowp + ((j ^ (row_in_tile & 7)) << 4)) = o[j];
+                    fence_proxy_async_smem();
+                    named_barrier(1, 128);   // the buffer is complete
+                    if (issuer) {
+                        if (col + c * EPI_COLS < p.n && row < p.m) tma_store_3d(&p.tm_c, smem_u32(cs), col + c * EPI_COLS, row, 0);
+                        bulk_commit();       // one group per chunk, stored or not: the wait below is for the other buffer's
+                        bulk_wait_read<1>();
+                    }
+                }
+            }
+            if (w.halves == 1) next ^= 1u;
+        }
+        if (issuer) bulk_wait<0>();
+        __syncwarp();
+    }
+    tc_fence_before();
+    cluster_arrive();   // neither CTA frees TMEM or leaves while the other may touch its TMEM, smem or barriers
+    cluster_wait();
+    if (warp == 1) tmem_dealloc<2>(tmem_base, TMEM_COLS);
+}
+
+}  // namespace int8
+}  // namespace tdist
+
+using namespace tdist;
+using tdist_host::fail;
+
+namespace {
+
+struct Plan {
+    bool few_rows, wide;
+    int bn, m_tiles, n_tiles, num_items, grid;
+    tdist_host::SkinnyPlan skinny;
+};
+
+const void* kernel_of(bool wide) {
+    return wide ? reinterpret_cast<const void*>(&tdist::int8::gemm_int8_kernel<true>) : reinterpret_cast<const void*>(&tdist::int8::gemm_int8_kernel<false>);
+}
+
+// CTAs of the pair kernel that are resident at once on the current device; opts in to its shared memory. Cached per device.
+int resident(bool wide) {
+    using namespace tdist::int8;
+    static int cache[64][2] = {};
+    int dev = 0;
+    const int nominal = tdist_host::sm_count() & ~1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return nominal;
+    }
+    int& slot = cache[dev][wide];
+    if (slot > 0) return slot;
+    int clusters = 0;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(nominal));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int result = nominal;
+    if (cudaFuncSetAttribute(kernel_of(wide), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&clusters, kernel_of(wide), &cfg) == cudaSuccess && clusters > 0)
+        result = 2 * clusters;
+    cudaGetLastError();
+    slot = result;
+    return result;
+}
+
+// The tiling whose rounds end soonest, by the times of a 128-byte K block that the bf16 kernel of the same shape has (a narrow tile 290 ns + 0.36
+// per column, a wide one 175 + 2.1 per column of a half), and the few-row kernel where its estimate is lower.
+Plan make_plan(const TdistGemmInt8Args* a) {
+    using namespace tdist::int8;
+    Plan best;
+    memset(&best, 0, sizeof(best));
+    double best_s = 1e30;
+    const int k_blocks = (a->k + BK - 1) / BK;
+    const double hbm_s = (static_cast<double>(a->n) * a->k + static_cast<double>(a->m) * a->k + 2.0 * a->m * a->n) / 6.3e12;
+    for (int wide = 1; wide >= 0; --wide)
+        for (int bn = BN; bn >= 128; bn -= 64) {
+            Plan c;
+            memset(&c, 0, sizeof(c));
+            c.wide = wide;
+            c.bn = bn;
+            c.m_tiles = (a->m + 2 * BM - 1) / (2 * BM);
+            c.n_tiles = (a->n + bn - 1) / bn;
+            if (wide && c.n_tiles < 2) continue;
+            c.num_items = c.m_tiles * (wide ? (c.n_tiles + 1) / 2 : c.n_tiles);
+            const int units = resident(wide) / 2, most = wide ? 2 * c.num_items : c.num_items;
+            c.grid = 2 * (units < most ? units : most);
+            const int u = c.grid / 2, full = c.num_items / u, rest = c.num_items - full * u;
+            const double narrow_s = k_blocks * (290 + 0.36 * bn) * 1e-9 + 0.3e-6, whole_s = wide ? k_blocks * (175 + 2.1 * bn) * 1e-9 + 3e-6 : narrow_s;
+            const double sm_s = full * whole_s + (rest == 0 ? 0.0 : (wide && 2 * rest <= u ? narrow_s : whole_s));
+            const double t = (sm_s > hbm_s ? sm_s : hbm_s) + 5e-6;
+            if (t < 0.96 * best_s) {
+                best_s = t;
+                best = c;
+            }
+        }
+    if (tdist_host::int8_skinny_plan(a->m, a->n, a->k, best_s, &best.skinny)) best.few_rows = true;
+    return best;
+}
+
+}  // namespace
+
+extern "C" int tdist_gemm_int8(const TdistGemmInt8Args* a) {
+    using namespace tdist::int8;
+    if (a->m < 0 || a->n < 0 || a->k < 1) return fail(TDIST_EINVAL, "int8 GEMM: bad shape");
+    if (a->n % 8 || a->k % 16) return fail(TDIST_EINVAL, "int8 GEMM: N must be a multiple of 8, K of 16");
+    if (a->k > 131071) return fail(TDIST_EINVAL, "int8 GEMM: K must be below 131072");
+    if (a->dtype != TDIST_BF16 && a->dtype != TDIST_F16) return fail(TDIST_EINVAL, "int8 GEMM: C must be bf16 or fp16");
+    if ((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->b) | reinterpret_cast<uintptr_t>(a->c) | reinterpret_cast<uintptr_t>(a->sb)) & 15)
+        return fail(TDIST_EINVAL, "int8 GEMM: A, B, C and SB must lie on 16 bytes");
+    if (a->m == 0 || a->n == 0) return 0;
+    const Plan plan = make_plan(a);
+    if (plan.few_rows) return tdist_host::int8_skinny_run(a, plan.skinny);
+    Params p;
+    memset(&p, 0, sizeof(p));
+    const uint64_t K = a->k, N = a->n, M = a->m;
+    int rc;
+    {
+        const uint64_t dims[3] = {K, M, 1}, strides[2] = {K, K * M};
+        const uint32_t box[3] = {BK, BM, 1};
+        if ((rc = tdist_host::encode_tmap(&p.tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 3, a->a, dims, strides, box, tdist_host::Swizzle::B128))) return rc;
+    }
+    {
+        const uint64_t dims[3] = {K, N, 1}, strides[2] = {K, K * N};
+        const uint32_t box[3] = {BK, static_cast<uint32_t>(plan.bn / 2), 1};
+        if ((rc = tdist_host::encode_tmap(&p.tm_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 3, a->b, dims, strides, box, tdist_host::Swizzle::B128))) return rc;
+    }
+    {
+        const uint64_t dims[3] = {N, M, 1}, strides[2] = {N * 2, N * M * 2};
+        const uint32_t box[3] = {EPI_COLS, BM, 1};
+        const CUtensorMapDataType dt = a->dtype == TDIST_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if ((rc = tdist_host::encode_tmap(&p.tm_c, dt, 2, 3, a->c, dims, strides, box, tdist_host::Swizzle::B128))) return rc;
+    }
+    p.sa = static_cast<const float*>(a->sa);
+    p.sb = static_cast<const float*>(a->sb);
+    p.m = a->m;
+    p.n = a->n;
+    p.k_blocks = (a->k + BK - 1) / BK;
+    p.m_tiles = plan.m_tiles;
+    p.n_tiles = plan.n_tiles;
+    p.bn = plan.bn;
+    p.num_items = plan.num_items;
+    p.is_f16 = a->dtype == TDIST_F16;
+    p.wctx.status = static_cast<Status*>(a->status);
+    p.wctx.timeout_ns = a->timeout_ns;
+    p.wctx.kernel_id = kKernelGemmInt8;
+    resident(plan.wide);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.grid));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.stream = static_cast<cudaStream_t>(a->stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1] = tdist_host::pdl_attribute();
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (plan.wide) TDIST_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_int8_kernel<true>, p));
+    else TDIST_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_int8_kernel<false>, p));
+    return 0;
+}
+
+// Replays the schedule on the host: every tile must be given to exactly one unit. Returns 0, or the number of the first check that failed.
+extern "C" int tdist_gemm_int8_schedule_check(int wide, int units, int m_tiles, int n_tiles) {
+    using namespace tdist::int8;
+    if (units < 1 || m_tiles < 1 || n_tiles < 1) return -1;
+    const int items = m_tiles * (wide ? (n_tiles + 1) / 2 : n_tiles);
+    char* seen = new char[static_cast<size_t>(m_tiles) * n_tiles]();
+    int rc = 0;
+    for (int u = 0; u < units && rc == 0; ++u) {
+        Work w;
+        for (int round = 0; rc == 0; ++round) {
+            if (!(wide ? get_work<true>(items, m_tiles, n_tiles, u, units, round, w) : get_work<false>(items, m_tiles, n_tiles, u, units, round, w))) break;
+            if (round > items / units + 1) rc = 1;
+            for (int h = 0; h < w.halves && rc == 0; ++h) {
+                if (w.m_tile < 0 || w.m_tile >= m_tiles || w.n_tile + h >= n_tiles) rc = 2;
+                else if (seen[static_cast<size_t>(w.m_tile) * n_tiles + w.n_tile + h]++) rc = 3;
+            }
+        }
+    }
+    for (size_t i = 0; rc == 0 && i < static_cast<size_t>(m_tiles) * n_tiles; ++i)
+        if (!seen[i]) rc = 4;
+    delete[] seen;
+    return rc;
+}

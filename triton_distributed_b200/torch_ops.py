@@ -26,6 +26,7 @@ from .ops import collectives as CO
 from .ops import flash_decode as FD
 from .ops import gemm as G
 from .ops import gemm_fp8 as F8
+from .ops import gemm_int8 as G8
 from .ops import moe_tp as MT
 from .ops import moe_utils as MU
 from .ops import paged_attention as PA
@@ -368,8 +369,31 @@ def _(q, k_codes, v_codes, k_scales, v_scales, kv_lens, block_table, window, sin
     return q.new_empty(q.shape)
 
 
+# ---------------------------------------------------------------------------- products of 8-bit integers
+@_op("tdist::quantize_int8_rowwise", mutates_args=())
+def quantize_int8_rowwise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(int8 [M, K], fp32 scales [M])"""
+    return G8.quantize_int8_rowwise(x)
+
+
+@quantize_int8_rowwise.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((x.shape[0],), dtype=torch.float32)
+
+
+@_op("tdist::gemm_int8", mutates_args=())
+def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    """(a @ b.T) sa[:, None] sb, sums in 32-bit integers"""
+    return G8.gemm_int8(a, sa, b, sb, out_dtype)
+
+
+@gemm_int8.register_fake
+def _(a, sa, b, sb, out_dtype):
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
+
+
 OP_NAMES = ["gemm", "ag_gemm", "gemm_rs", "gemm_fp8", "ag_gemm_fp8", "group_gemm", "reduce_scatter", "barrier_all", "moe_topk_softmax",
             "moe_ag_scatter_align_block_size", "moe_dispatch", "moe_combine", "ep_dispatch", "ep_combine", "gqa_fwd_batch_decode",
             "gqa_fwd_batch_decode_intra_rank", "sp_gqa_fwd_batch_decode", "lse_combine",
             "gqa_fwd_window_decode", "gqa_fwd_window_prefill", "gqa_fwd_shared_prefix_decode", "sample_tokens",
-            "kv_cache_write", "kv_cache_read", "gqa_fwd_quantized_decode"]
+            "kv_cache_write", "kv_cache_read", "gqa_fwd_quantized_decode", "quantize_int8_rowwise", "gemm_int8"]
