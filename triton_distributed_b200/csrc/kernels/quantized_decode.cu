@@ -3,12 +3,18 @@
 //   s_j = scale q . k_j, k_j = ks_j c_j             4 bits: k_j = step_jg c_j + least_jg in every group g of 64 dimensions
 //   o   = sum_j p_j vs_j c'_j / sum_j p_j           p_j = exp(s_j - max)
 //
-// The rows are never dequantised. Codes are small whole numbers, exact in fp16, so the products with them run on tensor cores
-// (mma.sync m16n8k16, fp16 operands, fp32 sums) and the scales are applied where they are one number per key: to the score (4 bits: to
-// a group's part of it, and least_jg times the sum of q over the group is added), and to the weight p_j vs_j, with the sum of p_j least_jg
-// kept beside the product. A query is brought to [2^13, 2^14) by a power of two first, so that bf16's range fits fp16 (values 2^-28 of
-// the largest lose bits). Weights are divided by a power of two above all vs_j so far, so that p_j vs_j / S lies in [0, 1] whatever the
-// values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest.
+// The rows are never dequantised: the scales are applied where they are one number per key, to the score (4 bits: to a group's part of it, and
+// least_jg times the sum of q over the group is added), and to the weight p_j vs_j, with the sum of p_j least_jg kept beside the product.
+//
+// K. Codes are 8-bit operands of the integer MMA (m16n8k32, u8 x s8) as they lie in memory, 4-bit ones after two logic instructions
+// per eight. A query is brought to 16 bits for it, rint(q 32512 / max |q|), as a high and a low byte with a product each: the sums are exact, the second
+// continues from 256 times the first, and 128 times the sum of q takes the codes' offset off. (As fp16 operands the codes of a tile cost 64
+// instructions, and the kernel was bound by its issue slots: 567 per tile of 16 x 128, 32 x 16384 keys of 8 kv heads 148 us.)
+// A score is off by up to 2^-17 max |q| sum |k_d|: a 16-bit query against bf16's 8 bits.
+//
+// V. Codes become fp16, exactly, two tokens per register. Weights are divided by a power of two above all vs_j so far, so that p_j vs_j / S lies
+// in [0, 1] whatever the values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest. 4-bit codes are taken as
+// c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
 // S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix. What is different is the way of the codes: a byte is no MMA operand, so they go
@@ -73,12 +79,20 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // A byte or nibble n under the exponent of 1024 is the fp16 number 1024 + n; in the upper nibble of a byte, 1024 + 16 n.
 constexpr uint32_t kMagic = 0x64006400u;
 constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a 0x64
 __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) { return hsub2(__byte_perm(w, kMagic, sel), 0x64806480u); }   // - 1152
-__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return hsub2((w & 0x000f000fu) | kMagic, kMagic); }
-__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return hfma2((w & 0x00f000f0u) | kMagic, 0x2c002c00u, 0xd400d400u); }   // / 16 - 64
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return hsub2((w & 0x000f000fu) | kMagic, 0x64086408u); }                     // - 1032: n - 8
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return hfma2((w & 0x00f000f0u) | kMagic, 0x2c002c00u, 0xd480d480u); }       // / 16 - 72: n - 8
+__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
+    return __byte_perm(__byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(b), 0x0040u), __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(d), 0x0040u), 0x5410u);
+}
 
 __device__ __forceinline__ uint32_t ldg32(const void* p) {
     uint32_t v;
@@ -160,85 +174,97 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
     const char* ksc = p.ks + kvh * p.scale_head;
     const char* vsc = p.vs + kvh * p.scale_head;
 
-    // A tile's place: its first token and the limits of what is seen of it
     auto first_token = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + t_lo) * TOK; };
-    // page (and row) of the tile's first token (WHOLE: pages of a multiple of 16), or of token `lane`; -1: not seen, or no page of the cache
-    auto lookup = [&](int i, int& page, int& row) {
-        page = -1;
-        row = 0;
+    // Where a tile lies: byte offsets of its first token (WHOLE: pages of a multiple of 16), or of token `lane` of it, in the codes and in the
+    // scales. A token that is not seen, or whose page the cache does not have, is read from the cache's first place and has `live` false.
+    struct Place {
+        long long code, scale;
+        bool live;
+    };
+    auto lookup = [&](int i) {
+        Place at{0, 0, false};
         if (i < i1 && (WHOLE || lane < TOK)) {
             const int t = first_token(i) + (WHOLE ? 0 : lane);
-            const bool seen = WHOLE || (i < sink_tiles ? t < first : t >= lo && t < n);
-            if (seen) {
+            if (WHOLE || (i < sink_tiles ? t < first : t >= lo && t < n)) {
                 const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-                page = static_cast<int>(ldg32(table + in_table));
-                row = t - in_table * p.page_size;
-                if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.blocks)) page = -1;
+                const int page = static_cast<int>(ldg32(table + in_table));
+                const int row = t - in_table * p.page_size;
+                if (static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks)) {
+                    at.code = page * p.code_block + row * p.code_token;
+                    at.scale = page * p.scale_block + row * p.scale_token;
+                    at.live = true;
+                }
             }
         }
+        return at;
     };
+    const uint8_t* k_lane = kc + c * (2 * BITS) + (WHOLE ? g * p.code_token : 0);
+    const uint8_t* v_lane = vc + g * (S::VB / 8) + (WHOLE ? 2 * c * p.code_token : 0);
+    const char* ks_lane = ksc + (WHOLE ? g * p.scale_token : 0);
+    const char* vs_lane = vsc + (WHOLE ? g * p.scale_token : 0);
+    const long long code8 = 8 * p.code_token, scale8 = 8 * p.scale_token;
     Words<S::KW> kw[2][S::KC];     // tokens g, g + 8
     Words<S::NG> kscale[2], vscale[2];
     Words<S::VW> vw[4][S::VC];     // tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-    auto place = [&](int page, int row, int r, long long block, long long token) -> long long {
-        if (WHOLE) return page < 0 ? -1 : page * block + (row + r) * token;
-        const int pg = __shfl_sync(0xffffffffu, page, r), rw = __shfl_sync(0xffffffffu, row, r);
-        return pg < 0 ? -1 : pg * block + rw * token;
-    };
-    auto load_k = [&](int page, int row) {
+    auto load_k = [&](const Place& at) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const long long at = place(page, row, g + 8 * r, p.code_block, p.code_token);
-            const long long sat = place(page, row, g + 8 * r, p.scale_block, p.scale_token);
-#pragma unroll
-            for (int j = 0; j < S::KC; ++j) {
-                if (at >= 0) kw[r][j] = load_words<S::KW>(kc + at + j * (64 * BITS / 8) + c * (16 * BITS / 8));
-                else
-#pragma unroll
-                    for (int w = 0; w < S::KW; ++w) kw[r][j].w[w] = 0;
-            }
-            if (sat >= 0) {
-                kscale[r] = load_words<S::NG>(ksc + sat);
+            const uint8_t* src;
+            const char* ssrc;
+            bool live = at.live;
+            if (WHOLE) {
+                src = k_lane + at.code + (r ? code8 : 0);
+                ssrc = ks_lane + at.scale + (r ? scale8 : 0);
             } else {
+                src = k_lane + __shfl_sync(0xffffffffu, at.code, g + 8 * r);
+                ssrc = ks_lane + __shfl_sync(0xffffffffu, at.scale, g + 8 * r);
+                live = __shfl_sync(0xffffffffu, static_cast<int>(at.live), g + 8 * r) != 0;
+            }
+#pragma unroll
+            for (int j = 0; j < S::KC; ++j) kw[r][j] = load_words<S::KW>(src + j * (8 * BITS));
+            kscale[r] = load_words<S::NG>(ssrc);
+            if (!live) {
 #pragma unroll
                 for (int w = 0; w < S::NG; ++w) kscale[r].w[w] = 0;
             }
         }
     };
-    auto load_v = [&](int page, int row) {
+    auto load_v = [&](const Place& at) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const long long at = place(page, row, 2 * c + (r & 1) + (r >> 1) * 8, p.code_block, p.code_token);
+            const uint8_t* src = WHOLE ? v_lane + at.code + (r & 1 ? p.code_token : 0) + (r >> 1 ? code8 : 0)
+                                       : v_lane + __shfl_sync(0xffffffffu, at.code, 2 * c + (r & 1) + (r >> 1) * 8);
 #pragma unroll
-            for (int j = 0; j < S::VC; ++j) {
-                if (at >= 0) vw[r][j] = load_words<S::VW>(vc + at + j * S::VB + g * (S::VB / 8));
-                else
-#pragma unroll
-                    for (int w = 0; w < S::VW; ++w) vw[r][j].w[w] = 0;
-            }
+            for (int j = 0; j < S::VC; ++j) vw[r][j] = load_words<S::VW>(src + j * S::VB);
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const long long sat = place(page, row, g + 8 * r, p.scale_block, p.scale_token);
-            if (sat >= 0) {
-                vscale[r] = load_words<S::NG>(vsc + sat);
+            const char* ssrc;
+            bool live = at.live;
+            if (WHOLE) {
+                ssrc = vs_lane + at.scale + (r ? scale8 : 0);
             } else {
+                ssrc = vs_lane + __shfl_sync(0xffffffffu, at.scale, g + 8 * r);
+                live = __shfl_sync(0xffffffffu, static_cast<int>(at.live), g + 8 * r) != 0;
+            }
+            vscale[r] = load_words<S::NG>(ssrc);
+            if (!live) {
 #pragma unroll
                 for (int w = 0; w < S::NG; ++w) vscale[r].w[w] = 0;
             }
         }
     };
 
-    int page, row;
-    lookup(i0, page, row);
-    load_k(page, row);
-    load_v(page, row);
-    lookup(i0 + WARPS, page, row);
+    Place next = lookup(i0);
+    load_k(next);
+    load_v(next);
+    next = lookup(i0 + WARPS);
 
     // ---- q as the second operand: column g of the MMA is head 8 h + g, its dimensions 16 c .. 16 c + 15 of every 64 are this lane's
-    uint32_t qf[NH][S::KC][4][2];
+    uint32_t qf[NH][S::KC][4][2];  // high and low bytes of four dimensions
     float factor[NH][2];           // of heads 8 h + 2 c + {0, 1}: what turns a product of codes into a score in units of log2
-    float qsum[NH][2][S::NG];      // 4 bits: the sum of the scaled q over a group
+    int bias[NH][2];               // 8 bits: 128 times the sum of the 16-bit q
+    float qsum[NH][2][S::NG];      // 4 bits: that sum over a group
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
         const int head = 8 * h + g;
@@ -263,40 +289,42 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^up brings the largest to [2^13, 2^14); none for zeros, infinities and NaN. 2^up and its inverse are normal numbers
-        const int e = static_cast<int>(top >> 23);
-        const int up = e == 0 || e == 255 ? 0 : min(100, 140 - e);
-        const float mul = head < heads ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : 0.f;
+        // magnitudes below 2^-100 count as that; a query with a NaN or an infinity has a factor of NaN, and so has its result
+        const bool good = top < 0x7f800000u;
+        const float most = fmaxf(good ? __uint_as_float(top) : 1.f, 7.888609052210118e-31f);
+        const float mul = head < heads && good ? 32512.f / most : 0.f;
+        int sum = 0;
 #pragma unroll
         for (int j = 0; j < S::KC; ++j) {
-            float sum = 0.f;
+            int part = 0, hi[16], low8[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                f[j][k] = head < heads ? __half2float(__float2half_rn(f[j][k] * mul)) : 0.f;
-                sum += f[j][k];
+                const int v = max(-32512, min(32512, __float2int_rn(f[j][k] * mul)));
+                hi[k] = (v + 128) >> 8;
+                low8[k] = v - 256 * hi[k];
+                part += v;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                // the order in which the codes of a chunk come out of their words
-                if (BITS == 8) {
-                    qf[h][j][k][0] = pack_f16x2(f[j][4 * k], f[j][4 * k + 1]);
-                    qf[h][j][k][1] = pack_f16x2(f[j][4 * k + 2], f[j][4 * k + 3]);
-                } else {
-                    const int d = (k >> 1) * 8 + (k & 1) * 2;
-                    qf[h][j][k][0] = pack_f16x2(f[j][d], f[j][d + 4]);
-                    qf[h][j][k][1] = pack_f16x2(f[j][d + 1], f[j][d + 5]);
-                }
+                // four codes of a register of the first operand
+                const int d = BITS == 8 ? 4 * k : 8 * (k >> 1) + (k & 1), e = BITS == 8 ? 1 : 2;
+                qf[h][j][k][0] = pack_bytes(hi[d], hi[d + e], hi[d + 2 * e], hi[d + 3 * e]);
+                qf[h][j][k][1] = pack_bytes(low8[d], low8[d + e], low8[d + 2 * e], low8[d + 3 * e]);
             }
+            part += __shfl_xor_sync(0xffffffffu, part, 1);
+            part += __shfl_xor_sync(0xffffffffu, part, 2);
+            sum += part;
             if (BITS == 4) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) qsum[h][r][j] = __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4);
+                for (int r = 0; r < 2; ++r) qsum[h][r][j] = static_cast<float>(__shfl_sync(0xffffffffu, part, (2 * c + r) * 4));
             }
         }
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * p.scale;
+        const float down = good ? most * (1.f / 32512.f) * p.scale : __uint_as_float(0x7fffffffu);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) factor[h][r] = __shfl_sync(0xffffffffu, down, (2 * c + r) * 4) * (p.soft_cap > 0.f ? 1.f : kLog2e);
+        for (int r = 0; r < 2; ++r) {
+            factor[h][r] = __shfl_sync(0xffffffffu, down, (2 * c + r) * 4) * (p.soft_cap > 0.f ? 1.f : kLog2e);
+            bias[h][r] = __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4) * 128;
+        }
     }
 
     // ---- sums: O^T in units of `unit` (a power of two), columns are heads 8 h + 2 c + {0, 1}
@@ -319,44 +347,39 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
     const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
 
     for (int i = i0; i < i1; i += WARPS) {
-        // ---- S^T = K Q^T, a sum per group of dimensions
+        // ---- S^T = K Q^T, a sum per group of dimensions: the high bytes of q, then 256 times that and the low ones
         float s[NH][4];
-        float acc[NH][S::NG][4];
+        int acc[NH][S::NG][4];
+        uint32_t ka[S::KC][4][2];    // [chunk][register][token]
+#pragma unroll
+        for (int j = 0; j < S::KC; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    ka[j][k][r] = BITS == 8 ? kw[r][j].w[k % S::KW] : (kw[r][j].w[(k >> 1) % S::KW] >> (4 * (k & 1))) & 0x0f0f0f0fu;
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int k = 0; k < S::NG; ++k) acc[h][k][0] = acc[h][k][1] = acc[h][k][2] = acc[h][k][3] = 0.f;
+            for (int k = 0; k < S::NG; ++k) {
+                acc[h][k][0] = acc[h][k][1] = acc[h][k][2] = acc[h][k][3] = 0;
 #pragma unroll
-        for (int j = 0; j < S::KC; ++j) {
-            constexpr int last = S::NG - 1;
+                for (int part = 0; part < 2; ++part) {
+                    if (part) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint32_t a[4];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    if (BITS == 8) {
-                        const uint32_t w = kw[r][j].w[k % S::KW];
-                        a[r] = bytes_to_half2(w, kLowBytes);
-                        a[2 + r] = bytes_to_half2(w, kHighBytes);
-                    } else {
-                        const uint32_t w = kw[r][j].w[k >> 1] >> ((k & 1) * 8);
-                        a[r] = low_nibbles(w);
-                        a[2 + r] = high_nibbles(w);
+                        for (int e = 0; e < 4; ++e) acc[h][k][e] = (acc[h][k][e] << 8) - (BITS == 8 ? bias[h][e & 1] : 0);
                     }
+#pragma unroll
+                    for (int j = k * (S::KC / S::NG); j < (k + 1) * (S::KC / S::NG); ++j)
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+                            mma_u8s8(acc[h][k], ka[j][2 * m][0], ka[j][2 * m][1], ka[j][2 * m + 1][0], ka[j][2 * m + 1][1], qf[h][j][2 * m][part], qf[h][j][2 * m + 1][part]);
                 }
-#pragma unroll
-                for (int h = 0; h < NH; ++h) mma_f16(acc[h][min(j, last)], a[0], a[1], a[2], a[3], qf[h][j][k][0], qf[h][j][k][1]);
             }
-        }
-        // ---- scales, cap, mask
+        // ---- scales, cap; masks at the ends of what is seen
         const int t0 = first_token(i);
-        const bool sink = i < sink_tiles;
-        bool higher = false, seen[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int t = t0 + g + 8 * r;
-            seen[r] = sink ? t < first : t >= lo && t < n;
-        }
+        const bool sink = i < sink_tiles, edge = sink || t0 < lo || t0 + TOK > n;
+        bool higher = false;
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -364,32 +387,51 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
                 const int r = e >> 1;
                 float v = 0.f;
                 if (BITS == 8) {
-                    v = acc[h][0][e] * __uint_as_float(kscale[r].w[0]);
+                    v = static_cast<float>(acc[h][0][e]) * __uint_as_float(kscale[r].w[0]);
                 } else {
 #pragma unroll
                     for (int k = 0; k < S::NG; ++k)
-                        v += __uint_as_float(kscale[r].w[k] << 16) * acc[h][k][e] + __uint_as_float(kscale[r].w[k] & 0xffff0000u) * qsum[h][e & 1][k];
+                        v += __uint_as_float(kscale[r].w[k] << 16) * static_cast<float>(acc[h][k][e]) + __uint_as_float(kscale[r].w[k] & 0xffff0000u) * qsum[h][e & 1][k];
                 }
-                v *= factor[h][e & 1];
-                if (p.soft_cap > 0.f) v = soft_cap(v * kLog2e, v * cap_inv, p.soft_cap * kLog2e);
-                v = seen[r] ? v : -CUDART_INF_F;
-                s[h][e] = v;
-                higher |= v > m_run[h][e & 1];
+                s[h][e] = v * factor[h][e & 1];
             }
+        if (p.soft_cap > 0.f) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[h][e] = soft_cap(s[h][e] * kLog2e, s[h][e] * cap_inv, p.soft_cap * kLog2e);
+        }
         // ---- the values' scales, as weights in units of `unit`
         float vmul[2][S::NG], vleast[2][S::NG];
         float most = 0.f;
+        if (edge) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int t = t0 + g + 8 * r;
+                const bool seen = sink ? t < first : t >= lo && t < n;
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) s[h][2 * r + e] = seen ? s[h][2 * r + e] : -CUDART_INF_F;
+#pragma unroll
+                for (int k = 0; k < S::NG; ++k) vscale[r].w[k] = seen ? vscale[r].w[k] : 0;
+            }
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) {
-                vmul[r][k] = seen[r] ? __uint_as_float(BITS == 8 ? vscale[r].w[k] : vscale[r].w[k] << 16) : 0.f;
-                if (BITS == 4) vleast[r][k] = seen[r] ? __uint_as_float(vscale[r].w[k] & 0xffff0000u) : 0.f;
+                vmul[r][k] = __uint_as_float(BITS == 8 ? vscale[r].w[k] : vscale[r].w[k] << 16);
+                if (BITS == 4) vleast[r][k] = fmaf(8.f, vmul[r][k], __uint_as_float(vscale[r].w[k] & 0xffff0000u));
                 most = fmaxf(most, vmul[r][k]);
             }
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) higher |= s[h][e] > m_run[h][e & 1];
         higher |= most > unit;
         // the next tile's keys: theirs are the registers that are free now
-        if (i + WARPS < i1) load_k(page, row);
+        if (i + WARPS < i1) load_k(next);
         if (__any_sync(0xffffffffu, higher)) {
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
@@ -485,8 +527,8 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
             }
         }
         if (i + WARPS < i1) {
-            load_v(page, row);
-            lookup(i + 2 * WARPS, page, row);
+            load_v(next);
+            next = lookup(i + 2 * WARPS);
         }
     }
 
@@ -704,6 +746,10 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     if ((reinterpret_cast<uintptr_t>(a->q) & 15) || (reinterpret_cast<uintptr_t>(a->out) & 3))
         return fail(TDIST_EINVAL, "quantised decode: q must lie on 16 bytes, out on 4");
     if (c.B == 0) return 0;
+    if (c.blocks == 0) {   // every page reads as zeros, and there is no place to read instead
+        TDIST_CUDA_OK(cudaMemsetAsync(a->out, 0, static_cast<size_t>(c.B) * a->Hq * c.head_dim * 2, static_cast<cudaStream_t>(c.stream)));
+        return 0;
+    }
     Params p;
     memset(&p, 0, sizeof(p));
     p.q = a->q;
