@@ -17,11 +17,11 @@
 // c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
-// S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix. What is different is the way of the codes: a byte is no MMA operand, so they go
-// through registers anyway, and they are loaded there straight from global memory, without shared memory. The sum over a row's dimensions may
-// run in any order and the output's dimensions may be dealt to the MMA's rows in any order, so both are chosen by what a wide load
-// gives: of 64 dimensions of a key, the four lanes of a quad take 16 neighbouring ones each, and of a value's each eighth lane an eighth.
-// A warp's next 16 tokens are loaded as soon as their registers are free: all 16 warps of an SM have 4 KB under way most of the time.
+// S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix, and every warp streams tiles of 16 tokens through a cp.async ring of its own.
+// The sum over a row's dimensions may run in any order, the output's dimensions may be dealt to the MMA's rows in any order and so may the
+// tokens, so all three are chosen by what a wide load from shared memory gives: of 64 dimensions of a key, the four lanes of a quad take 16 neighbouring
+// ones each, and of a value's each eighth lane an eighth. (Loads straight into registers, each as soon as the registers are free: too few bytes under
+// way, warps waited for memory half of their time.)
 //
 // A CTA is 8 warps of one (sequence, kv head, part of the keys); tiles of 16 tokens go round the warps. Warps meet in shared memory;
 // up to 8 parts are a cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); more parts go through a
@@ -119,6 +119,9 @@ __device__ __forceinline__ Words<W> load_words(const void* p) {
     return r;
 }
 
+// A tile in shared memory: 16 rows of K codes, 16 of V codes, the K rows' scales, the V rows'. Where row t and its 16-byte chunks lie makes every
+// load below free of bank conflicts: the loads of a key's row take tokens t and t + 4 (8 bits, eight lanes) or {0, 4, 1, 5} and {2, 6, 3, 7}
+// (half a warp) at once, those of the values four tokens in a row.
 template <int BITS, int D>
 struct Shape {
     static constexpr int NG = BITS == 8 ? 1 : D / 64;      // scales of a row
@@ -130,16 +133,74 @@ struct Shape {
     static constexpr int VW = VD * BITS / 32;
     static constexpr int VB = D * BITS / 8 / VC;           // bytes of a chunk
     static constexpr int MT = D / 16;                      // MMAs of a tile
+    static constexpr int ROW = D * BITS / 8;               // bytes of a row
+    static constexpr int SB = 4 * NG;                      // bytes of its scales
+    static constexpr int TILE = TOK * ROW;
+    static constexpr int STAGE = 2 * TILE + 2 * TOK * SB;
+
+    static __device__ __forceinline__ uint32_t at(int t, int byte) {
+        const int chunk = byte >> 4, rest = byte & 15;
+        int row = t, c2 = chunk;
+        if (ROW == 32) {
+            row = t ^ ((t >> 1) & 2);
+        } else if (ROW == 64) {
+            row = t ^ ((t >> 2) & 1);
+            c2 = chunk ^ (((row >> 1) ^ (row >> 2)) & 1) << 1;
+        } else if (BITS == 8) {
+            c2 = chunk ^ (((t & 3) << 1) | ((t >> 2) & 1));
+        } else {
+            c2 = chunk ^ ((((t & 3) ^ ((t >> 1) & 2))) << 1);
+        }
+        return static_cast<uint32_t>(row * ROW + c2 * 16 + rest);
+    }
+    // the 16 dimensions of 64-dimension chunk j that lane c of a quad holds: 8 bits 16 neighbouring codes, 4 bits 8 bytes of a group
+    static __device__ __forceinline__ int k_byte(int j, int c) {
+        return BITS == 4 ? j * 32 + c * 8 : (D == 64 ? c * 16 : ((j >> 1) * 8 + 2 * c + (j & 1)) * 16);
+    }
 };
+// token that row r of the MMA is
+__device__ __forceinline__ int token_of(int r) { return ((r & 7) >> 1) + 4 * (r & 1) + (r & 8); }
 
 // O and what belongs to it, per warp, in shared memory: heads [8 NH] rows of D + 4 floats
 __host__ __device__ constexpr int o_pitch(int d) { return d + 4; }
 
+template <int W>
+__device__ __forceinline__ Words<W> lds_words(uint32_t at) {
+    Words<W> r;
+    if constexpr (W == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r.w[0]) : "r"(at));
+    else if constexpr (W == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "r"(at));
+    else asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "r"(at));
+    return r;
+}
+// `bytes` 0: zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_small(uint32_t dst, const void* src, int bytes) {
+    if constexpr (N == 16) copy16(dst, src, bytes);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(N) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// CTAs per SM, and tiles of a warp's ring: what 208 KB per SM have room for, at most 8
+__host__ __device__ constexpr int ctas_per_sm(int d, int nh) { return d == 256 || nh == 2 ? 1 : 2; }
+__host__ __device__ constexpr int stages_of(int stage, int d, int nh) {
+    const int room = 208 * 1024 / ctas_per_sm(d, nh) / WARPS / stage;
+    return room < 8 ? room : 8;
+}
+
 template <int BITS, int D, int NH, bool WHOLE>
-__global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(const Params p) {
     using S = Shape<BITS, D>;
-    constexpr int HEADS = 8 * NH, OP = o_pitch(D);
-    extern __shared__ float o_s[];                          // [WARPS][HEADS][OP], then the cluster's slices
+    constexpr int HEADS = 8 * NH, OP = o_pitch(D), STAGES = stages_of(S::STAGE, D, NH);
+    static_assert(STAGES >= 3 && WARPS * STAGES * S::STAGE >= WARPS * HEADS * OP * 4, "the warps' sums reuse the ring");
+    extern __shared__ __align__(128) uint8_t smem[];        // rings [WARPS][STAGES][STAGE], the cluster's slices behind them
+    float* o_s = reinterpret_cast<float*>(smem);            // [WARPS][HEADS][OP], when the rings are done
     __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
     __shared__ float part_m[MAX_CLUSTER][HEADS], part_l[MAX_CLUSTER][HEADS];
     const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
@@ -175,90 +236,51 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
     const char* vsc = p.vs + kvh * p.scale_head;
 
     auto first_token = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + t_lo) * TOK; };
-    // Where a tile lies: byte offsets of its first token (WHOLE: pages of a multiple of 16), or of token `lane` of it, in the codes and in the
-    // scales. A token that is not seen, or whose page the cache does not have, is read from the cache's first place and has `live` false.
-    struct Place {
-        long long code, scale;
-        bool live;
-    };
+    // page of a tile's first token (WHOLE: pages of a multiple of 16 tokens), or of its token lane % 16; -1: not seen
+    const int my_token = lane & 15;
+    auto in_table = [&](int t) { return p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size; };
     auto lookup = [&](int i) {
-        Place at{0, 0, false};
-        if (i < i1 && (WHOLE || lane < TOK)) {
-            const int t = first_token(i) + (WHOLE ? 0 : lane);
-            if (WHOLE || (i < sink_tiles ? t < first : t >= lo && t < n)) {
-                const int in_table = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-                const int page = static_cast<int>(ldg32(table + in_table));
-                const int row = t - in_table * p.page_size;
-                if (static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks)) {
-                    at.code = page * p.code_block + row * p.code_token;
-                    at.scale = page * p.scale_block + row * p.scale_token;
-                    at.live = true;
-                }
-            }
+        int page = -1;
+        if (i < i1) {
+            const int t = first_token(i) + (WHOLE ? 0 : my_token);
+            if (WHOLE || (i < sink_tiles ? t < first : t >= lo && t < n)) page = static_cast<int>(ldg32(table + in_table(t)));
         }
-        return at;
+        return page;
     };
-    const uint8_t* k_lane = kc + c * (2 * BITS) + (WHOLE ? g * p.code_token : 0);
-    const uint8_t* v_lane = vc + g * (S::VB / 8) + (WHOLE ? 2 * c * p.code_token : 0);
-    const char* ks_lane = ksc + (WHOLE ? g * p.scale_token : 0);
-    const char* vs_lane = vsc + (WHOLE ? g * p.scale_token : 0);
-    const long long code8 = 8 * p.code_token, scale8 = 8 * p.scale_token;
-    Words<S::KW> kw[2][S::KC];     // tokens g, g + 8
-    Words<S::NG> kscale[2], vscale[2];
-    Words<S::VW> vw[4][S::VC];     // tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-    auto load_k = [&](const Place& at) {
+    // The copies of tile i into its place of this warp's ring; rows that are not seen, or whose page the cache does not have, are zeros.
+    constexpr int CHUNKS = S::ROW / 16, ROWS = CHUNKS >= 32 ? 1 : 32 / CHUNKS;   // rows that a warp copies at once
+    const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * STAGES * S::STAGE);
+    const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
+    const uint8_t* k_lane = kc + lchunk * 16 + (WHOLE ? lrow * p.code_token : 0);
+    const uint8_t* v_lane = vc + lchunk * 16 + (WHOLE ? lrow * p.code_token : 0);
+    const char* s_lane = lane < 16 ? ksc : vsc;             // lanes 0..15 copy the scales of the keys, 16..31 of the values
+    const long long next_rows = ROWS * p.code_token;
+    auto issue = [&](int i, int page, uint32_t stage) {
+        const int t = first_token(i) + (WHOLE ? 0 : my_token);
+        const int row = t - in_table(t) * p.page_size;
+        const bool live = static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks);
+        const long long off = live ? page * p.code_block + row * p.code_token : 0;
+        const long long soff = live ? page * p.scale_block + (row + (WHOLE ? my_token : 0)) * p.scale_token : 0;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint8_t* src;
-            const char* ssrc;
-            bool live = at.live;
-            if (WHOLE) {
-                src = k_lane + at.code + (r ? code8 : 0);
-                ssrc = ks_lane + at.scale + (r ? scale8 : 0);
-            } else {
-                src = k_lane + __shfl_sync(0xffffffffu, at.code, g + 8 * r);
-                ssrc = ks_lane + __shfl_sync(0xffffffffu, at.scale, g + 8 * r);
-                live = __shfl_sync(0xffffffffu, static_cast<int>(at.live), g + 8 * r) != 0;
-            }
-#pragma unroll
-            for (int j = 0; j < S::KC; ++j) kw[r][j] = load_words<S::KW>(src + j * (8 * BITS));
-            kscale[r] = load_words<S::NG>(ssrc);
-            if (!live) {
-#pragma unroll
-                for (int w = 0; w < S::NG; ++w) kscale[r].w[w] = 0;
-            }
+        for (int j = 0; j < TOK / ROWS; ++j) {
+            const int r = j * ROWS + lrow;
+            const long long at = WHOLE ? off + j * next_rows : __shfl_sync(0xffffffffu, off, r);
+            const int bytes = (WHOLE ? live : __shfl_sync(0xffffffffu, static_cast<int>(live), r) != 0) ? 16 : 0;
+            const uint32_t dst = stage + S::at(r, lchunk * 16);
+            copy16(dst, k_lane + (WHOLE && !live ? 0 : at), bytes);
+            copy16(dst + S::TILE, v_lane + (WHOLE && !live ? 0 : at), bytes);
         }
-    };
-    auto load_v = [&](const Place& at) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint8_t* src = WHOLE ? v_lane + at.code + (r & 1 ? p.code_token : 0) + (r >> 1 ? code8 : 0)
-                                       : v_lane + __shfl_sync(0xffffffffu, at.code, 2 * c + (r & 1) + (r >> 1) * 8);
-#pragma unroll
-            for (int j = 0; j < S::VC; ++j) vw[r][j] = load_words<S::VW>(src + j * S::VB);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const char* ssrc;
-            bool live = at.live;
-            if (WHOLE) {
-                ssrc = vs_lane + at.scale + (r ? scale8 : 0);
-            } else {
-                ssrc = vs_lane + __shfl_sync(0xffffffffu, at.scale, g + 8 * r);
-                live = __shfl_sync(0xffffffffu, static_cast<int>(at.live), g + 8 * r) != 0;
-            }
-            vscale[r] = load_words<S::NG>(ssrc);
-            if (!live) {
-#pragma unroll
-                for (int w = 0; w < S::NG; ++w) vscale[r].w[w] = 0;
-            }
-        }
+        copy_small<S::SB>(stage + 2 * S::TILE + lane * S::SB, s_lane + soff, live ? S::SB : 0);
     };
 
-    Place next = lookup(i0);
-    load_k(next);
-    load_v(next);
-    next = lookup(i0 + WARPS);
+    int page = lookup(i0);
+#pragma unroll
+    for (int a = 0; a < STAGES - 1; ++a) {
+        const int i = i0 + a * WARPS, now = page;
+        page = lookup(i + WARPS);
+        if (i < i1) issue(i, now, ring + a * S::STAGE);
+        copy_commit();
+    }
 
     // ---- q as the second operand: column g of the MMA is head 8 h + g, its dimensions 16 c .. 16 c + 15 of every 64 are this lane's
     uint32_t qf[NH][S::KC][4][2];  // high and low bytes of four dimensions
@@ -268,12 +290,13 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
         const int head = 8 * h + g;
-        const char* src = static_cast<const char*>(p.q) + (head0 + (head < heads ? head : 0)) * (D * 2) + c * 32;
+        const char* src = static_cast<const char*>(p.q) + (head0 + (head < heads ? head : 0)) * (D * 2);
         float f[S::KC][16];
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < S::KC; ++j) {
-            const Words<8> w = load_words<8>(src + j * 128);
+            // the dimensions whose codes lie in this lane's bytes of chunk j
+            const Words<8> w = load_words<8>(src + (BITS == 8 ? 2 : 4) * S::k_byte(j, c));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (p.is_f16) {
@@ -346,9 +369,37 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
     }
     const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
 
+    // what this lane reads of a tile: tokens of rows g and g + 8 of the MMA (keys and scales), of columns 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (values)
+    const int t_row = token_of(g);
+    uint32_t k_at[S::KC], v_at[4][S::VC];
+#pragma unroll
+    for (int j = 0; j < S::KC; ++j) k_at[j] = S::at(t_row, S::k_byte(j, c));
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(c + 4 * (r & 1) + 8 * (r >> 1), j * S::VB + g * (S::VB / 8));
+    const uint32_t s_at = 2 * S::TILE + t_row * S::SB;
+    uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
     for (int i = i0; i < i1; i += WARPS) {
+        copy_wait<STAGES - 2>();
+        __syncwarp();   // the tile is here, and the place of the one before it is free
+        {
+            const int ahead = i + (STAGES - 1) * WARPS, now = page;
+            page = lookup(ahead + WARPS);
+            if (ahead < i1) issue(ahead, now, free_stage);
+            copy_commit();
+        }
         // ---- S^T = K Q^T, a sum per group of dimensions: the high bytes of q, then 256 times that and the low ones
         float s[NH][4];
+        Words<S::KW> kw[2][S::KC];
+        Words<S::NG> kscale[2], vscale[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int j = 0; j < S::KC; ++j) kw[r][j] = lds_words<S::KW>(stage + k_at[j] + r * (8 * S::ROW));
+            kscale[r] = lds_words<S::NG>(stage + s_at + r * (8 * S::SB));
+            vscale[r] = lds_words<S::NG>(stage + s_at + TOK * S::SB + r * (8 * S::SB));
+        }
         int acc[NH][S::NG][4];
         uint32_t ka[S::KC][4][2];    // [chunk][register][token]
 #pragma unroll
@@ -407,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
         if (edge) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int t = t0 + g + 8 * r;
+                const int t = t0 + t_row + 8 * r;
                 const bool seen = sink ? t < first : t >= lo && t < n;
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
@@ -430,8 +481,6 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
 #pragma unroll
             for (int e = 0; e < 4; ++e) higher |= s[h][e] > m_run[h][e & 1];
         higher |= most > unit;
-        // the next tile's keys: theirs are the registers that are free now
-        if (i + WARPS < i1) load_k(next);
         if (__any_sync(0xffffffffu, higher)) {
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
@@ -491,6 +540,11 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
             }
         }
         // ---- O^T += V^T P^T: row g of MMA m is dimension 2 m of the lane's, row g + 8 the one after it
+        Words<S::VW> vw[4][S::VC];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r][j]);
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) {
             constexpr int last = S::NG - 1;
@@ -526,11 +580,11 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
                 }
             }
         }
-        if (i + WARPS < i1) {
-            load_v(next);
-            next = lookup(i + 2 * WARPS);
-        }
+        free_stage = stage;
+        stage = stage + S::STAGE == ring + STAGES * S::STAGE ? ring : stage + S::STAGE;
     }
+    copy_wait<0>();
+    __syncthreads();   // the rings are done: the sums take their place
 
     // ---- the warps meet in shared memory
 #pragma unroll
@@ -571,7 +625,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NH == 2) ? 1 : 2) decode
     const int total = heads * D;
     const int slices = in_cluster ? p.splits : 1;
     const int slice = ((total + slices - 1) / slices + 3) & ~3;
-    float* slice_s = o_s + WARPS * HEADS * OP;              // [splits][slice]
+    float* slice_s = reinterpret_cast<float*>(smem + WARPS * STAGES * S::STAGE);   // [splits][slice]
     const bool to_workspace = p.splits > MAX_CLUSTER;
     for (int idx = static_cast<int>(threadIdx.x); idx < total; idx += THREADS) {
         const int head = idx / D, d = idx % D;
@@ -684,7 +738,8 @@ template <int BITS, int D, int NH, bool WHOLE>
 int launch(const Params& p, int grid, cudaStream_t stream) {
     const int cluster = p.splits > 1 && p.splits <= MAX_CLUSTER ? p.splits : 1;
     // slices: a part's share of 8 NH heads, rounded up to 4 floats
-    const int smem = (WARPS * 8 * NH * o_pitch(D) + 8 * NH * D + 4 * MAX_CLUSTER) * 4;
+    using S = Shape<BITS, D>;
+    const int smem = WARPS * stages_of(S::STAGE, D, NH) * S::STAGE + (8 * NH * D + 4 * MAX_CLUSTER) * 4;
     const auto fn = decode_kernel<BITS, D, NH, WHOLE>;
     TDIST_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg;
