@@ -353,3 +353,20 @@ def test_two_streams_at_once():
             got.append(((1, 4, 20)[i % 3], tdist.gqa_fwd_quantized_decode(q, gpu, lens, dt, kv_split=(1, 4, 20)[i % 3])))
     torch.cuda.synchronize()
     assert all(torch.equal(want[s], o) for s, o in got)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("D,page,splits", [(128, 16, 1), (128, 16, 2), (64, 16, 1), (256, 16, 1), (128, 5, 1)])
+def test_decode_goes_round_its_rings_often(bits, D, page, splits):
+    """Many tiles per warp, whose loads land in any order, on a full machine: the same result every time, and the right one."""
+    B, Hkv, n = 40, 4, 6000
+    table, blocks = _table(1, -(-n // page))
+    cpu, gpu = _fill(blocks, page, Hkv, D, bits, seed=11)
+    q = torch.randn(B, 8, D, generator=torch.Generator().manual_seed(13)).to(torch.float16)
+    lens = torch.tensor([n - 16 * b for b in range(B)], dtype=torch.int32)
+    args = q.cuda(), gpu, lens.cuda(), table.expand(B, -1).cuda()
+    got = [tdist.gqa_fwd_quantized_decode(*args, kv_split=splits) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[0], o) for o in got)
+    one = _check_decode(q[-1:], cpu, [int(lens[-1])], table, kv_split=splits)
+    assert torch.equal(one[0], got[0][-1].cpu())

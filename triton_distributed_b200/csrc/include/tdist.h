@@ -496,6 +496,8 @@ typedef struct TdistQuantDecodeArgs {
     void* part;                  /* fp32 [B, Hq, splits, D + 2] where splits > 8 */
     int Hq, splits, window, sinks;
     float scale, soft_cap;
+    void* status;
+    uint64_t timeout_ns;
 } TdistQuantDecodeArgs;
 
 int tdist_quant_cache_write(const TdistQuantCacheArgs* args);

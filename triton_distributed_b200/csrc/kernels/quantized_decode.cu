@@ -26,6 +26,7 @@
 // A CTA is 8 warps of one (sequence, kv head, part of the keys); tiles of 16 tokens go round the warps. Warps meet in shared memory;
 // up to 8 parts are a cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); more parts go through a
 // workspace and a second kernel. No counters: nothing has to be zero before a call, and calls share nothing.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,6 +36,7 @@
 #include <string>
 
 #include "../device/ptx.cuh"
+#include "../device/signal.cuh"
 #include "../device/soft_cap.cuh"
 #include "../include/tdist.h"
 #include "../runtime/host_common.h"
@@ -43,11 +45,19 @@ namespace tdist {
 namespace qdecode {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
+// warps that compute: where tiles come by TMA, one warp loads for the others
+__host__ __device__ constexpr int consumers(bool paged) { return paged ? WARPS - 1 : WARPS; }
 constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
+constexpr int kKernelQuantDecode = 13;
+// Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled: a weight
+// times its scale's share of the unit is rounded to fp16 whatever its size, and 2^8 is far below fp16's largest.
+constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
+    CUtensorMap tm_k, tm_v;        // PAGED: codes as bytes {ROW, Hkv, page, blocks}, box {BOX, 1, 16, 1}
+    CUtensorMap tm_ks, tm_vs;      // scales as words {page NG, Hkv, blocks}, box {16 NG, 1, 1}
     const void* q;                 // [B, Hq, D]
     const uint8_t *k, *v;
     const char *ks, *vs;
@@ -57,16 +67,18 @@ struct Params {
     long long code_block, code_token, code_head, scale_block, scale_head, scale_token;   // bytes
     int Hq, Hkv, head_tiles, page_size, page_shift, max_blocks, blocks, splits, window, sinks, table_keys, is_f16;
     float scale, soft_cap;
+    uint32_t page_mul;             // t / page_size = (t page_mul) >> page_shift for t < 2^31
+    WaitCtx wctx;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
     return r;
 }
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
@@ -74,22 +86,24 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same from c0 (rows of a register pair's first column) and c1
+__device__ __forceinline__ void mma_u8s8_from(int (&d)[4], int c0, int c1, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
 }
 // A byte or nibble n under the exponent of 1024 is the fp16 number 1024 + n; in the upper nibble of a byte, 1024 + 16 n.
 constexpr uint32_t kMagic = 0x64006400u;
 constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a 0x64
 __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) { return hsub2(__byte_perm(w, kMagic, sel), 0x64806480u); }   // - 1152
 __device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return hsub2((w & 0x000f000fu) | kMagic, 0x64086408u); }                     // - 1032: n - 8
-__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return hfma2((w & 0x00f000f0u) | kMagic, 0x2c002c00u, 0xd480d480u); }       // / 16 - 72: n - 8
+// 16 (n - 8): the rows of the MMA that take it are off by that factor until the end (a multiply-add here has two constants to keep in registers)
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return hsub2((w & 0x00f000f0u) | kMagic, 0x64806480u); }                     // - 1152
 __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
     return __byte_perm(__byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(b), 0x0040u), __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(d), 0x0040u), 0x5410u);
 }
@@ -119,9 +133,10 @@ __device__ __forceinline__ Words<W> load_words(const void* p) {
     return r;
 }
 
-// A tile in shared memory: 16 rows of K codes, 16 of V codes, the K rows' scales, the V rows'. Where row t and its 16-byte chunks lie makes every
-// load below free of bank conflicts: the loads of a key's row take tokens t and t + 4 (8 bits, eight lanes) or {0, 4, 1, 5} and {2, 6, 3, 7}
-// (half a warp) at once, those of the values four tokens in a row.
+// A tile in shared memory: 16 rows of K codes, 16 of V codes, and apart from them the rows' scales. The 16-byte chunks of a row lie as a TMA load with the
+// swizzle of the row's width leaves them (rows of 256 bytes as two halves of 128), and the MMA's rows are tokens in an order that makes
+// the loads below free of bank conflicts but for two of K's in twos (4 bits, heads of 64 and 256): a key's load takes two rows whose tokens differ in
+// bit 0, or four whose tokens differ in bits 0 and 2, and a value's four columns whose tokens differ in bits 0 and 2, and in bits 1 and 2.
 template <int BITS, int D>
 struct Shape {
     static constexpr int NG = BITS == 8 ? 1 : D / 64;      // scales of a row
@@ -134,24 +149,17 @@ struct Shape {
     static constexpr int VB = D * BITS / 8 / VC;           // bytes of a chunk
     static constexpr int MT = D / 16;                      // MMAs of a tile
     static constexpr int ROW = D * BITS / 8;               // bytes of a row
+    static constexpr int BOX = ROW < 128 ? ROW : 128;      // bytes of a row that lie together
     static constexpr int SB = 4 * NG;                      // bytes of its scales
-    static constexpr int TILE = TOK * ROW;
-    static constexpr int STAGE = 2 * TILE + 2 * TOK * SB;
+    static constexpr int TILE = TOK * ROW;                 // K; V behind it
+    static constexpr int SCALES = TOK * SB < 128 ? 128 : TOK * SB;   // K's, on 128 bytes as TMA wants them; V's behind them
+    static constexpr int STAGE = 2 * TILE + 2 * SCALES;    // bytes of a place in the ring
+    static constexpr int LOADED = 2 * TILE + 2 * TOK * SB;
 
     static __device__ __forceinline__ uint32_t at(int t, int byte) {
-        const int chunk = byte >> 4, rest = byte & 15;
-        int row = t, c2 = chunk;
-        if (ROW == 32) {
-            row = t ^ ((t >> 1) & 2);
-        } else if (ROW == 64) {
-            row = t ^ ((t >> 2) & 1);
-            c2 = chunk ^ (((row >> 1) ^ (row >> 2)) & 1) << 1;
-        } else if (BITS == 8) {
-            c2 = chunk ^ (((t & 3) << 1) | ((t >> 2) & 1));
-        } else {
-            c2 = chunk ^ ((((t & 3) ^ ((t >> 1) & 2))) << 1);
-        }
-        return static_cast<uint32_t>(row * ROW + c2 * 16 + rest);
+        const int chunk = (byte & (BOX - 1)) >> 4;
+        const int swizzled = BOX == 32 ? chunk ^ ((t >> 2) & 1) : (BOX == 64 ? chunk ^ ((t >> 1) & 3) : chunk ^ (t & 7));
+        return static_cast<uint32_t>((byte / BOX) * (TOK * BOX) + t * BOX + swizzled * 16 + (byte & 15));
     }
     // the 16 dimensions of 64-dimension chunk j that lane c of a quad holds: 8 bits 16 neighbouring codes, 4 bits 8 bytes of a group
     static __device__ __forceinline__ int k_byte(int j, int c) {
@@ -159,7 +167,7 @@ struct Shape {
     }
 };
 // token that row r of the MMA is
-__device__ __forceinline__ int token_of(int r) { return ((r & 7) >> 1) + 4 * (r & 1) + (r & 8); }
+__device__ __forceinline__ int token_of(int r) { return static_cast<int>((0x76234510u >> (4 * (r & 7))) & 7u) + (r & 8); }
 
 // O and what belongs to it, per warp, in shared memory: heads [8 NH] rows of D + 4 floats
 __host__ __device__ constexpr int o_pitch(int d) { return d + 4; }
@@ -172,14 +180,19 @@ __device__ __forceinline__ Words<W> lds_words(uint32_t at) {
     else asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "r"(at));
     return r;
 }
-// `bytes` 0: zeros
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// `none`: zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool none) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, p;\n\t}" ::"r"(dst), "l"(src),
+                 "r"(static_cast<uint32_t>(none))
+                 : "memory");
 }
 template <int N>
-__device__ __forceinline__ void copy_small(uint32_t dst, const void* src, int bytes) {
-    if constexpr (N == 16) copy16(dst, src, bytes);
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(N) : "memory");
+__device__ __forceinline__ void copy_small(uint32_t dst, const void* src, bool none) {
+    if constexpr (N == 16) copy16(dst, src, none);
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tcp.async.ca.shared.global [%0], [%1], %3, p;\n\t}" ::"r"(dst), "l"(src),
+                     "r"(static_cast<uint32_t>(none)), "n"(N)
+                     : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -187,26 +200,39 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// CTAs per SM, and tiles of a warp's ring: what 208 KB per SM have room for, at most 8
+// CTAs per SM, and tiles that the rings of a CTA have room for in 206 KB per SM: at most 8 per warp, and as many for each. (A place belongs to one
+// warp: only a warp that has waited for a place's earlier tiles itself can tell by a barrier's parity that the next one is there.)
 __host__ __device__ constexpr int ctas_per_sm(int d, int nh) { return d == 256 || nh == 2 ? 1 : 2; }
-__host__ __device__ constexpr int stages_of(int stage, int d, int nh) {
-    const int room = 208 * 1024 / ctas_per_sm(d, nh) / WARPS / stage;
-    return room < 8 ? room : 8;
+__host__ __device__ constexpr int places_of(int stage, int d, int nh, bool paged) {
+    const int each = 206 * 1024 / ctas_per_sm(d, nh) / stage / consumers(paged);
+    return (each < 8 ? each : 8) * consumers(paged);
 }
 
-template <int BITS, int D, int NH, bool WHOLE>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(const Params p) {
+template <int BITS, int D, int NH, bool PAGED>
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(const __grid_constant__ Params p) {
     using S = Shape<BITS, D>;
-    constexpr int HEADS = 8 * NH, OP = o_pitch(D), STAGES = stages_of(S::STAGE, D, NH);
-    static_assert(STAGES >= 3 && WARPS * STAGES * S::STAGE >= WARPS * HEADS * OP * 4, "the warps' sums reuse the ring");
-    extern __shared__ __align__(128) uint8_t smem[];        // rings [WARPS][STAGES][STAGE], the cluster's slices behind them
-    float* o_s = reinterpret_cast<float*>(smem);            // [WARPS][HEADS][OP], when the rings are done
-    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    constexpr int HEADS = 8 * NH, OP = o_pitch(D), CW = consumers(PAGED);
+    constexpr int PLACES = places_of(S::STAGE, D, NH, PAGED), STAGES = PLACES / CW;   // of all rings; of a warp's own
+    static_assert(STAGES >= 3 && PLACES * S::STAGE >= CW * HEADS * OP * 4, "the warps' sums reuse the ring");
+    extern __shared__ uint8_t smem_raw[];
+    // [PLACES] K and V codes, [PLACES] scales, the cluster's slices
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* o_s = reinterpret_cast<float*>(smem);            // [CW][HEADS][OP], when the rings are done
+    __shared__ uint64_t bars[2][PAGED ? PLACES : 1];       // PAGED: a tile's bytes are there; its place is free
+    __shared__ float m_s[CW][HEADS], l_s[CW][HEADS];
     __shared__ float part_m[MAX_CLUSTER][HEADS], part_l[MAX_CLUSTER][HEADS];
-    const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = static_cast<int>(threadIdx.x) & 31;
     const int g = lane >> 2, c = lane & 3;
     const bool in_cluster = p.splits > 1 && p.splits <= MAX_CLUSTER;
     if (in_cluster) cluster_arrive();                       // waited for before the first store into another CTA
+    if (PAGED) {
+        if (threadIdx.x < PLACES) {
+            mbar_init(smem_u32(&bars[0][threadIdx.x]), 1);
+            mbar_init(smem_u32(&bars[1][threadIdx.x]), 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
     pdl_wait_and_release();
 
     int x = static_cast<int>(blockIdx.x);
@@ -227,65 +253,92 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
     const int t_lo = lo / TOK;
     const int tiles = sink_tiles + (n + TOK - 1) / TOK - t_lo;
     const int per = (tiles + p.splits - 1) / p.splits;
-    const int i0 = min(split * per, tiles) + warp, i1 = min((split + 1) * per, tiles);
+    const int first_tile = min(split * per, tiles), i0 = first_tile + warp, i1 = min((split + 1) * per, tiles);
 
     const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
-    const uint8_t* kc = p.k + kvh * p.code_head;
-    const uint8_t* vc = p.v + kvh * p.code_head;
-    const char* ksc = p.ks + kvh * p.scale_head;
-    const char* vsc = p.vs + kvh * p.scale_head;
-
     auto first_token = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + t_lo) * TOK; };
-    // page of a tile's first token (WHOLE: pages of a multiple of 16 tokens), or of its token lane % 16; -1: not seen
-    const int my_token = lane & 15;
-    auto in_table = [&](int t) { return p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size; };
-    auto lookup = [&](int i) {
-        int page = -1;
-        if (i < i1) {
-            const int t = first_token(i) + (WHOLE ? 0 : my_token);
-            if (WHOLE || (i < sink_tiles ? t < first : t >= lo && t < n)) page = static_cast<int>(ldg32(table + in_table(t)));
+    auto in_table = [&](int t) { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * p.page_mul) >> p.page_shift); };
+    auto codes_at = [&](int place) { return smem_u32(smem) + static_cast<uint32_t>(place * 2 * S::TILE); };
+    auto scales_at = [&](int place) { return smem_u32(smem) + static_cast<uint32_t>(PLACES * 2 * S::TILE + place * 2 * S::SCALES); };
+
+    if (PAGED && warp == CW) {
+        // ---- the loading warp: a lane looks up the page of one of the next 32 tiles, then tile after tile is sent on its way. A page that the
+        // cache does not have is out of the tensor map's bounds and reads as zeros.
+        auto lookup = [&](int i) { return i < i1 ? static_cast<int>(ldg32(table + in_table(first_token(i)))) : 0; };
+        int place = 0;
+        uint32_t parity = 1;
+        int pages = lookup(first_tile + lane);
+        for (int base = first_tile; base < i1; base += 32) {
+            const int now = pages, row = first_token(base + lane) - in_table(first_token(base + lane)) * p.page_size;
+            pages = lookup(base + 32 + lane);
+            const int count = min(32, i1 - base);
+            for (int j = 0; j < count; ++j) {
+                const int page_j = __shfl_sync(0xffffffffu, now, j), row_j = __shfl_sync(0xffffffffu, row, j);
+                mbar_wait(smem_u32(&bars[1][place]), parity, p.wctx, 2);
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&bars[0][place]), codes = codes_at(place), scales = scales_at(place);
+                    mbar_expect_tx(bar, S::LOADED);
+                    tma_load_4d(codes, &p.tm_k, bar, 0, kvh, row_j, page_j);
+                    if (S::ROW > S::BOX) tma_load_4d(codes + TOK * S::BOX, &p.tm_k, bar, S::BOX, kvh, row_j, page_j);
+                    tma_load_3d(scales, &p.tm_ks, bar, row_j * S::NG, kvh, page_j);
+                    tma_load_4d(codes + S::TILE, &p.tm_v, bar, 0, kvh, row_j, page_j);
+                    if (S::ROW > S::BOX) tma_load_4d(codes + S::TILE + TOK * S::BOX, &p.tm_v, bar, S::BOX, kvh, row_j, page_j);
+                    tma_load_3d(scales + S::SCALES, &p.tm_vs, bar, row_j * S::NG, kvh, page_j);
+                }
+                __syncwarp();
+                if (++place == PLACES) {
+                    place = 0;
+                    parity ^= 1u;
+                }
+            }
         }
-        return page;
+    } else {
+    // ---- not PAGED (pages of other sizes, scales with strides): every warp copies its own tiles, 16 bytes of a row per lane. A lane looks up token
+    // lane % 16; -1: not seen. Rows that are not seen, or whose page the cache does not have, are zeros.
+    const int my_token = lane & 15;
+    auto lookup = [&](int i) {
+        const int t = first_token(i) + my_token;
+        return i < i1 && (i < sink_tiles ? t < first : t >= lo && t < n) ? static_cast<int>(ldg32(table + in_table(t))) : -1;
     };
-    // The copies of tile i into its place of this warp's ring; rows that are not seen, or whose page the cache does not have, are zeros.
-    constexpr int CHUNKS = S::ROW / 16, ROWS = CHUNKS >= 32 ? 1 : 32 / CHUNKS;   // rows that a warp copies at once
-    const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * STAGES * S::STAGE);
+    constexpr int CHUNKS = S::ROW / 16, ROWS = 32 / CHUNKS;   // rows that a warp copies at once
     const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
-    const uint8_t* k_lane = kc + lchunk * 16 + (WHOLE ? lrow * p.code_token : 0);
-    const uint8_t* v_lane = vc + lchunk * 16 + (WHOLE ? lrow * p.code_token : 0);
-    const char* s_lane = lane < 16 ? ksc : vsc;             // lanes 0..15 copy the scales of the keys, 16..31 of the values
-    const long long next_rows = ROWS * p.code_token;
-    auto issue = [&](int i, int page, uint32_t stage) {
-        const int t = first_token(i) + (WHOLE ? 0 : my_token);
+    const uint8_t* k_lane = p.k + kvh * p.code_head + lchunk * 16;
+    const uint8_t* v_lane = p.v + kvh * p.code_head + lchunk * 16;
+    const char* s_lane = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head;   // lanes 0..15 copy the scales of the keys, 16..31 of the values
+    auto issue = [&](int i, int page, int place) {
+        const int t = first_token(i) + my_token;
         const int row = t - in_table(t) * p.page_size;
         const bool live = static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks);
-        const long long off = live ? page * p.code_block + row * p.code_token : 0;
-        const long long soff = live ? page * p.scale_block + (row + (WHOLE ? my_token : 0)) * p.scale_token : 0;
+        const long long from = live ? page : 0;
+        const long long off = from * p.code_block + row * p.code_token, soff = from * p.scale_block + row * p.scale_token;
+        const uint32_t codes = codes_at(place);
 #pragma unroll
         for (int j = 0; j < TOK / ROWS; ++j) {
             const int r = j * ROWS + lrow;
-            const long long at = WHOLE ? off + j * next_rows : __shfl_sync(0xffffffffu, off, r);
-            const int bytes = (WHOLE ? live : __shfl_sync(0xffffffffu, static_cast<int>(live), r) != 0) ? 16 : 0;
-            const uint32_t dst = stage + S::at(r, lchunk * 16);
-            copy16(dst, k_lane + (WHOLE && !live ? 0 : at), bytes);
-            copy16(dst + S::TILE, v_lane + (WHOLE && !live ? 0 : at), bytes);
+            const long long at = __shfl_sync(0xffffffffu, off, r);
+            const bool none = !__shfl_sync(0xffffffffu, static_cast<int>(live), r);
+            const uint32_t dst = codes + S::at(r, lchunk * 16);
+            copy16(dst, k_lane + at, none);
+            copy16(dst + S::TILE, v_lane + at, none);
         }
-        copy_small<S::SB>(stage + 2 * S::TILE + lane * S::SB, s_lane + soff, live ? S::SB : 0);
+        copy_small<S::SB>(scales_at(place) + (lane >> 4) * S::SCALES + my_token * S::SB, s_lane + soff, !live);
     };
-
-    int page = lookup(i0);
+    int page = -1;
+    if (!PAGED) {
+        page = lookup(i0);
 #pragma unroll
-    for (int a = 0; a < STAGES - 1; ++a) {
-        const int i = i0 + a * WARPS, now = page;
-        page = lookup(i + WARPS);
-        if (i < i1) issue(i, now, ring + a * S::STAGE);
-        copy_commit();
+        for (int a = 0; a < STAGES - 1; ++a) {
+            const int i = i0 + a * WARPS, now = page;
+            page = lookup(i + WARPS);
+            if (i < i1) issue(i, now, warp * STAGES + a);
+            copy_commit();
+        }
     }
 
     // ---- q as the second operand: column g of the MMA is head 8 h + g, its dimensions 16 c .. 16 c + 15 of every 64 are this lane's
     uint32_t qf[NH][S::KC][4][2];  // high and low bytes of four dimensions
     float factor[NH][2];           // of heads 8 h + 2 c + {0, 1}: what turns a product of codes into a score in units of log2
-    int bias[NH][2];               // 8 bits: 128 times the sum of the 16-bit q
+    int bias[NH][2];               // 8 bits: -128 times the sum of the 16-bit q
     float qsum[NH][2][S::NG];      // 4 bits: that sum over a group
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
@@ -346,13 +399,13 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             factor[h][r] = __shfl_sync(0xffffffffu, down, (2 * c + r) * 4) * (p.soft_cap > 0.f ? 1.f : kLog2e);
-            bias[h][r] = __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4) * 128;
+            bias[h][r] = BITS == 8 ? __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4) * -128 : 0;
         }
     }
 
     // ---- sums: O^T in units of `unit` (a power of two), columns are heads 8 h + 2 c + {0, 1}
     float o[NH][S::MT][4];
-    float m_run[NH][2], m_use[NH][2], l_run[NH][2];
+    float limit[NH][2], m_use[NH][2], l_run[NH][2];   // weights are relative to 2^m_use; it is raised when a score passes `limit`
     float low[NH][2][S::NG];       // 4 bits: sum of p least, of this lane's tokens
     float unit = 0.f, inv_unit = 0.f;
 #pragma unroll
@@ -361,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
         for (int j = 0; j < S::MT; ++j) o[h][j][0] = o[h][j][1] = o[h][j][2] = o[h][j][3] = 0.f;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            m_run[h][r] = -CUDART_INF_F;
+            limit[h][r] = -CUDART_INF_F;
             m_use[h][r] = l_run[h][r] = 0.f;
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) low[h][r][k] = 0.f;
@@ -371,36 +424,39 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
 
     // what this lane reads of a tile: tokens of rows g and g + 8 of the MMA (keys and scales), of columns 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (values)
     const int t_row = token_of(g);
-    uint32_t k_at[S::KC], v_at[4][S::VC];
+    uint32_t k_at[S::KC], v_at[2][S::VC];
 #pragma unroll
     for (int j = 0; j < S::KC; ++j) k_at[j] = S::at(t_row, S::k_byte(j, c));
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(c + 4 * (r & 1) + 8 * (r >> 1), j * S::VB + g * (S::VB / 8));
-    const uint32_t s_at = 2 * S::TILE + t_row * S::SB;
-    uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
-    for (int i = i0; i < i1; i += WARPS) {
-        copy_wait<STAGES - 2>();
-        __syncwarp();   // the tile is here, and the place of the one before it is free
-        {
+        for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
+    int place = PAGED ? warp : warp * STAGES, free_place = warp * STAGES + STAGES - 1;
+    uint32_t parity = 0;
+    for (int i = i0; i < i1; i += CW) {
+        if (PAGED) {
+            mbar_wait(smem_u32(&bars[0][place]), parity, p.wctx, 1);
+        } else {
+            copy_wait<STAGES - 2>();
+            __syncwarp();   // the tile is here, and the place of the one before it is free
             const int ahead = i + (STAGES - 1) * WARPS, now = page;
             page = lookup(ahead + WARPS);
-            if (ahead < i1) issue(ahead, now, free_stage);
+            if (ahead < i1) issue(ahead, now, free_place);
             copy_commit();
         }
-        // ---- S^T = K Q^T, a sum per group of dimensions: the high bytes of q, then 256 times that and the low ones
+        const uint32_t stage = codes_at(place), scales = scales_at(place) + static_cast<uint32_t>(t_row * S::SB);
+        // ---- S^T = K Q^T, a sum per group of dimensions and byte of q
         float s[NH][4];
         Words<S::KW> kw[2][S::KC];
         Words<S::NG> kscale[2], vscale[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
-            for (int j = 0; j < S::KC; ++j) kw[r][j] = lds_words<S::KW>(stage + k_at[j] + r * (8 * S::ROW));
-            kscale[r] = lds_words<S::NG>(stage + s_at + r * (8 * S::SB));
-            vscale[r] = lds_words<S::NG>(stage + s_at + TOK * S::SB + r * (8 * S::SB));
+            for (int j = 0; j < S::KC; ++j) kw[r][j] = lds_words<S::KW>(stage + k_at[j] + r * (8 * S::BOX));
+            kscale[r] = lds_words<S::NG>(scales + r * (8 * S::SB));
+            vscale[r] = lds_words<S::NG>(scales + S::SCALES + r * (8 * S::SB));
         }
-        int acc[NH][S::NG][4];
+        int acc[NH][S::NG][4], acc_low[NH][S::NG][4];
         uint32_t ka[S::KC][4][2];    // [chunk][register][token]
 #pragma unroll
         for (int j = 0; j < S::KC; ++j)
@@ -413,19 +469,21 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) {
-                acc[h][k][0] = acc[h][k][1] = acc[h][k][2] = acc[h][k][3] = 0;
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    if (part) {
+                for (int j = k * (S::KC / S::NG); j < (k + 1) * (S::KC / S::NG); ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[h][k][e] = (acc[h][k][e] << 8) - (BITS == 8 ? bias[h][e & 1] : 0);
+                    for (int m = 0; m < 2; ++m) {
+                        const uint32_t a0 = ka[j][2 * m][0], a1 = ka[j][2 * m][1], a2 = ka[j][2 * m + 1][0], a3 = ka[j][2 * m + 1][1];
+                        if (m == 0 && j == k * (S::KC / S::NG)) {
+                            mma_u8s8_from(acc[h][k], 0, 0, a0, a1, a2, a3, qf[h][j][0][0], qf[h][j][1][0]);
+                            mma_u8s8_from(acc_low[h][k], bias[h][0], bias[h][1], a0, a1, a2, a3, qf[h][j][0][1], qf[h][j][1][1]);
+                        } else {
+                            mma_u8s8(acc[h][k], a0, a1, a2, a3, qf[h][j][2 * m][0], qf[h][j][2 * m + 1][0]);
+                            mma_u8s8(acc_low[h][k], a0, a1, a2, a3, qf[h][j][2 * m][1], qf[h][j][2 * m + 1][1]);
+                        }
                     }
 #pragma unroll
-                    for (int j = k * (S::KC / S::NG); j < (k + 1) * (S::KC / S::NG); ++j)
-#pragma unroll
-                        for (int m = 0; m < 2; ++m)
-                            mma_u8s8(acc[h][k], ka[j][2 * m][0], ka[j][2 * m][1], ka[j][2 * m + 1][0], ka[j][2 * m + 1][1], qf[h][j][2 * m][part], qf[h][j][2 * m + 1][part]);
-                }
+                for (int e = 0; e < 4; ++e) acc[h][k][e] = acc[h][k][e] * 256 + acc_low[h][k][e];
             }
         // ---- scales, cap; masks at the ends of what is seen
         const int t0 = first_token(i);
@@ -479,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) higher |= s[h][e] > m_run[h][e & 1];
+            for (int e = 0; e < 4; ++e) higher |= s[h][e] > limit[h][e & 1];
         higher |= most > unit;
         if (__any_sync(0xffffffffu, higher)) {
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
@@ -502,10 +560,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float m_new = fmaxf(m_run[h][r], mx);
+                    const float m_old = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r], m_new = fmaxf(m_old, mx);
                     m_use[h][r] = m_new == -CUDART_INF_F ? 0.f : m_new;
-                    const float alpha = exp2f(m_run[h][r] - m_use[h][r]);
-                    m_run[h][r] = m_new;
+                    limit[h][r] = m_new + kSlack;
+                    const float alpha = exp2f(m_old - m_use[h][r]);
                     l_run[h][r] *= alpha;
 #pragma unroll
                     for (int k = 0; k < S::NG; ++k) low[h][r][k] *= alpha;
@@ -544,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r][j]);
+            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) {
             constexpr int last = S::NG - 1;
@@ -580,11 +638,22 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
                 }
             }
         }
-        free_stage = stage;
-        stage = stage + S::STAGE == ring + STAGES * S::STAGE ? ring : stage + S::STAGE;
+        if (PAGED) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars[1][place]));
+            place += CW;
+            if (place >= PLACES) {
+                place -= PLACES;
+                parity ^= 1u;
+            }
+        } else {
+            free_place = place;
+            if (++place == warp * STAGES + STAGES) place = warp * STAGES;
+        }
     }
-    copy_wait<0>();
-    __syncthreads();   // the rings are done: the sums take their place
+    if (!PAGED) copy_wait<0>();
+    // the rings are done once every warp is here: the sums take their place
+    named_barrier(1, CW * 32);
 
     // ---- the warps meet in shared memory
 #pragma unroll
@@ -597,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
             if (g == 0) {
-                m_s[warp][head] = m_run[h][r];
+                m_s[warp][head] = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r];
                 l_s[warp][head] = l;
             }
             float* dst = o_s + (warp * HEADS + head) * OP;
@@ -614,10 +683,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
                 for (int k = 0; k < S::VD / 2; ++k) {
                     const int m = j * (S::VD / 2) + k;
                     *reinterpret_cast<float2*>(dst + j * (D / S::VC) + g * S::VD + 2 * k) =
-                        make_float2(o[h][m][r] * unit + add, o[h][m][2 + r] * unit + add);
+                        make_float2(o[h][m][r] * unit + add, o[h][m][2 + r] * (BITS == 8 ? unit : unit * 0.0625f) + add);
                 }
             }
         }
+    }
     __syncthreads();
     if (in_cluster) cluster_wait();   // every CTA of the cluster runs
 
@@ -625,17 +695,17 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
     const int total = heads * D;
     const int slices = in_cluster ? p.splits : 1;
     const int slice = ((total + slices - 1) / slices + 3) & ~3;
-    float* slice_s = reinterpret_cast<float*>(smem + WARPS * STAGES * S::STAGE);   // [splits][slice]
+    float* slice_s = reinterpret_cast<float*>(smem + PLACES * S::STAGE);   // [splits][slice]
     const bool to_workspace = p.splits > MAX_CLUSTER;
     for (int idx = static_cast<int>(threadIdx.x); idx < total; idx += THREADS) {
         const int head = idx / D, d = idx % D;
         float m = -CUDART_INF_F;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w][head]);
+        for (int w = 0; w < CW; ++w) m = fmaxf(m, m_s[w][head]);
         const float mu = m == -CUDART_INF_F ? 0.f : m;
         float l = 0.f, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
+        for (int w = 0; w < CW; ++w) {
             const float f = exp2f(m_s[w][head] - mu);
             l += l_s[w][head] * f;
             sum += o_s[(w * HEADS + head) * OP + d] * f;
@@ -734,13 +804,13 @@ __global__ void __launch_bounds__(128) merge_kernel(const float* part, int split
     *reinterpret_cast<uint32_t*>(static_cast<char*>(out) + (head * D + d) * 2) = w;
 }
 
-template <int BITS, int D, int NH, bool WHOLE>
+template <int BITS, int D, int NH, bool PAGED>
 int launch(const Params& p, int grid, cudaStream_t stream) {
     const int cluster = p.splits > 1 && p.splits <= MAX_CLUSTER ? p.splits : 1;
     // slices: a part's share of 8 NH heads, rounded up to 4 floats
     using S = Shape<BITS, D>;
-    const int smem = WARPS * stages_of(S::STAGE, D, NH) * S::STAGE + (8 * NH * D + 4 * MAX_CLUSTER) * 4;
-    const auto fn = decode_kernel<BITS, D, NH, WHOLE>;
+    const int smem = 1024 + places_of(S::STAGE, D, NH, PAGED) * S::STAGE + (8 * NH * D + 4 * MAX_CLUSTER) * 4;
+    const auto fn = decode_kernel<BITS, D, NH, PAGED>;
     TDIST_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
@@ -761,18 +831,18 @@ int launch(const Params& p, int grid, cudaStream_t stream) {
 }
 
 template <int BITS, int D>
-int launch_heads(const Params& p, int nh, bool whole, int grid, cudaStream_t stream) {
+int launch_heads(const Params& p, int nh, bool paged, int grid, cudaStream_t stream) {
     // heads of 256 take one tile of query heads: two would need more registers than there are
     if constexpr (D != 256) {
-        if (nh == 2) return whole ? launch<BITS, D, 2, true>(p, grid, stream) : launch<BITS, D, 2, false>(p, grid, stream);
+        if (nh == 2) return paged ? launch<BITS, D, 2, true>(p, grid, stream) : launch<BITS, D, 2, false>(p, grid, stream);
     }
-    return whole ? launch<BITS, D, 1, true>(p, grid, stream) : launch<BITS, D, 1, false>(p, grid, stream);
+    return paged ? launch<BITS, D, 1, true>(p, grid, stream) : launch<BITS, D, 1, false>(p, grid, stream);
 }
 
 template <int BITS>
-int launch_dim(const Params& p, int head_dim, int nh, bool whole, int grid, cudaStream_t stream) {
-    return head_dim == 64 ? launch_heads<BITS, 64>(p, nh, whole, grid, stream)
-                          : (head_dim == 128 ? launch_heads<BITS, 128>(p, nh, whole, grid, stream) : launch_heads<BITS, 256>(p, nh, whole, grid, stream));
+int launch_dim(const Params& p, int head_dim, int nh, bool paged, int grid, cudaStream_t stream) {
+    return head_dim == 64 ? launch_heads<BITS, 64>(p, nh, paged, grid, stream)
+                          : (head_dim == 128 ? launch_heads<BITS, 128>(p, nh, paged, grid, stream) : launch_heads<BITS, 256>(p, nh, paged, grid, stream));
 }
 
 }  // namespace qdecode
@@ -828,9 +898,11 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     const int nh = G > 8 && c.head_dim != 256 ? 2 : 1;
     p.head_tiles = (G + 8 * nh - 1) / (8 * nh);
     p.page_size = c.page_size;
-    p.page_shift = -1;
-    for (int i = 0; i < 31; ++i)
-        if (c.page_size == 1 << i) p.page_shift = i;
+    // with 2^l >= page_size the multiplier ceil(2^(31 + l) / page_size) is off by less than one, so t < 2^31 times it by less than 2^31 <= 2^(31 + l) / page_size
+    int l = 0;
+    while ((1ll << l) < c.page_size) ++l;
+    p.page_shift = 31 + l;
+    p.page_mul = static_cast<uint32_t>(((1ull << (31 + l)) + static_cast<uint64_t>(c.page_size) - 1) / static_cast<uint64_t>(c.page_size));
     p.max_blocks = c.max_blocks;
     p.blocks = c.blocks;
     p.splits = a->splits;
@@ -843,10 +915,31 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.soft_cap = a->soft_cap;
     const long long grid = static_cast<long long>(c.B) * c.Hkv * p.head_tiles * a->splits;
     if (grid > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many sequences");
-    const bool whole = c.page_size % TOK == 0;
+    p.wctx.status = static_cast<Status*>(a->status);
+    p.wctx.timeout_ns = a->timeout_ns;
+    p.wctx.kernel_id = kKernelQuantDecode;
+    // pages of whole tiles whose rows' scales lie side by side are loaded by TMA
+    const int groups = c.bits == 8 ? 1 : c.head_dim / 64, row_bytes = c.head_dim * c.bits / 8;
+    const bool paged = c.page_size % TOK == 0 && c.scale_token == 4 * groups &&
+                       ((reinterpret_cast<uintptr_t>(c.k_scales) | reinterpret_cast<uintptr_t>(c.v_scales) | static_cast<uintptr_t>(c.scale_block | c.scale_head)) & 15) == 0;
+    if (paged) {
+        const uint32_t box_bytes = static_cast<uint32_t>(row_bytes < 128 ? row_bytes : 128);
+        const tdist_host::Swizzle sw = box_bytes == 128 ? tdist_host::Swizzle::B128 : (box_bytes == 64 ? tdist_host::Swizzle::B64 : tdist_host::Swizzle::B32);
+        const uint64_t dims[4] = {static_cast<uint64_t>(row_bytes), static_cast<uint64_t>(c.Hkv), static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(c.blocks)};
+        const uint64_t strides[3] = {static_cast<uint64_t>(c.code_head), static_cast<uint64_t>(c.code_token), static_cast<uint64_t>(c.code_block)};
+        const uint32_t box[4] = {box_bytes, 1, TOK, 1};
+        const uint64_t sdims[3] = {static_cast<uint64_t>(c.page_size) * groups, static_cast<uint64_t>(c.Hkv), static_cast<uint64_t>(c.blocks)};
+        const uint64_t sstrides[2] = {static_cast<uint64_t>(c.scale_head), static_cast<uint64_t>(c.scale_block)};
+        const uint32_t sbox[3] = {static_cast<uint32_t>(TOK * groups), 1, 1};
+        int rc;
+        if ((rc = tdist_host::encode_tmap(&p.tm_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 4, c.k_codes, dims, strides, box, sw))) return rc;
+        if ((rc = tdist_host::encode_tmap(&p.tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 4, c.v_codes, dims, strides, box, sw))) return rc;
+        if ((rc = tdist_host::encode_tmap(&p.tm_ks, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, 3, c.k_scales, sdims, sstrides, sbox, tdist_host::Swizzle::None))) return rc;
+        if ((rc = tdist_host::encode_tmap(&p.tm_vs, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, 3, c.v_scales, sdims, sstrides, sbox, tdist_host::Swizzle::None))) return rc;
+    }
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
-    const int rc = c.bits == 8 ? launch_dim<8>(p, c.head_dim, nh, whole, static_cast<int>(grid), stream)
-                               : launch_dim<4>(p, c.head_dim, nh, whole, static_cast<int>(grid), stream);
+    const int rc = c.bits == 8 ? launch_dim<8>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream)
+                               : launch_dim<4>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream);
     if (rc) return rc;
     if (a->splits > MAX_CLUSTER)
         TDIST_CUDA_OK(tdist_host::launch_pdl(merge_kernel, dim3(static_cast<unsigned>(c.B * a->Hq)), 128, 0, stream, p.part, a->splits, c.head_dim,

@@ -33,7 +33,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import _lib
-from ..runtime import stream_ptr
+from ..runtime import default_timeout_ns, stream_ptr
 from ..utils.profile import nvtx_range
 from . import flash_decode as FD
 from . import paged_attention as PA
@@ -394,6 +394,7 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
     if q.data_ptr() % 16:
         q = q.clone()
     a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.status, a.timeout_ns = PA._status_ptr(), default_timeout_ns()
     if a.splits > 8:
         part = torch.empty(a.cache.B * a.Hq * a.splits * (a.cache.head_dim + 2), dtype=torch.float32, device=q.device)
         a.part = part.data_ptr()
