@@ -227,9 +227,8 @@ class QuantDecodeArgs(C.Structure):
     _fields_ = [
         ("cache", QuantCacheArgs),
         ("q", C.c_void_p), ("out", C.c_void_p), ("part", C.c_void_p),
-        ("Hq", C.c_int), ("splits", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
+        ("Hq", C.c_int), ("splits", C.c_int), ("shares", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
         ("scale", C.c_float), ("soft_cap", C.c_float),
-        ("status", C.c_void_p), ("timeout_ns", C.c_uint64),
     ]
 
 

@@ -488,16 +488,15 @@ typedef struct TdistQuantCacheArgs {
     void* stream;
 } TdistQuantCacheArgs;
 
-#define TDIST_QUANT_DECODE_SPLITS 512
 typedef struct TdistQuantDecodeArgs {
     TdistQuantCacheArgs cache;
     const void* q;               /* [B, Hq, D] */
     void* out;                   /* [B, Hq, D] */
-    void* part;                  /* fp32 [B, Hq, splits, D + 2] where splits > 8 */
-    int Hq, splits, window, sinks;
+    void* part;                  /* splits 0: fp32 [shares][4 + 2 x 16 x (D + 2)], on 16 bytes */
+    int Hq;
+    int splits;                  /* CTAs per (sequence, kv head), up to 8; 0: `shares` CTAs take equal shares of all keys (up to 511 sequences) */
+    int shares, window, sinks;
     float scale, soft_cap;
-    void* status;
-    uint64_t timeout_ns;
 } TdistQuantDecodeArgs;
 
 int tdist_quant_cache_write(const TdistQuantCacheArgs* args);

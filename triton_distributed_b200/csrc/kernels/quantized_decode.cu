@@ -20,13 +20,15 @@
 // S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix, and every warp streams tiles of 16 tokens through a cp.async ring of its own.
 // The sum over a row's dimensions may run in any order, the output's dimensions may be dealt to the MMA's rows in any order and so may the
 // tokens, so all three are chosen by what a wide load from shared memory gives: of 64 dimensions of a key, the four lanes of a quad take 16 neighbouring
-// ones each, and of a value's each eighth lane an eighth. (Loads straight into registers, each as soon as the registers are free: too few bytes under
-// way, warps waited for memory half of their time.)
+// ones each, and of a value's each eighth lane an eighth. Not by TMA: a box of 16 rows of one head costs it some 5 clocks a row and SM, whatever the rows' width
+// (16 x 16384 keys of 8 kv heads of 128, loads alone: 4 bits 75 us, these copies 55; 8 bits 93 and 88). Not straight into registers: too few bytes under
+// way, warps waited for memory half of their time.
 //
-// A CTA is 8 warps of one (sequence, kv head, part of the keys); tiles of 16 tokens go round the warps. Warps meet in shared memory;
-// up to 8 parts are a cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); more parts go through a
-// workspace and a second kernel. No counters: nothing has to be zero before a call, and calls share nothing.
-#include <cuda.h>
+// Work. A segment is the keys of one (sequence, kv head, tile of query heads), cut into tiles of 16 tokens. Either a segment has `splits` CTAs, up to 8, a
+// cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); or the machine is filled once and every CTA takes an equal
+// share of all segments' tiles in a row, from the lengths on the device: pieces of segments, of which the first and the last may be shared with other
+// CTAs. Those leave their sums in a workspace, and a second kernel adds them up. The copies run on from one piece to the next: while a piece's sums meet, the next one's
+// first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -36,7 +38,6 @@
 #include <string>
 
 #include "../device/ptx.cuh"
-#include "../device/signal.cuh"
 #include "../device/soft_cap.cuh"
 #include "../include/tdist.h"
 #include "../runtime/host_common.h"
@@ -44,31 +45,26 @@
 namespace tdist {
 namespace qdecode {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-// warps that compute: where tiles come by TMA, one warp loads for the others
-__host__ __device__ constexpr int consumers(bool paged) { return paged ? WARPS - 1 : WARPS; }
 constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
-constexpr int kKernelQuantDecode = 13;
 // Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled: a weight
 // times its scale's share of the unit is rounded to fp16 whatever its size, and 2^8 is far below fp16's largest.
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
-    CUtensorMap tm_k, tm_v;        // PAGED: codes as bytes {ROW, Hkv, page, blocks}, box {BOX, 1, 16, 1}
-    CUtensorMap tm_ks, tm_vs;      // scales as words {page NG, Hkv, blocks}, box {16 NG, 1, 1}
     const void* q;                 // [B, Hq, D]
     const uint8_t *k, *v;
     const char *ks, *vs;
     const int *table, *lens;
-    float* part;                   // [B * Hq][splits][D + 2]: sums, maximum, sum of weights (more than MAX_CLUSTER parts)
+    float* part;                   // shares: [CTAs][2][8 NH][D + 2]: sums, maximum, sum of weights of a CTA's first and last piece
+    int4* info;                    // shares: [CTAs]: the segment that this CTA's first piece goes on with (see merge_kernel)
     void* out;
     long long code_block, code_token, code_head, scale_block, scale_head, scale_token;   // bytes
+    int B, shares;                 // shares: CTAs that share all tiles equally, 0: `splits` CTAs per segment
     int Hq, Hkv, head_tiles, page_size, page_shift, max_blocks, blocks, splits, window, sinks, table_keys, is_f16;
     float scale, soft_cap;
-    uint32_t page_mul;             // t / page_size = (t page_mul) >> page_shift for t < 2^31
-    WaitCtx wctx;
+    uint32_t page_mul;             // not PAGED: t / page_size = (t page_mul) >> page_shift for t < 2^31
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -133,8 +129,8 @@ __device__ __forceinline__ Words<W> load_words(const void* p) {
     return r;
 }
 
-// A tile in shared memory: 16 rows of K codes, 16 of V codes, and apart from them the rows' scales. The 16-byte chunks of a row lie as a TMA load with the
-// swizzle of the row's width leaves them (rows of 256 bytes as two halves of 128), and the MMA's rows are tokens in an order that makes
+// A tile in shared memory: 16 rows of K codes, 16 of V codes, the rows' scales. The 16-byte chunks of a row are swizzled with its number (rows
+// of 256 bytes as two halves of 128), and the MMA's rows are tokens in an order that makes
 // the loads below free of bank conflicts but for two of K's in twos (4 bits, heads of 64 and 256): a key's load takes two rows whose tokens differ in
 // bit 0, or four whose tokens differ in bits 0 and 2, and a value's four columns whose tokens differ in bits 0 and 2, and in bits 1 and 2.
 template <int BITS, int D>
@@ -152,9 +148,8 @@ struct Shape {
     static constexpr int BOX = ROW < 128 ? ROW : 128;      // bytes of a row that lie together
     static constexpr int SB = 4 * NG;                      // bytes of its scales
     static constexpr int TILE = TOK * ROW;                 // K; V behind it
-    static constexpr int SCALES = TOK * SB < 128 ? 128 : TOK * SB;   // K's, on 128 bytes as TMA wants them; V's behind them
-    static constexpr int STAGE = 2 * TILE + 2 * SCALES;    // bytes of a place in the ring
-    static constexpr int LOADED = 2 * TILE + 2 * TOK * SB;
+    static constexpr int SCALES = TOK * SB;                // K's; V's behind them
+    static constexpr int STAGE = 2 * TILE + 2 * SCALES;
 
     static __device__ __forceinline__ uint32_t at(int t, int byte) {
         const int chunk = (byte & (BOX - 1)) >> 4;
@@ -200,206 +195,348 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// CTAs per SM, and tiles that the rings of a CTA have room for in 206 KB per SM: at most 8 per warp, and as many for each. (A place belongs to one
-// warp: only a warp that has waited for a place's earlier tiles itself can tell by a barrier's parity that the next one is there.)
+// Shared memory behind the rings: buffers in which the warps' sums meet, q, then a cluster's slices or the shares' lengths and prefix sums.
+constexpr int MAX_SHARED = 511;   // sequences of a call that is dealt out in shares
+// CTAs per SM and their warps: two of six, which then have up to 168 registers per thread, or one of eight or (rings of 4 x 8 KB) six where a thread needs more
 __host__ __device__ constexpr int ctas_per_sm(int d, int nh) { return d == 256 || nh == 2 ? 1 : 2; }
-__host__ __device__ constexpr int places_of(int stage, int d, int nh, bool paged) {
-    const int each = 206 * 1024 / ctas_per_sm(d, nh) / stage / consumers(paged);
-    return (each < 8 ? each : 8) * consumers(paged);
+__host__ __device__ constexpr int warps_of(int d, int nh) { return nh == 2 ? 8 : 6; }
+__host__ __device__ constexpr int buffers_of(int d, int nh) { return warps_of(d, nh) - 4; }
+__host__ __device__ constexpr int sums_bytes(int d, int nh) { return buffers_of(d, nh) * 8 * nh * o_pitch(d) * 4; }
+__host__ __device__ constexpr int last_bytes(int d, int nh) {
+    return (8 * nh * d + 4 * MAX_CLUSTER) * 4 > 8 * (MAX_SHARED + 1) ? (8 * nh * d + 4 * MAX_CLUSTER) * 4 : 8 * (MAX_SHARED + 1);
+}
+__host__ __device__ constexpr int behind_rings(int d, int nh) { return sums_bytes(d, nh) + 16 * nh * d + last_bytes(d, nh); }
+// tiles that a warp's ring has room for, 8 at most: of 228 KB per SM, 1 KB per CTA the system's and 2 KB for static shared memory
+__host__ __device__ constexpr int stages_of(int stage, int d, int nh) {
+    const int each = (228 * 1024 / ctas_per_sm(d, nh) - 3 * 1024 - behind_rings(d, nh)) / stage / warps_of(d, nh);
+    return each < 8 ? each : 8;
 }
 
+// A sequence's keys as tiles: those of the first `first` tokens, then those from the window's first token on (a tile's first token is a multiple of 16)
+struct Keys {
+    int n, lo, first, sink_tiles, t_lo, tiles;
+    __device__ __forceinline__ int first_token(int i) const { return (i < sink_tiles ? i : i - sink_tiles + t_lo) * TOK; }
+};
+__device__ __forceinline__ Keys keys_of(const Params& p, int length) {
+    Keys k;
+    k.n = min(max(length, 0), p.table_keys);
+    k.lo = max(0, k.n - p.window);
+    k.first = min(p.sinks, k.lo);
+    k.sink_tiles = (k.first + TOK - 1) / TOK;
+    k.t_lo = k.lo / TOK;
+    k.tiles = k.sink_tiles + (k.n + TOK - 1) / TOK - k.t_lo;
+    return k;
+}
+
+// Tiles i0 .. i1 - 1 of segment (b, of_b)
+struct Piece {
+    int b, of_b, i0, i1;
+};
+// The pieces of this CTA, one after the other
+struct Pieces {
+    const uint32_t* prefix;   // shares: tiles of a kv head of the sequences before b; nullptr: one piece
+    uint32_t at, end;         // shares: tiles of this CTA
+    int per_b;                // segments of a sequence
+    int b, i0, i1;            // one piece: its segment is `b`
+
+    __device__ __forceinline__ bool next(Piece& x) {
+        if (prefix == nullptr) {
+            if (per_b == 0) return false;
+            x.b = b / per_b;
+            x.of_b = b - x.b * per_b;
+            x.i0 = i0;
+            x.i1 = i1;
+            per_b = 0;
+            return true;
+        }
+        if (at >= end) return false;
+        while (prefix[b + 1] * per_b <= at) ++b;
+        const uint32_t tiles = prefix[b + 1] - prefix[b], rest = at - prefix[b] * per_b;
+        x.b = b;
+        x.of_b = static_cast<int>(rest / tiles);
+        x.i0 = static_cast<int>(rest - x.of_b * tiles);
+        const uint32_t take = min(tiles - x.i0, end - at);
+        x.i1 = x.i0 + static_cast<int>(take);
+        at += take;
+        return true;
+    }
+};
+
 template <int BITS, int D, int NH, bool PAGED>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) decode_kernel(const __grid_constant__ Params p) {
     using S = Shape<BITS, D>;
-    constexpr int HEADS = 8 * NH, OP = o_pitch(D), CW = consumers(PAGED);
-    constexpr int PLACES = places_of(S::STAGE, D, NH, PAGED), STAGES = PLACES / CW;   // of all rings; of a warp's own
-    static_assert(STAGES >= 3 && PLACES * S::STAGE >= CW * HEADS * OP * 4, "the warps' sums reuse the ring");
-    extern __shared__ uint8_t smem_raw[];
-    // [PLACES] K and V codes, [PLACES] scales, the cluster's slices
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* o_s = reinterpret_cast<float*>(smem);            // [CW][HEADS][OP], when the rings are done
-    __shared__ uint64_t bars[2][PAGED ? PLACES : 1];       // PAGED: a tile's bytes are there; its place is free
-    __shared__ float m_s[CW][HEADS], l_s[CW][HEADS];
+    constexpr int WARPS = warps_of(D, NH), THREADS = 32 * WARPS, BUFS = buffers_of(D, NH);
+    constexpr int HEADS = 8 * NH, OP = o_pitch(D), STAGES = stages_of(S::STAGE, D, NH);
+    static_assert(STAGES >= 3, "two tiles ahead at least");
+    extern __shared__ __align__(128) uint8_t smem[];
+    // rings [WARPS][STAGES][STAGE], the sums' buffers, q as bytes [2][HEADS][D], a cluster's slices or lengths and prefix sums
+    float* sums_s = reinterpret_cast<float*>(smem + WARPS * STAGES * S::STAGE);   // [BUFS][HEADS][OP]
+    uint8_t* q_s = smem + WARPS * STAGES * S::STAGE + sums_bytes(D, NH);
+    uint8_t* last_s = q_s + 2 * HEADS * D;
+    __shared__ float m_s[BUFS][HEADS], l_s[BUFS][HEADS];
+    __shared__ float factor_s[HEADS], qsum_s[HEADS][S::NG];
+    __shared__ int bias_s[HEADS];
     __shared__ float part_m[MAX_CLUSTER][HEADS], part_l[MAX_CLUSTER][HEADS];
+    __shared__ uint32_t scan_s[WARPS];
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = static_cast<int>(threadIdx.x) & 31;
     const int g = lane >> 2, c = lane & 3;
-    const bool in_cluster = p.splits > 1 && p.splits <= MAX_CLUSTER;
+    const bool in_cluster = p.shares == 0 && p.splits > 1;
     if (in_cluster) cluster_arrive();                       // waited for before the first store into another CTA
-    if (PAGED) {
-        if (threadIdx.x < PLACES) {
-            mbar_init(smem_u32(&bars[0][threadIdx.x]), 1);
-            mbar_init(smem_u32(&bars[1][threadIdx.x]), 1);
-            fence_mbar_init();
-        }
-        __syncthreads();
-    }
     pdl_wait_and_release();
 
-    int x = static_cast<int>(blockIdx.x);
-    const int split = x % p.splits;
-    x /= p.splits;
-    const int tile_of_heads = x % p.head_tiles;
-    x /= p.head_tiles;
-    const int kvh = x % p.Hkv, b = x / p.Hkv;
     const int G = p.Hq / p.Hkv;
-    const int heads = min(HEADS, G - tile_of_heads * HEADS);
-    const size_t head0 = static_cast<size_t>(b) * p.Hq + kvh * G + tile_of_heads * HEADS;
-
-    // ---- the keys: tiles of the first `first` tokens, then those from the window's first token on (a tile's first token is a multiple of 16)
-    const int n = min(max(p.lens[b], 0), p.table_keys);
-    const int lo = max(0, n - p.window);
-    const int first = min(p.sinks, lo);
-    const int sink_tiles = (first + TOK - 1) / TOK;
-    const int t_lo = lo / TOK;
-    const int tiles = sink_tiles + (n + TOK - 1) / TOK - t_lo;
-    const int per = (tiles + p.splits - 1) / p.splits;
-    const int first_tile = min(split * per, tiles), i0 = first_tile + warp, i1 = min((split + 1) * per, tiles);
-
-    const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
-    auto first_token = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + t_lo) * TOK; };
-    auto in_table = [&](int t) { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * p.page_mul) >> p.page_shift); };
-    auto codes_at = [&](int place) { return smem_u32(smem) + static_cast<uint32_t>(place * 2 * S::TILE); };
-    auto scales_at = [&](int place) { return smem_u32(smem) + static_cast<uint32_t>(PLACES * 2 * S::TILE + place * 2 * S::SCALES); };
-
-    if (PAGED && warp == CW) {
-        // ---- the loading warp: a lane looks up the page of one of the next 32 tiles, then tile after tile is sent on its way. A page that the
-        // cache does not have is out of the tensor map's bounds and reads as zeros.
-        auto lookup = [&](int i) { return i < i1 ? static_cast<int>(ldg32(table + in_table(first_token(i)))) : 0; };
-        int place = 0;
-        uint32_t parity = 1;
-        int pages = lookup(first_tile + lane);
-        for (int base = first_tile; base < i1; base += 32) {
-            const int now = pages, row = first_token(base + lane) - in_table(first_token(base + lane)) * p.page_size;
-            pages = lookup(base + 32 + lane);
-            const int count = min(32, i1 - base);
-            for (int j = 0; j < count; ++j) {
-                const int page_j = __shfl_sync(0xffffffffu, now, j), row_j = __shfl_sync(0xffffffffu, row, j);
-                mbar_wait(smem_u32(&bars[1][place]), parity, p.wctx, 2);
-                if (elect_one()) {
-                    const uint32_t bar = smem_u32(&bars[0][place]), codes = codes_at(place), scales = scales_at(place);
-                    mbar_expect_tx(bar, S::LOADED);
-                    tma_load_4d(codes, &p.tm_k, bar, 0, kvh, row_j, page_j);
-                    if (S::ROW > S::BOX) tma_load_4d(codes + TOK * S::BOX, &p.tm_k, bar, S::BOX, kvh, row_j, page_j);
-                    tma_load_3d(scales, &p.tm_ks, bar, row_j * S::NG, kvh, page_j);
-                    tma_load_4d(codes + S::TILE, &p.tm_v, bar, 0, kvh, row_j, page_j);
-                    if (S::ROW > S::BOX) tma_load_4d(codes + S::TILE + TOK * S::BOX, &p.tm_v, bar, S::BOX, kvh, row_j, page_j);
-                    tma_load_3d(scales + S::SCALES, &p.tm_vs, bar, row_j * S::NG, kvh, page_j);
+    const int split = in_cluster ? static_cast<int>(blockIdx.x) % p.splits : 0;
+    Pieces pieces;
+    pieces.prefix = nullptr;
+    pieces.per_b = p.Hkv * p.head_tiles;
+    pieces.b = 0;
+    uint32_t total_tiles = 0, ctas = 0, from = 0;           // shares: all tiles, the CTAs that have some, this CTA's first
+    if (p.shares > 0) {
+        uint32_t* prefix = reinterpret_cast<uint32_t*>(last_s);
+        int* lens = reinterpret_cast<int*>(last_s) + MAX_SHARED + 1;
+        uint32_t carry = 0;
+        for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+            const int b = b0 + static_cast<int>(threadIdx.x);
+            const int length = b < p.B ? p.lens[b] : 0;
+            if (b < p.B) lens[b] = length;
+            uint32_t sum = static_cast<uint32_t>(keys_of(p, length).tiles);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+                sum += lane >= o ? v : 0u;
+            }
+            if (lane == 31) scan_s[warp] = sum;
+            __syncthreads();
+            uint32_t all = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                if (w == warp) sum += carry + all;
+                all += scan_s[w];
+            }
+            if (b < p.B) prefix[b + 1] = sum;
+            carry += all;
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) prefix[0] = 0;
+        __syncthreads();
+        total_tiles = carry * pieces.per_b;
+        ctas = min(static_cast<uint32_t>(p.shares), total_tiles);
+        const uint32_t cta = blockIdx.x;
+        if (cta < ctas) {
+            from = static_cast<uint32_t>(static_cast<uint64_t>(cta) * total_tiles / ctas);
+            pieces.at = from;
+            pieces.end = static_cast<uint32_t>(static_cast<uint64_t>(cta + 1) * total_tiles / ctas);
+            int lo = 0, hi = p.B;   // the sequence of the first tile: the last one that starts at it or before (those without tiles start where the next does)
+            while (hi - lo > 1) {
+                const int m = (lo + hi) >> 1;
+                if (prefix[m] * pieces.per_b <= from) lo = m;
+                else hi = m;
+            }
+            pieces.b = lo;
+        } else {
+            pieces.at = pieces.end = 0;
+        }
+        pieces.prefix = prefix;
+        if (threadIdx.x == 0) {
+            // for the second kernel: head 0 and heads of the segment that goes on here, and the CTAs that have some of it
+            int4 info = make_int4(-1, 0, 0, 0);
+            Pieces first = pieces;
+            Piece x;
+            if (cta < ctas && first.next(x) && x.i0 > 0) {
+                const uint32_t start = from - x.i0, stop = start + (prefix[x.b + 1] - prefix[x.b]);
+                const uint32_t c0 = static_cast<uint32_t>(((static_cast<uint64_t>(start) + 1) * ctas - 1) / total_tiles);
+                const uint32_t c1 = static_cast<uint32_t>((static_cast<uint64_t>(stop) * ctas - 1) / total_tiles);
+                if (cta == c0 + 1) {
+                    const int kvh = x.of_b / p.head_tiles, tile_of_heads = x.of_b % p.head_tiles;
+                    const bool whole = static_cast<uint32_t>(static_cast<uint64_t>(c0) * total_tiles / ctas) == start;   // c0's first piece, not its last
+                    info = make_int4(x.b * p.Hq + kvh * G + tile_of_heads * HEADS, min(HEADS, G - tile_of_heads * HEADS), static_cast<int>(2 * c0 + (whole ? 0 : 1)), static_cast<int>(c1));
                 }
-                __syncwarp();
-                if (++place == PLACES) {
-                    place = 0;
-                    parity ^= 1u;
+            }
+            p.info[cta] = info;
+        }
+        // sequences without keys
+        for (int b = static_cast<int>(cta); b < p.B; b += p.shares)
+            if (prefix[b + 1] == prefix[b])
+                for (int i = static_cast<int>(threadIdx.x); i < p.Hq * D / 2; i += THREADS) static_cast<uint32_t*>(p.out)[static_cast<size_t>(b) * (p.Hq * D / 2) + i] = 0u;
+    } else {
+        pieces.b = static_cast<int>(blockIdx.x) / p.splits;
+        const int tiles = keys_of(p, p.lens[pieces.b / pieces.per_b]).tiles, per = (tiles + p.splits - 1) / p.splits;
+        pieces.i0 = min(split * per, tiles);
+        pieces.i1 = min((split + 1) * per, tiles);
+    }
+    auto keys_in = [&](int b) { return keys_of(p, p.shares > 0 ? reinterpret_cast<const int*>(last_s)[MAX_SHARED + 1 + b] : p.lens[b]); };
+
+    // ---- The copies. A cursor goes over this warp's tiles of all pieces, STAGES - 1 of them ahead of the sums. PAGED (pages of 16, 32, 64 .. tokens): a tile lies
+    // in one page, every lane knows where. Otherwise lane r and r + 16 look token r up and tell the others. -1: not seen; rows that are
+    // not seen, or whose page the cache does not have, are zeros.
+    constexpr int CHUNKS = S::ROW / 16, ROWS = 32 / CHUNKS;   // a warp copies ROWS rows at once, 16 bytes a lane
+    const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS, my_token = lane & 15;
+    const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * STAGES * S::STAGE);
+    uint32_t dst_at[TOK / ROWS];
+#pragma unroll
+    for (int j = 0; j < TOK / ROWS; ++j) dst_at[j] = S::at(j * ROWS + lrow, lchunk * 16);
+    const uint32_t code_token = static_cast<uint32_t>(p.code_token), scale_token = static_cast<uint32_t>(p.scale_token);   // PAGED: strides fit 32 bits
+    auto in_table = [&](int t) {
+        return PAGED ? t >> p.page_shift : static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * p.page_mul) >> p.page_shift);
+    };
+    Pieces coming = pieces;
+    Keys c_keys;
+    const int* c_table = nullptr;
+    const uint8_t *c_k = nullptr, *c_v = nullptr;
+    const char* c_s = nullptr;               // lanes 0..15 copy the scales of the keys, 16..31 of the values
+    int c_i = 0, c_end = 0, c_turn = 0, c_page = -1;
+    c_keys.n = c_keys.lo = c_keys.first = c_keys.sink_tiles = c_keys.t_lo = 0;
+    bool c_more = true;
+    // to the next tile, and its page's number
+    auto advance = [&]() {
+        c_i += WARPS;
+        while (c_i >= c_end && c_more) {
+            Piece x;
+            c_more = coming.next(x);
+            if (!c_more) break;
+            c_keys = keys_in(x.b);
+            const int kvh = x.of_b / p.head_tiles;
+            c_table = p.table + static_cast<size_t>(x.b) * p.max_blocks;
+            c_k = p.k + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
+            c_v = p.v + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
+            c_s = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head + (PAGED ? my_token * p.scale_token : 0);
+            c_i = x.i0 + (warp + WARPS - c_turn) % WARPS;
+            c_end = x.i1;
+            c_turn = (c_turn + x.i1 - x.i0) % WARPS;
+        }
+        if (c_i < c_end) {
+            const int t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
+            const bool seen = PAGED || (c_i < c_keys.sink_tiles ? t < c_keys.first : t >= c_keys.lo && t < c_keys.n);
+            c_page = seen ? static_cast<int>(ldg32(c_table + in_table(t))) : -1;
+        }
+    };
+    auto copy_next = [&](uint32_t to) {
+        if (c_i < c_end) {
+            const int t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
+            const bool live = static_cast<unsigned>(c_page) < static_cast<unsigned>(p.blocks);
+            const uint32_t from = live ? static_cast<uint32_t>(c_page) : 0u;
+            if (PAGED) {
+                const uint32_t row = static_cast<uint32_t>(t) & static_cast<uint32_t>(p.page_size - 1), block = static_cast<uint32_t>(p.code_block);
+                const uint8_t* k = c_k + static_cast<uint64_t>(from) * block + static_cast<uint64_t>(row) * code_token;
+                const uint8_t* v = c_v + static_cast<uint64_t>(from) * block + static_cast<uint64_t>(row) * code_token;
+#pragma unroll
+                for (int j = 0; j < TOK / ROWS; ++j) {
+                    copy16(to + dst_at[j], k + static_cast<uint64_t>(code_token) * (j * ROWS), !live);
+                    copy16(to + dst_at[j] + S::TILE, v + static_cast<uint64_t>(code_token) * (j * ROWS), !live);
+                }
+                copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + static_cast<uint64_t>(from) * static_cast<uint32_t>(p.scale_block) + static_cast<uint64_t>(row) * scale_token, !live);
+            } else {
+                const int row = t - in_table(t) * p.page_size;
+                const long long off = live ? from * p.code_block + row * p.code_token : 0;
+#pragma unroll
+                for (int j = 0; j < TOK / ROWS; ++j) {
+                    const long long at = __shfl_sync(0xffffffffu, off, j * ROWS + lrow);
+                    const bool none = !__shfl_sync(0xffffffffu, static_cast<int>(live), j * ROWS + lrow);
+                    copy16(to + dst_at[j], c_k + at, none);
+                    copy16(to + dst_at[j] + S::TILE, c_v + at, none);
+                }
+                copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + (live ? from * p.scale_block + row * p.scale_token : 0), !live);
+            }
+            advance();
+        }
+        copy_commit();
+    };
+    advance();
+#pragma unroll
+    for (int a = 0; a < STAGES - 1; ++a) copy_next(ring + a * S::STAGE);
+
+    // what this lane reads of a tile: tokens of rows g and g + 8 of the MMA (keys and scales), of columns 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (values)
+    const int t_row = token_of(g);
+    uint32_t k_at[S::KC], v_at[2][S::VC];
+#pragma unroll
+    for (int j = 0; j < S::KC; ++j) k_at[j] = S::at(t_row, S::k_byte(j, c));
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
+    const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
+    uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
+    int turn = 0;            // the warp that has a piece's first tile: tiles go round the warps from piece to piece
+    bool first_piece = true;
+    Piece x;
+    while (pieces.next(x)) {
+    const Keys keys = keys_in(x.b);
+    const int kvh = x.of_b / p.head_tiles, tile_of_heads = x.of_b % p.head_tiles;
+    const int heads = min(HEADS, G - tile_of_heads * HEADS);
+    const size_t head0 = static_cast<size_t>(x.b) * p.Hq + kvh * G + tile_of_heads * HEADS;
+    const int i0 = x.i0 + (warp + WARPS - turn) % WARPS, i1 = x.i1;
+
+    // ---- q to 16 bits, a warp per head: the high and the low bytes in the order in which the codes' registers have their dimensions
+    for (int head = warp; head < HEADS; head += WARPS) {
+        constexpr int E = D / 32;                // dimensions of a lane
+        float f[E];
+        const bool there = head < heads;
+        {
+            const Words<E / 2> w = load_words<E / 2>(static_cast<const char*>(p.q) + (head0 + (there ? head : 0)) * (D * 2) + lane * (E * 2));
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                if (p.is_f16) {
+                    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w.w[e]));
+                    f[2 * e] = t.x;
+                    f[2 * e + 1] = t.y;
+                } else {
+                    f[2 * e] = __uint_as_float(w.w[e] << 16);
+                    f[2 * e + 1] = __uint_as_float(w.w[e] & 0xffff0000u);
                 }
             }
         }
-    } else {
-    // ---- not PAGED (pages of other sizes, scales with strides): every warp copies its own tiles, 16 bytes of a row per lane. A lane looks up token
-    // lane % 16; -1: not seen. Rows that are not seen, or whose page the cache does not have, are zeros.
-    const int my_token = lane & 15;
-    auto lookup = [&](int i) {
-        const int t = first_token(i) + my_token;
-        return i < i1 && (i < sink_tiles ? t < first : t >= lo && t < n) ? static_cast<int>(ldg32(table + in_table(t))) : -1;
-    };
-    constexpr int CHUNKS = S::ROW / 16, ROWS = 32 / CHUNKS;   // rows that a warp copies at once
-    const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
-    const uint8_t* k_lane = p.k + kvh * p.code_head + lchunk * 16;
-    const uint8_t* v_lane = p.v + kvh * p.code_head + lchunk * 16;
-    const char* s_lane = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head;   // lanes 0..15 copy the scales of the keys, 16..31 of the values
-    auto issue = [&](int i, int page, int place) {
-        const int t = first_token(i) + my_token;
-        const int row = t - in_table(t) * p.page_size;
-        const bool live = static_cast<unsigned>(page) < static_cast<unsigned>(p.blocks);
-        const long long from = live ? page : 0;
-        const long long off = from * p.code_block + row * p.code_token, soff = from * p.scale_block + row * p.scale_token;
-        const uint32_t codes = codes_at(place);
+        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < TOK / ROWS; ++j) {
-            const int r = j * ROWS + lrow;
-            const long long at = __shfl_sync(0xffffffffu, off, r);
-            const bool none = !__shfl_sync(0xffffffffu, static_cast<int>(live), r);
-            const uint32_t dst = codes + S::at(r, lchunk * 16);
-            copy16(dst, k_lane + at, none);
-            copy16(dst + S::TILE, v_lane + at, none);
+        for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+        top = __reduce_max_sync(0xffffffffu, top);
+        // magnitudes below 2^-100 count as that; a query with a NaN or an infinity has a factor of NaN, and so has its result
+        const bool good = top < 0x7f800000u;
+        const float most = fmaxf(good ? __uint_as_float(top) : 1.f, 7.888609052210118e-31f);
+        const float mul = there && good ? 32512.f / most : 0.f;
+        int sum = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int v = max(-32512, min(32512, __float2int_rn(f[e] * mul)));
+            const int hi = (v + 128) >> 8, d = lane * E + e;
+            const int at = BITS == 8 ? d : (d & ~7) + (d & 1) * 4 + ((d >> 1) & 3);
+            q_s[head * D + at] = static_cast<uint8_t>(hi);
+            q_s[(HEADS + head) * D + at] = static_cast<uint8_t>(v - 256 * hi);
+            sum += v;
         }
-        copy_small<S::SB>(scales_at(place) + (lane >> 4) * S::SCALES + my_token * S::SB, s_lane + soff, !live);
-    };
-    int page = -1;
-    if (!PAGED) {
-        page = lookup(i0);
+        constexpr int PER = 32 / S::NG;          // lanes of a group (8 bits: all)
 #pragma unroll
-        for (int a = 0; a < STAGES - 1; ++a) {
-            const int i = i0 + a * WARPS, now = page;
-            page = lookup(i + WARPS);
-            if (i < i1) issue(i, now, warp * STAGES + a);
-            copy_commit();
+        for (int o = 1; o < PER; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane % PER == 0) qsum_s[head][lane / PER] = static_cast<float>(sum);
+        if (lane == 0) {
+            bias_s[head] = BITS == 8 ? sum * -128 : 0;
+            factor_s[head] = (good ? most * (1.f / 32512.f) * p.scale : __uint_as_float(0x7fffffffu)) * (p.soft_cap > 0.f ? 1.f : kLog2e);
         }
     }
+    __syncthreads();
 
-    // ---- q as the second operand: column g of the MMA is head 8 h + g, its dimensions 16 c .. 16 c + 15 of every 64 are this lane's
+    // ---- q as the second operand: column g of the MMA is head 8 h + g
     uint32_t qf[NH][S::KC][4][2];  // high and low bytes of four dimensions
     float factor[NH][2];           // of heads 8 h + 2 c + {0, 1}: what turns a product of codes into a score in units of log2
     int bias[NH][2];               // 8 bits: -128 times the sum of the 16-bit q
     float qsum[NH][2][S::NG];      // 4 bits: that sum over a group
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-        const int head = 8 * h + g;
-        const char* src = static_cast<const char*>(p.q) + (head0 + (head < heads ? head : 0)) * (D * 2);
-        float f[S::KC][16];
-        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < S::KC; ++j) {
-            // the dimensions whose codes lie in this lane's bytes of chunk j
-            const Words<8> w = load_words<8>(src + (BITS == 8 ? 2 : 4) * S::k_byte(j, c));
+        for (int j = 0; j < S::KC; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (p.is_f16) {
-                    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w.w[e]));
-                    f[j][2 * e] = t.x;
-                    f[j][2 * e + 1] = t.y;
-                } else {
-                    f[j][2 * e] = __uint_as_float(w.w[e] << 16);
-                    f[j][2 * e + 1] = __uint_as_float(w.w[e] & 0xffff0000u);
-                }
-                top = max(top, max(__float_as_uint(f[j][2 * e]) & 0x7fffffffu, __float_as_uint(f[j][2 * e + 1]) & 0x7fffffffu));
+            for (int part = 0; part < 2; ++part) {
+                const uint4 w = *reinterpret_cast<const uint4*>(q_s + (part * HEADS + 8 * h + g) * D + (BITS == 8 ? 1 : 2) * S::k_byte(j, c));
+                qf[h][j][0][part] = w.x;
+                qf[h][j][1][part] = w.y;
+                qf[h][j][2][part] = w.z;
+                qf[h][j][3][part] = w.w;
             }
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // magnitudes below 2^-100 count as that; a query with a NaN or an infinity has a factor of NaN, and so has its result
-        const bool good = top < 0x7f800000u;
-        const float most = fmaxf(good ? __uint_as_float(top) : 1.f, 7.888609052210118e-31f);
-        const float mul = head < heads && good ? 32512.f / most : 0.f;
-        int sum = 0;
-#pragma unroll
-        for (int j = 0; j < S::KC; ++j) {
-            int part = 0, hi[16], low8[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int v = max(-32512, min(32512, __float2int_rn(f[j][k] * mul)));
-                hi[k] = (v + 128) >> 8;
-                low8[k] = v - 256 * hi[k];
-                part += v;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                // four codes of a register of the first operand
-                const int d = BITS == 8 ? 4 * k : 8 * (k >> 1) + (k & 1), e = BITS == 8 ? 1 : 2;
-                qf[h][j][k][0] = pack_bytes(hi[d], hi[d + e], hi[d + 2 * e], hi[d + 3 * e]);
-                qf[h][j][k][1] = pack_bytes(low8[d], low8[d + e], low8[d + 2 * e], low8[d + 3 * e]);
-            }
-            part += __shfl_xor_sync(0xffffffffu, part, 1);
-            part += __shfl_xor_sync(0xffffffffu, part, 2);
-            sum += part;
-            if (BITS == 4) {
-#pragma unroll
-                for (int r = 0; r < 2; ++r) qsum[h][r][j] = static_cast<float>(__shfl_sync(0xffffffffu, part, (2 * c + r) * 4));
-            }
-        }
-        const float down = good ? most * (1.f / 32512.f) * p.scale : __uint_as_float(0x7fffffffu);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            factor[h][r] = __shfl_sync(0xffffffffu, down, (2 * c + r) * 4) * (p.soft_cap > 0.f ? 1.f : kLog2e);
-            bias[h][r] = BITS == 8 ? __shfl_sync(0xffffffffu, sum, (2 * c + r) * 4) * -128 : 0;
+            factor[h][r] = factor_s[8 * h + 2 * c + r];
+            bias[h][r] = bias_s[8 * h + 2 * c + r];
+#pragma unroll
+            for (int k = 0; k < S::NG; ++k) qsum[h][r][k] = qsum_s[8 * h + 2 * c + r][k];
         }
     }
 
@@ -420,31 +557,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
             for (int k = 0; k < S::NG; ++k) low[h][r][k] = 0.f;
         }
     }
-    const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
 
-    // what this lane reads of a tile: tokens of rows g and g + 8 of the MMA (keys and scales), of columns 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (values)
-    const int t_row = token_of(g);
-    uint32_t k_at[S::KC], v_at[2][S::VC];
-#pragma unroll
-    for (int j = 0; j < S::KC; ++j) k_at[j] = S::at(t_row, S::k_byte(j, c));
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
-    int place = PAGED ? warp : warp * STAGES, free_place = warp * STAGES + STAGES - 1;
-    uint32_t parity = 0;
-    for (int i = i0; i < i1; i += CW) {
-        if (PAGED) {
-            mbar_wait(smem_u32(&bars[0][place]), parity, p.wctx, 1);
-        } else {
-            copy_wait<STAGES - 2>();
-            __syncwarp();   // the tile is here, and the place of the one before it is free
-            const int ahead = i + (STAGES - 1) * WARPS, now = page;
-            page = lookup(ahead + WARPS);
-            if (ahead < i1) issue(ahead, now, free_place);
-            copy_commit();
-        }
-        const uint32_t stage = codes_at(place), scales = scales_at(place) + static_cast<uint32_t>(t_row * S::SB);
+    for (int i = i0; i < i1; i += WARPS) {
+        copy_wait<STAGES - 2>();
+        __syncwarp();   // the tile is here, and the place of the one before it is free
+        copy_next(free_stage);
+        const uint32_t scales = stage + 2 * S::TILE + static_cast<uint32_t>(t_row * S::SB);
         // ---- S^T = K Q^T, a sum per group of dimensions and byte of q
         float s[NH][4];
         Words<S::KW> kw[2][S::KC];
@@ -486,8 +604,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
                 for (int e = 0; e < 4; ++e) acc[h][k][e] = acc[h][k][e] * 256 + acc_low[h][k][e];
             }
         // ---- scales, cap; masks at the ends of what is seen
-        const int t0 = first_token(i);
-        const bool sink = i < sink_tiles, edge = sink || t0 < lo || t0 + TOK > n;
+        const int t0 = keys.first_token(i);
+        const bool sink = i < keys.sink_tiles, edge = sink || t0 < keys.lo || t0 + TOK > keys.n;
         bool higher = false;
 #pragma unroll
         for (int h = 0; h < NH; ++h)
@@ -517,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int t = t0 + t_row + 8 * r;
-                const bool seen = sink ? t < first : t >= lo && t < n;
+                const bool seen = sink ? t < keys.first : t >= keys.lo && t < keys.n;
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -638,38 +756,21 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
                 }
             }
         }
-        if (PAGED) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars[1][place]));
-            place += CW;
-            if (place >= PLACES) {
-                place -= PLACES;
-                parity ^= 1u;
-            }
-        } else {
-            free_place = place;
-            if (++place == warp * STAGES + STAGES) place = warp * STAGES;
-        }
+        free_stage = stage;
+        stage = stage + S::STAGE == ring + STAGES * S::STAGE ? ring : stage + S::STAGE;
     }
-    if (!PAGED) copy_wait<0>();
-    // the rings are done once every warp is here: the sums take their place
-    named_barrier(1, CW * 32);
+    turn = (turn + x.i1 - x.i0) % WARPS;
 
-    // ---- the warps meet in shared memory
+    // ---- the warps' sums, in the values' units
+    float m_run[NH][2];
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int head = 8 * h + 2 * c + r;
-            float l = l_run[h][r];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (g == 0) {
-                m_s[warp][head] = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r];
-                l_s[warp][head] = l;
-            }
-            float* dst = o_s + (warp * HEADS + head) * OP;
+            m_run[h][r] = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r];
+            l_run[h][r] += __shfl_xor_sync(0xffffffffu, l_run[h][r], 4);
+            l_run[h][r] += __shfl_xor_sync(0xffffffffu, l_run[h][r], 8);
+            l_run[h][r] += __shfl_xor_sync(0xffffffffu, l_run[h][r], 16);
 #pragma unroll
             for (int j = 0; j < S::VC; ++j) {
                 float add = 0.f;
@@ -682,140 +783,183 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NH)) decode_kernel(con
 #pragma unroll
                 for (int k = 0; k < S::VD / 2; ++k) {
                     const int m = j * (S::VD / 2) + k;
-                    *reinterpret_cast<float2*>(dst + j * (D / S::VC) + g * S::VD + 2 * k) =
-                        make_float2(o[h][m][r] * unit + add, o[h][m][2 + r] * (BITS == 8 ? unit : unit * 0.0625f) + add);
+                    o[h][m][r] = o[h][m][r] * unit + add;
+                    o[h][m][2 + r] = o[h][m][2 + r] * (BITS == 8 ? unit : unit * 0.0625f) + add;
                 }
             }
         }
+    // they meet two and two: warps 4 .. give theirs to 0 .., 2 and 3 to 0 and 1, 1 to 0
+    auto give = [&](int buf) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int head = 8 * h + 2 * c + r;
+                if (head >= heads) continue;
+                if (g == 0) {
+                    m_s[buf][head] = m_run[h][r];
+                    l_s[buf][head] = l_run[h][r];
+                }
+                float* dst = sums_s + (buf * HEADS + head) * OP + g * S::VD;
+#pragma unroll
+                for (int m = 0; m < S::MT; ++m)
+                    *reinterpret_cast<float2*>(dst + (m / (S::VD / 2)) * (D / S::VC) + 2 * (m % (S::VD / 2))) = make_float2(o[h][m][r], o[h][m][2 + r]);
+            }
+    };
+    auto take = [&](int buf) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int head = 8 * h + 2 * c + r;
+                if (head >= heads) continue;
+                const float m_other = m_s[buf][head], m = fmaxf(m_run[h][r], m_other), mu = m == -CUDART_INF_F ? 0.f : m;
+                const float fa = exp2f(m_run[h][r] - mu), fb = exp2f(m_other - mu);
+                l_run[h][r] = l_run[h][r] * fa + l_s[buf][head] * fb;
+                m_run[h][r] = m;
+                const float* src = sums_s + (buf * HEADS + head) * OP + g * S::VD;
+#pragma unroll
+                for (int k = 0; k < S::MT; ++k) {
+                    const float2 v = *reinterpret_cast<const float2*>(src + (k / (S::VD / 2)) * (D / S::VC) + 2 * (k % (S::VD / 2)));
+                    o[h][k][r] = o[h][k][r] * fa + v.x * fb;
+                    o[h][k][2 + r] = o[h][k][2 + r] * fa + v.y * fb;
+                }
+            }
+    };
+    if (warp >= 4) give(warp - 4);
+    __syncthreads();
+    if (warp < WARPS - 4) take(warp);
+    __syncthreads();
+    if (warp == 2 || warp == 3) give(warp - 2);
+    __syncthreads();
+    if (warp < 2) take(warp);
+    if (warp == 1) give(1);
+    __syncthreads();
+    if (warp == 0) {
+        take(1);
+        give(0);
     }
     __syncthreads();
-    if (in_cluster) cluster_wait();   // every CTA of the cluster runs
 
-    // A part's sums go to the slice's owner (the CTA itself without a cluster), relative to the part's maximum
     const int total = heads * D;
-    const int slices = in_cluster ? p.splits : 1;
-    const int slice = ((total + slices - 1) / slices + 3) & ~3;
-    float* slice_s = reinterpret_cast<float*>(smem + PLACES * S::STAGE);   // [splits][slice]
-    const bool to_workspace = p.splits > MAX_CLUSTER;
-    for (int idx = static_cast<int>(threadIdx.x); idx < total; idx += THREADS) {
-        const int head = idx / D, d = idx % D;
-        float m = -CUDART_INF_F;
-#pragma unroll
-        for (int w = 0; w < CW; ++w) m = fmaxf(m, m_s[w][head]);
-        const float mu = m == -CUDART_INF_F ? 0.f : m;
-        float l = 0.f, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < CW; ++w) {
-            const float f = exp2f(m_s[w][head] - mu);
-            l += l_s[w][head] * f;
-            sum += o_s[(w * HEADS + head) * OP + d] * f;
-        }
-        if (to_workspace) {
-            float* dst = p.part + ((head0 + head) * p.splits + split) * (D + 2);
-            dst[d] = sum;
-            if (d == 0) {
-                dst[D] = m;
-                dst[D + 1] = l;
-            }
-        } else {
-            const int owner = idx / slice;
-            float* at = slice_s + split * slice + (idx - owner * slice);
-            if (in_cluster) st_shared_cluster_f32(mapa_u32(smem_u32(at), static_cast<uint32_t>(owner)), sum);
-            else *at = sum;
-            if (d == 0) {
-                for (int o2 = 0; o2 < slices; ++o2) {
-                    if (in_cluster) {
-                        st_shared_cluster_f32(mapa_u32(smem_u32(&part_m[split][head]), static_cast<uint32_t>(o2)), m);
-                        st_shared_cluster_f32(mapa_u32(smem_u32(&part_l[split][head]), static_cast<uint32_t>(o2)), l);
-                    } else {
-                        part_m[0][head] = m;
-                        part_l[0][head] = l;
-                    }
-                }
-            }
-        }
-    }
-    if (to_workspace) return;
     if (in_cluster) {
+        // ---- the parts' sums go to their slice's owner, relative to the part's maximum
+        cluster_wait();   // every CTA of the cluster runs
+        const int slice = ((total + p.splits - 1) / p.splits + 3) & ~3;
+        float* slice_s = reinterpret_cast<float*>(last_s);   // [splits][slice]
+        for (int idx = static_cast<int>(threadIdx.x); idx < total; idx += THREADS) {
+            const int head = idx / D, d = idx % D, owner = idx / slice;
+            st_shared_cluster_f32(mapa_u32(smem_u32(slice_s + split * slice + (idx - owner * slice)), static_cast<uint32_t>(owner)), sums_s[head * OP + d]);
+        }
+        for (int idx = static_cast<int>(threadIdx.x); idx < heads * p.splits; idx += THREADS) {
+            const int head = idx % heads;
+            const uint32_t to = static_cast<uint32_t>(idx / heads);
+            st_shared_cluster_f32(mapa_u32(smem_u32(&part_m[split][head]), to), m_s[0][head]);
+            st_shared_cluster_f32(mapa_u32(smem_u32(&part_l[split][head]), to), l_s[0][head]);
+        }
         cluster_arrive();
         cluster_wait();
-    } else {
-        __syncthreads();
-    }
-    const int base = in_cluster ? split * slice : 0;
-    const int mine = min(slice, total - base);
-    for (int idx = static_cast<int>(threadIdx.x) * 2; idx < mine; idx += THREADS * 2) {   // (D and slices are even)
-        const int head = (base + idx) / D;
-        float m = -CUDART_INF_F;
-        for (int s2 = 0; s2 < slices; ++s2) m = fmaxf(m, part_m[s2][head]);
-        const float mu = m == -CUDART_INF_F ? 0.f : m;
-        float l = 0.f, a0 = 0.f, a1 = 0.f;
-        for (int s2 = 0; s2 < slices; ++s2) {
-            const float f = exp2f(part_m[s2][head] - mu);
-            l += part_l[s2][head] * f;
-            const float2 v = *reinterpret_cast<const float2*>(slice_s + s2 * slice + idx);
-            a0 += v.x * f;
-            a1 += v.y * f;
+        const int base = split * slice, mine = min(slice, total - base);
+        for (int idx = static_cast<int>(threadIdx.x) * 2; idx < mine; idx += THREADS * 2) {   // (D and slices are even)
+            const int head = (base + idx) / D;
+            float m = -CUDART_INF_F;
+            for (int s2 = 0; s2 < p.splits; ++s2) m = fmaxf(m, part_m[s2][head]);
+            const float mu = m == -CUDART_INF_F ? 0.f : m;
+            float l = 0.f, a0 = 0.f, a1 = 0.f;
+            for (int s2 = 0; s2 < p.splits; ++s2) {
+                const float f = exp2f(part_m[s2][head] - mu);
+                l += part_l[s2][head] * f;
+                const float2 v = *reinterpret_cast<const float2*>(slice_s + s2 * slice + idx);
+                a0 += v.x * f;
+                a1 += v.y * f;
+            }
+            // a sum of weights that is not positive: no keys (zeros), or a NaN among the scores
+            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            const uint32_t w = p.is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
+            *reinterpret_cast<uint32_t*>(static_cast<char*>(p.out) + (head0 * D + base + idx) * 2) = w;
         }
-        // a sum of weights that is not positive: no keys (zeros), or a NaN among the scores
-        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-        const uint32_t w = p.is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
-        *reinterpret_cast<uint32_t*>(static_cast<char*>(p.out) + (head0 * D + base + idx) * 2) = w;
+    } else if (p.shares > 0 && (x.i0 > 0 || x.i1 < keys.tiles)) {
+        float* dst = p.part + (2 * static_cast<size_t>(blockIdx.x) + (first_piece ? 0 : 1)) * (HEADS * (D + 2));
+        for (int idx = static_cast<int>(threadIdx.x); idx < total; idx += THREADS) dst[idx / D * (D + 2) + idx % D] = sums_s[idx / D * OP + idx % D];
+        if (threadIdx.x < heads) {
+            dst[threadIdx.x * (D + 2) + D] = m_s[0][threadIdx.x];
+            dst[threadIdx.x * (D + 2) + D + 1] = l_s[0][threadIdx.x];
+        }
+    } else {
+        for (int idx = static_cast<int>(threadIdx.x) * 2; idx < total; idx += THREADS * 2) {
+            const int head = idx / D;
+            const float l = l_s[0][head], inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            const float a0 = sums_s[head * OP + idx % D], a1 = sums_s[head * OP + idx % D + 1];
+            const uint32_t w = p.is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
+            *reinterpret_cast<uint32_t*>(static_cast<char*>(p.out) + (head0 * D + idx) * 2) = w;
+        }
+    }
+    first_piece = false;
     }
 }
 
-// The parts of a head, from the workspace: a CTA per head, a thread per two dimensions.
-__global__ void __launch_bounds__(128) merge_kernel(const float* part, int splits, int D, int is_f16, void* out) {
-    __shared__ float f_s[512];
-    __shared__ float l_s;
+// Shares: the sums of a segment that several CTAs have pieces of. Block (c, h): head h of the segment whose second piece is CTA c's first; its
+// first piece is in CTA info.z / 2 (its last piece where info.z is odd), the others are the first ones of CTAs c .. info.w. Four threads per two dimensions.
+template <int D>
+__global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const int4* info, int heads, int is_f16, void* out) {
+    constexpr int GROUPS = 4;
+    __shared__ float a_s[GROUPS][D], l_s[GROUPS], m_s[GROUPS];
     pdl_wait_and_release();
-    const size_t head = blockIdx.x;
-    const float* src = part + head * splits * (D + 2);
-    const int lane = static_cast<int>(threadIdx.x) & 31;
-    if (threadIdx.x < 32) {
-        float m = -CUDART_INF_F;
-        for (int s = lane; s < splits; s += 32) m = fmaxf(m, src[s * (D + 2) + D]);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float mu = m == -CUDART_INF_F ? 0.f : m;
-        float l = 0.f;
-        for (int s = lane; s < splits; s += 32) {
-            const float f = exp2f(src[s * (D + 2) + D] - mu);
-            f_s[s] = f;
-            l += f * src[s * (D + 2) + D + 1];
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) l_s = l;
+    const int4 x = info[blockIdx.x];
+    const int h = static_cast<int>(blockIdx.y);
+    if (x.x < 0 || h >= x.y) return;
+    const int group = static_cast<int>(threadIdx.x) / (D / 2), d = static_cast<int>(threadIdx.x) % (D / 2) * 2;
+    const int first = static_cast<int>(blockIdx.x) - 1, count = x.w - first + 1;
+    auto at = [&](int i) { return part + (static_cast<size_t>(i == 0 ? x.z : 2 * (first + i)) * heads + h) * (D + 2); };
+    float m = -CUDART_INF_F, l = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll 4
+    for (int i = group; i < count; i += GROUPS) {
+        const float* src = at(i);
+        const float mi = src[D], li = src[D + 1];
+        const float2 v = *reinterpret_cast<const float2*>(src + d);
+        const float m_new = fmaxf(m, mi), mu = m_new == -CUDART_INF_F ? 0.f : m_new;
+        const float fa = exp2f(m - mu), fb = exp2f(mi - mu);
+        l = l * fa + li * fb;
+        a0 = a0 * fa + v.x * fb;
+        a1 = a1 * fa + v.y * fb;
+        m = m_new;
+    }
+    a_s[group][d] = a0;
+    a_s[group][d + 1] = a1;
+    if (d == 0) {
+        l_s[group] = l;
+        m_s[group] = m;
     }
     __syncthreads();
-    const float l = l_s;
-    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    const int d = static_cast<int>(threadIdx.x) * 2;
-    if (d >= D) return;
-    float a0 = 0.f, a1 = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) {
-        const float2 v = *reinterpret_cast<const float2*>(src + s * (D + 2) + d);
-        a0 += v.x * f_s[s];
-        a1 += v.y * f_s[s];
+    if (group != 0) return;
+    m = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, m_s[i]);
+    const float mu = m == -CUDART_INF_F ? 0.f : m;
+    l = a0 = a1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+        const float f = exp2f(m_s[i] - mu);
+        l += l_s[i] * f;
+        a0 += a_s[i][d] * f;
+        a1 += a_s[i][d + 1] * f;
     }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint32_t w = is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
-    *reinterpret_cast<uint32_t*>(static_cast<char*>(out) + (head * D + d) * 2) = w;
+    *reinterpret_cast<uint32_t*>(static_cast<char*>(out) + ((static_cast<size_t>(x.x) + h) * D + d) * 2) = w;
 }
 
 template <int BITS, int D, int NH, bool PAGED>
 int launch(const Params& p, int grid, cudaStream_t stream) {
-    const int cluster = p.splits > 1 && p.splits <= MAX_CLUSTER ? p.splits : 1;
-    // slices: a part's share of 8 NH heads, rounded up to 4 floats
+    const int cluster = p.shares == 0 ? p.splits : 1;
     using S = Shape<BITS, D>;
-    const int smem = 1024 + places_of(S::STAGE, D, NH, PAGED) * S::STAGE + (8 * NH * D + 4 * MAX_CLUSTER) * 4;
+    const int smem = warps_of(D, NH) * stages_of(S::STAGE, D, NH) * S::STAGE + behind_rings(D, NH);
     const auto fn = decode_kernel<BITS, D, NH, PAGED>;
     TDIST_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(32 * warps_of(D, NH));
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -859,7 +1003,7 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     if (c.Hkv < 1 || a->Hq < 1 || a->Hq % c.Hkv || c.page_size < 1 || c.B < 0 || c.blocks < 0 || c.max_blocks < 0)
         return fail(TDIST_EINVAL, "quantised decode: bad shape");
     if (c.dtype != TDIST_BF16 && c.dtype != TDIST_F16) return fail(TDIST_EINVAL, "quantised decode: q must be bf16 or fp16");
-    if (a->splits < 1 || a->splits > TDIST_QUANT_DECODE_SPLITS || (a->splits > MAX_CLUSTER && a->part == nullptr))
+    if (a->splits < 0 || a->splits > MAX_CLUSTER || (a->splits == 0 && (a->part == nullptr || a->shares < 1 || c.B > MAX_SHARED)))
         return fail(TDIST_EINVAL, "quantised decode: parts");
     if (a->window < 1 || a->sinks < 0 || !(a->soft_cap >= 0.f)) return fail(TDIST_EINVAL, "quantised decode: window, sinks or soft cap");
     const uintptr_t code_align = reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.v_codes) |
@@ -898,14 +1042,18 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     const int nh = G > 8 && c.head_dim != 256 ? 2 : 1;
     p.head_tiles = (G + 8 * nh - 1) / (8 * nh);
     p.page_size = c.page_size;
-    // with 2^l >= page_size the multiplier ceil(2^(31 + l) / page_size) is off by less than one, so t < 2^31 times it by less than 2^31 <= 2^(31 + l) / page_size
     int l = 0;
     while ((1ll << l) < c.page_size) ++l;
-    p.page_shift = 31 + l;
+    const bool paged = c.page_size == 1 << l && l >= 4 && ((c.code_block | c.code_token | c.scale_block | c.scale_token) >> 32) == 0;
+    // PAGED: t >> l. Otherwise, with 2^l >= page_size, the multiplier ceil(2^(31 + l) / page_size) is off by less than one, so its product with
+    // t < 2^31 by less than 2^31, and the quotient's fraction is at most 1 - 1 / page_size
+    p.page_shift = paged ? l : 31 + l;
     p.page_mul = static_cast<uint32_t>(((1ull << (31 + l)) + static_cast<uint64_t>(c.page_size) - 1) / static_cast<uint64_t>(c.page_size));
     p.max_blocks = c.max_blocks;
     p.blocks = c.blocks;
-    p.splits = a->splits;
+    p.splits = a->splits > 0 ? a->splits : 1;
+    p.shares = a->splits > 0 ? 0 : a->shares;
+    p.B = c.B;
     p.window = a->window;
     p.sinks = a->sinks;
     const long long keys = static_cast<long long>(c.max_blocks) * c.page_size;
@@ -913,36 +1061,27 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.is_f16 = c.dtype == TDIST_F16;
     p.scale = a->scale;
     p.soft_cap = a->soft_cap;
-    const long long grid = static_cast<long long>(c.B) * c.Hkv * p.head_tiles * a->splits;
+    const long long segments = static_cast<long long>(c.B) * c.Hkv * p.head_tiles, grid = p.shares > 0 ? p.shares : segments * p.splits;
     if (grid > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many sequences");
-    p.wctx.status = static_cast<Status*>(a->status);
-    p.wctx.timeout_ns = a->timeout_ns;
-    p.wctx.kernel_id = kKernelQuantDecode;
-    // pages of whole tiles whose rows' scales lie side by side are loaded by TMA
-    const int groups = c.bits == 8 ? 1 : c.head_dim / 64, row_bytes = c.head_dim * c.bits / 8;
-    const bool paged = c.page_size % TOK == 0 && c.scale_token == 4 * groups &&
-                       ((reinterpret_cast<uintptr_t>(c.k_scales) | reinterpret_cast<uintptr_t>(c.v_scales) | static_cast<uintptr_t>(c.scale_block | c.scale_head)) & 15) == 0;
-    if (paged) {
-        const uint32_t box_bytes = static_cast<uint32_t>(row_bytes < 128 ? row_bytes : 128);
-        const tdist_host::Swizzle sw = box_bytes == 128 ? tdist_host::Swizzle::B128 : (box_bytes == 64 ? tdist_host::Swizzle::B64 : tdist_host::Swizzle::B32);
-        const uint64_t dims[4] = {static_cast<uint64_t>(row_bytes), static_cast<uint64_t>(c.Hkv), static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(c.blocks)};
-        const uint64_t strides[3] = {static_cast<uint64_t>(c.code_head), static_cast<uint64_t>(c.code_token), static_cast<uint64_t>(c.code_block)};
-        const uint32_t box[4] = {box_bytes, 1, TOK, 1};
-        const uint64_t sdims[3] = {static_cast<uint64_t>(c.page_size) * groups, static_cast<uint64_t>(c.Hkv), static_cast<uint64_t>(c.blocks)};
-        const uint64_t sstrides[2] = {static_cast<uint64_t>(c.scale_head), static_cast<uint64_t>(c.scale_block)};
-        const uint32_t sbox[3] = {static_cast<uint32_t>(TOK * groups), 1, 1};
-        int rc;
-        if ((rc = tdist_host::encode_tmap(&p.tm_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 4, c.k_codes, dims, strides, box, sw))) return rc;
-        if ((rc = tdist_host::encode_tmap(&p.tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 4, c.v_codes, dims, strides, box, sw))) return rc;
-        if ((rc = tdist_host::encode_tmap(&p.tm_ks, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, 3, c.k_scales, sdims, sstrides, sbox, tdist_host::Swizzle::None))) return rc;
-        if ((rc = tdist_host::encode_tmap(&p.tm_vs, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, 3, c.v_scales, sdims, sstrides, sbox, tdist_host::Swizzle::None))) return rc;
+    if (p.shares > 0) {
+        // (tiles are counted in 32 bits)
+        if (segments * ((p.table_keys + TOK - 1) / TOK + 2) > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many keys to deal out in shares");
+        p.info = reinterpret_cast<int4*>(p.part);
+        p.part += 4ll * p.shares;
     }
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
     const int rc = c.bits == 8 ? launch_dim<8>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream)
                                : launch_dim<4>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream);
     if (rc) return rc;
-    if (a->splits > MAX_CLUSTER)
-        TDIST_CUDA_OK(tdist_host::launch_pdl(merge_kernel, dim3(static_cast<unsigned>(c.B * a->Hq)), 128, 0, stream, p.part, a->splits, c.head_dim,
-                                             p.is_f16, a->out));
+    if (p.shares > 0) {
+        const dim3 blocks(static_cast<unsigned>(p.shares), static_cast<unsigned>(8 * nh));
+        const float* part = p.part;
+        const int4* info = p.info;
+        cudaError_t e;
+        if (c.head_dim == 64) e = tdist_host::launch_pdl(merge_kernel<64>, blocks, 128, 0, stream, part, info, 8 * nh, p.is_f16, a->out);
+        else if (c.head_dim == 128) e = tdist_host::launch_pdl(merge_kernel<128>, blocks, 256, 0, stream, part, info, 8 * nh, p.is_f16, a->out);
+        else e = tdist_host::launch_pdl(merge_kernel<256>, blocks, 512, 0, stream, part, info, 8 * nh, p.is_f16, a->out);
+        TDIST_CUDA_OK(e);
+    }
     return 0;
 }

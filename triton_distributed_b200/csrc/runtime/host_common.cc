@@ -63,7 +63,7 @@ int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int
     std::memset(&key, 0, sizeof(key));
     key.words[0] = reinterpret_cast<uint64_t>(base);
     key.words[1] = (static_cast<uint64_t>(dtype) << 32) | (static_cast<uint64_t>(rank_) << 8) |
-                   static_cast<uint64_t>(sw);
+                   static_cast<uint64_t>(sw == Swizzle::B128);
     for (int i = 0; i < rank_; ++i) {
         key.words[2 + i] = dims[i];
         key.words[9 + i] = box[i];
@@ -94,9 +94,7 @@ int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, int
     for (int i = 0; i + 1 < rank_; ++i) gstrides[i] = strides_bytes[i];
     CUresult r = encode(out, dtype, static_cast<cuuint32_t>(rank_), const_cast<void*>(base), gdims, gstrides,
                         gbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        sw == Swizzle::B128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                        : sw == Swizzle::B64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                        : sw == Swizzle::B32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        sw == Swizzle::B128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(TDIST_EINVAL, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(static_cast<int>(r)));

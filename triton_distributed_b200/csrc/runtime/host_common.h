@@ -23,7 +23,7 @@ int fail(int code, const std::string& msg);
 // Returns nullptr (and records an error) if the driver does not export `name`.
 void* driver_fn(const char* name);
 
-enum class Swizzle { None, B128, B64, B32 };
+enum class Swizzle { None, B128 };
 
 // Encodes (or fetches from the cache; `keep` false: neither looks there nor leaves it there) a tiled tensor map of rank 2 to 4. dims/box
 // are in elements, innermost first; strides_bytes[i] is the byte stride of dimension i+1.

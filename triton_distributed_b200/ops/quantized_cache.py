@@ -33,7 +33,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import _lib
-from ..runtime import default_timeout_ns, stream_ptr
+from ..runtime import stream_ptr
 from ..utils.profile import nvtx_range
 from . import flash_decode as FD
 from . import paged_attention as PA
@@ -334,10 +334,20 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
     return k, v
 
 
-def _decode_splits(B: int, Hkv: int, head_tiles: int, most: int, sms: int, per_sm: int) -> int:
-    """Parts of a sequence's keys: one wave of CTAs, at least 256 keys each; above 8 (a cluster) a second kernel merges."""
-    want = max(1, per_sm * sms // max(1, B * Hkv * head_tiles))
-    return max(1, min(want, -(-most // 256), 512))
+MOST_SHARED = 511   # sequences of a call whose keys are dealt out in shares
+
+
+def _decode_parts(B: int, Hkv: int, head_tiles: int, most: int, table_keys: int, asked: int, sms: int, per_sm: int):
+    """(splits, shares) of a decode over at most ``most`` keys per sequence: CTAs per (sequence, kv head, tile of heads), or 0 and the CTAs
+    that take equal shares of all of them."""
+    segments, slots = B * Hkv * head_tiles, per_sm * sms
+    may_share = B <= MOST_SHARED and segments * (-(-table_keys // 16) + 2) < 1 << 31
+    if asked > 0:
+        return (asked, 0) if asked <= 8 else ((0, min(slots, segments * asked)) if may_share else (8, 0))
+    splits = max(1, min(slots // max(1, segments), -(-most // 256)))
+    if may_share and (splits > 8 or segments * most > slots * 1024):
+        return 0, slots
+    return min(splits, 8), 0
 
 
 @nvtx_range("tdist.gqa_fwd_quantized_decode")
@@ -346,7 +356,8 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
                              out: Optional[torch.Tensor] = None, kv_split: int = -1) -> torch.Tensor:
     """Decode attention of one query token per sequence over a quantised cache: the query of a sequence of n keys sees key j if
     j >= n - window or j < sinks (``window=None``: all keys). ``q [B, Hq, D]`` bf16 or fp16, contiguous; returns its shape and type. A
-    query that sees no key (or none whose score is above -inf) gives zeros. Pages without a visible key are not read."""
+    query that sees no key (or none whose score is above -inf) gives zeros. Pages without a visible key are not read. ``kv_split``: parts of a
+    sequence's keys, up to 8; more: equal shares of all sequences' keys, as many as fit the machine; -1: chosen by sizes."""
     window, sinks, scale, soft_cap = PA._settings(window, sinks, scale, soft_cap)
     key = (gqa_fwd_quantized_decode, PA._layout(q, *cache, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
     args = _PLANS.get(key)
@@ -372,8 +383,6 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
             raise TypeError("q must be bf16 or fp16")
         if not q.is_contiguous():
             raise ValueError("q must be contiguous")
-        if kv_split > 512:
-            raise ValueError("kv_split must be at most 512")
         args = _lib.QuantDecodeArgs()
         args.cache = _cache_args(cache, q.dtype)
         args.cache.B, args.cache.max_blocks = B, block_table.shape[1]
@@ -381,8 +390,8 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
         args.scale, args.soft_cap = factor, soft_cap
         wide = Hq // Hkv > 8 and D != 256
         most = min(cache.k.shape[1] * block_table.shape[1], args.window + sinks)
-        args.splits = kv_split if kv_split > 0 else _decode_splits(B, Hkv, -(-(Hq // Hkv) // (16 if wide else 8)), most, FD._sm_count(q.device),
-                                                                   1 if wide or D == 256 else 2)
+        args.splits, args.shares = _decode_parts(B, Hkv, -(-(Hq // Hkv) // (16 if wide else 8)), most, cache.k.shape[1] * block_table.shape[1],
+                                                 kv_split, FD._sm_count(q.device), 1 if wide or D == 256 else 2)
         _remember(key, args)
     out = PA._output(out, q)
     if args.cache.B == 0:
@@ -394,9 +403,8 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
     if q.data_ptr() % 16:
         q = q.clone()
     a.q, a.out = q.data_ptr(), out.data_ptr()
-    a.status, a.timeout_ns = PA._status_ptr(), default_timeout_ns()
-    if a.splits > 8:
-        part = torch.empty(a.cache.B * a.Hq * a.splits * (a.cache.head_dim + 2), dtype=torch.float32, device=q.device)
+    if a.splits == 0:
+        part = torch.empty(a.shares * (4 + 32 * (a.cache.head_dim + 2)), dtype=torch.float32, device=q.device)
         a.part = part.data_ptr()
     _launch(_lib.lib().tdist_quant_decode, a, q.device, "tdist_quant_decode")
     return out
