@@ -229,6 +229,7 @@ class QuantDecodeArgs(C.Structure):
         ("q", C.c_void_p), ("out", C.c_void_p), ("part", C.c_void_p),
         ("Hq", C.c_int), ("splits", C.c_int), ("shares", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
         ("scale", C.c_float), ("soft_cap", C.c_float),
+        ("scratch", C.c_longlong),
     ]
 
 

@@ -492,11 +492,12 @@ typedef struct TdistQuantDecodeArgs {
     TdistQuantCacheArgs cache;
     const void* q;               /* [B, Hq, D] */
     void* out;                   /* [B, Hq, D] */
-    void* part;                  /* splits 0: fp32 [shares][4 + 2 x 16 x (D + 2)], on 16 bytes */
+    void* part;                  /* splits 0: fp32 [CTAs][4 + 2 x heads x (D + 2)], on 16 bytes; CTAs: shares x Hkv x tiles of heads (8, or 16 where Hq / Hkv > 8 and D < 256) */
     int Hq;
-    int splits;                  /* CTAs per (sequence, kv head), up to 8; 0: `shares` CTAs take equal shares of all keys (up to 511 sequences) */
+    int splits;                  /* CTAs per (sequence, kv head), up to 8; 0: `shares` CTAs of each kv head take equal shares of all keys (up to 511 sequences) */
     int shares, window, sinks;
     float scale, soft_cap;
+    long long scratch;           /* floats of `part` */
 } TdistQuantDecodeArgs;
 
 int tdist_quant_cache_write(const TdistQuantCacheArgs* args);

@@ -25,10 +25,12 @@
 // way, warps waited for memory half of their time.
 //
 // Work. A segment is the keys of one (sequence, kv head, tile of query heads), cut into tiles of 16 tokens. Either a segment has `splits` CTAs, up to 8, a
-// cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); or the machine is filled once and every CTA takes an equal
-// share of all segments' tiles in a row, from the lengths on the device: pieces of segments, of which the first and the last may be shared with other
-// CTAs. Those leave their sums in a workspace, and a second kernel adds them up. The copies run on from one piece to the next: while a piece's sums meet, the next one's
-// first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
+// cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); or the machine is filled once by groups of CTAs, one
+// for each segment of a sequence, and every group takes an equal share of all sequences' tiles in a row, from the lengths on the device: pieces
+// of sequences, of which the first and the last may be shared with other groups. Those leave their sums in a workspace, and a second kernel
+// adds them up. (The heads of a key lie side by side in memory, so they are read side by side: with shares dealt out head by head 4-bit rows of 64 bytes were
+// read from HBM twice, and 16 x 16384 keys took 107 us in 8 bits.) The copies run on from one piece to the next: while a piece's sums meet,
+// the next one's first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -61,7 +63,7 @@ struct Params {
     int4* info;                    // shares: [CTAs]: the segment that this CTA's first piece goes on with (see merge_kernel)
     void* out;
     long long code_block, code_token, code_head, scale_block, scale_head, scale_token;   // bytes
-    int B, shares;                 // shares: CTAs that share all tiles equally, 0: `splits` CTAs per segment
+    int B, shares;                 // shares: groups of CTAs that share all tiles equally, 0: `splits` CTAs per segment
     int Hq, Hkv, head_tiles, page_size, page_shift, max_blocks, blocks, splits, window, sinks, table_keys, is_f16;
     float scale, soft_cap;
     uint32_t page_mul;             // not PAGED: t / page_size = (t page_mul) >> page_shift for t < 2^31
@@ -228,34 +230,27 @@ __device__ __forceinline__ Keys keys_of(const Params& p, int length) {
     return k;
 }
 
-// Tiles i0 .. i1 - 1 of segment (b, of_b)
+// Tiles i0 .. i1 - 1 of sequence b
 struct Piece {
-    int b, of_b, i0, i1;
+    int b, i0, i1;
 };
 // The pieces of this CTA, one after the other
 struct Pieces {
-    const uint32_t* prefix;   // shares: tiles of a kv head of the sequences before b; nullptr: one piece
-    uint32_t at, end;         // shares: tiles of this CTA
-    int per_b;                // segments of a sequence
-    int b, i0, i1;            // one piece: its segment is `b`
+    const uint32_t* prefix;   // shares: tiles of the sequences before b; nullptr: one piece
+    uint32_t at, end;         // tiles of this CTA; one piece: whether it is still to come
+    int b, i0, i1;
 
     __device__ __forceinline__ bool next(Piece& x) {
+        if (at >= end) return false;
         if (prefix == nullptr) {
-            if (per_b == 0) return false;
-            x.b = b / per_b;
-            x.of_b = b - x.b * per_b;
-            x.i0 = i0;
-            x.i1 = i1;
-            per_b = 0;
+            x = Piece{b, i0, i1};
+            at = end;
             return true;
         }
-        if (at >= end) return false;
-        while (prefix[b + 1] * per_b <= at) ++b;
-        const uint32_t tiles = prefix[b + 1] - prefix[b], rest = at - prefix[b] * per_b;
+        while (prefix[b + 1] <= at) ++b;
         x.b = b;
-        x.of_b = static_cast<int>(rest / tiles);
-        x.i0 = static_cast<int>(rest - x.of_b * tiles);
-        const uint32_t take = min(tiles - x.i0, end - at);
+        x.i0 = static_cast<int>(at - prefix[b]);
+        const uint32_t take = min(prefix[b + 1] - at, end - at);
         x.i1 = x.i0 + static_cast<int>(take);
         at += take;
         return true;
@@ -288,9 +283,12 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     const int split = in_cluster ? static_cast<int>(blockIdx.x) % p.splits : 0;
     Pieces pieces;
     pieces.prefix = nullptr;
-    pieces.per_b = p.Hkv * p.head_tiles;
-    pieces.b = 0;
-    uint32_t total_tiles = 0, ctas = 0, from = 0;           // shares: all tiles, the CTAs that have some, this CTA's first
+    const int per_b = p.Hkv * p.head_tiles;                 // segments of a sequence
+    const int group = static_cast<int>(blockIdx.x) / (p.shares > 0 ? per_b : p.splits);   // shares: this CTA's group; otherwise its segment
+    const int of_b = p.shares > 0 ? static_cast<int>(blockIdx.x) % per_b : group % per_b;
+    const int kvh = of_b / p.head_tiles, tile_of_heads = of_b % p.head_tiles;
+    const int heads = min(HEADS, G - tile_of_heads * HEADS);
+    const int head_of_b = kvh * G + tile_of_heads * HEADS;
     if (p.shares > 0) {
         uint32_t* prefix = reinterpret_cast<uint32_t*>(last_s);
         int* lens = reinterpret_cast<int*>(last_s) + MAX_SHARED + 1;
@@ -319,50 +317,45 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
         }
         if (threadIdx.x == 0) prefix[0] = 0;
         __syncthreads();
-        total_tiles = carry * pieces.per_b;
-        ctas = min(static_cast<uint32_t>(p.shares), total_tiles);
-        const uint32_t cta = blockIdx.x;
-        if (cta < ctas) {
-            from = static_cast<uint32_t>(static_cast<uint64_t>(cta) * total_tiles / ctas);
-            pieces.at = from;
-            pieces.end = static_cast<uint32_t>(static_cast<uint64_t>(cta + 1) * total_tiles / ctas);
+        const uint32_t total = carry, groups = min(static_cast<uint32_t>(p.shares), total);   // all tiles, the groups that have some
+        auto first_of = [&](uint32_t of) { return static_cast<uint32_t>(static_cast<uint64_t>(of) * total / groups); };
+        auto group_of = [&](uint32_t tile) { return static_cast<uint32_t>(((static_cast<uint64_t>(tile) + 1) * groups - 1) / total); };
+        const uint32_t mine = static_cast<uint32_t>(group);
+        pieces.b = 0;
+        pieces.at = pieces.end = 0;
+        if (mine < groups) {
+            pieces.at = first_of(mine);
+            pieces.end = first_of(mine + 1);
             int lo = 0, hi = p.B;   // the sequence of the first tile: the last one that starts at it or before (those without tiles start where the next does)
             while (hi - lo > 1) {
                 const int m = (lo + hi) >> 1;
-                if (prefix[m] * pieces.per_b <= from) lo = m;
+                if (prefix[m] <= pieces.at) lo = m;
                 else hi = m;
             }
             pieces.b = lo;
-        } else {
-            pieces.at = pieces.end = 0;
         }
         pieces.prefix = prefix;
         if (threadIdx.x == 0) {
-            // for the second kernel: head 0 and heads of the segment that goes on here, and the CTAs that have some of it
+            // for the second kernel: head 0 and heads of the segment that goes on here, where its first sums are, the last CTA that has some
             int4 info = make_int4(-1, 0, 0, 0);
-            Pieces first = pieces;
-            Piece x;
-            if (cta < ctas && first.next(x) && x.i0 > 0) {
-                const uint32_t start = from - x.i0, stop = start + (prefix[x.b + 1] - prefix[x.b]);
-                const uint32_t c0 = static_cast<uint32_t>(((static_cast<uint64_t>(start) + 1) * ctas - 1) / total_tiles);
-                const uint32_t c1 = static_cast<uint32_t>((static_cast<uint64_t>(stop) * ctas - 1) / total_tiles);
-                if (cta == c0 + 1) {
-                    const int kvh = x.of_b / p.head_tiles, tile_of_heads = x.of_b % p.head_tiles;
-                    const bool whole = static_cast<uint32_t>(static_cast<uint64_t>(c0) * total_tiles / ctas) == start;   // c0's first piece, not its last
-                    info = make_int4(x.b * p.Hq + kvh * G + tile_of_heads * HEADS, min(HEADS, G - tile_of_heads * HEADS), static_cast<int>(2 * c0 + (whole ? 0 : 1)), static_cast<int>(c1));
-                }
+            if (mine < groups && pieces.at > prefix[pieces.b]) {
+                const uint32_t start = prefix[pieces.b], g0 = group_of(start), g1 = group_of(prefix[pieces.b + 1] - 1);
+                if (mine == g0 + 1)   // (the sequence is that group's first piece or its last)
+                    info = make_int4(pieces.b * p.Hq + head_of_b, heads, static_cast<int>(2 * (g0 * per_b + of_b) + (first_of(g0) == start ? 0 : 1)), static_cast<int>(g1 * per_b + of_b));
             }
-            p.info[cta] = info;
+            p.info[blockIdx.x] = info;
         }
         // sequences without keys
-        for (int b = static_cast<int>(cta); b < p.B; b += p.shares)
+        for (int b = static_cast<int>(blockIdx.x); b < p.B; b += static_cast<int>(gridDim.x))
             if (prefix[b + 1] == prefix[b])
                 for (int i = static_cast<int>(threadIdx.x); i < p.Hq * D / 2; i += THREADS) static_cast<uint32_t*>(p.out)[static_cast<size_t>(b) * (p.Hq * D / 2) + i] = 0u;
     } else {
-        pieces.b = static_cast<int>(blockIdx.x) / p.splits;
-        const int tiles = keys_of(p, p.lens[pieces.b / pieces.per_b]).tiles, per = (tiles + p.splits - 1) / p.splits;
+        pieces.b = group / per_b;
+        const int tiles = keys_of(p, p.lens[pieces.b]).tiles, per = (tiles + p.splits - 1) / p.splits;
         pieces.i0 = min(split * per, tiles);
         pieces.i1 = min((split + 1) * per, tiles);
+        pieces.at = 0;
+        pieces.end = 1;
     }
     auto keys_in = [&](int b) { return keys_of(p, p.shares > 0 ? reinterpret_cast<const int*>(last_s)[MAX_SHARED + 1 + b] : p.lens[b]); };
 
@@ -382,8 +375,10 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     Pieces coming = pieces;
     Keys c_keys;
     const int* c_table = nullptr;
-    const uint8_t *c_k = nullptr, *c_v = nullptr;
-    const char* c_s = nullptr;               // lanes 0..15 copy the scales of the keys, 16..31 of the values
+    const uint8_t* c_k = p.k + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
+    const uint8_t* c_v = p.v + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
+    // lanes 0..15 copy the scales of the keys, 16..31 of the values
+    const char* c_s = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head + (PAGED ? my_token * p.scale_token : 0);
     int c_i = 0, c_end = 0, c_turn = 0, c_page = -1;
     c_keys.n = c_keys.lo = c_keys.first = c_keys.sink_tiles = c_keys.t_lo = 0;
     bool c_more = true;
@@ -395,11 +390,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
             c_more = coming.next(x);
             if (!c_more) break;
             c_keys = keys_in(x.b);
-            const int kvh = x.of_b / p.head_tiles;
             c_table = p.table + static_cast<size_t>(x.b) * p.max_blocks;
-            c_k = p.k + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
-            c_v = p.v + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
-            c_s = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head + (PAGED ? my_token * p.scale_token : 0);
             c_i = x.i0 + (warp + WARPS - c_turn) % WARPS;
             c_end = x.i1;
             c_turn = (c_turn + x.i1 - x.i0) % WARPS;
@@ -461,9 +452,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     Piece x;
     while (pieces.next(x)) {
     const Keys keys = keys_in(x.b);
-    const int kvh = x.of_b / p.head_tiles, tile_of_heads = x.of_b % p.head_tiles;
-    const int heads = min(HEADS, G - tile_of_heads * HEADS);
-    const size_t head0 = static_cast<size_t>(x.b) * p.Hq + kvh * G + tile_of_heads * HEADS;
+    const size_t head0 = static_cast<size_t>(x.b) * p.Hq + head_of_b;
     const int i0 = x.i0 + (warp + WARPS - turn) % WARPS, i1 = x.i1;
 
     // ---- q to 16 bits, a warp per head: the high and the low bytes in the order in which the codes' registers have their dimensions
@@ -899,9 +888,10 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 }
 
 // Shares: the sums of a segment that several CTAs have pieces of. Block (c, h): head h of the segment whose second piece is CTA c's first; its
-// first piece is in CTA info.z / 2 (its last piece where info.z is odd), the others are the first ones of CTAs c .. info.w. Four threads per two dimensions.
+// first piece is in CTA info.z / 2 (its last piece where info.z is odd), the others are the first ones of every per_b-th CTA from c to info.w.
+// Four threads per two dimensions.
 template <int D>
-__global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const int4* info, int heads, int is_f16, void* out) {
+__global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const int4* info, int per_b, int heads, int is_f16, void* out) {
     constexpr int GROUPS = 4;
     __shared__ float a_s[GROUPS][D], l_s[GROUPS], m_s[GROUPS];
     pdl_wait_and_release();
@@ -909,8 +899,8 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const i
     const int h = static_cast<int>(blockIdx.y);
     if (x.x < 0 || h >= x.y) return;
     const int group = static_cast<int>(threadIdx.x) / (D / 2), d = static_cast<int>(threadIdx.x) % (D / 2) * 2;
-    const int first = static_cast<int>(blockIdx.x) - 1, count = x.w - first + 1;
-    auto at = [&](int i) { return part + (static_cast<size_t>(i == 0 ? x.z : 2 * (first + i)) * heads + h) * (D + 2); };
+    const int c = static_cast<int>(blockIdx.x), count = (x.w - c) / per_b + 2;
+    auto at = [&](int i) { return part + (static_cast<size_t>(i == 0 ? x.z : 2 * (c + (i - 1) * per_b)) * heads + h) * (D + 2); };
     float m = -CUDART_INF_F, l = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll 4
     for (int i = group; i < count; i += GROUPS) {
@@ -1061,26 +1051,28 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.is_f16 = c.dtype == TDIST_F16;
     p.scale = a->scale;
     p.soft_cap = a->soft_cap;
-    const long long segments = static_cast<long long>(c.B) * c.Hkv * p.head_tiles, grid = p.shares > 0 ? p.shares : segments * p.splits;
+    const long long segments = static_cast<long long>(c.B) * c.Hkv * p.head_tiles, grid = p.shares > 0 ? static_cast<long long>(p.shares) * c.Hkv * p.head_tiles : segments * p.splits;
     if (grid > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many sequences");
     if (p.shares > 0) {
         // (tiles are counted in 32 bits)
-        if (segments * ((p.table_keys + TOK - 1) / TOK + 2) > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many keys to deal out in shares");
+        if (c.B * static_cast<long long>((p.table_keys + TOK - 1) / TOK + 2) > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many keys to deal out in shares");
+        if (a->scratch < grid * (4 + 2ll * 8 * nh * (c.head_dim + 2))) return fail(TDIST_EINVAL, "quantised decode: too little scratch");
         p.info = reinterpret_cast<int4*>(p.part);
-        p.part += 4ll * p.shares;
+        p.part += 4 * grid;
     }
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
     const int rc = c.bits == 8 ? launch_dim<8>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream)
                                : launch_dim<4>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream);
     if (rc) return rc;
     if (p.shares > 0) {
-        const dim3 blocks(static_cast<unsigned>(p.shares), static_cast<unsigned>(8 * nh));
+        const dim3 blocks(static_cast<unsigned>(grid), static_cast<unsigned>(8 * nh));
+        const int per_b = c.Hkv * p.head_tiles;
         const float* part = p.part;
         const int4* info = p.info;
         cudaError_t e;
-        if (c.head_dim == 64) e = tdist_host::launch_pdl(merge_kernel<64>, blocks, 128, 0, stream, part, info, 8 * nh, p.is_f16, a->out);
-        else if (c.head_dim == 128) e = tdist_host::launch_pdl(merge_kernel<128>, blocks, 256, 0, stream, part, info, 8 * nh, p.is_f16, a->out);
-        else e = tdist_host::launch_pdl(merge_kernel<256>, blocks, 512, 0, stream, part, info, 8 * nh, p.is_f16, a->out);
+        if (c.head_dim == 64) e = tdist_host::launch_pdl(merge_kernel<64>, blocks, 128, 0, stream, part, info, per_b, 8 * nh, p.is_f16, a->out);
+        else if (c.head_dim == 128) e = tdist_host::launch_pdl(merge_kernel<128>, blocks, 256, 0, stream, part, info, per_b, 8 * nh, p.is_f16, a->out);
+        else e = tdist_host::launch_pdl(merge_kernel<256>, blocks, 512, 0, stream, part, info, per_b, 8 * nh, p.is_f16, a->out);
         TDIST_CUDA_OK(e);
     }
     return 0;

@@ -337,16 +337,15 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
 MOST_SHARED = 511   # sequences of a call whose keys are dealt out in shares
 
 
-def _decode_parts(B: int, Hkv: int, head_tiles: int, most: int, table_keys: int, asked: int, sms: int, per_sm: int):
-    """(splits, shares) of a decode over at most ``most`` keys per sequence: CTAs per (sequence, kv head, tile of heads), or 0 and the CTAs
-    that take equal shares of all of them."""
-    segments, slots = B * Hkv * head_tiles, per_sm * sms
-    may_share = B <= MOST_SHARED and segments * (-(-table_keys // 16) + 2) < 1 << 31
+def _decode_parts(B: int, per_b: int, most: int, table_keys: int, asked: int, slots: int):
+    """(splits, shares) of a decode over at most ``most`` keys per sequence, ``per_b`` CTAs side by side for a sequence's heads: CTAs per
+    sequence and head, or 0 and the CTAs that take equal shares of all sequences."""
+    may_share = B <= MOST_SHARED and B * (-(-table_keys // 16) + 2) < 1 << 31
     if asked > 0:
-        return (asked, 0) if asked <= 8 else ((0, min(slots, segments * asked)) if may_share else (8, 0))
-    splits = max(1, min(slots // max(1, segments), -(-most // 256)))
-    if may_share and (splits > 8 or segments * most > slots * 1024):
-        return 0, slots
+        return (asked, 0) if asked <= 8 else ((0, max(1, min(slots // per_b, B * asked))) if may_share else (8, 0))
+    splits = max(1, min(slots // max(1, B * per_b), -(-most // 256)))
+    if may_share and (splits > 8 or B * per_b * most > slots * 1024):
+        return 0, max(1, slots // per_b)
     return min(splits, 8), 0
 
 
@@ -390,8 +389,11 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
         args.scale, args.soft_cap = factor, soft_cap
         wide = Hq // Hkv > 8 and D != 256
         most = min(cache.k.shape[1] * block_table.shape[1], args.window + sinks)
-        args.splits, args.shares = _decode_parts(B, Hkv, -(-(Hq // Hkv) // (16 if wide else 8)), most, cache.k.shape[1] * block_table.shape[1],
-                                                 kv_split, FD._sm_count(q.device), 1 if wide or D == 256 else 2)
+        per_b = Hkv * -(-(Hq // Hkv) // (16 if wide else 8))
+        args.splits, args.shares = _decode_parts(B, per_b, most, cache.k.shape[1] * block_table.shape[1], kv_split,
+                                                 (1 if wide or D == 256 else 2) * FD._sm_count(q.device))
+        # scratch of the shares: per CTA four words, and two times the sums of its heads
+        args.scratch = args.shares * per_b * (4 + 2 * (16 if wide else 8) * (D + 2))
         _remember(key, args)
     out = PA._output(out, q)
     if args.cache.B == 0:
@@ -404,7 +406,7 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
         q = q.clone()
     a.q, a.out = q.data_ptr(), out.data_ptr()
     if a.splits == 0:
-        part = torch.empty(a.shares * (4 + 32 * (a.cache.head_dim + 2)), dtype=torch.float32, device=q.device)
+        part = torch.empty(a.scratch, dtype=torch.float32, device=q.device)
         a.part = part.data_ptr()
     _launch(_lib.lib().tdist_quant_decode, a, q.device, "tdist_quant_decode")
     return out
