@@ -379,31 +379,35 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     const uint8_t* c_v = p.v + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
     // lanes 0..15 copy the scales of the keys, 16..31 of the values
     const char* c_s = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head + (PAGED ? my_token * p.scale_token : 0);
-    int c_i = 0, c_end = 0, c_turn = 0, c_page = -1;
+    // the next tile, its first token (not PAGED: this lane's), the end of the run of tiles whose tokens follow one another (the first keys, or the
+    // window), the piece's end, the page
+    int c_i = 0, c_t = 0, c_run = 0, c_end = 0, c_turn = 0, c_page = -1;
     c_keys.n = c_keys.lo = c_keys.first = c_keys.sink_tiles = c_keys.t_lo = 0;
-    bool c_more = true;
-    // to the next tile, and its page's number
     auto advance = [&]() {
         c_i += WARPS;
-        while (c_i >= c_end && c_more) {
-            Piece x;
-            c_more = coming.next(x);
-            if (!c_more) break;
-            c_keys = keys_in(x.b);
-            c_table = p.table + static_cast<size_t>(x.b) * p.max_blocks;
-            c_i = x.i0 + (warp + WARPS - c_turn) % WARPS;
-            c_end = x.i1;
-            c_turn = (c_turn + x.i1 - x.i0) % WARPS;
+        c_t += WARPS * TOK;
+        if (c_i >= c_run) {
+            while (c_i >= c_end) {
+                Piece x;
+                if (!coming.next(x)) {
+                    c_i = c_run = 0;
+                    return;
+                }
+                c_keys = keys_in(x.b);
+                c_table = p.table + static_cast<size_t>(x.b) * p.max_blocks;
+                c_i = x.i0 + (warp + WARPS - c_turn) % WARPS;
+                c_end = x.i1;
+                c_turn = (c_turn + x.i1 - x.i0) % WARPS;
+            }
+            c_run = c_i < c_keys.sink_tiles ? min(c_keys.sink_tiles, c_end) : c_end;
+            c_t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
         }
-        if (c_i < c_end) {
-            const int t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
-            const bool seen = PAGED || (c_i < c_keys.sink_tiles ? t < c_keys.first : t >= c_keys.lo && t < c_keys.n);
-            c_page = seen ? static_cast<int>(ldg32(c_table + in_table(t))) : -1;
-        }
+        const bool seen = PAGED || (c_i < c_keys.sink_tiles ? c_t < c_keys.first : c_t >= c_keys.lo && c_t < c_keys.n);
+        c_page = seen ? static_cast<int>(ldg32(c_table + in_table(c_t))) : -1;
     };
     auto copy_next = [&](uint32_t to) {
-        if (c_i < c_end) {
-            const int t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
+        if (c_i < c_run) {
+            const int t = c_t;
             const bool live = static_cast<unsigned>(c_page) < static_cast<unsigned>(p.blocks);
             const uint32_t from = live ? static_cast<uint32_t>(c_page) : 0u;
             if (PAGED) {
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
         copy_commit();
     };
     advance();
-#pragma unroll
+#pragma unroll 1
     for (int a = 0; a < STAGES - 1; ++a) copy_next(ring + a * S::STAGE);
 
     // what this lane reads of a tile: tokens of rows g and g + 8 of the MMA (keys and scales), of columns 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (values)
@@ -454,6 +458,9 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     const Keys keys = keys_in(x.b);
     const size_t head0 = static_cast<size_t>(x.b) * p.Hq + head_of_b;
     const int i0 = x.i0 + (warp + WARPS - turn) % WARPS, i1 = x.i1;
+    // tiles that are seen whole
+    const int whole0 = keys.sink_tiles - keys.t_lo + (keys.lo + TOK - 1) / TOK;
+    const unsigned whole = static_cast<unsigned>(max(0, keys.sink_tiles - keys.t_lo + keys.n / TOK - whole0));
 
     // ---- q to 16 bits, a warp per head: the high and the low bytes in the order in which the codes' registers have their dimensions
     for (int head = warp; head < HEADS; head += WARPS) {
@@ -593,8 +600,6 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                 for (int e = 0; e < 4; ++e) acc[h][k][e] = acc[h][k][e] * 256 + acc_low[h][k][e];
             }
         // ---- scales, cap; masks at the ends of what is seen
-        const int t0 = keys.first_token(i);
-        const bool sink = i < keys.sink_tiles, edge = sink || t0 < keys.lo || t0 + TOK > keys.n;
         bool higher = false;
 #pragma unroll
         for (int h = 0; h < NH; ++h)
@@ -620,7 +625,9 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
         // ---- the values' scales, as weights in units of `unit`
         float vmul[2][S::NG], vleast[2][S::NG];
         float most = 0.f;
-        if (edge) {
+        if (static_cast<unsigned>(i - whole0) >= whole) {
+            const int t0 = keys.first_token(i);
+            const bool sink = i < keys.sink_tiles;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int t = t0 + t_row + 8 * r;
