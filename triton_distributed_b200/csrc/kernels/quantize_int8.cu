@@ -2,7 +2,9 @@
 // A row with a NaN or an infinity gets a scale of NaN and codes of 0. Quotients and products are IEEE's (compiled without fast math), so the
 // codes are those of the statement in torch.
 //
-// Bound by bytes: a CTA per row holds up to 64 values of it per thread in registers between the two passes; longer rows are read again (L2).
+// Bound by bytes: a row is read once, into the registers of 32 to 256 threads (up to 64 values each; what is longer is read again, from L2), so
+// that every thread has all its loads under way. Few instructions per value: magnitudes are compared as pairs of 16-bit integers (the order
+// of bf16 and fp16 bits is the numbers'), and rounding is the addition of 1.5 2^23, whose low byte is the code.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -14,82 +16,108 @@
 namespace tdist {
 namespace quant8 {
 
-constexpr int THREADS = 256, HELD = 8;       // HELD x 8 values of a thread stay in registers
+constexpr int THREADS = 256, HELD = 8;       // chunks of 8 values that a thread holds
 constexpr float kLeast = 7.888609052210118e-31f;   // 2^-100
 
+// eight values as they lie in memory
 template <int DT>
-__device__ __forceinline__ void load8(const char* row, long long i, float (&f)[8]) {
-    if (DT == TDIST_F32) {
-        const uint4 a = ld_v4(row + i * 32), b = ld_v4(row + i * 32 + 16);
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+struct Chunk {
+    uint32_t w[DT == TDIST_F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const char* p) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
-    } else {
-        const uint4 a = ld_v4(row + i * 16);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (DT == TDIST_F16) {
-                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                f[2 * j] = t.x;
-                f[2 * j + 1] = t.y;
-            } else {
-                f[2 * j] = __uint_as_float(w[j] << 16);
-                f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
+        for (int i = 0; i < (DT == TDIST_F32 ? 2 : 1); ++i) {
+            const uint4 v = ld_v4(p + 16 * i);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
         }
     }
+    __device__ __forceinline__ float get(int i) const {
+        if (DT == TDIST_F32) return __uint_as_float(w[i]);
+        if (DT == TDIST_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+        const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+        return i & 1 ? __high2float(h) : __low2float(h);
+    }
+    // the largest magnitude so far, as bits: of fp32, or of 16 bits in each half
+    __device__ __forceinline__ uint32_t most(uint32_t top) const {
+        if (DT == TDIST_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, w[i] & 0x7fffffffu);
+            return top;
+        }
+        top = __vimax3_u16x2(top, w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
+        return __vimax3_u16x2(top, w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu);
+    }
+    __device__ __forceinline__ uint2 codes(float inv) const {
+        uint32_t b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(get(i), inv), 12582912.f));
+        return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                          __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+    }
+};
+
+// ROW threads hold a row
+template <int DT, int ROW>
+__global__ void __launch_bounds__(THREADS) quantize_kernel(const char* x, long long row_bytes, long long rows, int chunks, int8_t* out, float* scale) {
+    constexpr int SIZE = DT == TDIST_F32 ? 32 : 16;
+    __shared__ uint32_t top_s[THREADS / 32];
+    const int t = static_cast<int>(threadIdx.x) % ROW;
+    const long long r = static_cast<long long>(blockIdx.x) * (THREADS / ROW) + static_cast<int>(threadIdx.x) / ROW;
+    const bool live = r < rows;
+    pdl_wait_and_release();
+    const char* row = x + r * row_bytes;
+    Chunk<DT> c[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        if (live && t + i * ROW < chunks) c[i].load(row + static_cast<long long>(t + i * ROW) * SIZE);
+        else c[i] = Chunk<DT>{};
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) top = c[i].most(top);
+    if (ROW == THREADS)
+        for (int i = t + HELD * ROW; i < chunks; i += ROW) {
+            Chunk<DT> more;
+            more.load(row + static_cast<long long>(i) * SIZE);
+            top = more.most(top);
+        }
+    if (DT != TDIST_F32) top = max(top & 0xffffu, top >> 16);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (ROW > 32) {
+        if ((threadIdx.x & 31) == 0) top_s[threadIdx.x >> 5] = top;
+        __syncthreads();
+        const int first = static_cast<int>(threadIdx.x) / ROW * (ROW / 32);
+#pragma unroll
+        for (int w = 0; w < ROW / 32; ++w) top = max(top, top_s[first + w]);
+    }
+    if (!live) return;
+    const float most = DT == TDIST_F32 ? __uint_as_float(top) : (DT == TDIST_BF16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(top))));
+    const bool good = most < __uint_as_float(0x7f800000u);   // (false for NaN)
+    const float a = good ? fmaxf(most, kLeast) : 1.f;
+    const float inv = __fdiv_rn(127.f, a);
+    if (t == 0) scale[r] = good ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fffffffu);
+    uint2* dst = reinterpret_cast<uint2*>(out + r * chunks * 8);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (t + i * ROW < chunks) dst[t + i * ROW] = good ? c[i].codes(inv) : make_uint2(0u, 0u);
+    if (ROW == THREADS)
+        for (int i = t + HELD * ROW; i < chunks; i += ROW) {
+            Chunk<DT> more;
+            more.load(row + static_cast<long long>(i) * SIZE);
+            dst[i] = good ? more.codes(inv) : make_uint2(0u, 0u);
+        }
 }
 
 template <int DT>
-__global__ void __launch_bounds__(THREADS) quantize_kernel(const char* x, long long row_bytes, int chunks, int8_t* out, float* scale) {
-    __shared__ uint32_t top_s[THREADS / 32];
-    pdl_wait_and_release();
-    const char* row = x + static_cast<long long>(blockIdx.x) * row_bytes;
-    const int t = static_cast<int>(threadIdx.x);
-    float f[HELD][8];
-    uint32_t top = 0;   // bits of the largest magnitude; a NaN's lie above an infinity's
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (t + i * THREADS < chunks) load8<DT>(row, t + i * THREADS, f[i]);
-        else
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < HELD; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[i][j]) & 0x7fffffffu);
-    for (int i = t + HELD * THREADS; i < chunks; i += THREADS) {
-        float g[8];
-        load8<DT>(row, i, g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(g[j]) & 0x7fffffffu);
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((t & 31) == 0) top_s[t >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) top = max(top, top_s[w]);
-    const bool good = top < 0x7f800000u;
-    const float a = fmaxf(good ? __uint_as_float(top) : 1.f, kLeast);
-    const float inv = __fdiv_rn(127.f, a);
-    if (t == 0) scale[blockIdx.x] = good ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fffffffu);
-    int8_t* dst = out + static_cast<long long>(blockIdx.x) * chunks * 8;
-    auto put = [&](int i, const float (&v)[8]) {
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= (static_cast<uint32_t>(good ? __float2int_rn(__fmul_rn(v[j], inv)) : 0) & 255u) << (8 * (j & 3));
-        *reinterpret_cast<uint2*>(dst + static_cast<long long>(i) * 8) = make_uint2(w[0], w[1]);
-    };
-#pragma unroll
-    for (int i = 0; i < HELD; ++i)
-        if (t + i * THREADS < chunks) put(t + i * THREADS, f[i]);
-    for (int i = t + HELD * THREADS; i < chunks; i += THREADS) {
-        float g[8];
-        load8<DT>(row, i, g);
-        put(i, g);
-    }
+cudaError_t launch(const char* x, long long row_bytes, long long rows, int chunks, int8_t* out, float* scale, cudaStream_t s) {
+    const int row = chunks <= 32 * HELD ? 32 : (chunks <= 64 * HELD ? 64 : (chunks <= 128 * HELD ? 128 : 256));
+    const dim3 grid(static_cast<unsigned>((rows * row + THREADS - 1) / THREADS));
+    if (row == 32) return tdist_host::launch_pdl(quantize_kernel<DT, 32>, grid, THREADS, 0, s, x, row_bytes, rows, chunks, out, scale);
+    if (row == 64) return tdist_host::launch_pdl(quantize_kernel<DT, 64>, grid, THREADS, 0, s, x, row_bytes, rows, chunks, out, scale);
+    if (row == 128) return tdist_host::launch_pdl(quantize_kernel<DT, 128>, grid, THREADS, 0, s, x, row_bytes, rows, chunks, out, scale);
+    return tdist_host::launch_pdl(quantize_kernel<DT, 256>, grid, THREADS, 0, s, x, row_bytes, rows, chunks, out, scale);
 }
 
 }  // namespace quant8
@@ -106,15 +134,12 @@ extern "C" int tdist_quant_int8_rowwise(const void* x, long long row_stride, voi
     if ((reinterpret_cast<uintptr_t>(x) & 15) || (row_stride * size) % 16 || (reinterpret_cast<uintptr_t>(out) & 7))
         return fail(TDIST_EINVAL, "int8 quantiser: rows must lie on 16 bytes");
     if (rows == 0) return 0;
-    const dim3 grid(static_cast<unsigned>(rows));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const char* src = static_cast<const char*>(x);
     int8_t* dst = static_cast<int8_t*>(out);
     float* sc = static_cast<float*>(scale);
-    cudaError_t e;
-    if (dtype == TDIST_F32) e = tdist_host::launch_pdl(quantize_kernel<TDIST_F32>, grid, THREADS, 0, s, src, row_stride * size, k / 8, dst, sc);
-    else if (dtype == TDIST_F16) e = tdist_host::launch_pdl(quantize_kernel<TDIST_F16>, grid, THREADS, 0, s, src, row_stride * size, k / 8, dst, sc);
-    else e = tdist_host::launch_pdl(quantize_kernel<TDIST_BF16>, grid, THREADS, 0, s, src, row_stride * size, k / 8, dst, sc);
-    TDIST_CUDA_OK(e);
+    TDIST_CUDA_OK(dtype == TDIST_F32 ? launch<TDIST_F32>(src, row_stride * size, rows, k / 8, dst, sc, s)
+                                     : (dtype == TDIST_F16 ? launch<TDIST_F16>(src, row_stride * size, rows, k / 8, dst, sc, s)
+                                                           : launch<TDIST_BF16>(src, row_stride * size, rows, k / 8, dst, sc, s)));
     return 0;
 }

@@ -8,8 +8,9 @@
 // bf16 rows do not, one of fp32 would make 5 bits of 4.5.
 // Quotients and products are IEEE's (this file is compiled without fast math): the same codes as the statement in torch.
 //
-// Bound by bytes. A lane takes 8 values (16 bytes) of a k row and of the v row beside it when writing, 16 codes of each when reading:
-// two loads of each lane under way at once, and 2048 threads per SM.
+// Bound by bytes. A lane takes 8 values (16 bytes) of a k row and of the v row beside it when writing, 16 codes of each of two places when reading:
+// two and four loads of each lane under way at once. Quotients of places by heads and page sizes go by a multiplication, rounding by
+// the addition of 1.5 2^23, whose low byte is the code.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -39,7 +40,11 @@ struct Params {
     long long code_block, code_token, code_head, scale_block, scale_head, scale_token;   // bytes
     long long rows;        // write: tokens; read: rows of the output
     int B, Hkv, blocks, page_size, max_blocks, is_f16, rows_per_cta;
+    uint32_t head_mul, page_mul;   // n / Hkv = (n head_mul) >> head_shift for n < 2^31, the same for page_size
+    int head_shift, page_shift;
 };
+
+__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t mul, int shift) { return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift); }
 
 __device__ __forceinline__ void unpack8(const uint4& v, int is_f16, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -65,18 +70,18 @@ __device__ __forceinline__ uint32_t bf16_down(float x) {
 template <int BITS, int D>
 __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
     constexpr int LANES = D / 8, GROUP = BITS == 8 ? LANES : 8;   // lanes that share a scale
-    const long long item = (static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x) / LANES;
+    const uint32_t item = static_cast<uint32_t>((static_cast<uint64_t>(blockIdx.x) * THREADS + threadIdx.x) / LANES);
     const int l = static_cast<int>(threadIdx.x) % LANES;
     pdl_wait_and_release();
-    const long long t = item / p.Hkv;
-    const int h = static_cast<int>(item - t * p.Hkv);
+    const long long t = quotient(item, p.head_mul, p.head_shift);
+    const int h = static_cast<int>(item - static_cast<uint32_t>(t) * p.Hkv);
     const bool live = t < p.rows;
     const int slot = live ? p.slots[t] : -1;
     uint4 raw[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         raw[i] = live ? ld_v4(p.x[i] + t * p.x_token[i] + h * p.x_head[i] + l * 16) : make_uint4(0u, 0u, 0u, 0u);
-    const int page = slot / p.page_size;
+    const int page = slot < 0 ? 0 : static_cast<int>(quotient(static_cast<uint32_t>(slot), p.page_mul, p.page_shift));
     const int row = slot - page * p.page_size;
     const bool kept = slot >= 0 && page < p.blocks;
 #pragma unroll
@@ -105,10 +110,11 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
         if (BITS == 8) {
             const float a = fmaxf(good ? __uint_as_float(top) : 1.f, kLeast);
             const float inv = __fdiv_rn(127.f, a);
-            uint32_t w[2] = {0u, 0u};
+            uint32_t b[8];   // 1.5 2^23 + 128 + the code: the low byte is what is stored
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j >> 2] |= static_cast<uint32_t>(good ? 128 + __float2int_rn(__fmul_rn(f[j], inv)) : 128) << (8 * (j & 3));
+            for (int j = 0; j < 8; ++j) b[j] = good ? __float_as_uint(__fadd_rn(__fmul_rn(f[j], inv), 12583040.f)) : 128u;
+            const uint32_t w[2] = {__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                                   __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410)};
             if (kept) {
                 *reinterpret_cast<uint2*>(dst + l * 8) = make_uint2(w[0], w[1]);
                 if (l == 0) *reinterpret_cast<float*>(sdst) = good ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fffffffu);
@@ -122,8 +128,9 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
             uint32_t w = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int c = good ? __float2int_rn(__fmul_rn(__fsub_rn(f[j], base), inv)) : 0;   // (NaN gives 0)
-                w |= static_cast<uint32_t>(min(15, max(0, c))) << (4 * j);
+                // (a NaN, from a range beyond fp32's, gives 0)
+                const float c = fminf(15.f, fmaxf(0.f, __fmul_rn(__fsub_rn(f[j], base), inv)));
+                w |= (good ? __float_as_uint(__fadd_rn(c, 12582912.f)) & 15u : 0u) << (4 * j);
             }
             if (kept) {
                 *reinterpret_cast<uint32_t*>(dst + l * 4) = w;
@@ -164,7 +171,7 @@ __global__ void __launch_bounds__(THREADS) read_kernel(const Params p) {
         int page = -1, row = 0;
         if (a > 0 && r < p.starts[a]) {
             const int j = r - p.starts[a - 1];
-            const int in_table = j / p.page_size;
+            const int in_table = static_cast<int>(quotient(static_cast<uint32_t>(j), p.page_mul, p.page_shift));
             if (j < p.lens[a - 1] && in_table < p.max_blocks) {
                 page = p.table[static_cast<long long>(a - 1) * p.max_blocks + in_table];
                 row = j - in_table * p.page_size;
@@ -177,45 +184,67 @@ __global__ void __launch_bounds__(THREADS) read_kernel(const Params p) {
     __syncthreads();
     const int l = static_cast<int>(threadIdx.x) % LANES;
     const int items = n * p.Hkv;
-    for (int item = static_cast<int>(threadIdx.x) / LANES; item < items; item += THREADS / LANES) {
-        const int r = item / p.Hkv, h = item - r * p.Hkv;
-        const int page = page_s[r], row = row_s[r];
-        uint4 codes[2];
-        float scale[2], least[2] = {0.f, 0.f};
+    constexpr int STEP = THREADS / LANES, AT_ONCE = 2;
+    for (int first = static_cast<int>(threadIdx.x) / LANES; first < items; first += STEP * AT_ONCE) {
+        uint4 codes[AT_ONCE][2];
+        float scale[AT_ONCE][2], least[AT_ONCE][2];
+        bool there[AT_ONCE];
+        int r[AT_ONCE], h[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            codes[i] = make_uint4(0u, 0u, 0u, 0u);
-            scale[i] = 0.f;
-            if (page < 0) continue;
-            const uint8_t* src = p.codes[i] + page * p.code_block + row * p.code_token + h * p.code_head;
-            const char* ssrc = p.scales[i] + page * p.scale_block + h * p.scale_head + row * p.scale_token;
-            if (BITS == 8) {
-                codes[i] = ld_v4(src + l * 16);
-                scale[i] = *reinterpret_cast<const float*>(ssrc);
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(src + l * 8);
-                codes[i].x = w.x;
-                codes[i].y = w.y;
-                const uint32_t pair = *reinterpret_cast<const uint32_t*>(ssrc + (l >> 2) * 4);
-                scale[i] = __uint_as_float(pair << 16);
-                least[i] = __uint_as_float(pair & 0xffff0000u);
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int item = first + u * STEP;
+            r[u] = static_cast<int>(quotient(static_cast<uint32_t>(item), p.head_mul, p.head_shift));
+            h[u] = item - r[u] * p.Hkv;
+            const int page = item < items ? page_s[r[u]] : -1;
+            there[u] = page >= 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                codes[u][i] = make_uint4(0u, 0u, 0u, 0u);
+                scale[u][i] = least[u][i] = 0.f;
+                if (!there[u]) continue;
+                const int row = row_s[r[u]];
+                const uint8_t* src = p.codes[i] + page * p.code_block + row * p.code_token + h[u] * p.code_head;
+                const char* ssrc = p.scales[i] + page * p.scale_block + h[u] * p.scale_head + row * p.scale_token;
+                if (BITS == 8) {
+                    codes[u][i] = ld_v4(src + l * 16);
+                    scale[u][i] = *reinterpret_cast<const float*>(ssrc);
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(src + l * 8);
+                    codes[u][i].x = w.x;
+                    codes[u][i].y = w.y;
+                    const uint32_t pair = *reinterpret_cast<const uint32_t*>(ssrc + (l >> 2) * 4);
+                    scale[u][i] = __uint_as_float(pair << 16);
+                    least[u][i] = __uint_as_float(pair & 0xffff0000u);
+                }
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float f[16];
-            values16<BITS>(codes[i], scale[i], least[i], f);
-            uint32_t o[8];
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (first + u * STEP >= items) break;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float a = page < 0 ? 0.f : f[2 * j], b = page < 0 ? 0.f : f[2 * j + 1];
-                o[j] = p.is_f16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+            for (int i = 0; i < 2; ++i) {
+                float f[16];
+                values16<BITS>(codes[u][i], scale[u][i], least[u][i], f);
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    o[j] = p.is_f16 ? pack_f16x2(f[2 * j], f[2 * j + 1]) : pack_bf16x2(f[2 * j], f[2 * j + 1]);
+                    if (!there[u]) o[j] = 0u;   // (codes of 0 would be -128 times 0: a negative zero)
+                }
+                uint4* dst = reinterpret_cast<uint4*>(p.out[i] + ((r0 + r[u]) * p.Hkv + h[u]) * (D * 2ll) + l * 32);
+                dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
             }
-            uint4* dst = reinterpret_cast<uint4*>(p.out[i] + ((r0 + r) * p.Hkv + h) * (D * 2ll) + l * 32);
-            dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }
     }
+}
+
+static void multiplier(int n, uint32_t* mul, int* shift) {
+    // with 2^l >= n the multiplier ceil(2^(31 + l) / n) is off by less than one, so its product with a number below 2^31 by less than 2^31
+    int l = 0;
+    while ((1ll << l) < n) ++l;
+    *shift = 31 + l;
+    *mul = static_cast<uint32_t>(((1ull << (31 + l)) + static_cast<uint64_t>(n) - 1) / static_cast<uint64_t>(n));
 }
 
 static int fill(const TdistQuantCacheArgs* a, Params& p) {
@@ -241,6 +270,8 @@ static int fill(const TdistQuantCacheArgs* a, Params& p) {
     p.max_blocks = a->max_blocks;
     p.is_f16 = a->dtype == TDIST_F16;
     p.rows = a->rows;
+    multiplier(a->Hkv, &p.head_mul, &p.head_shift);
+    multiplier(a->page_size, &p.page_mul, &p.page_shift);
     const uintptr_t code_align = reinterpret_cast<uintptr_t>(a->k_codes) | reinterpret_cast<uintptr_t>(a->v_codes) |
                                  static_cast<uintptr_t>(a->code_block | a->code_token | a->code_head);
     const uintptr_t scale_align = reinterpret_cast<uintptr_t>(a->k_scales) | reinterpret_cast<uintptr_t>(a->v_scales) |
@@ -284,7 +315,7 @@ extern "C" int tdist_quant_cache_write(const TdistQuantCacheArgs* a) {
         return fail(TDIST_EINVAL, "quantised cache: rows must lie on 16 bytes");
     const long long lanes = a->head_dim / 8, threads = a->rows * a->Hkv * lanes;
     const long long grid = (threads + qcache::THREADS - 1) / qcache::THREADS;
-    if (grid > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised cache: too many rows in one call");
+    if (a->rows * a->Hkv > 0x7ffffff0ll) return fail(TDIST_EINVAL, "quantised cache: too many rows in one call");
     TDIST_BY_CACHE(qcache::write_kernel, a->bits, a->head_dim, dim3(static_cast<unsigned>(grid)), qcache::THREADS, 0, static_cast<cudaStream_t>(a->stream), p);
     return 0;
 }
