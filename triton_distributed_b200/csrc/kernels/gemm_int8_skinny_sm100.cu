@@ -32,7 +32,7 @@ constexpr int SMEM_BYTES = STAGE_AREA + 1024 + 256;
 // the partials of one cluster share: split x ceil(tok / split) tokens x 128 rows of 32 bits
 static_assert((MAX_TOK + MAX_SPLIT) * ROWS * 4 <= STAGE_AREA, "the partial sums reuse the stages");
 
-constexpr int kKernelSkinny = 12;   // reported as the int8 GEMM
+constexpr int kKernelSkinny = 10;   // reported as the int8 GEMM
 
 struct Params {
     CUtensorMap tm_w;   // {K, N}, box {128, 128}

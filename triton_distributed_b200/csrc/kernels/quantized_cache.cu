@@ -8,8 +8,8 @@
 // bf16 rows do not, one of fp32 would make 5 bits of 4.5.
 // Quotients and products are IEEE's (this file is compiled without fast math): the same codes as the statement in torch.
 //
-// Bound by bytes. A lane takes 8 values (16 bytes) of a k row and of the v row beside it when writing, 16 codes of each of two places when reading:
-// two and four loads of each lane under way at once. Quotients of places by heads and page sizes go by a multiplication, rounding by
+// Bound by bytes. A lane takes 16 values (32 bytes) of a k row and of the v row beside it when writing, 16 codes of each of two places when reading:
+// four loads of each lane under way at once. Quotients of places by heads and page sizes go by a multiplication, rounding by
 // the addition of 1.5 2^23, whose low byte is the code.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,30 +46,41 @@ struct Params {
 
 __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t mul, int shift) { return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift); }
 
-__device__ __forceinline__ void unpack8(const uint4& v, int is_f16, float (&f)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (is_f16) {
-            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = t.x;
-            f[2 * i + 1] = t.y;
-        } else {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-}
 // the largest bf16 that is not above x (x finite), as its 16 bits
 __device__ __forceinline__ uint32_t bf16_down(float x) {
     const uint32_t u = __float_as_uint(x);
     return (u >> 16) + ((u >> 31) && (u & 0xffffu) ? 1u : 0u);
 }
 
-// LANES lanes hold a row, 8 values each
-template <int BITS, int D>
+// pairs of 16-bit numbers
+template <bool F16>
+struct Pair {
+    static __device__ __forceinline__ float low(uint32_t w) { return F16 ? __low2float(*reinterpret_cast<const __half2*>(&w)) : __uint_as_float(w << 16); }
+    static __device__ __forceinline__ float high(uint32_t w) { return F16 ? __high2float(*reinterpret_cast<const __half2*>(&w)) : __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ uint32_t least(uint32_t a, uint32_t b) {
+        if (F16) {
+            const __half2 r = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        }
+        const __nv_bfloat162 r = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) {
+        if (F16) {
+            const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        }
+        const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+
+// LANES lanes hold a row, 16 values each: what a row costs once (its place, the scale's quotients, the exchange between its lanes) counts as much as its
+// values (8 per lane: 16384 tokens of 8 heads of 128 24.2 us in 8 bits, 33.6 in 4). Magnitudes are compared as 16-bit integers, whose order is the numbers'.
+template <int BITS, int D, bool F16>
 __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
-    constexpr int LANES = D / 8, GROUP = BITS == 8 ? LANES : 8;   // lanes that share a scale
+    using P = Pair<F16>;
+    constexpr int LANES = D / 16, GROUP = BITS == 8 ? LANES : 4;   // lanes that share a scale
     const uint32_t item = static_cast<uint32_t>((static_cast<uint64_t>(blockIdx.x) * THREADS + threadIdx.x) / LANES);
     const int l = static_cast<int>(threadIdx.x) % LANES;
     pdl_wait_and_release();
@@ -77,64 +88,77 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
     const int h = static_cast<int>(item - static_cast<uint32_t>(t) * p.Hkv);
     const bool live = t < p.rows;
     const int slot = live ? p.slots[t] : -1;
-    uint4 raw[2];
+    uint32_t w[2][8];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        raw[i] = live ? ld_v4(p.x[i] + t * p.x_token[i] + h * p.x_head[i] + l * 16) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint4 v = live ? ld_v4(p.x[i] + t * p.x_token[i] + h * p.x_head[i] + l * 32 + j * 16) : make_uint4(0u, 0u, 0u, 0u);
+            w[i][4 * j] = v.x;
+            w[i][4 * j + 1] = v.y;
+            w[i][4 * j + 2] = v.z;
+            w[i][4 * j + 3] = v.w;
+        }
     const int page = slot < 0 ? 0 : static_cast<int>(quotient(static_cast<uint32_t>(slot), p.page_mul, p.page_shift));
     const int row = slot - page * p.page_size;
     const bool kept = slot >= 0 && page < p.blocks;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float f[8];
-        unpack8(raw[i], p.is_f16, f);
-        uint32_t top = 0;   // bits of the largest magnitude; a NaN's lie above an infinity's
-        float lo = f[0], hi = f[0];
+        uint32_t top = 0, lo2 = w[i][0], hi2 = w[i][0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-            lo = fminf(lo, f[j]);
-            hi = fmaxf(hi, f[j]);
+        for (int j = 0; j < 4; ++j) top = __vimax3_u16x2(top, w[i][2 * j] & 0x7fff7fffu, w[i][2 * j + 1] & 0x7fff7fffu);
+        top = max(top & 0xffffu, top >> 16);
+        if (BITS == 4) {
+#pragma unroll
+            for (int j = 1; j < 8; ++j) {
+                lo2 = P::least(lo2, w[i][j]);
+                hi2 = P::most(hi2, w[i][j]);
+            }
         }
 #pragma unroll
         for (int o = 1; o < GROUP; o <<= 1) {
             top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             if (BITS == 4) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                lo2 = P::least(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
+                hi2 = P::most(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
             }
         }
-        const bool good = top < 0x7f800000u;
+        const bool good = top < (F16 ? 0x7c00u : 0x7f80u);
         uint8_t* dst = p.codes[i] + page * p.code_block + row * p.code_token + h * p.code_head;
         char* sdst = p.scales[i] + page * p.scale_block + h * p.scale_head + row * p.scale_token;
         if (BITS == 8) {
-            const float a = fmaxf(good ? __uint_as_float(top) : 1.f, kLeast);
+            const float a = good ? fmaxf(P::low(top), kLeast) : 1.f;
             const float inv = __fdiv_rn(127.f, a);
-            uint32_t b[8];   // 1.5 2^23 + 128 + the code: the low byte is what is stored
+            uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = good ? __float_as_uint(__fadd_rn(__fmul_rn(f[j], inv), 12583040.f)) : 128u;
-            const uint32_t w[2] = {__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
-                                   __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410)};
+            for (int j = 0; j < 4; ++j) {
+                // 1.5 2^23 + 128 + the code: the low byte is what is stored
+                const uint32_t b0 = __float_as_uint(__fadd_rn(__fmul_rn(P::low(w[i][2 * j]), inv), 12583040.f)), b1 = __float_as_uint(__fadd_rn(__fmul_rn(P::high(w[i][2 * j]), inv), 12583040.f));
+                const uint32_t b2 = __float_as_uint(__fadd_rn(__fmul_rn(P::low(w[i][2 * j + 1]), inv), 12583040.f)), b3 = __float_as_uint(__fadd_rn(__fmul_rn(P::high(w[i][2 * j + 1]), inv), 12583040.f));
+                o[j] = good ? __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410) : 0x80808080u;
+            }
             if (kept) {
-                *reinterpret_cast<uint2*>(dst + l * 8) = make_uint2(w[0], w[1]);
+                *reinterpret_cast<uint4*>(dst + l * 16) = make_uint4(o[0], o[1], o[2], o[3]);
                 if (l == 0) *reinterpret_cast<float*>(sdst) = good ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fffffffu);
             }
         } else {
+            const float lo = fminf(P::low(lo2), P::high(lo2)), hi = fmaxf(P::low(hi2), P::high(hi2));
             const uint32_t least = bf16_down(lo);
             const float base = __uint_as_float(least << 16);
             const float wide = fmaxf(__fdiv_rn(__fsub_rn(hi, base), 15.f), kLeast);
             const uint32_t step = bf16_down(-wide) & 0x7fffu;   // up: down of the negative (a range beyond fp32's: infinite)
             const float inv = __fdiv_rn(1.f, __uint_as_float(step << 16));
-            uint32_t w = 0;
+            uint32_t o[2] = {0u, 0u};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 // (a NaN, from a range beyond fp32's, gives 0)
-                const float c = fminf(15.f, fmaxf(0.f, __fmul_rn(__fsub_rn(f[j], base), inv)));
-                w |= (good ? __float_as_uint(__fadd_rn(c, 12582912.f)) & 15u : 0u) << (4 * j);
+                const float c0 = fminf(15.f, fmaxf(0.f, __fmul_rn(__fsub_rn(P::low(w[i][j]), base), inv))), c1 = fminf(15.f, fmaxf(0.f, __fmul_rn(__fsub_rn(P::high(w[i][j]), base), inv)));
+                const uint32_t pair = (__float_as_uint(__fadd_rn(c0, 12582912.f)) & 15u) | (__float_as_uint(__fadd_rn(c1, 12582912.f)) & 15u) << 4;
+                o[j >> 2] |= pair << (8 * (j & 3));
             }
             if (kept) {
-                *reinterpret_cast<uint32_t*>(dst + l * 4) = w;
-                if ((l & 7) == 0) *reinterpret_cast<uint32_t*>(sdst + (l >> 3) * 4) = good ? step | (least << 16) : 0x7fff7fffu;
+                *reinterpret_cast<uint2*>(dst + l * 8) = good ? make_uint2(o[0], o[1]) : make_uint2(0u, 0u);
+                if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(sdst + (l >> 2) * 4) = good ? step | (least << 16) : 0x7fff7fffu;
             }
         }
     }
@@ -287,17 +311,17 @@ static int fill(const TdistQuantCacheArgs* a, Params& p) {
 using namespace tdist;
 using tdist_host::fail;
 
-#define TDIST_BY_CACHE(kernel, bits, dim, ...)                                                                      \
-    do {                                                                                                            \
-        cudaError_t e;                                                                                              \
-        if (bits == 8)                                                                                              \
-            e = dim == 64 ? tdist_host::launch_pdl(kernel<8, 64>, __VA_ARGS__)                                      \
-                          : (dim == 128 ? tdist_host::launch_pdl(kernel<8, 128>, __VA_ARGS__) : tdist_host::launch_pdl(kernel<8, 256>, __VA_ARGS__)); \
-        else                                                                                                        \
-            e = dim == 64 ? tdist_host::launch_pdl(kernel<4, 64>, __VA_ARGS__)                                      \
-                          : (dim == 128 ? tdist_host::launch_pdl(kernel<4, 128>, __VA_ARGS__) : tdist_host::launch_pdl(kernel<4, 256>, __VA_ARGS__)); \
-        TDIST_CUDA_OK(e);                                                                                           \
-    } while (0)
+namespace {
+template <int BITS, int D>
+cudaError_t write_rows(bool f16, dim3 grid, cudaStream_t stream, const qcache::Params& p) {
+    return f16 ? tdist_host::launch_pdl(qcache::write_kernel<BITS, D, true>, grid, qcache::THREADS, 0, stream, p)
+               : tdist_host::launch_pdl(qcache::write_kernel<BITS, D, false>, grid, qcache::THREADS, 0, stream, p);
+}
+template <int BITS, int D>
+cudaError_t read_rows(dim3 grid, cudaStream_t stream, const qcache::Params& p) {
+    return tdist_host::launch_pdl(qcache::read_kernel<BITS, D>, grid, qcache::THREADS, 0, stream, p);
+}
+}  // namespace
 
 extern "C" int tdist_quant_cache_write(const TdistQuantCacheArgs* a) {
     qcache::Params p;
@@ -313,10 +337,18 @@ extern "C" int tdist_quant_cache_write(const TdistQuantCacheArgs* a) {
     p.slots = static_cast<const int*>(a->slots);
     if ((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v) | static_cast<uintptr_t>(a->k_token | a->k_head | a->v_token | a->v_head)) & 15)
         return fail(TDIST_EINVAL, "quantised cache: rows must lie on 16 bytes");
-    const long long lanes = a->head_dim / 8, threads = a->rows * a->Hkv * lanes;
+    const long long lanes = a->head_dim / 16, threads = a->rows * a->Hkv * lanes;
     const long long grid = (threads + qcache::THREADS - 1) / qcache::THREADS;
     if (a->rows * a->Hkv > 0x7ffffff0ll) return fail(TDIST_EINVAL, "quantised cache: too many rows in one call");
-    TDIST_BY_CACHE(qcache::write_kernel, a->bits, a->head_dim, dim3(static_cast<unsigned>(grid)), qcache::THREADS, 0, static_cast<cudaStream_t>(a->stream), p);
+    const dim3 blocks(static_cast<unsigned>(grid));
+    const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+    const bool f16 = a->dtype == TDIST_F16;
+    cudaError_t e;
+    if (a->bits == 8)
+        e = (a->head_dim == 64 ? write_rows<8, 64>(f16, blocks, stream, p) : (a->head_dim == 128 ? write_rows<8, 128>(f16, blocks, stream, p) : write_rows<8, 256>(f16, blocks, stream, p)));
+    else
+        e = (a->head_dim == 64 ? write_rows<4, 64>(f16, blocks, stream, p) : (a->head_dim == 128 ? write_rows<4, 128>(f16, blocks, stream, p) : write_rows<4, 256>(f16, blocks, stream, p)));
+    TDIST_CUDA_OK(e);
     return 0;
 }
 
@@ -335,9 +367,16 @@ extern "C" int tdist_quant_cache_read(const TdistQuantCacheArgs* a) {
     p.table = static_cast<const int*>(a->table);
     // few rows: a CTA each, so that all lookups run side by side
     int per = qcache::MAX_ROWS;
-    while (per > 1 && (a->rows + per - 1) / per < 4ll * tdist_host::sm_count()) per >>= 1;
+    while (per > 1 && (a->rows + per - 1) / per < 8ll * tdist_host::sm_count()) per >>= 1;
     p.rows_per_cta = per;
     const long long grid = (a->rows + per - 1) / per;
-    TDIST_BY_CACHE(qcache::read_kernel, a->bits, a->head_dim, dim3(static_cast<unsigned>(grid)), qcache::THREADS, 0, static_cast<cudaStream_t>(a->stream), p);
+    const dim3 blocks(static_cast<unsigned>(grid));
+    const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+    cudaError_t e;
+    if (a->bits == 8)
+        e = (a->head_dim == 64 ? read_rows<8, 64>(blocks, stream, p) : (a->head_dim == 128 ? read_rows<8, 128>(blocks, stream, p) : read_rows<8, 256>(blocks, stream, p)));
+    else
+        e = (a->head_dim == 64 ? read_rows<4, 64>(blocks, stream, p) : (a->head_dim == 128 ? read_rows<4, 128>(blocks, stream, p) : read_rows<4, 256>(blocks, stream, p)));
+    TDIST_CUDA_OK(e);
     return 0;
 }

@@ -43,16 +43,22 @@ def ref_gemm_int8(a, sa, b, sb, out_dtype=torch.bfloat16) -> torch.Tensor:
     return (acc.float() * sa.float().view(-1, 1) * sb.float()).to(out_dtype)
 
 
-def _on(device):
-    return None if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call(index, fn, *args):
+    """The native call with device ``index`` as the current one."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
 
 
-def _call(device, fn, *args):
-    guard = _on(device)
-    if guard is None:
-        return fn(*args)
-    with guard:
-        return fn(*args)
+# What the checks found, by shapes, strides, types and devices (never by addresses or contents)
+_CHECKED: set = set()
+
+
+def _remember(key):
+    if len(_CHECKED) >= 4096:
+        _CHECKED.clear()
+    _CHECKED.add(key)
 
 
 @nvtx_range("tdist.quantize_int8_rowwise")
@@ -68,10 +74,10 @@ def quantize_int8_rowwise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     M, K = x.shape
     if x.stride(1) != 1 or (x.stride(0) * x.element_size()) % 16 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    codes, scale = torch.empty((M, K), dtype=torch.int8, device=x.device), torch.empty(M, dtype=torch.float32, device=x.device)
+    codes, scale = x.new_empty((M, K), dtype=torch.int8), x.new_empty((M,), dtype=torch.float32)
     if M:
-        code = _call(x.device, _lib.lib().tdist_quant_int8_rowwise, x.data_ptr(), x.stride(0), codes.data_ptr(), scale.data_ptr(), M, K, _ROWS[x.dtype],
-                     stream_ptr(x.device))
+        code = _call(x.get_device(), _lib.lib().tdist_quant_int8_rowwise, x.data_ptr(), x.stride(0), codes.data_ptr(), scale.data_ptr(), M, K,
+                     _ROWS[x.dtype], stream_ptr(x.device))
         if code:
             _lib.check(code, "tdist_quant_int8_rowwise")
         launch_count += 1
@@ -106,11 +112,16 @@ def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tens
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a [M, K]``, ``b [N, K]`` int8, ``sa [M]``, ``sb [N]`` fp32 -> ``[M, N]`` bf16 or fp16. K a multiple of 16, N of 8."""
     global launch_count
-    _check(a, sa, b, sb, out_dtype, out)
-    if a.device.type != "cuda":
+    index = a.get_device()
+    key = (a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype, b.get_device(), sa.shape, sa.stride(), sa.dtype, sa.get_device(), sb.shape, sb.stride(),
+           sb.dtype, sb.get_device(), index, out_dtype, None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
+    if index < 0 or key not in _CHECKED:
+        _check(a, sa, b, sb, out_dtype, out)
+        _remember(key)
+    if index < 0:
         c = ref_gemm_int8(a, sa, b, sb, out_dtype)
         return c if out is None else out.copy_(c)
-    c = out if out is not None else torch.empty((a.shape[0], b.shape[0]), dtype=out_dtype, device=a.device)
+    c = out if out is not None else a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
     if c.numel() == 0:
         return c
     g = _lib.GemmInt8Args()
@@ -120,7 +131,7 @@ def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tens
     g.status = st.device_ptr if st is not None else None
     g.timeout_ns = default_timeout_ns()
     g.stream = stream_ptr(a.device)
-    code = _call(a.device, _lib.lib().tdist_gemm_int8, C.byref(g))
+    code = _call(index, _lib.lib().tdist_gemm_int8, C.byref(g))
     if code:
         _lib.check(code, "tdist_gemm_int8")
     launch_count += 1

@@ -228,6 +228,15 @@ def _cache_args(cache: QuantizedKVCache, dtype) -> "_lib.QuantCacheArgs":
     return a
 
 
+def _layout(cache: QuantizedKVCache, *others):
+    """What a plan is found by: codes and scales of k and v have to be alike, so theirs are compared and k's told."""
+    k, v, ks, vs = cache
+    same = (k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and ks.shape == vs.shape and ks.stride() == vs.stride()
+            and ks.dtype == vs.dtype and k.get_device() == v.get_device() == ks.get_device() == vs.get_device())
+    return (same, k.shape, k.stride(), k.dtype, ks.shape, ks.stride(), ks.dtype, k.get_device()) + tuple(
+        x for t in others for x in (t.shape, t.stride(), t.dtype, t.get_device()))
+
+
 def _point(a, cache: QuantizedKVCache):
     a.k_codes, a.v_codes, a.k_scales, a.v_scales = cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scales.data_ptr(), cache.v_scales.data_ptr()
     a.stream = stream_ptr(cache.k.device)
@@ -236,7 +245,7 @@ def _point(a, cache: QuantizedKVCache):
 def _launch(fn, a, device, what):
     """The native call with ``device`` as the current one."""
     global launch_count
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         code = fn(C.byref(a))
     else:
         with torch.cuda.device(device):
@@ -257,7 +266,7 @@ def _aligned(x):
 def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantises ``k, v [T, Hkv, D]`` (bf16 or fp16; views of a fused projection are read in place) into their places ``slots [T]``.
     What the slots do not name keeps its bytes."""
-    layout = PA._layout(*cache, k, v, slots)
+    layout = _layout(cache, k, v, slots)
     args = _PLANS.get((kv_cache_write, layout))
     if args is None:
         _check_cache(cache)
@@ -300,7 +309,7 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
     sequence are zeros."""
     rows = int(rows)
     given = () if out is None else tuple(out)
-    key = (kv_cache_read, PA._layout(*cache, starts, kv_lens, block_table, *given), rows, dtype)
+    key = (kv_cache_read, _layout(cache, starts, kv_lens, block_table, *given), rows, dtype)
     args = _PLANS.get(key)
     if args is None:
         _check_cache(cache)
@@ -320,7 +329,8 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
         args.rows, args.B, args.max_blocks = rows, B, block_table.shape[1]
         _remember(key, args)
     if out is None:
-        k, v = (torch.empty((rows, args.Hkv, args.head_dim), dtype=dtype, device=cache.k.device) for _ in range(2))
+        shape = (rows, args.Hkv, args.head_dim)
+        k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
     else:
         k, v = given
     if rows == 0:
@@ -344,7 +354,7 @@ def _decode_parts(B: int, per_b: int, most: int, table_keys: int, asked: int, sl
     if asked > 0:
         return (asked, 0) if asked <= 8 else ((0, max(1, min(slots // per_b, B * asked))) if may_share else (8, 0))
     splits = max(1, min(slots // max(1, B * per_b), -(-most // 256)))
-    if may_share and (splits > 8 or B * per_b * most > slots * 1024):
+    if may_share and (splits > 8 or (most >= 1024 and B * per_b * most > slots * 2048)):
         return 0, max(1, slots // per_b)
     return min(splits, 8), 0
 
@@ -358,7 +368,7 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
     query that sees no key (or none whose score is above -inf) gives zeros. Pages without a visible key are not read. ``kv_split``: parts of a
     sequence's keys, up to 8; more: equal shares of all sequences' keys, as many as fit the machine; -1: chosen by sizes."""
     window, sinks, scale, soft_cap = PA._settings(window, sinks, scale, soft_cap)
-    key = (gqa_fwd_quantized_decode, PA._layout(q, *cache, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
+    key = (gqa_fwd_quantized_decode, _layout(cache, q, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
     args = _PLANS.get(key)
     if args is None:
         _check_cache(cache)
