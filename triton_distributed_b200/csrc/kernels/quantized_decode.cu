@@ -49,9 +49,11 @@ namespace qdecode {
 
 constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
-// Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled: a weight
-// times its scale's share of the unit is rounded to fp16 whatever its size, and 2^8 is far below fp16's largest.
-constexpr float kSlack = 8.f;
+// Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled. 8 bits: a
+// weight times its scale is rounded whatever its size, and 2^8 is far below fp16's largest. 4 bits: none, as the largest weight, 1, times a step of 8
+// bits is exact, which is most of a result that few keys make up (64 heads on 8, 16384 keys, fp16: error 2.7e-4 of the result, 3.8e-4
+// with a slack of 2^8, of which 2.1e-4 the result's own rounding; 16 x 16384 keys 102 and 100 us).
+__host__ __device__ constexpr float slack_of(int bits) { return bits == 8 ? 8.f : 0.f; }
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -450,6 +452,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
     const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
+    const bool fine = p.is_f16 != 0;   // 8 bits: weights as two fp16 numbers, which costs little beside the loads (fp16 results: error 3.0e-4 with one)
     uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
     int turn = 0;            // the warp that has a piece's first tile: tiles go round the warps from piece to piece
     bool first_piece = true;
@@ -676,7 +679,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     const float m_old = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r], m_new = fmaxf(m_old, mx);
                     m_use[h][r] = m_new == -CUDART_INF_F ? 0.f : m_new;
-                    limit[h][r] = m_new + kSlack;
+                    limit[h][r] = m_new + slack_of(BITS);
                     const float alpha = exp2f(m_old - m_use[h][r]);
                     l_run[h][r] *= alpha;
 #pragma unroll
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) vmul[r][k] *= inv_unit;
         // ---- P^T times the scales as the second operand: tokens in pairs per lane, heads over lane / 4
-        uint32_t pb[NH][S::NG][2];
+        uint32_t pb[NH][S::NG][2], pl[NH][2];
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
             const float p0 = exp2f(s[h][0] - m_use[h][0]), p1 = exp2f(s[h][1] - m_use[h][1]);
@@ -707,8 +710,16 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                     low[h][0][k] += p0 * vleast[0][k] + p2 * vleast[1][k];
                     low[h][1][k] += p1 * vleast[0][k] + p3 * vleast[1][k];
                 }
-                pb[h][k][0] = movmatrix_trans(pack_f16x2(p0 * vmul[0][k], p1 * vmul[0][k]));
-                pb[h][k][1] = movmatrix_trans(pack_f16x2(p2 * vmul[1][k], p3 * vmul[1][k]));
+                const float w0 = p0 * vmul[0][k], w1 = p1 * vmul[0][k], w2 = p2 * vmul[1][k], w3 = p3 * vmul[1][k];
+                const uint32_t a = pack_f16x2(w0, w1), bb = pack_f16x2(w2, w3);
+                pb[h][k][0] = movmatrix_trans(a);
+                pb[h][k][1] = movmatrix_trans(bb);
+                if (BITS == 8 && fine) {
+                    // what the rounding left
+                    const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&a)), rb = __half22float2(*reinterpret_cast<const __half2*>(&bb));
+                    pl[h][0] = movmatrix_trans(pack_f16x2(w0 - ra.x, w1 - ra.y));
+                    pl[h][1] = movmatrix_trans(pack_f16x2(w2 - rb.x, w3 - rb.y));
+                }
             }
         }
         // ---- O^T += V^T P^T: row g of MMA m is dimension 2 m of the lane's, row g + 8 the one after it
@@ -733,7 +744,10 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                         const uint32_t x0 = bytes_to_half2(a, kLowBytes), x1 = bytes_to_half2(a, kHighBytes);
                         const uint32_t x2 = bytes_to_half2(bb, kLowBytes), x3 = bytes_to_half2(bb, kHighBytes);
 #pragma unroll
-                        for (int h = 0; h < NH; ++h) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
+                        for (int h = 0; h < NH; ++h) {
+                            mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
+                            if (fine) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pl[h][0], pl[h][1]);
+                        }
                     }
                 } else {
 #pragma unroll
