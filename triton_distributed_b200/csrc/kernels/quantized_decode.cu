@@ -36,6 +36,7 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <atomic>
 #include <cstring>
 #include <string>
 
@@ -370,75 +371,85 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     uint32_t dst_at[TOK / ROWS];
 #pragma unroll
     for (int j = 0; j < TOK / ROWS; ++j) dst_at[j] = S::at(j * ROWS + lrow, lchunk * 16);
-    const uint32_t code_token = static_cast<uint32_t>(p.code_token), scale_token = static_cast<uint32_t>(p.scale_token);   // PAGED: strides fit 32 bits
+    const uint32_t code_token = static_cast<uint32_t>(p.code_token);   // PAGED: fits 32 bits
+    const uint64_t code_rows = static_cast<uint64_t>(code_token) * ROWS;
     auto in_table = [&](int t) {
         return PAGED ? t >> p.page_shift : static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * p.page_mul) >> p.page_shift);
     };
     Pieces coming = pieces;
-    Keys c_keys;
-    const int* c_table = nullptr;
+    Keys c_keys = keys_of(p, 0);
+    const int* c_table = p.table;
     const uint8_t* c_k = p.k + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
     const uint8_t* c_v = p.v + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
     // lanes 0..15 copy the scales of the keys, 16..31 of the values
     const char* c_s = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head + (PAGED ? my_token * p.scale_token : 0);
-    // the next tile, its first token (not PAGED: this lane's), the end of the run of tiles whose tokens follow one another (the first keys, or the
-    // window), the piece's end, the page
-    int c_i = 0, c_t = 0, c_run = 0, c_end = 0, c_turn = 0, c_page = -1;
-    c_keys.n = c_keys.lo = c_keys.first = c_keys.sink_tiles = c_keys.t_lo = 0;
-    auto advance = [&]() {
-        c_i += WARPS;
-        c_t += WARPS * TOK;
-        if (c_i >= c_run) {
-            while (c_i >= c_end) {
-                Piece x;
-                if (!coming.next(x)) {
-                    c_i = c_run = 0;
-                    return;
-                }
-                c_keys = keys_in(x.b);
-                c_table = p.table + static_cast<size_t>(x.b) * p.max_blocks;
-                c_i = x.i0 + (warp + WARPS - c_turn) % WARPS;
-                c_end = x.i1;
-                c_turn = (c_turn + x.i1 - x.i0) % WARPS;
+    // A run: tiles whose tokens follow one another (the first keys, or the window's). Tiles left of it, the next one's first token (not PAGED: this lane's),
+    // the last one's, the next one's page; whether there are no more
+    int c_left = 0, c_t = 0, c_last = 0, c_page = -1;
+    int c_i = 0, c_end = 0, c_turn = 0;   // the piece's next tile behind the run, its end
+    bool c_done = false;
+    auto page_of = [&]() {
+        const bool seen = !c_done && (PAGED || c_t < c_keys.first || (c_t >= c_keys.lo && c_t < c_keys.n));
+        return seen ? static_cast<int>(ldg32(c_table + in_table(c_t))) : -1;
+    };
+    auto new_run = [&]() {
+        while (c_i >= c_end) {
+            Piece x;
+            if (!coming.next(x)) {
+                // nothing from here on: what is "copied" are zeros
+                c_left = 0x7fffffff;
+                c_last = c_t;
+                c_page = -1;
+                c_done = true;
+                return;
             }
-            c_run = c_i < c_keys.sink_tiles ? min(c_keys.sink_tiles, c_end) : c_end;
-            c_t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
+            c_keys = keys_in(x.b);
+            c_table = p.table + static_cast<size_t>(x.b) * p.max_blocks;
+            c_i = x.i0 + (warp + WARPS - c_turn) % WARPS;
+            c_end = x.i1;
+            c_turn = (c_turn + x.i1 - x.i0) % WARPS;
         }
-        const bool seen = PAGED || (c_i < c_keys.sink_tiles ? c_t < c_keys.first : c_t >= c_keys.lo && c_t < c_keys.n);
-        c_page = seen ? static_cast<int>(ldg32(c_table + in_table(c_t))) : -1;
+        const int stop = c_i < c_keys.sink_tiles ? min(c_keys.sink_tiles, c_end) : c_end;
+        c_left = (stop - c_i + WARPS - 1) / WARPS;
+        c_t = c_keys.first_token(c_i) + (PAGED ? 0 : my_token);
+        c_last = c_t + (c_left - 1) * (WARPS * TOK);
+        c_i += c_left * WARPS;
+        c_page = page_of();
     };
     auto copy_next = [&](uint32_t to) {
-        if (c_i < c_run) {
-            const int t = c_t;
-            const bool live = static_cast<unsigned>(c_page) < static_cast<unsigned>(p.blocks);
-            const uint32_t from = live ? static_cast<uint32_t>(c_page) : 0u;
-            if (PAGED) {
-                const uint32_t row = static_cast<uint32_t>(t) & static_cast<uint32_t>(p.page_size - 1), block = static_cast<uint32_t>(p.code_block);
-                const uint8_t* k = c_k + static_cast<uint64_t>(from) * block + static_cast<uint64_t>(row) * code_token;
-                const uint8_t* v = c_v + static_cast<uint64_t>(from) * block + static_cast<uint64_t>(row) * code_token;
+        if (c_left == 0) new_run();
+        const bool live = static_cast<unsigned>(c_page) < static_cast<unsigned>(p.blocks);
+        const uint32_t from = live ? static_cast<uint32_t>(c_page) : 0u;
+        if (PAGED) {
+            // (pages follow one another: a place's number times the tokens' distance)
+            const uint32_t row = static_cast<uint32_t>(c_t) & static_cast<uint32_t>(p.page_size - 1);
+            const uint64_t off = static_cast<uint64_t>(from * static_cast<uint32_t>(p.page_size) + row) * code_token;
+            const uint8_t *k = c_k + off, *v = c_v + off;
 #pragma unroll
-                for (int j = 0; j < TOK / ROWS; ++j) {
-                    copy16(to + dst_at[j], k + static_cast<uint64_t>(code_token) * (j * ROWS), !live);
-                    copy16(to + dst_at[j] + S::TILE, v + static_cast<uint64_t>(code_token) * (j * ROWS), !live);
-                }
-                copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + static_cast<uint64_t>(from) * static_cast<uint32_t>(p.scale_block) + static_cast<uint64_t>(row) * scale_token, !live);
-            } else {
-                const int row = t - in_table(t) * p.page_size;
-                const long long off = live ? from * p.code_block + row * p.code_token : 0;
-#pragma unroll
-                for (int j = 0; j < TOK / ROWS; ++j) {
-                    const long long at = __shfl_sync(0xffffffffu, off, j * ROWS + lrow);
-                    const bool none = !__shfl_sync(0xffffffffu, static_cast<int>(live), j * ROWS + lrow);
-                    copy16(to + dst_at[j], c_k + at, none);
-                    copy16(to + dst_at[j] + S::TILE, c_v + at, none);
-                }
-                copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + (live ? from * p.scale_block + row * p.scale_token : 0), !live);
+            for (int j = 0; j < TOK / ROWS; ++j) {
+                copy16(to + dst_at[j], k, !live);
+                copy16(to + dst_at[j] + S::TILE, v, !live);
+                k += code_rows;
+                v += code_rows;
             }
-            advance();
+            copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + (static_cast<uint64_t>(from) * static_cast<uint32_t>(p.scale_block) + row * static_cast<uint32_t>(S::SB)), !live);
+        } else {
+            const int row = c_t - in_table(c_t) * p.page_size;
+            const long long off = live ? from * p.code_block + row * p.code_token : 0;
+#pragma unroll
+            for (int j = 0; j < TOK / ROWS; ++j) {
+                const long long at = __shfl_sync(0xffffffffu, off, j * ROWS + lrow);
+                const bool none = !__shfl_sync(0xffffffffu, static_cast<int>(live), j * ROWS + lrow);
+                copy16(to + dst_at[j], c_k + at, none);
+                copy16(to + dst_at[j] + S::TILE, c_v + at, none);
+            }
+            copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + (live ? from * p.scale_block + row * p.scale_token : 0), !live);
         }
         copy_commit();
+        --c_left;
+        c_t = c_t < c_last ? c_t + WARPS * TOK : c_last;   // (no further than a token whose page the table has)
+        c_page = page_of();
     };
-    advance();
 #pragma unroll 1
     for (int a = 0; a < STAGES - 1; ++a) copy_next(ring + a * S::STAGE);
 
@@ -966,7 +977,12 @@ int launch(const Params& p, int grid, cudaStream_t stream) {
     using S = Shape<BITS, D>;
     const int smem = warps_of(D, NH) * stages_of(S::STAGE, D, NH) * S::STAGE + behind_rings(D, NH);
     const auto fn = decode_kernel<BITS, D, NH, PAGED>;
-    TDIST_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<bool> opted_in[64];   // (for each instance of this template)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !opted_in[dev]) {
+        TDIST_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (dev >= 0 && dev < 64) opted_in[dev] = true;
+    }
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
@@ -1055,7 +1071,8 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.page_size = c.page_size;
     int l = 0;
     while ((1ll << l) < c.page_size) ++l;
-    const bool paged = c.page_size == 1 << l && l >= 4 && ((c.code_block | c.code_token | c.scale_block | c.scale_token) >> 32) == 0;
+    const bool paged = c.page_size == 1 << l && l >= 4 && c.code_block == c.code_token * c.page_size && c.scale_token == 4 * (c.bits == 8 ? 1 : c.head_dim / 64) &&
+                       ((c.code_token | c.scale_block | static_cast<long long>(c.blocks) * c.page_size) >> 32) == 0;
     // PAGED: t >> l. Otherwise, with 2^l >= page_size, the multiplier ceil(2^(31 + l) / page_size) is off by less than one, so its product with
     // t < 2^31 by less than 2^31, and the quotient's fraction is at most 1 - 1 / page_size
     p.page_shift = paged ? l : 31 + l;

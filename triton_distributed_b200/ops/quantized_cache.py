@@ -354,7 +354,7 @@ def _decode_parts(B: int, per_b: int, most: int, table_keys: int, asked: int, sl
     if asked > 0:
         return (asked, 0) if asked <= 8 else ((0, max(1, min(slots // per_b, B * asked))) if may_share else (8, 0))
     splits = max(1, min(slots // max(1, B * per_b), -(-most // 256)))
-    if may_share and (splits > 8 or (most >= 1024 and B * per_b * most > slots * 2048)):
+    if may_share and ((splits > 8 and most > 8 * 768) or (most >= 1024 and B * per_b * most > slots * 2048)):
         return 0, max(1, slots // per_b)
     return min(splits, 8), 0
 
