@@ -67,7 +67,7 @@ struct Params {
     void* out;
     long long code_block, code_token, code_head, scale_block, scale_head, scale_token;   // bytes
     int B, shares;                 // shares: groups of CTAs that share all tiles equally, 0: `splits` CTAs per segment
-    int Hq, Hkv, head_tiles, page_size, page_shift, max_blocks, blocks, splits, window, sinks, table_keys, is_f16;
+    int Hq, Hkv, head_tiles, page_size, page_shift, max_blocks, blocks, splits, window, sinks, table_keys;
     float scale, soft_cap;
     uint32_t page_mul;             // not PAGED: t / page_size = (t page_mul) >> page_shift for t < 2^31
 };
@@ -98,13 +98,24 @@ __device__ __forceinline__ void mma_u8s8_from(int (&d)[4], int c0, int c1, uint3
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
 }
-// A byte or nibble n under the exponent of 1024 is the fp16 number 1024 + n; in the upper nibble of a byte, 1024 + 16 n.
-constexpr uint32_t kMagic = 0x64006400u;
-constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a 0x64
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) { return hsub2(__byte_perm(w, kMagic, sel), 0x64806480u); }   // - 1152
-__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return hsub2((w & 0x000f000fu) | kMagic, 0x64086408u); }                     // - 1032: n - 8
-// 16 (n - 8): the rows of the MMA that take it are off by that factor until the end (a multiply-add here has two constants to keep in registers)
-__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return hsub2((w & 0x00f000f0u) | kMagic, 0x64806480u); }                     // - 1152
+// Codes as operands of the fp16 MMA, exactly. Plain: a byte or nibble n alone is fp16's subnormal n 2^-24, and in the upper nibble of a byte n 2^-20; the sums
+// have the codes' offset in them, which is taken off at the end. FINE: under the exponent of 1024 it is 1024 + n or 1024 + 16 n, and a subtraction leaves
+// n - 128, n - 8 or 16 (n - 8). Rows of the MMA that take an upper nibble are off by 16 until the end.
+template <bool FINE>
+__device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t offset) {
+    if constexpr (FINE) return hsub2(w, offset);
+    return w;
+}
+constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a byte of `magic`
+template <bool FINE>
+constexpr uint32_t magic = FINE ? 0x64006400u : 0u;
+template <bool FINE>
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) { return centred<FINE>(__byte_perm(w, magic<FINE>, sel), 0x64806480u); }
+template <bool FINE>
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return centred<FINE>((w & 0x000f000fu) | magic<FINE>, 0x64086408u); }
+template <bool FINE>
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return centred<FINE>((w & 0x00f000f0u) | magic<FINE>, 0x64806480u); }
+__host__ __device__ constexpr uint32_t offset_of(int bits) { return bits == 8 ? 0x00800080u : 0x00080008u; }   // 128 or 8, as such subnormals
 __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
     return __byte_perm(__byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(b), 0x0040u), __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(d), 0x0040u), 0x5410u);
 }
@@ -260,7 +271,7 @@ struct Pieces {
     }
 };
 
-template <int BITS, int D, int NH, bool PAGED>
+template <int BITS, int D, int NH, bool PAGED, bool F16>
 __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) decode_kernel(const __grid_constant__ Params p) {
     using S = Shape<BITS, D>;
     constexpr int WARPS = warps_of(D, NH), THREADS = 32 * WARPS, BUFS = buffers_of(D, NH);
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
     const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
-    const bool fine = p.is_f16 != 0;   // 8 bits: weights as two fp16 numbers, which costs little beside the loads (fp16 results: error 3.0e-4 with one)
+    constexpr bool FINE = F16;   // see centred(); 8 bits: weights as two fp16 numbers, which costs little beside the loads (error 3.0e-4 with one)
     uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
     int turn = 0;            // the warp that has a piece's first tile: tiles go round the warps from piece to piece
     bool first_piece = true;
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
             const Words<E / 2> w = load_words<E / 2>(static_cast<const char*>(p.q) + (head0 + (there ? head : 0)) * (D * 2) + lane * (E * 2));
 #pragma unroll
             for (int e = 0; e < E / 2; ++e) {
-                if (p.is_f16) {
+                if (F16) {
                     const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w.w[e]));
                     f[2 * e] = t.x;
                     f[2 * e + 1] = t.y;
@@ -553,7 +564,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
     // ---- sums: O^T in units of `unit` (a power of two), columns are heads 8 h + 2 c + {0, 1}
     float o[NH][S::MT][4];
     float limit[NH][2], m_use[NH][2], l_run[NH][2];   // weights are relative to 2^m_use; it is raised when a score passes `limit`
-    float low[NH][2][S::NG];       // 4 bits: sum of p least, of this lane's tokens
+    float low[NH][2][S::NG];       // 4 bits: sum of p (least + 8 step), of this lane's tokens
+    float off[NH][(S::NG + 1) / 2][4];   // not fine: of the weights times the codes' offset: in rows 0 .. 7 those of even groups, in 8 .. 15 of odd ones
     float unit = 0.f, inv_unit = 0.f;
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
@@ -566,6 +578,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) low[h][r][k] = 0.f;
         }
+#pragma unroll
+        for (int j = 0; j < (S::NG + 1) / 2; ++j) off[h][j][0] = off[h][j][1] = off[h][j][2] = off[h][j][3] = 0.f;
     }
 
     for (int i = i0; i < i1; i += WARPS) {
@@ -701,6 +715,11 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                         o[h][j][r] *= both;
                         o[h][j][2 + r] *= both;
                     }
+#pragma unroll
+                    for (int j = 0; j < (S::NG + 1) / 2; ++j) {
+                        off[h][j][r] *= both;
+                        off[h][j][2 + r] *= both;
+                    }
                 }
         }
 #pragma unroll
@@ -725,7 +744,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                 const uint32_t a = pack_f16x2(w0, w1), bb = pack_f16x2(w2, w3);
                 pb[h][k][0] = movmatrix_trans(a);
                 pb[h][k][1] = movmatrix_trans(bb);
-                if (BITS == 8 && fine) {
+                if (BITS == 8 && FINE) {
                     // what the rounding left
                     const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&a)), rb = __half22float2(*reinterpret_cast<const __half2*>(&bb));
                     pl[h][0] = movmatrix_trans(pack_f16x2(w0 - ra.x, w1 - ra.y));
@@ -739,6 +758,15 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
+        if (!FINE) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int k = 0; k < S::NG; ++k) {
+                    const uint32_t even = k & 1 ? 0u : offset_of(BITS), odd = k & 1 ? offset_of(BITS) : 0u;
+                    mma_f16(off[h][k / 2], even, odd, even, odd, pb[h][k][0], pb[h][k][1]);
+                }
+        }
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) {
             constexpr int last = S::NG - 1;
@@ -752,12 +780,12 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         const uint32_t a = m ? a23 : a01, bb = m ? b23 : b01;
-                        const uint32_t x0 = bytes_to_half2(a, kLowBytes), x1 = bytes_to_half2(a, kHighBytes);
-                        const uint32_t x2 = bytes_to_half2(bb, kLowBytes), x3 = bytes_to_half2(bb, kHighBytes);
+                        const uint32_t x0 = bytes_to_half2<FINE>(a, kLowBytes), x1 = bytes_to_half2<FINE>(a, kHighBytes);
+                        const uint32_t x2 = bytes_to_half2<FINE>(bb, kLowBytes), x3 = bytes_to_half2<FINE>(bb, kHighBytes);
 #pragma unroll
                         for (int h = 0; h < NH; ++h) {
                             mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
-                            if (fine) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pl[h][0], pl[h][1]);
+                            if (FINE) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pl[h][0], pl[h][1]);
                         }
                     }
                 } else {
@@ -767,8 +795,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
                         const uint32_t a = __byte_perm(w0, w1, half ? 0x7632u : 0x5410u), bb = __byte_perm(w2, w3, half ? 0x7632u : 0x5410u);
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
-                            const uint32_t x0 = low_nibbles(a >> (8 * m)), x1 = high_nibbles(a >> (8 * m));
-                            const uint32_t x2 = low_nibbles(bb >> (8 * m)), x3 = high_nibbles(bb >> (8 * m));
+                            const uint32_t x0 = low_nibbles<FINE>(a >> (8 * m)), x1 = high_nibbles<FINE>(a >> (8 * m));
+                            const uint32_t x2 = low_nibbles<FINE>(bb >> (8 * m)), x3 = high_nibbles<FINE>(bb >> (8 * m));
 #pragma unroll
                             for (int h = 0; h < NH; ++h)
                                 mma_f16(o[h][j * (S::VD / 2) + w * 4 + half * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
@@ -784,6 +812,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 
     // ---- the warps' sums, in the values' units
     float m_run[NH][2];
+    const float up = FINE ? 1.f : 16777216.f;   // 2^24
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -804,8 +833,11 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 #pragma unroll
                 for (int k = 0; k < S::VD / 2; ++k) {
                     const int m = j * (S::VD / 2) + k;
+                    const float offset = off[h][min(j, S::NG - 1) / 2][(min(j, S::NG - 1) & 1) * 2 + r];
+                    o[h][m][r] = (o[h][m][r] - offset) * up;
+                    o[h][m][2 + r] = (o[h][m][2 + r] * (BITS == 8 ? 1.f : 0.0625f) - offset) * up;
                     o[h][m][r] = o[h][m][r] * unit + add;
-                    o[h][m][2 + r] = o[h][m][2 + r] * (BITS == 8 ? unit : unit * 0.0625f) + add;
+                    o[h][m][2 + r] = o[h][m][2 + r] * unit + add;
                 }
             }
         }
@@ -896,7 +928,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
             }
             // a sum of weights that is not positive: no keys (zeros), or a NaN among the scores
             const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-            const uint32_t w = p.is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
+            const uint32_t w = F16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
             *reinterpret_cast<uint32_t*>(static_cast<char*>(p.out) + (head0 * D + base + idx) * 2) = w;
         }
     } else if (p.shares > 0 && (x.i0 > 0 || x.i1 < keys.tiles)) {
@@ -911,7 +943,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
             const int head = idx / D;
             const float l = l_s[0][head], inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
             const float a0 = sums_s[head * OP + idx % D], a1 = sums_s[head * OP + idx % D + 1];
-            const uint32_t w = p.is_f16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
+            const uint32_t w = F16 ? pack_f16x2(a0 * inv, a1 * inv) : pack_bf16x2(a0 * inv, a1 * inv);
             *reinterpret_cast<uint32_t*>(static_cast<char*>(p.out) + (head0 * D + idx) * 2) = w;
         }
     }
@@ -923,7 +955,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH), ctas_per_sm(D, NH)) deco
 // first piece is in CTA info.z / 2 (its last piece where info.z is odd), the others are the first ones of every per_b-th CTA from c to info.w.
 // Four threads per two dimensions.
 template <int D>
-__global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const int4* info, int per_b, int heads, int is_f16, void* out) {
+__global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const int4* info, int per_b, int heads, bool is_f16, void* out) {
     constexpr int GROUPS = 4;
     __shared__ float a_s[GROUPS][D], l_s[GROUPS], m_s[GROUPS];
     pdl_wait_and_release();
@@ -971,12 +1003,12 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const i
     *reinterpret_cast<uint32_t*>(static_cast<char*>(out) + ((static_cast<size_t>(x.x) + h) * D + d) * 2) = w;
 }
 
-template <int BITS, int D, int NH, bool PAGED>
+template <int BITS, int D, int NH, bool PAGED, bool F16>
 int launch(const Params& p, int grid, cudaStream_t stream) {
     const int cluster = p.shares == 0 ? p.splits : 1;
     using S = Shape<BITS, D>;
     const int smem = warps_of(D, NH) * stages_of(S::STAGE, D, NH) * S::STAGE + behind_rings(D, NH);
-    const auto fn = decode_kernel<BITS, D, NH, PAGED>;
+    const auto fn = decode_kernel<BITS, D, NH, PAGED, F16>;
     static std::atomic<bool> opted_in[64];   // (for each instance of this template)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !opted_in[dev]) {
@@ -1001,19 +1033,24 @@ int launch(const Params& p, int grid, cudaStream_t stream) {
     return 0;
 }
 
-template <int BITS, int D>
+template <int BITS, int D, bool F16>
 int launch_heads(const Params& p, int nh, bool paged, int grid, cudaStream_t stream) {
     // heads of 256 take one tile of query heads: two would need more registers than there are
     if constexpr (D != 256) {
-        if (nh == 2) return paged ? launch<BITS, D, 2, true>(p, grid, stream) : launch<BITS, D, 2, false>(p, grid, stream);
+        if (nh == 2) return paged ? launch<BITS, D, 2, true, F16>(p, grid, stream) : launch<BITS, D, 2, false, F16>(p, grid, stream);
     }
-    return paged ? launch<BITS, D, 1, true>(p, grid, stream) : launch<BITS, D, 1, false>(p, grid, stream);
+    return paged ? launch<BITS, D, 1, true, F16>(p, grid, stream) : launch<BITS, D, 1, false, F16>(p, grid, stream);
+}
+
+template <int BITS, bool F16>
+int launch_dim(const Params& p, int head_dim, int nh, bool paged, int grid, cudaStream_t stream) {
+    return head_dim == 64 ? launch_heads<BITS, 64, F16>(p, nh, paged, grid, stream)
+                          : (head_dim == 128 ? launch_heads<BITS, 128, F16>(p, nh, paged, grid, stream) : launch_heads<BITS, 256, F16>(p, nh, paged, grid, stream));
 }
 
 template <int BITS>
-int launch_dim(const Params& p, int head_dim, int nh, bool paged, int grid, cudaStream_t stream) {
-    return head_dim == 64 ? launch_heads<BITS, 64>(p, nh, paged, grid, stream)
-                          : (head_dim == 128 ? launch_heads<BITS, 128>(p, nh, paged, grid, stream) : launch_heads<BITS, 256>(p, nh, paged, grid, stream));
+int launch_type(const Params& p, int head_dim, int nh, bool paged, bool f16, int grid, cudaStream_t stream) {
+    return f16 ? launch_dim<BITS, true>(p, head_dim, nh, paged, grid, stream) : launch_dim<BITS, false>(p, head_dim, nh, paged, grid, stream);
 }
 
 }  // namespace qdecode
@@ -1086,7 +1123,7 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.sinks = a->sinks;
     const long long keys = static_cast<long long>(c.max_blocks) * c.page_size;
     p.table_keys = static_cast<int>(keys < 0x7fffffc0ll ? keys : 0x7fffffc0ll);
-    p.is_f16 = c.dtype == TDIST_F16;
+    const bool f16 = c.dtype == TDIST_F16;
     p.scale = a->scale;
     p.soft_cap = a->soft_cap;
     const long long segments = static_cast<long long>(c.B) * c.Hkv * p.head_tiles, grid = p.shares > 0 ? static_cast<long long>(p.shares) * c.Hkv * p.head_tiles : segments * p.splits;
@@ -1099,8 +1136,8 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
         p.part += 4 * grid;
     }
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
-    const int rc = c.bits == 8 ? launch_dim<8>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream)
-                               : launch_dim<4>(p, c.head_dim, nh, paged, static_cast<int>(grid), stream);
+    const int rc = c.bits == 8 ? launch_type<8>(p, c.head_dim, nh, paged, f16, static_cast<int>(grid), stream)
+                               : launch_type<4>(p, c.head_dim, nh, paged, f16, static_cast<int>(grid), stream);
     if (rc) return rc;
     if (p.shares > 0) {
         const dim3 blocks(static_cast<unsigned>(grid), static_cast<unsigned>(8 * nh));
@@ -1108,9 +1145,9 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
         const float* part = p.part;
         const int4* info = p.info;
         cudaError_t e;
-        if (c.head_dim == 64) e = tdist_host::launch_pdl(merge_kernel<64>, blocks, 128, 0, stream, part, info, per_b, 8 * nh, p.is_f16, a->out);
-        else if (c.head_dim == 128) e = tdist_host::launch_pdl(merge_kernel<128>, blocks, 256, 0, stream, part, info, per_b, 8 * nh, p.is_f16, a->out);
-        else e = tdist_host::launch_pdl(merge_kernel<256>, blocks, 512, 0, stream, part, info, per_b, 8 * nh, p.is_f16, a->out);
+        if (c.head_dim == 64) e = tdist_host::launch_pdl(merge_kernel<64>, blocks, 128, 0, stream, part, info, per_b, 8 * nh, f16, a->out);
+        else if (c.head_dim == 128) e = tdist_host::launch_pdl(merge_kernel<128>, blocks, 256, 0, stream, part, info, per_b, 8 * nh, f16, a->out);
+        else e = tdist_host::launch_pdl(merge_kernel<256>, blocks, 512, 0, stream, part, info, per_b, 8 * nh, f16, a->out);
         TDIST_CUDA_OK(e);
     }
     return 0;
