@@ -183,6 +183,20 @@ def test_decode_parts_meet(bits, splits):
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("splits", [0, 1, 2, 40])
+@pytest.mark.parametrize("D,Hq,Hkv,page", [(64, 3, 3, 32), (64, 13, 1, 6), (128, 8, 1, 16), (128, 40, 2, 16), (256, 12, 1, 64), (256, 3, 1, 1)])
+def test_decode_ways_of_dealing_out(bits, dtype, splits, D, Hq, Hkv, page):
+    """Small CTAs, large ones, clusters and shares over the same sequences: ends inside a tile and at its border, none, one past the table."""
+    lens = [0, 1, 96, 403, 17, 10 ** 6]
+    table, blocks = _table(len(lens), -(-410 // page))
+    cache, _ = _fill(blocks, page, Hkv, D, bits, seed=12)
+    q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(13)).to(dtype)
+    _check_decode(q, cache, lens, table, kv_split=splits)
+    _check_decode(q, cache, lens, table, window=33, sinks=3, kv_split=splits)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("page", [1, 16, 24])
 @pytest.mark.parametrize("window,sinks,cap", [(1, 0, 0.0), (17, 4, 30.0), (100, 37, 0.0), (333, 1, 1000.0), (5000, 4, 5.0)])
 def test_decode_windows_and_caps(bits, page, window, sinks, cap):

@@ -494,7 +494,7 @@ typedef struct TdistQuantDecodeArgs {
     void* out;                   /* [B, Hq, D] */
     void* part;                  /* splits 0: fp32 [CTAs][4 + 2 x heads x (D + 2)], on 16 bytes; CTAs: shares x Hkv x tiles of heads (8, or 16 where Hq / Hkv > 8 and D < 256) */
     int Hq;
-    int splits;                  /* CTAs per (sequence, kv head), up to 8; 0: `shares` CTAs of each kv head take equal shares of all keys (up to 511 sequences) */
+    int splits;                  /* CTAs per (sequence, kv head), up to 8; 0: `shares` CTAs of each kv head take equal shares of all keys (up to 511 sequences); both 0: a small CTA each */
     int shares, window, sinks;
     float scale, soft_cap;
     long long scratch;           /* floats of `part` */

@@ -347,14 +347,25 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
 MOST_SHARED = 511   # sequences of a call whose keys are dealt out in shares
 
 
-def _decode_parts(B: int, per_b: int, most: int, table_keys: int, asked: int, slots: int):
-    """(splits, shares) of a decode over at most ``most`` keys per sequence, ``per_b`` CTAs side by side for a sequence's heads: CTAs per
-    sequence and head, or 0 and the CTAs that take equal shares of all sequences."""
+def _decode_parts(B: int, per_b: int, most: int, table_keys: int, asked: int, slots: int, wide: bool):
+    """(splits, shares) of a decode over at most ``most`` keys per sequence, ``per_b`` segments side by side for a sequence's heads; the machine
+    has room for ``slots`` large CTAs (``wide``: one per SM, otherwise two). CTAs per segment; or 0 and the CTAs that take equal shares of
+    all sequences; or 0, 0: a small CTA per segment.
+
+    Small CTAs leave room for three (wide: two) times as many: a short segment is mostly latency and the meeting of its warps' sums (8 bits, heads
+    of 128, 8 of kv: 256 sequences of 512 keys 74.2 us with large CTAs, 58.8 with small ones, of 128 keys 42.6 and 22.2; 24 sequences
+    of 512 keys 10.3 and 10.9; wide, heads of 256, 500 sequences of 1024 keys 75.0 and 59.8, of 8192 ones 403 and 416). A cluster's 8
+    parts merge without a second kernel (one sequence, 4096 keys 10.3 us and 12.8 as shares, 8192 keys 14.4 and 13.7)."""
     may_share = B <= MOST_SHARED and B * (-(-table_keys // 16) + 2) < 1 << 31
+    segments = B * per_b
+    if asked == 0:
+        return 0, 0
     if asked > 0:
         return (asked, 0) if asked <= 8 else ((0, max(1, min(slots // per_b, B * asked))) if may_share else (8, 0))
-    splits = max(1, min(slots // max(1, B * per_b), -(-most // 256)))
-    if may_share and ((splits > 8 and most > 8 * 768) or (most >= 1024 and B * per_b * most > slots * 2048)):
+    if most <= (256 if segments <= slots else 4096 if wide else min(2048, 256 + segments)):
+        return 0, 0
+    splits = max(1, min(slots // max(1, segments), -(-most // 256)))
+    if may_share and ((splits > 8 and most > 8 * 768) or (most >= 1024 and segments * most > slots * 2048)):
         return 0, max(1, slots // per_b)
     return min(splits, 8), 0
 
@@ -366,7 +377,8 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
     """Decode attention of one query token per sequence over a quantised cache: the query of a sequence of n keys sees key j if
     j >= n - window or j < sinks (``window=None``: all keys). ``q [B, Hq, D]`` bf16 or fp16, contiguous; returns its shape and type. A
     query that sees no key (or none whose score is above -inf) gives zeros. Pages without a visible key are not read. ``kv_split``: parts of a
-    sequence's keys, up to 8; more: equal shares of all sequences' keys, as many as fit the machine; -1: chosen by sizes."""
+    sequence's keys, up to 8; more: equal shares of all sequences' keys, as many as fit the machine; 0: one part by few warps, for many short
+    sequences; -1: chosen by sizes."""
     window, sinks, scale, soft_cap = PA._settings(window, sinks, scale, soft_cap)
     key = (gqa_fwd_quantized_decode, _layout(cache, q, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
     args = _PLANS.get(key)
@@ -397,13 +409,14 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
         args.cache.B, args.cache.max_blocks = B, block_table.shape[1]
         args.Hq, args.window, args.sinks = Hq, PA.NO_WINDOW if window is None else window, sinks
         args.scale, args.soft_cap = factor, soft_cap
-        wide = Hq // Hkv > 8 and D != 256
+        two = Hq // Hkv > 8 and D != 256   # tiles of 8 query heads per segment
+        wide = two or D == 256
         most = min(cache.k.shape[1] * block_table.shape[1], args.window + sinks)
-        per_b = Hkv * -(-(Hq // Hkv) // (16 if wide else 8))
+        per_b = Hkv * -(-(Hq // Hkv) // (16 if two else 8))
         args.splits, args.shares = _decode_parts(B, per_b, most, cache.k.shape[1] * block_table.shape[1], kv_split,
-                                                 (1 if wide or D == 256 else 2) * FD._sm_count(q.device))
+                                                 (1 if wide else 2) * FD._sm_count(q.device), wide)
         # scratch of the shares: per CTA four words, and two times the sums of its heads
-        args.scratch = args.shares * per_b * (4 + 2 * (16 if wide else 8) * (D + 2))
+        args.scratch = args.shares * per_b * (4 + 2 * (16 if two else 8) * (D + 2))
         _remember(key, args)
     out = PA._output(out, q)
     if args.cache.B == 0:
@@ -415,7 +428,7 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
     if q.data_ptr() % 16:
         q = q.clone()
     a.q, a.out = q.data_ptr(), out.data_ptr()
-    if a.splits == 0:
+    if a.shares:
         part = torch.empty(a.scratch, dtype=torch.float32, device=q.device)
         a.part = part.data_ptr()
     _launch(_lib.lib().tdist_quant_decode, a, q.device, "tdist_quant_decode")
