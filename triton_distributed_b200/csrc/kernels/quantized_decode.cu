@@ -112,7 +112,7 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.page_size = c.page_size;
     int l = 0;
     while ((1ll << l) < c.page_size) ++l;
-    const bool paged = c.page_size == 1 << l && l >= 4 && ((c.code_block | c.code_token | c.scale_block | c.scale_token) >> 32) == 0;
+    const bool paged = c.page_size == 1 << l && l >= 4 && ((c.code_block | c.code_token | c.scale_block | c.scale_token << l) >> 32) == 0;
     // PAGED: t >> l. Otherwise, with 2^l >= page_size, the multiplier ceil(2^(31 + l) / page_size) is off by less than one, so its product with
     // t < 2^31 by less than 2^31, and the quotient's fraction is at most 1 - 1 / page_size
     p.page_shift = paged ? l : 31 + l;

@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
     const int* c_table = p.table;
     const uint8_t* c_k = p.k + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
     const uint8_t* c_v = p.v + kvh * p.code_head + lchunk * 16 + (PAGED ? lrow * p.code_token : 0);
+    const ptrdiff_t v_from_k = static_cast<ptrdiff_t>(reinterpret_cast<uintptr_t>(c_v) - reinterpret_cast<uintptr_t>(c_k));   // (an instruction less than two sums)
     // lanes 0..15 copy the scales of the keys, 16..31 of the values
     const char* c_s = (lane < 16 ? p.ks : p.vs) + kvh * p.scale_head + (PAGED ? my_token * p.scale_token : 0);
     // A run: tiles whose tokens follow one another (the first keys, or the window's). Tiles left of it, the next one's first token (not PAGED: this lane's),
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         if (PAGED) {
             const uint32_t row = static_cast<uint32_t>(c_t) & static_cast<uint32_t>(p.page_size - 1);
             const uint64_t off = static_cast<uint64_t>(from) * static_cast<uint32_t>(p.code_block) + static_cast<uint64_t>(row) * code_token;
-            const uint8_t *k = c_k + off, *v = c_v + off;
+            const uint8_t *k = c_k + off, *v = k + v_from_k;
 #pragma unroll
             for (int j = 0; j < TOK / ROWS; ++j) {
                 copy16(to + dst_at[j], k, !live);
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                 k += code_rows;
                 v += code_rows;
             }
-            copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + (static_cast<uint64_t>(from) * static_cast<uint32_t>(p.scale_block) + static_cast<uint64_t>(row) * static_cast<uint32_t>(p.scale_token)), !live);
+            copy_small<S::SB>(to + 2 * S::TILE + lane * S::SB, c_s + (static_cast<uint64_t>(from) * static_cast<uint32_t>(p.scale_block) + row * static_cast<uint32_t>(p.scale_token)), !live);
         } else {
             const int row = c_t - in_table(c_t) * p.page_size;
             const long long off = live ? from * p.code_block + row * p.code_token : 0;
