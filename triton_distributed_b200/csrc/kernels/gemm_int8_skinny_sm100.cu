@@ -4,6 +4,8 @@
 // tcgen05.mma (kind::i8), up to 128 tokens its N operand, and the K ranges of a tile (`split` of them) form a cluster whose CTAs
 // add their sums through shared memory, in 32-bit integers: exact in any order. CTA r of a cluster scales and writes the r-th share of the tokens.
 //
+// Measured: 16 x 6144 x 12288 17.0 us (75 MB, 11.6 at HBM's copy rate), 1 x 4096 x 4096 6.7 (2.6: start, one tile's latency, the exchange), 128 tokens 10.9.
+//
 // Warps (192 threads): 0 = TMA producer, 1 = MMA issuer and TMEM owner, 2..5 = epilogue. One tile per CTA, two CTAs per SM.
 #include <cuda.h>
 #include <cuda_runtime.h>

@@ -11,6 +11,10 @@
 // per stage, TMA fills 128-byte-swizzled stages, one thread of the leader issues the MMAs, sums lie in two TMEM slots of 256 columns.
 // What follows the product differs: an epilogue thread owns a row, so SA is one number per thread, and SB four columns per load, from L1.
 //
+// Measured, quantised inputs: 8192 x 14336 x 16384 1184 - 1290 us with the clock, 3.0 - 3.25 POP/s, twice the bf16 GEMM's measured rate at best; 8192 x 14336 x 4096
+// 371 us. Below that rounds bound it: 1000 x 5504 x 4096 32 us, 14 of them MMAs at their full rate: one round of 60 items of 256 x 384 on 74 pairs, its
+// prologue and its exposed epilogue.
+//
 // Warps (192 threads): 0 = TMA producer, 1 = MMA issuer and TMEM owner, 2..5 = epilogue (TMEM -> scale -> swizzled smem -> TMA store).
 #include <cuda.h>
 #include <cuda_runtime.h>

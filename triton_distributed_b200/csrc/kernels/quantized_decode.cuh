@@ -13,8 +13,8 @@
 // A score is off by up to 2^-17 max |q| sum |k_d|: a 16-bit query against bf16's 8 bits.
 //
 // V. Codes become fp16, exactly, two tokens per register. Weights are divided by a power of two above all vs_j so far, so that p_j vs_j / S lies
-// in [0, 1] whatever the values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest. 4-bit codes are taken as
-// c - 8 with least + 8 step, so that the sums stay small.
+// in [0, 1] whatever the values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest; fp16 results over 8 bits take what the
+// rounding left as a second weight. 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
 // S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix, and every warp streams tiles of 16 tokens through a cp.async ring of its own.
@@ -25,12 +25,18 @@
 // way, warps waited for memory half of their time.
 //
 // Work. A segment is the keys of one (sequence, kv head, tile of query heads), cut into tiles of 16 tokens. Either a segment has `splits` CTAs, up to 8, a
-// cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); or the machine is filled once by groups of CTAs, one
+// cluster that exchanges slices of the sums (CTA r adds up the r-th slice of all parts); or, where there are many short ones, a small CTA of two or four
+// warps each; or the machine is filled once by groups of CTAs, one
 // for each segment of a sequence, and every group takes an equal share of all sequences' tiles in a row, from the lengths on the device: pieces
 // of sequences, of which the first and the last may be shared with other groups. Those leave their sums in a workspace, and a second kernel
 // adds them up. (The heads of a key lie side by side in memory, so they are read side by side: with shares dealt out head by head 4-bit rows of 64 bytes were
 // read from HBM twice, and 16 x 16384 keys took 107 us in 8 bits.) The copies run on from one piece to the next: while a piece's sums meet,
 // the next one's first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
+//
+// Measured, heads of 128, 8 of kv, 4 query heads each, 16 x 16384 keys: 8 bits 91.5 us, 6.05 TB/s of codes and scales, HBM. 4 bits 97 us where HBM would take
+// 46: issue slots, some 430 instructions per tile of 16 tokens, 62 % of the slots in use, the integer pipe 60 % (nibbles 72 instructions, scales 16). One
+// sequence of 4096 keys, 8 bits: 9.8 us, a chain of latencies: length, page, codes, merge.
+
 #pragma once
 
 #include <cuda_bf16.h>
@@ -84,11 +90,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
     return r;
 }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
@@ -100,24 +101,21 @@ __device__ __forceinline__ void mma_u8s8_from(int (&d)[4], int c0, int c1, uint3
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
 }
-// Codes as operands of the fp16 MMA, exactly. Plain: a byte or nibble n alone is fp16's subnormal n 2^-24, and in the upper nibble of a byte n 2^-20; the sums
-// have the codes' offset in them, which is taken off at the end. FINE: under the exponent of 1024 it is 1024 + n or 1024 + 16 n, and a subtraction leaves
-// n - 128, n - 8 or 16 (n - 8). Rows of the MMA that take an upper nibble are off by 16 until the end.
-template <bool FINE>
-__device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t offset) {
-    if constexpr (FINE) return hsub2(w, offset);
-    return w;
+// Codes as operands of the fp16 MMA, exactly. A byte n under the exponent of 1024 is 1024 + n, from which 1152 is taken. A nibble n alone is the subnormal n 2^-24,
+// and in the upper nibble of a byte n 2^-20: rows of the MMA that take those are off by 16 until the end, and the offset of 8 is taken off by a product of its
+// own with the same weights, one MMA for four subtractions (fp16, 64 ragged sequences to 16384 keys of 8 kv heads: 193 us, 210 with subtractions; 8 bits, whose
+// weights are two numbers in fp16 and would need two such products, 16 x 16384 keys 98 and 94). The sums stay small either way; with the offset
+// in them until the end, their roundings come to 1.5e-3 of a flat result over 524288 keys.
+constexpr uint32_t kMagic = 0x64006400u;
+constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a 0x64
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(w, kMagic, sel)), "r"(0x64806480u));
+    return r;
 }
-constexpr uint32_t kLowBytes = 0x7150u, kHighBytes = 0x7352u;   // bytes 0, 1 / 2, 3 of a word, each under a byte of `magic`
-template <bool FINE>
-constexpr uint32_t magic = FINE ? 0x64006400u : 0u;
-template <bool FINE>
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) { return centred<FINE>(__byte_perm(w, magic<FINE>, sel), 0x64806480u); }
-template <bool FINE>
-__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return centred<FINE>((w & 0x000f000fu) | magic<FINE>, 0x64086408u); }
-template <bool FINE>
-__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return centred<FINE>((w & 0x00f000f0u) | magic<FINE>, 0x64806480u); }
-__host__ __device__ constexpr uint32_t offset_of(int bits) { return bits == 8 ? 0x00800080u : 0x00080008u; }   // 128 or 8, as such subnormals
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return w & 0x00f000f0u; }
+constexpr uint32_t kLowOffset = 0x80088008u, kHighOffset = 0x80808080u;   // -8 2^-24, -8 2^-20
 __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
     return __byte_perm(__byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(b), 0x0040u), __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(d), 0x0040u), 0x5410u);
 }
@@ -480,7 +478,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
     const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
-    constexpr bool FINE = F16;   // see centred(); 8 bits: weights as two fp16 numbers, which costs little beside the loads (error 3.0e-4 with one)
+    constexpr bool FINE = BITS == 8 && F16;   // weights as two fp16 numbers, which costs little beside the loads (error 3.0e-4 with one)
     uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
     int turn = 0;            // the warp that has a piece's first tile: tiles go round the warps from piece to piece
     bool first_piece = true;
@@ -571,7 +569,6 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
     float o[NH][S::MT][4];
     float limit[NH][2], m_use[NH][2], l_run[NH][2];   // weights are relative to 2^m_use; it is raised when a score passes `limit`
     float low[NH][2][S::NG];       // 4 bits: sum of p (least + 8 step), of this lane's tokens
-    float off[NH][(S::NG + 1) / 2][4];   // not fine: of the weights times the codes' offset: in rows 0 .. 7 those of even groups, in 8 .. 15 of odd ones
     float unit = 0.f, inv_unit = 0.f;
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
@@ -584,8 +581,6 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) low[h][r][k] = 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < (S::NG + 1) / 2; ++j) off[h][j][0] = off[h][j][1] = off[h][j][2] = off[h][j][3] = 0.f;
     }
 
     for (int i = i0; i < i1; i += WARPS) {
@@ -721,11 +716,6 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                         o[h][j][r] *= both;
                         o[h][j][2 + r] *= both;
                     }
-#pragma unroll
-                    for (int j = 0; j < (S::NG + 1) / 2; ++j) {
-                        off[h][j][r] *= both;
-                        off[h][j][2 + r] *= both;
-                    }
                 }
         }
 #pragma unroll
@@ -750,7 +740,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                 const uint32_t a = pack_f16x2(w0, w1), bb = pack_f16x2(w2, w3);
                 pb[h][k][0] = movmatrix_trans(a);
                 pb[h][k][1] = movmatrix_trans(bb);
-                if (BITS == 8 && FINE) {
+                if (FINE) {
                     // what the rounding left
                     const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&a)), rb = __half22float2(*reinterpret_cast<const __half2*>(&bb));
                     pl[h][0] = movmatrix_trans(pack_f16x2(w0 - ra.x, w1 - ra.y));
@@ -764,13 +754,13 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
-        if (!FINE) {
+        if (BITS == 4) {
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int k = 0; k < S::NG; ++k) {
-                    const uint32_t even = k & 1 ? 0u : offset_of(BITS), odd = k & 1 ? offset_of(BITS) : 0u;
-                    mma_f16(off[h][k / 2], even, odd, even, odd, pb[h][k][0], pb[h][k][1]);
+                for (int m = 0; m < S::MT; ++m) {
+                    const int k = min(m / (S::VD / 2), S::NG - 1);
+                    mma_f16(o[h][m], kLowOffset, kHighOffset, kLowOffset, kHighOffset, pb[h][k][0], pb[h][k][1]);
                 }
         }
 #pragma unroll
@@ -786,8 +776,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         const uint32_t a = m ? a23 : a01, bb = m ? b23 : b01;
-                        const uint32_t x0 = bytes_to_half2<FINE>(a, kLowBytes), x1 = bytes_to_half2<FINE>(a, kHighBytes);
-                        const uint32_t x2 = bytes_to_half2<FINE>(bb, kLowBytes), x3 = bytes_to_half2<FINE>(bb, kHighBytes);
+                        const uint32_t x0 = bytes_to_half2(a, kLowBytes), x1 = bytes_to_half2(a, kHighBytes);
+                        const uint32_t x2 = bytes_to_half2(bb, kLowBytes), x3 = bytes_to_half2(bb, kHighBytes);
 #pragma unroll
                         for (int h = 0; h < NH; ++h) {
                             mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
@@ -801,8 +791,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                         const uint32_t a = __byte_perm(w0, w1, half ? 0x7632u : 0x5410u), bb = __byte_perm(w2, w3, half ? 0x7632u : 0x5410u);
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
-                            const uint32_t x0 = low_nibbles<FINE>(a >> (8 * m)), x1 = high_nibbles<FINE>(a >> (8 * m));
-                            const uint32_t x2 = low_nibbles<FINE>(bb >> (8 * m)), x3 = high_nibbles<FINE>(bb >> (8 * m));
+                            const uint32_t x0 = low_nibbles(a >> (8 * m)), x1 = high_nibbles(a >> (8 * m));
+                            const uint32_t x2 = low_nibbles(bb >> (8 * m)), x3 = high_nibbles(bb >> (8 * m));
 #pragma unroll
                             for (int h = 0; h < NH; ++h)
                                 mma_f16(o[h][j * (S::VD / 2) + w * 4 + half * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
@@ -818,7 +808,6 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 
     // ---- the warps' sums, in the values' units
     float m_run[NH][2];
-    const float up = FINE ? 1.f : 16777216.f;   // 2^24
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -839,9 +828,10 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
                 for (int k = 0; k < S::VD / 2; ++k) {
                     const int m = j * (S::VD / 2) + k;
-                    const float offset = off[h][min(j, S::NG - 1) / 2][(min(j, S::NG - 1) & 1) * 2 + r];
-                    o[h][m][r] = (o[h][m][r] - offset) * up;
-                    o[h][m][2 + r] = (o[h][m][2 + r] * (BITS == 8 ? 1.f : 0.0625f) - offset) * up;
+                    if (BITS == 4) {
+                        o[h][m][r] *= 16777216.f;   // 2^24
+                        o[h][m][2 + r] *= 1048576.f;
+                    }
                     o[h][m][r] = o[h][m][r] * unit + add;
                     o[h][m][2 + r] = o[h][m][2 + r] * unit + add;
                 }
