@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ..runtime import default_timeout_ns, global_status, stream_ptr
+from ..runtime import default_timeout_ns, global_status
 from ..utils.profile import nvtx_range
 from .quantized_cache import LEAST, quotient
 
@@ -51,33 +51,39 @@ def _call(index, fn, *args):
         return fn(*args)
 
 
-# What the checks found, by shapes, strides, types and devices (never by addresses or contents)
-_CHECKED: set = set()
+# What the checks found, by shapes, layouts, types and devices (never by addresses or contents): of a call's operands the arguments that they settle
+_PLANS: dict = {}
 
 
-def _remember(key):
-    if len(_CHECKED) >= 4096:
-        _CHECKED.clear()
-    _CHECKED.add(key)
+def _remember(key, plan):
+    if len(_PLANS) >= 4096:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
 
 
 @nvtx_range("tdist.quantize_int8_rowwise")
 def quantize_int8_rowwise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x [M, K]`` (bf16, fp16 or fp32; rows any distance apart) to int8 and one fp32 scale per row; K a multiple of 16."""
     global launch_count
-    if x.dim() != 2 or x.shape[1] % 16 or x.shape[1] < 16:
-        raise ValueError(f"expected [M, K] with K a multiple of 16, got {tuple(x.shape)}")
-    if x.dtype not in _ROWS:
-        raise TypeError("rows must be bf16, fp16 or fp32")
-    if x.device.type != "cuda":
-        return ref_quantize_int8_rowwise(x)
-    M, K = x.shape
-    if x.stride(1) != 1 or (x.stride(0) * x.element_size()) % 16 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    codes, scale = x.new_empty((M, K), dtype=torch.int8), x.new_empty((M,), dtype=torch.float32)
+    index = x.get_device()
+    key = (x.shape, x.stride(), x.dtype)
+    plan = _PLANS.get(key) if index >= 0 else None
+    if plan is None:
+        if x.dim() != 2 or x.shape[1] % 16 or x.shape[1] < 16:
+            raise ValueError(f"expected [M, K] with K a multiple of 16, got {tuple(x.shape)}")
+        if x.dtype not in _ROWS:
+            raise TypeError("rows must be bf16, fp16 or fp32")
+        if x.device.type != "cuda":
+            return ref_quantize_int8_rowwise(x)
+        plan = _remember(key, (x.shape[0], x.shape[1], x.stride(0), _ROWS[x.dtype], x.stride(1) == 1 and (x.stride(0) * x.element_size()) % 16 == 0))
+    M, K, row, dtype, loads = plan
+    if not loads or x.data_ptr() % 16:
+        x, row = x.clone(memory_format=torch.contiguous_format), K
+    codes, scale = x.new_empty(M, K, dtype=torch.int8), x.new_empty(M, dtype=torch.float32)
     if M:
-        code = _call(x.get_device(), _lib.lib().tdist_quant_int8_rowwise, x.data_ptr(), x.stride(0), codes.data_ptr(), scale.data_ptr(), M, K,
-                     _ROWS[x.dtype], stream_ptr(x.device))
+        code = _call(index, _lib.lib().tdist_quant_int8_rowwise, x.data_ptr(), row, codes.data_ptr(), scale.data_ptr(), M, K, dtype,
+                     torch._C._cuda_getCurrentRawStream(index))
         if code:
             _lib.check(code, "tdist_quant_int8_rowwise")
         launch_count += 1
@@ -113,24 +119,27 @@ def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tens
     """``a [M, K]``, ``b [N, K]`` int8, ``sa [M]``, ``sb [N]`` fp32 -> ``[M, N]`` bf16 or fp16. K a multiple of 16, N of 8."""
     global launch_count
     index = a.get_device()
-    key = (a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype, b.get_device(), sa.shape, sa.stride(), sa.dtype, sa.get_device(), sb.shape, sb.stride(),
-           sb.dtype, sb.get_device(), index, out_dtype, None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
-    if index < 0 or key not in _CHECKED:
+    key = (a.shape, b.shape, sa.shape, sb.shape, a.dtype, b.dtype, sa.dtype, sb.dtype, index, b.get_device(), sa.get_device(), sb.get_device(),
+           a.is_contiguous() and b.is_contiguous() and sa.is_contiguous() and sb.is_contiguous(), out_dtype,
+           None if out is None else (out.shape, out.is_contiguous(), out.dtype, out.get_device()))
+    plan = _PLANS.get(key) if index >= 0 else None
+    if plan is None:
         _check(a, sa, b, sb, out_dtype, out)
-        _remember(key)
-    if index < 0:
-        c = ref_gemm_int8(a, sa, b, sb, out_dtype)
-        return c if out is None else out.copy_(c)
-    c = out if out is not None else a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
+        if index < 0:
+            c = ref_gemm_int8(a, sa, b, sb, out_dtype)
+            return c if out is None else out.copy_(c)
+        plan = _lib.GemmInt8Args()
+        plan.m, plan.n, plan.k, plan.dtype = a.shape[0], b.shape[0], a.shape[1], _OUT[out_dtype]
+        _remember(key, plan)
+    c = out if out is not None else a.new_empty(plan.m, plan.n, dtype=out_dtype)
     if c.numel() == 0:
         return c
-    g = _lib.GemmInt8Args()
+    g = _lib.GemmInt8Args.from_buffer_copy(plan)
     g.a, g.b, g.sa, g.sb, g.c = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), c.data_ptr()
-    g.m, g.n, g.k, g.dtype = a.shape[0], b.shape[0], a.shape[1], _OUT[out_dtype]
     st = global_status()
     g.status = st.device_ptr if st is not None else None
     g.timeout_ns = default_timeout_ns()
-    g.stream = stream_ptr(a.device)
+    g.stream = torch._C._cuda_getCurrentRawStream(index)
     code = _call(index, _lib.lib().tdist_gemm_int8, C.byref(g))
     if code:
         _lib.check(code, "tdist_gemm_int8")

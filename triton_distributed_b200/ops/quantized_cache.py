@@ -33,7 +33,6 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import _lib
-from ..runtime import stream_ptr
 from ..utils.profile import nvtx_range
 from . import flash_decode as FD
 from . import paged_attention as PA
@@ -228,47 +227,48 @@ def _cache_args(cache: QuantizedKVCache, dtype) -> "_lib.QuantCacheArgs":
     return a
 
 
-def _layout(cache: QuantizedKVCache, *others):
-    """What a plan is found by: codes and scales of k and v have to be alike, so theirs are compared and k's told."""
+def _of(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype, t.get_device()
+
+
+def _layout(cache: QuantizedKVCache):
+    """What a plan is found by, the device last: codes and scales of k and v have to be alike, so theirs are compared and k's told."""
     k, v, ks, vs = cache
-    same = (k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and ks.shape == vs.shape and ks.stride() == vs.stride()
-            and ks.dtype == vs.dtype and k.get_device() == v.get_device() == ks.get_device() == vs.get_device())
-    return (same, k.shape, k.stride(), k.dtype, ks.shape, ks.stride(), ks.dtype, k.get_device()) + tuple(
-        x for t in others for x in (t.shape, t.stride(), t.dtype, t.get_device()))
+    codes, scales = _of(k), _of(ks)
+    return _of(v) == codes and _of(vs) == scales, codes, scales, codes[3]
 
 
-def _point(a, cache: QuantizedKVCache):
-    a.k_codes, a.v_codes, a.k_scales, a.v_scales = cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scales.data_ptr(), cache.v_scales.data_ptr()
-    a.stream = stream_ptr(cache.k.device)
+def _plain(*ints):
+    return all(t.dtype == torch.int32 and t.is_contiguous() for t in ints)
 
 
-def _launch(fn, a, device, what):
-    """The native call with ``device`` as the current one."""
+def _point(a, cache: QuantizedKVCache, index: int):
+    k, v, ks, vs = cache
+    a.k_codes, a.v_codes, a.k_scales, a.v_scales = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
+    a.stream = torch._C._cuda_getCurrentRawStream(index)
+
+
+def _launch(fn, a, index: int, what: str):
+    """The native call with device ``index`` as the current one."""
     global launch_count
-    if device.index == torch._C._cuda_getDevice():
+    if index == torch._C._cuda_getDevice():
         code = fn(C.byref(a))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             code = fn(C.byref(a))
     if code:
         _lib.check(code, what)
     launch_count += 1
 
 
-def _aligned(x):
-    """x [T, Hkv, D] with rows on 16 bytes."""
-    if x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
 @nvtx_range("tdist.kv_cache_write")
 def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantises ``k, v [T, Hkv, D]`` (bf16 or fp16; views of a fused projection are read in place) into their places ``slots [T]``.
     What the slots do not name keeps its bytes."""
-    layout = _layout(cache, k, v, slots)
-    args = _PLANS.get((kv_cache_write, layout))
-    if args is None:
+    layout = _layout(cache)
+    key = (kv_cache_write, layout, _of(k), _of(v), _of(slots))
+    plan = _PLANS.get(key)
+    if plan is None:
         _check_cache(cache)
         want = (slots.shape[0] if slots.dim() else 0, cache.k.shape[2], cache.head_dim)
         if k.shape != want or v.shape != want:
@@ -283,18 +283,23 @@ def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, sl
             return
         args = _cache_args(cache, k.dtype)
         args.rows = k.shape[0]
-        _remember((kv_cache_write, layout), args)
+        args.k_token, args.k_head, args.v_token, args.v_head = 2 * k.stride(0), 2 * k.stride(1), 2 * v.stride(0), 2 * v.stride(1)
+        # rows are loaded by 16 bytes
+        plan = _remember(key, (args, _plain(slots), all(x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 for x in (k, v))))
+    args, plain, loads = plan
     if args.rows == 0 or args.blocks == 0:
         return
     a = _lib.QuantCacheArgs.from_buffer_copy(args)
-    if slots.dtype != torch.int32:
+    if not plain:
         # no place of the cache is beyond 32 bits, but a slot may be
-        slots = slots.clamp(-1, 0x7FFFFFFF).to(torch.int32)
-    slots, k, v = slots.contiguous(), _aligned(k), _aligned(v)
+        slots = slots.clamp(-1, 0x7FFFFFFF).to(torch.int32).contiguous()
+    if not loads or (k.data_ptr() | v.data_ptr()) % 16:
+        k, v = (x.clone(memory_format=torch.contiguous_format) for x in (k, v))
+        a.k_token = a.v_token = 2 * a.Hkv * a.head_dim
+        a.k_head = a.v_head = 2 * a.head_dim
     a.k, a.v, a.slots = k.data_ptr(), v.data_ptr(), slots.data_ptr()
-    a.k_token, a.k_head, a.v_token, a.v_head = 2 * k.stride(0), 2 * k.stride(1), 2 * v.stride(0), 2 * v.stride(1)
-    _point(a, cache)
-    _launch(_lib.lib().tdist_quant_cache_write, a, cache.k.device, "tdist_quant_cache_write")
+    _point(a, cache, layout[-1])
+    _launch(_lib.lib().tdist_quant_cache_write, a, layout[-1], "tdist_quant_cache_write")
 
 
 def _int32(t):
@@ -309,9 +314,10 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
     sequence are zeros."""
     rows = int(rows)
     given = () if out is None else tuple(out)
-    key = (kv_cache_read, _layout(cache, starts, kv_lens, block_table, *given), rows, dtype)
-    args = _PLANS.get(key)
-    if args is None:
+    layout = _layout(cache)
+    key = (kv_cache_read, layout, _of(starts), _of(kv_lens), _of(block_table), rows, dtype, given and tuple(map(_of, given)))
+    plan = _PLANS.get(key)
+    if plan is None:
         _check_cache(cache)
         if rows < 0 or rows >= 1 << 31:
             raise ValueError("rows must lie in [0, 2^31)")
@@ -327,20 +333,22 @@ def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.
             return ref if out is None else (given[0].copy_(ref[0]), given[1].copy_(ref[1]))
         args = _cache_args(cache, dtype)
         args.rows, args.B, args.max_blocks = rows, B, block_table.shape[1]
-        _remember(key, args)
+        plan = _remember(key, (args, _plain(starts, kv_lens, block_table)))
+    args, plain = plan
     if out is None:
-        shape = (rows, args.Hkv, args.head_dim)
-        k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
+        k = cache.k.new_empty(rows, args.Hkv, args.head_dim, dtype=dtype)
+        v = torch.empty_like(k)
     else:
         k, v = given
     if rows == 0:
         return k, v
     a = _lib.QuantCacheArgs.from_buffer_copy(args)
-    starts, lens, table = _int32(starts), _int32(kv_lens), _int32(block_table)
-    a.starts, a.lens, a.table = starts.data_ptr(), lens.data_ptr(), table.data_ptr()
+    if not plain:
+        starts, kv_lens, block_table = _int32(starts), _int32(kv_lens), _int32(block_table)
+    a.starts, a.lens, a.table = starts.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr()
     a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
-    _point(a, cache)
-    _launch(_lib.lib().tdist_quant_cache_read, a, cache.k.device, "tdist_quant_cache_read")
+    _point(a, cache, layout[-1])
+    _launch(_lib.lib().tdist_quant_cache_read, a, layout[-1], "tdist_quant_cache_read")
     return k, v
 
 
@@ -380,9 +388,10 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
     sequence's keys, up to 8; more: equal shares of all sequences' keys, as many as fit the machine; 0: one part by few warps, for many short
     sequences; -1: chosen by sizes."""
     window, sinks, scale, soft_cap = PA._settings(window, sinks, scale, soft_cap)
-    key = (gqa_fwd_quantized_decode, _layout(cache, q, kv_lens, block_table), window, sinks, scale, soft_cap, kv_split)
-    args = _PLANS.get(key)
-    if args is None:
+    layout = _layout(cache)
+    key = (gqa_fwd_quantized_decode, layout, _of(q), _of(kv_lens), _of(block_table), window, sinks, scale, soft_cap, kv_split)
+    plan = _PLANS.get(key)
+    if plan is None:
         _check_cache(cache)
         if q.dim() != 3 or q.shape[2] != cache.head_dim:
             raise ValueError("q must be [B, Hq, D] with the cache's head_dim")
@@ -417,19 +426,22 @@ def gqa_fwd_quantized_decode(q: torch.Tensor, cache: QuantizedKVCache, kv_lens: 
                                                  (1 if wide else 2) * FD._sm_count(q.device), wide)
         # scratch of the shares: per CTA four words, and two times the sums of its heads
         args.scratch = args.shares * per_b * (4 + 2 * (16 if two else 8) * (D + 2))
-        _remember(key, args)
-    out = PA._output(out, q)
-    if args.cache.B == 0:
-        return out
+        plan = _remember(key, (args, _plain(kv_lens, block_table)))
+    args, plain = plan
+    out = torch.empty_like(q) if out is None else PA._output(out, q)
     a = _lib.QuantDecodeArgs.from_buffer_copy(args)
-    lens, table = _int32(kv_lens), _int32(block_table)
-    _point(a.cache, cache)
-    a.cache.lens, a.cache.table = lens.data_ptr(), table.data_ptr()
+    if a.cache.B == 0:
+        return out
+    if not plain:
+        kv_lens, block_table = _int32(kv_lens), _int32(block_table)
+    c = a.cache
+    _point(c, cache, layout[-1])
+    c.lens, c.table = kv_lens.data_ptr(), block_table.data_ptr()
     if q.data_ptr() % 16:
         q = q.clone()
     a.q, a.out = q.data_ptr(), out.data_ptr()
     if a.shares:
         part = torch.empty(a.scratch, dtype=torch.float32, device=q.device)
         a.part = part.data_ptr()
-    _launch(_lib.lib().tdist_quant_decode, a, q.device, "tdist_quant_decode")
+    _launch(_lib.lib().tdist_quant_decode, a, layout[-1], "tdist_quant_decode")
     return out
