@@ -9,11 +9,12 @@
 // its MMAs are those of the bf16 GEMM with K / 2, and the kernel is built like that one's CTA-pair tilings (gemm_sm100.cu): a cluster of two CTAs
 // computes 256 x bn (narrow) or 256 x 2 bn (WIDE, both halves sharing the A rows through the collector), K advances 128 bytes
 // per stage, TMA fills 128-byte-swizzled stages, one thread of the leader issues the MMAs, sums lie in two TMEM slots of 256 columns.
-// What follows the product differs: an epilogue thread owns a row, so SA is one number per thread, and SB four columns per load, from L1.
+// What follows the product differs: an epilogue thread owns a row, so SA is one number per thread, and SB of a tile's columns is
+// fetched into shared memory while the product is made (from L1 and L2 as it was needed: 2048 x 14336 x 256 56 us).
 //
-// Measured, quantised inputs: 8192 x 14336 x 16384 1184 - 1290 us with the clock, 3.0 - 3.25 POP/s, twice the bf16 GEMM's measured rate at best; 8192 x 14336 x 4096
-// 371 us. Below that rounds bound it: 1000 x 5504 x 4096 32 us, 14 of them MMAs at their full rate: one round of 60 items of 256 x 384 on 74 pairs, its
-// prologue and its exposed epilogue.
+// Measured, quantised inputs: 8192 x 14336 x 16384 1159 - 1196 us with the clock, 3.2 - 3.3 POP/s, twice the bf16 GEMM's measured rate; 8192 x 14336 x 4096
+// 330 us, 4096^3 51. Below that rounds bound it: 1000 x 5504 x 4096 24 us, 14 of them MMAs at their full rate: one round of 60 items of 256 x 384 on 74
+// pairs, its prologue and its exposed epilogue.
 //
 // Warps (192 threads): 0 = TMA producer, 1 = MMA issuer and TMEM owner, 2..5 = epilogue (TMEM -> scale -> swizzled smem -> TMA store).
 #include <cuda.h>
@@ -35,7 +36,7 @@ constexpr int A_BYTES = BM * BK;
 constexpr int EPI_COLS = 64, EPI_BYTES = BM * EPI_COLS * 2;
 constexpr int PIPE_BYTES = 192 * 1024;
 constexpr int SMEM_TILES = PIPE_BYTES + 2 * EPI_BYTES;
-constexpr int SMEM_BYTES = SMEM_TILES + 1024 + 256;
+constexpr int SMEM_BYTES = SMEM_TILES + 1024 + 256 + BN * 4;   // alignment, barriers, the scales of a tile's columns
 constexpr int THREADS = 192, TMEM_COLS = 512, MAX_STAGES = 6, GROUP_M = 8;
 constexpr int kKernelGemmInt8 = 10;
 
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_int8_kernel(const __grid_cons
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SMEM_TILES);   // full, empty, tmem full (2), tmem empty (2)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * MAX_STAGES + 4);
+    float* sb_s = reinterpret_cast<float*>(smem + SMEM_TILES + 256);   // [BN]
     const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
     const int cta_rank = static_cast<int>(cluster_ctarank());
     const int unit = static_cast<int>(blockIdx.x) >> 1, units = static_cast<int>(gridDim.x) >> 1;
@@ -209,10 +211,16 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_int8_kernel(const __grid_cons
             const float sa = row + row_in_tile < p.m ? p.sa[row + row_in_tile] : 0.f;
             for (int h = 0; h < w.halves; ++h) {
                 const uint32_t slot = w.halves == 2 ? static_cast<uint32_t>(h) : next;
+                const int col = (w.n_tile + h) * p.bn;
+                // the columns' scales, while the product is made (the barriers of the last chunk say that they have been read)
+                for (int i = 2 * row_in_tile; i < p.bn; i += 256) {
+                    const float2 sb = col + i < p.n ? *reinterpret_cast<const float2*>(p.sb + col + i) : make_float2(0.f, 0.f);   // N is a multiple of 8
+                    *reinterpret_cast<float2*>(sb_s + i) = sb;
+                }
+                named_barrier(1, 128);
                 mbar_wait(bar_tfull(slot), uses[slot] & 1u, p.wctx, 5);
                 tc_fence_after();
                 ++uses[slot];
-                const int col = (w.n_tile + h) * p.bn;
 #pragma unroll 1
                 for (int c = 0; c < p.bn / EPI_COLS; ++c) {
                     uint32_t r[2][32];
@@ -229,11 +237,10 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_int8_kernel(const __grid_cons
                     uint4 o[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int at = col + c * EPI_COLS + 8 * j;
                         uint32_t v[4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float4 sb = at < p.n ? *reinterpret_cast<const float4*>(p.sb + at + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);   // N is a multiple of 8
+                            const float4 sb = *reinterpret_cast<const float4*>(sb_s + c * EPI_COLS + 8 * j + 4 * i);
                             const uint32_t* x = r[j >> 2] + 8 * (j & 3) + 4 * i;
                             const float f0 = static_cast<float>(static_cast<int>(x[0])) * sa * sb.x, f1 = static_cast<float>(static_cast<int>(x[1])) * sa * sb.y;
                             const float f2 = static_cast<float>(static_cast<int>(x[2])) * sa * sb.z, f3 = static_cast<float>(static_cast<int>(x[3])) * sa * sb.w;
@@ -318,8 +325,10 @@ int resident(bool wide) {
     return result;
 }
 
-// The tiling whose rounds end soonest, by the times of a 128-byte K block that the bf16 kernel of the same shape has (a narrow tile 290 ns + 0.36
-// per column, a wide one 175 + 2.1 per column of a half), and the few-row kernel where its estimate is lower.
+// The tiling whose rounds end soonest, by measured times of a 128-byte K block, and the few-row kernel where its estimate is lower. A narrow tile takes
+// 250 ns + 0.25 per column, a wide one 110 + 2.05 per column of a half and 1.5 us more per tile; a product of more than 150 us runs into the power cap, where
+// the narrow tiles' second reading of A tells: 310 + 0.36, and 175 + 2.1 and 3 us (us, wide and narrow tiles of 256: 256 x 14336 x 4096 20.6, 18.2; 4096^3 53.7,
+// 50.9; 8192 x 14336 x 4096 334.6, 329.7; 8192 x 14336 x 16384 1195, 1287; 1000 x 5504 x 4096 29.2, 27.2, of 192 24.1, 26.7).
 Plan make_plan(const TdistGemmInt8Args* a) {
     using namespace tdist::int8;
     Plan best;
@@ -327,6 +336,7 @@ Plan make_plan(const TdistGemmInt8Args* a) {
     double best_s = 1e30;
     const int k_blocks = (a->k + BK - 1) / BK;
     const double hbm_s = (static_cast<double>(a->n) * a->k + static_cast<double>(a->m) * a->k + 2.0 * a->m * a->n) / 6.3e12;
+    const bool lasts = 2.0 * a->m * a->n * a->k > 5e11;
     for (int wide = 1; wide >= 0; --wide)
         for (int bn = BN; bn >= 128; bn -= 64) {
             Plan c;
@@ -340,10 +350,12 @@ Plan make_plan(const TdistGemmInt8Args* a) {
             const int units = resident(wide) / 2, most = wide ? 2 * c.num_items : c.num_items;
             c.grid = 2 * (units < most ? units : most);
             const int u = c.grid / 2, full = c.num_items / u, rest = c.num_items - full * u;
-            const double narrow_s = k_blocks * (290 + 0.36 * bn) * 1e-9 + 0.3e-6, whole_s = wide ? k_blocks * (175 + 2.1 * bn) * 1e-9 + 3e-6 : narrow_s;
-            const double sm_s = full * whole_s + (rest == 0 ? 0.0 : (wide && 2 * rest <= u ? narrow_s : whole_s));
+            const double narrow_s = k_blocks * (lasts ? 310 + 0.36 * bn : 250 + 0.25 * bn) * 1e-9 + 0.3e-6;
+            const double wide_s = k_blocks * (lasts ? 175 + 2.1 * bn : 110 + 2.05 * bn) * 1e-9 + (lasts ? 3e-6 : 1.5e-6);
+            const double whole_s = wide ? wide_s : narrow_s;
+            const double sm_s = full * whole_s + (rest == 0 ? 0.0 : (wide && 2 * rest <= u ? narrow_s + 1.5e-6 : whole_s));
             const double t = (sm_s > hbm_s ? sm_s : hbm_s) + 5e-6;
-            if (t < 0.96 * best_s) {
+            if (t < 0.98 * best_s) {
                 best_s = t;
                 best = c;
             }
