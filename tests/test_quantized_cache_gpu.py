@@ -5,7 +5,8 @@ Bound of the attention, per element, with A = sum_j p_j |v_j| / sum_j p_j, vmax 
 * a weight times its value's scale is rounded to fp16: 2^-11 of itself, or 2^-25 of a unit that is at most four times the largest scale
   (the next power of two above it, reached when the largest comes last): n 2^-23 vmax / sum p
 * a score is a sum of D / 16 fp32 steps that may truncate (2^-23 of the sum of |q_d k_d| scale each) and a few roundings of its own size, and its
-  exponential is good to 2^-21: both move weights and their sum, so twice. The same for 4 bits with |step c| + |least| in the place of |k_d|.
+  exponential is good to 2^-21: both move weights and their sum, so twice. The query is brought to 16 bits, rint(q 32512 / max |q|), which is off by
+  half a step, max |q| / 65024 < 2^-15.98 max |q|, in each dimension: that times the sum of |k_d| scale is a score's share. The same for 4 bits with |step c| + |least| in the place of |k_d|.
 """
 import math
 
@@ -64,7 +65,8 @@ def _check_decode(q, cache, lens, table, window=None, sinks=0, scale=None, soft_
         p = torch.exp(t - t.amax(-1, keepdim=True))
         l = p.sum(-1, keepdim=True)
         ref, A = p @ vb / l, p @ vab / l
-        moved = 2 * ((D / 16 + 6) * 2.0 ** -23 * size + (2.0 ** -20 * soft_cap if soft_cap > 0 else 0.0) + 2.0 ** -20)
+        query = 2.0 ** -15.98 * qq.abs().amax(-1, keepdim=True) * kab.sum(-1).amax(-1).view(-1, 1, 1) * abs(scale)
+        moved = 2 * (query + (D / 16 + 6) * 2.0 ** -23 * size + (2.0 ** -20 * soft_cap if soft_cap > 0 else 0.0) + 2.0 ** -20)
         tol = HALF[q.dtype] * ref.abs() + (2.0 ** -11 + moved) * 1.01 * A + at.numel() * 2.0 ** -23 * vab.amax() / l + 2.0 ** -24
         err = (got[b].double().view(Hkv, -1, D) - ref).abs()
         assert bool((err <= tol).all()), (b, n, float(err.max()), float((err / tol).max()))

@@ -10,11 +10,11 @@
 // per eight. A query is brought to 16 bits for it, rint(q 32512 / max |q|), as a high and a low byte with a product each: the sums are exact, the second
 // continues from 256 times the first, and 128 times the sum of q takes the codes' offset off. (As fp16 operands the codes of a tile cost 64
 // instructions, and the kernel was bound by its issue slots: 567 per tile of 16 x 128, 32 x 16384 keys of 8 kv heads 148 us.)
-// A score is off by up to 2^-17 max |q| sum |k_d|: a 16-bit query against bf16's 8 bits.
+// A score is off by up to 2^-16 max |q| sum |k_d| scale: a 16-bit query against bf16's 8 bits.
 //
 // V. Codes become fp16, exactly, two tokens per register. Weights are divided by a power of two above all vs_j so far, so that p_j vs_j / S lies
-// in [0, 1] whatever the values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest; fp16 results over 8 bits take what the
-// rounding left as a second weight. 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
+// in [0, 1] whatever the values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest; for fp16 results what that
+// rounding left is a second weight (without it errors of 3.0e-4 of a result where its own rounding is 2.1e-4). 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
 // S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix, and every warp streams tiles of 16 tokens through a cp.async ring of its own.
@@ -60,8 +60,7 @@ constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
 // Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled. 8 bits: a
 // weight times its scale is rounded whatever its size, and 2^8 is far below fp16's largest. 4 bits: none, as the largest weight, 1, times a step of 8
-// bits is exact, which is most of a result that few keys make up (64 heads on 8, 16384 keys, fp16: error 2.7e-4 of the result, 3.8e-4
-// with a slack of 2^8, of which 2.1e-4 the result's own rounding; 16 x 16384 keys 102 and 100 us).
+// bits is exact, which is most of a result that few keys make up (16 x 16384 keys 102 us, 100 with a slack of 2^8).
 __host__ __device__ constexpr float slack_of(int bits) { return bits == 8 ? 8.f : 0.f; }
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -478,7 +477,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
         for (int j = 0; j < S::VC; ++j) v_at[r][j] = S::TILE + S::at(token_of(2 * c + r), j * S::VB + g * (S::VB / 8));   // tokens 8 further on: 8 rows
     const float cap_inv = p.soft_cap > 0.f ? 1.f / p.soft_cap : 0.f;
-    constexpr bool FINE = BITS == 8 && F16;   // weights as two fp16 numbers, which costs little beside the loads (error 3.0e-4 with one)
+    constexpr bool FINE = F16;   // weights as two fp16 numbers, what the first one's rounding leaves in the second
     uint32_t stage = ring, free_stage = ring + (STAGES - 1) * S::STAGE;
     int turn = 0;            // the warp that has a piece's first tile: tiles go round the warps from piece to piece
     bool first_piece = true;
@@ -723,7 +722,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
             for (int k = 0; k < S::NG; ++k) vmul[r][k] *= inv_unit;
         // ---- P^T times the scales as the second operand: tokens in pairs per lane, heads over lane / 4
-        uint32_t pb[NH][S::NG][2], pl[NH][2];
+        uint32_t pb[NH][S::NG][2], pl[NH][S::NG][2];
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
             const float p0 = exp2f(s[h][0] - m_use[h][0]), p1 = exp2f(s[h][1] - m_use[h][1]);
@@ -741,10 +740,14 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                 pb[h][k][0] = movmatrix_trans(a);
                 pb[h][k][1] = movmatrix_trans(bb);
                 if (FINE) {
-                    // what the rounding left
                     const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&a)), rb = __half22float2(*reinterpret_cast<const __half2*>(&bb));
-                    pl[h][0] = movmatrix_trans(pack_f16x2(w0 - ra.x, w1 - ra.y));
-                    pl[h][1] = movmatrix_trans(pack_f16x2(w2 - rb.x, w3 - rb.y));
+                    const float l0 = w0 - ra.x, l1 = w1 - ra.y, l2 = w2 - rb.x, l3 = w3 - rb.y;
+                    pl[h][k][0] = movmatrix_trans(pack_f16x2(l0, l1));
+                    pl[h][k][1] = movmatrix_trans(pack_f16x2(l2, l3));
+                    if (BITS == 4) {   // their codes' offset
+                        low[h][0][k] -= 8.f * unit * (l0 + l2);
+                        low[h][1][k] -= 8.f * unit * (l1 + l3);
+                    }
                 }
             }
         }
@@ -781,7 +784,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
                         for (int h = 0; h < NH; ++h) {
                             mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
-                            if (FINE) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pl[h][0], pl[h][1]);
+                            if (FINE) mma_f16(o[h][j * (S::VD / 2) + w * 2 + m], x0, x1, x2, x3, pl[h][min(j, last)][0], pl[h][min(j, last)][1]);
                         }
                     }
                 } else {
@@ -794,8 +797,10 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                             const uint32_t x0 = low_nibbles(a >> (8 * m)), x1 = high_nibbles(a >> (8 * m));
                             const uint32_t x2 = low_nibbles(bb >> (8 * m)), x3 = high_nibbles(bb >> (8 * m));
 #pragma unroll
-                            for (int h = 0; h < NH; ++h)
+                            for (int h = 0; h < NH; ++h) {
                                 mma_f16(o[h][j * (S::VD / 2) + w * 4 + half * 2 + m], x0, x1, x2, x3, pb[h][min(j, last)][0], pb[h][min(j, last)][1]);
+                                if (FINE) mma_f16(o[h][j * (S::VD / 2) + w * 4 + half * 2 + m], x0, x1, x2, x3, pl[h][min(j, last)][0], pl[h][min(j, last)][1]);
+                            }
                         }
                     }
                 }
