@@ -33,7 +33,7 @@
 // read from HBM twice, and 16 x 16384 keys took 107 us in 8 bits.) The copies run on from one piece to the next: while a piece's sums meet,
 // the next one's first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
 //
-// Measured, heads of 128, 8 of kv, 4 query heads each, 16 x 16384 keys: 8 bits 91.5 us, 6.05 TB/s of codes and scales, HBM. 4 bits 97 us where HBM would take
+// Measured, heads of 128, 8 of kv, 4 query heads each, 16 x 16384 keys: 8 bits 93 us, 5.95 TB/s of codes and scales, HBM. 4 bits 95 us where HBM would take
 // 46: issue slots, some 430 instructions per tile of 16 tokens, 62 % of the slots in use, the integer pipe 60 % (nibbles 72 instructions, scales 16). One
 // sequence of 4096 keys, 8 bits: 9.8 us, a chain of latencies: length, page, codes, merge.
 
@@ -58,10 +58,9 @@ namespace qdecode {
 
 constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
-// Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled. 8 bits: a
-// weight times its scale is rounded whatever its size, and 2^8 is far below fp16's largest. 4 bits: none, as the largest weight, 1, times a step of 8
-// bits is exact, which is most of a result that few keys make up (16 x 16384 keys 102 us, 100 with a slack of 2^8).
-__host__ __device__ constexpr float slack_of(int bits) { return bits == 8 ? 8.f : 0.f; }
+// Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled: a weight times its
+// scale is rounded whatever its size, and 2^8 is far below fp16's largest (4 bits, 16 x 16384 keys 94.7 us, 97.6 without).
+constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -102,7 +101,7 @@ __device__ __forceinline__ void mma_u8s8_from(int (&d)[4], int c0, int c1, uint3
 }
 // Codes as operands of the fp16 MMA, exactly. A byte n under the exponent of 1024 is 1024 + n, from which 1152 is taken. A nibble n alone is the subnormal n 2^-24,
 // and in the upper nibble of a byte n 2^-20: rows of the MMA that take those are off by 16 until the end, and the offset of 8 is taken off by a product of its
-// own with the same weights, one MMA for four subtractions (fp16, 64 ragged sequences to 16384 keys of 8 kv heads: 193 us, 210 with subtractions; 8 bits, whose
+// own with the same weights, one MMA for four subtractions (64 ragged sequences to 16384 keys of 8 kv heads 193 us, 210 with subtractions; 8 bits, whose
 // weights are two numbers in fp16 and would need two such products, 16 x 16384 keys 98 and 94). The sums stay small either way; with the offset
 // in them until the end, their roundings come to 1.5e-3 of a flat result over 524288 keys.
 constexpr uint32_t kMagic = 0x64006400u;
@@ -704,7 +703,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     const float m_old = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r], m_new = fmaxf(m_old, mx);
                     m_use[h][r] = m_new == -CUDART_INF_F ? 0.f : m_new;
-                    limit[h][r] = m_new + slack_of(BITS);
+                    limit[h][r] = m_new + kSlack;
                     const float alpha = exp2f(m_old - m_use[h][r]);
                     l_run[h][r] *= alpha;
 #pragma unroll
