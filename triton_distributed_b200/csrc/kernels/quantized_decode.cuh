@@ -34,7 +34,7 @@
 // the next one's first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
 //
 // Measured, heads of 128, 8 of kv, 4 query heads each, 16 x 16384 keys: 8 bits 93 us, 5.95 TB/s of codes and scales, HBM. 4 bits 95 us where HBM would take
-// 46: issue slots, some 430 instructions per tile of 16 tokens, 62 % of the slots in use, the integer pipe 60 % (nibbles 72 instructions, scales 16). One
+// 46: issue slots and the integer pipe, 413 instructions per tile of 16 tokens (nibbles 72, scales 16). One
 // sequence of 4096 keys, 8 bits: 9.8 us, a chain of latencies: length, page, codes, merge.
 
 #pragma once

@@ -15,7 +15,7 @@ The format, per row of D values (one token's key or value of one head):
 
 So a key and value of 128 dimensions take 264 and 144 bytes where bf16 takes 512. A row (64 values) that holds a NaN or an infinity is
 stored with a scale of NaN: it reads as NaN, and so does the result of every query that sees it. Codes are exact in every product; a result
-differs from attention over the rows read back only by the roundings of the weights and of the result.
+differs from attention over the rows read back only by the roundings of the query to 16 bits, of the weights and of the result.
 
 Slots must differ, as a server's pages do: of two tokens with one slot either's codes may stay beside the other's scale. Tokens whose slot is
 no place of the cache (a negative one: padding) are left out. Lengths are cut to what the table has room for, and a page that the cache does not
