@@ -43,6 +43,13 @@ def test_results_are_the_statement_bit_for_bit(m, n, k, dtype):
     _check(*_operands(m, n, k, seed=m + n), dtype)
 
 
+@pytest.mark.parametrize("m,n,k", [(513, 3080, 2064), (2049, 4104, 528), (513, 7176, 1040), (2600, 7176, 4112), (2049, 4104, 4112), (1500, 5512, 144),
+                                   (6200, 5512, 144), (6200, 12296, 144)])
+def test_every_tiling(m, n, k):
+    """Narrow and wide tiles of 256, 192 and 128 columns: one round and more of them, a last one in halves, odd last tiles."""
+    _check(*_operands(m, n, k, seed=n), torch.bfloat16)
+
+
 @pytest.mark.parametrize("m", [5, 300])
 def test_the_longest_and_largest_sums(m):
     """-128 x -128 throughout at the largest K: 2147221504, 262144 below 2^31; cancelling sums beside them."""

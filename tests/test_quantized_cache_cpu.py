@@ -162,3 +162,19 @@ def test_refusals():
                       ({"table": table.float()}, TypeError), ({"out": q[:, :2]}, ValueError), ({"q": q.to("meta")}, ValueError)):
         with pytest.raises(error):
             decode(**kw)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_the_ways_a_decode_is_dealt_out_are_ones_the_kernel_has(wide):
+    """CTAs per sequence and head from 1 to 8, shares of at most 511 sequences that the machine has room for, or a small CTA each."""
+    slots = 148 if wide else 296
+    for B in (1, 2, 7, 64, 511, 512, 5000):
+        for per_b in (1, 3, 8, 64, 500):
+            for most in (0, 1, 17, 256, 1000, 6144, 6145, 524288, 1 << 30):
+                for asked in (-1, 0, 1, 8, 9, 1000):
+                    splits, shares = QC._decode_parts(B, per_b, most, max(most, 16), asked, slots, wide)
+                    assert 0 <= splits <= 8 and shares >= 0 and not (splits and shares)
+                    if shares:
+                        assert B <= QC.MOST_SHARED and (shares == 1 or shares * per_b <= slots)
+                    if 0 < asked <= 8:
+                        assert splits == asked
