@@ -1,0 +1,132 @@
+"""Attention over a quantised cache where weights, values and scores lie far apart, against 64 bits.
+
+Bound per element, with p the weights relative to the largest, l their sum, A = sum p |v| / l:
+* half a step of the result's type, of itself (fp16: or half of its least step, 2^-25; results beyond its largest are infinite)
+* a weight times its value's scale (a group's step) is rounded to fp16: 2^-11 of itself, or 2^-25 of a unit that is at most 2^-5 of the largest such product of
+  that group; codes reach 127 (8): per key 2^-30 max_j(p_j scale_j) 127 / l (4 bits: 8 step for 127 scale)
+* scores move weights and their sum: the query's share 2^-15 max|q| sum |k_d| scale, 2^-23 (D / 16 + 6) of sum |q_d k_d| scale, the exponential 2^-20; sums of n / 16 fp32 steps
+"""
+import math
+
+import pytest
+import torch
+
+import triton_distributed_b200 as tdist
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _cache(k, v, bits, page=16):
+    """A sequence [n, Hkv, D] in a cache of its own, on the CPU, and its table."""
+    n, Hkv, D = k.shape
+    pages = -(-n // page)
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(n)).to(torch.int32).view(1, -1)
+    cache = tdist.create_quantized_kv_cache(pages, page, Hkv, D, bits, "cpu")
+    at = torch.arange(n)
+    tdist.kv_cache_write(cache, k, v, table[0].long()[at // page] * page + at % page)
+    return cache, table
+
+
+def _rows(cache, table, n, i):
+    """What is stored, in 64 bits: [Hkv, n, D]; |step c| + |least| of each; the product's size per unit of weight [Hkv, n, D]."""
+    page = cache.k.shape[1]
+    at = torch.arange(n)
+    pages, rows = table[0].long()[at // page], at % page
+    c, s = cache[i][pages, rows].transpose(0, 1), cache[2 + i].transpose(1, 2)[pages, rows].double().transpose(0, 1)
+    if cache.bits == 8:
+        v = (c.double() - 128.0) * s.unsqueeze(-1)
+        return v, v.abs(), (127.0 * s).unsqueeze(-1).expand_as(v)
+    c = torch.stack([c & 15, c >> 4], -1).flatten(-2).double().unflatten(-1, (-1, 64))
+    step, least = s[..., 0:1], s[..., 1:2]
+    return (c * step + least).flatten(-2), (c * step + least.abs()).flatten(-2), (8.0 * step).expand_as(c).flatten(-2)
+
+
+def _check(q, cache, table, n, scale=None, **kw):
+    got = tdist.gqa_fwd_quantized_decode(q.cuda(), tdist.QuantizedKVCache(*(t.cuda() for t in cache)), torch.tensor([n], dtype=torch.int32).cuda(), table.cuda(),
+                                         scale=scale, **kw).cpu()
+    D, Hkv = q.shape[2], cache.k.shape[2]
+    scale = D ** -0.5 if scale is None else scale
+    (k, ka, _), (v, va, size) = _rows(cache, table, n, 0), _rows(cache, table, n, 1)
+    qq = q[0].double().view(Hkv, -1, D)
+    t = qq @ k.transpose(1, 2) * scale
+    p = torch.exp(t - t.amax(-1, keepdim=True))
+    l = p.sum(-1, keepdim=True)
+    ref, A = p @ v / l, p @ va / l
+    # a score's error counts with the key's weight: what weighs nothing may be off by much
+    off = 2.0 ** -15 * qq.abs().amax(-1, keepdim=True) * ka.sum(-1).unsqueeze(1) * abs(scale) + (D / 16 + 6) * 2.0 ** -23 * (qq.abs() @ ka.transpose(1, 2)) * abs(scale)
+    moved = (p * torch.expm1(off + 2.0 ** -20)) @ va / l + (p * torch.expm1(off + 2.0 ** -20)).sum(-1, keepdim=True) / l * A
+    least = torch.stack([(p[..., None] * size.unsqueeze(1)[..., d:d + 64]).amax(2) for d in range(0, D, 64)], 2).flatten(2) * n * 2.0 ** -30 / l
+    tol = HALF[q.dtype] * ref.abs() + 1.01 * ((2.0 ** -11 + n / 16 * 2.0 ** -23) * A + moved + least) + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -120)
+    out = got[0].double().view(Hkv, -1, D)
+    most = torch.finfo(q.dtype).max
+    inf = out.abs() == math.inf                   # where the bound reaches beyond the type's range, and has to where it lies beyond
+    assert bool((out == ref.sign() * math.inf)[inf].all()) and bool((ref.abs() + tol > most)[inf].all()) and bool(inf[ref.abs() - tol > most].all())
+    err = (out - ref).abs().masked_fill(inf, 0.0)
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+    return got
+
+
+def _keys(n, G, D, scores, seed):
+    """Query heads of one kind and keys whose scores (scale 1 / D) are about `scores`, with some noise."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.where(torch.rand(1, 1, D, generator=g) < 0.5, -1.0, 1.0).expand(1, G, D) * (1.0 + torch.arange(G).view(1, G, 1) / 64)
+    k = q[:, :1] * scores.view(n, 1, 1) + 0.3 * torch.randn(n, 1, D, generator=g)
+    return q, k, torch.randn(n, 1, D, generator=g)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("split", [0, 1, 3, 40])
+@pytest.mark.parametrize("D,G,n", [(64, 3, 200), (128, 4, 700), (128, 12, 333), (256, 6, 500)])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+def test_a_large_value_without_weight(bits, dtype, split, D, G, n, where):
+    """One value 2^30 times the others, at a key that weighs e^-60: the others' sum is the result."""
+    at = {"first": 0, "middle": n // 2, "last": n - 1}[where]
+    scores = torch.zeros(n)
+    scores[at] = -60.0
+    q, k, v = _keys(n, G, D, scores, n + D)
+    v[at] *= 2.0 ** 30
+    _check(q.to(dtype).contiguous(), *_cache(k.bfloat16(), v.bfloat16(), bits), n, scale=1.0 / D, kv_split=split)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("gap,ratio", [(60.0, 30), (20.8, 30), (5.0, 30), (60.0, 80), (0.5, 20)])
+@pytest.mark.parametrize("least", [-60.0, 0.0])
+def test_scores_rise_past_large_values(bits, dtype, split, gap, ratio, least):
+    """Tile by tile scores rise by `gap` and values shrink by 2^ratio, down to 2^least: what was the largest product comes to nothing, or does not."""
+    n, D = 512, 128
+    step = torch.arange(n) // 96                # every warp of 6 takes part in each
+    q, k, v = _keys(n, 4, D, gap * step.float(), 3)
+    v = v * torch.exp2(60.0 - ratio * step.float()).clamp_min(2.0 ** least).view(n, 1, 1)
+    _check(q.to(dtype).contiguous(), *_cache(k.bfloat16(), v.bfloat16(), bits), n, scale=1.0 / D, kv_split=split)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,G", [(128, 4), (128, 16), (256, 8)])
+def test_groups_of_values_far_apart(dtype, D, G):
+    """4 bits: the dimensions of one group are 2^40 times those of another, which keeps its own."""
+    n = 300
+    q, k, v = _keys(n, G, D, torch.zeros(n), 5)
+    v = v * torch.exp2(40.0 * (torch.arange(D) // 64 % 2))
+    v[7, 0, :64] *= 2.0 ** 60
+    for j in (0, 64):
+        w = v.clone()
+        w[:, :, j:j + 64] *= 2.0 ** -40
+        _check(q.to(dtype).contiguous(), *_cache(k.bfloat16(), w.bfloat16(), 4), n, scale=1.0 / D)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_long_tail_of_small_weights(bits, dtype):
+    """One key of most of the weight whose value is nearly zero, and 65536 keys of 2^-26 each whose values are alike: their sum is the result."""
+    n, D = 65537, 64
+    scores = torch.full((n,), -26 * math.log(2.0))
+    scores[100] = 0.0
+    q, k, v = _keys(n, 2, D, scores, 6)
+    k = q[:, :1] * scores.view(n, 1, 1) + 0.0 * k
+    v = 1.0 + 0.01 * v
+    v[100] = 2.0 ** -20
+    _check(q.to(dtype).contiguous(), *_cache(k.bfloat16(), v.bfloat16(), bits), n, scale=1.0 / D, kv_split=8)

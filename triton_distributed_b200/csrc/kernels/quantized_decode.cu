@@ -19,14 +19,14 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const i
     const int group = static_cast<int>(threadIdx.x) / (D / 2), d = static_cast<int>(threadIdx.x) % (D / 2) * 2;
     const int c = static_cast<int>(blockIdx.x), count = (x.w - c) / per_b + 2;
     auto at = [&](int i) { return part + (static_cast<size_t>(i == 0 ? x.z : 2 * (c + (i - 1) * per_b)) * heads + h) * (D + 2); };
-    float m = -CUDART_INF_F, l = 0.f, a0 = 0.f, a1 = 0.f;
+    float m = kNoScore, l = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll 4
     for (int i = group; i < count; i += GROUPS) {
         const float* src = at(i);
         const float mi = src[D], li = src[D + 1];
         const float2 v = *reinterpret_cast<const float2*>(src + d);
-        const float m_new = fmaxf(m, mi), mu = m_new == -CUDART_INF_F ? 0.f : m_new;
-        const float fa = exp2f(m - mu), fb = exp2f(mi - mu);
+        const float m_new = fmaxf(m, mi);
+        const float fa = exp2f(m - m_new), fb = exp2f(mi - m_new);
         l = l * fa + li * fb;
         a0 = a0 * fa + v.x * fb;
         a1 = a1 * fa + v.y * fb;
@@ -40,14 +40,13 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const float* part, const i
     }
     __syncthreads();
     if (group != 0) return;
-    m = -CUDART_INF_F;
+    m = kNoScore;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, m_s[i]);
-    const float mu = m == -CUDART_INF_F ? 0.f : m;
     l = a0 = a1 = 0.f;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
-        const float f = exp2f(m_s[i] - mu);
+        const float f = exp2f(m_s[i] - m);
         l += l_s[i] * f;
         a0 += a_s[i][d] * f;
         a1 += a_s[i][d + 1] * f;

@@ -12,9 +12,11 @@
 // instructions, and the kernel was bound by its issue slots: 567 per tile of 16 x 128, 32 x 16384 keys of 8 kv heads 148 us.)
 // A score is off by up to 2^-16 max |q| sum |k_d| scale: a 16-bit query against bf16's 8 bits.
 //
-// V. Codes become fp16, exactly, two tokens per register. Weights are divided by a power of two above all vs_j so far, so that p_j vs_j / S lies
-// in [0, 1] whatever the values' magnitude: rounded to fp16 it is off by 2^-12 of itself, or 2^-25 of the largest; for fp16 results what that
-// rounding left is a second weight (without it errors of 3.0e-4 of a result where its own rounding is 2.1e-4). 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
+// V. Codes become fp16, exactly, two tokens per register. The weights p_j vs_j of a head (4 bits: p_j step_jg of a head and group) are held in units of a power of two
+// that follows the largest of them so far: 2^-5 of it or less where it is set, down again as the maximum of the scores rises. So they stay below 2^15 whatever the values' magnitude, and
+// rounded to fp16 one is off by 2^-11 of itself, or by 2^-25 of a unit, 2^-30 of the largest (one below 2^-126 is zero). In units of the largest scale, which may be one
+// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights costs 16 x 16384 keys in 4 bits 1 %, heads of 256 5 %.
+// For fp16 results what that rounding left is a second weight (without it errors of 3.0e-4 of a result where its own rounding is 2.1e-4). 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
 // S^T = K Q^T, O^T = V^T P^T, P transposed by movmatrix, and every warp streams tiles of 16 tokens through a cp.async ring of its own.
@@ -58,10 +60,14 @@ namespace qdecode {
 
 constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
-// Scores may pass the maximum that weights are relative to by this much (in powers of two) before it is raised and the sums are scaled: a weight times its
-// scale is rounded whatever its size, and 2^8 is far below fp16's largest (4 bits, 16 x 16384 keys 94.7 us, 97.6 without).
-constexpr float kSlack = 8.f;
+// The maximum that weights are relative to is raised, and the sums scaled, when two weights of a lane come to more than 2^8 (4 bits, 16 x 16384 keys 94.7 us, 97.6
+// where every higher score raises it). Before the first score it is fp32's lowest number.
+constexpr float kMostPair = 256.f, kNoScore = -3.4028234663852886e38f;
 constexpr float kLog2e = 1.4426950408889634f;
+// Units of weights: powers of two from 2^-110, far below the least scale there is, to 2^123, as biased exponents. A new one is at least 2^-5 and more
+// than 2^-6 of the largest weighted scale, which is looked for among products with 2^-20.
+constexpr int kLeastExponent = 17, kMostExponent = 250, kTopExponent = 20 - 5;
+constexpr float kLeastUnit = 7.703719777548943e-34f, kTopScale = 9.5367431640625e-07f;   // 2^-110, 2^-20
 
 struct Params {
     const void* q;                 // [B, Hq, D]
@@ -114,6 +120,8 @@ __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
 __device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return w & 0x00f000f0u; }
 constexpr uint32_t kLowOffset = 0x80088008u, kHighOffset = 0x80808080u;   // -8 2^-24, -8 2^-20
+// of a power of two whose inverse is a normal number too
+__device__ __forceinline__ float one_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
     return __byte_perm(__byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(b), 0x0040u), __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(d), 0x0040u), 0x5410u);
 }
@@ -565,19 +573,23 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 
     // ---- sums: O^T in units of `unit` (a power of two), columns are heads 8 h + 2 c + {0, 1}
     float o[NH][S::MT][4];
-    float limit[NH][2], m_use[NH][2], l_run[NH][2];   // weights are relative to 2^m_use; it is raised when a score passes `limit`
+    float m_run[NH][2], l_run[NH][2];   // weights are relative to 2^m_run, which is raised late
     float low[NH][2][S::NG];       // 4 bits: sum of p (least + 8 step), of this lane's tokens
-    float unit = 0.f, inv_unit = 0.f;
+    float inv_unit[NH][2][S::NG];  // 1 / unit
+    float seconds[NH][2][S::NG];   // 4 bits, FINE: sum of the second weights, in units, of this lane's tokens
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
 #pragma unroll
         for (int j = 0; j < S::MT; ++j) o[h][j][0] = o[h][j][1] = o[h][j][2] = o[h][j][3] = 0.f;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            limit[h][r] = -CUDART_INF_F;
-            m_use[h][r] = l_run[h][r] = 0.f;
+            m_run[h][r] = kNoScore;
+            l_run[h][r] = 0.f;
 #pragma unroll
-            for (int k = 0; k < S::NG; ++k) low[h][r][k] = 0.f;
+            for (int k = 0; k < S::NG; ++k) {
+                low[h][r][k] = seconds[h][r][k] = 0.f;
+                inv_unit[h][r][k] = one_over(kLeastUnit);
+            }
         }
     }
 
@@ -649,9 +661,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[h][e] = soft_cap(s[h][e] * kLog2e, s[h][e] * cap_inv, p.soft_cap * kLog2e);
         }
-        // ---- the values' scales, as weights in units of `unit`
+        // ---- the values' scales
         float vmul[2][S::NG], vleast[2][S::NG];
-        float most = 0.f;
         if (static_cast<unsigned>(i - whole0) >= whole) {
             const int t0 = keys.first_token(i);
             const bool sink = i < keys.sink_tiles;
@@ -673,26 +684,52 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
             for (int k = 0; k < S::NG; ++k) {
                 vmul[r][k] = __uint_as_float(BITS == 8 ? vscale[r].w[k] : vscale[r].w[k] << 16);
                 if (BITS == 4) vleast[r][k] = fmaf(8.f, vmul[r][k], __uint_as_float(vscale[r].w[k] & 0xffff0000u));
-                most = fmaxf(most, vmul[r][k]);
             }
+        // the values' codes, on their way while the weights are made
+        Words<S::VW> vw[4][S::VC];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
+        // ---- P^T times the scales, in units, as the second operand: tokens in pairs per lane, heads over lane / 4
+        float pr[NH][4], pair[NH][2], rest[NH][2][S::NG];
+        uint32_t pb[NH][S::NG][2], pl[NH][S::NG][2];
+        __half2 all;             // a sum of weights that is at least the largest
+        auto weights = [&]() {
+            all = __half2half2(__ushort_as_half(0));
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pr[h][e] = exp2f(s[h][e] - m_run[h][e & 1]);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) pair[h][r] = pr[h][r] + pr[h][2 + r];
+#pragma unroll
+                for (int k = 0; k < S::NG; ++k) {
+                    const float w0 = pr[h][0] * vmul[0][k] * inv_unit[h][0][k], w1 = pr[h][1] * vmul[0][k] * inv_unit[h][1][k];
+                    const float w2 = pr[h][2] * vmul[1][k] * inv_unit[h][0][k], w3 = pr[h][3] * vmul[1][k] * inv_unit[h][1][k];
+                    const uint32_t a = pack_f16x2(w0, w1), bb = pack_f16x2(w2, w3);
+                    all = __hadd2(all, __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bb)));
+                    pb[h][k][0] = movmatrix_trans(a);
+                    pb[h][k][1] = movmatrix_trans(bb);
+                    if (FINE) {
+                        const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&a)), rb = __half22float2(*reinterpret_cast<const __half2*>(&bb));
+                        const float l0 = w0 - ra.x, l1 = w1 - ra.y, l2 = w2 - rb.x, l3 = w3 - rb.y;
+                        pl[h][k][0] = movmatrix_trans(pack_f16x2(l0, l1));
+                        pl[h][k][1] = movmatrix_trans(pack_f16x2(l2, l3));
+                        rest[h][0][k] = l0 + l2;
+                        rest[h][1][k] = l1 + l3;
+                    }
+                }
+            }
+        };
+        weights();
+        bool again = !__hblt2(all, __half2half2(__ushort_as_half(0x7800)));   // 2^15 and above, infinities and NaN
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) higher |= s[h][e] > limit[h][e & 1];
-        higher |= most > unit;
-        if (__any_sync(0xffffffffu, higher)) {
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-            float shrink = 1.f;
-            if (most > unit) {
-                // the next power of two, whose inverse is a normal number too
-                const uint32_t e = min((__float_as_uint(most) >> 23) + 1u, 250u);
-                const float up = __uint_as_float(e << 23);
-                shrink = unit / up;
-                unit = up;
-                inv_unit = __uint_as_float((254u - e) << 23);
-            }
+            for (int r = 0; r < 2; ++r) again |= pair[h][r] > kMostPair;
+        if (__any_sync(0xffffffffu, again)) {
+            float alpha[NH][2];
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -701,61 +738,52 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float m_old = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r], m_new = fmaxf(m_old, mx);
-                    m_use[h][r] = m_new == -CUDART_INF_F ? 0.f : m_new;
-                    limit[h][r] = m_new + kSlack;
-                    const float alpha = exp2f(m_old - m_use[h][r]);
-                    l_run[h][r] *= alpha;
+                    mx = fmaxf(m_run[h][r], mx);
+                    alpha[h][r] = exp2f(m_run[h][r] - mx);
+                    m_run[h][r] = mx;
+                    l_run[h][r] *= alpha[h][r];
+                }
 #pragma unroll
-                    for (int k = 0; k < S::NG; ++k) low[h][r][k] *= alpha;
-                    const float both = alpha * shrink;
+            for (int h = 0; h < NH; ++h)
 #pragma unroll
-                    for (int j = 0; j < S::MT; ++j) {
-                        o[h][j][r] *= both;
-                        o[h][j][2 + r] *= both;
+                for (int r = 0; r < 2; ++r) {
+                    const float p0 = exp2f(s[h][r] - m_run[h][r]), p1 = exp2f(s[h][2 + r] - m_run[h][r]);
+#pragma unroll
+                    for (int k = 0; k < S::NG; ++k) {
+                        float top = fmaxf(p0 * (vmul[0][k] * kTopScale), p1 * (vmul[1][k] * kTopScale));   // (not beyond fp32)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const int e_alpha = static_cast<int>(__float_as_uint(alpha[h][r]) >> 23), e_old = 254 - static_cast<int>(__float_as_uint(inv_unit[h][r][k]) >> 23);
+                        const int e_new = min(max(max(static_cast<int>(__float_as_uint(top) >> 23) + kTopExponent, e_old + e_alpha - 127), kLeastExponent), kMostExponent);
+                        inv_unit[h][r][k] = __uint_as_float(static_cast<uint32_t>(254 - e_new) << 23);
+                        const int e_both = e_alpha + e_old - e_new;   // alpha times the old unit over the new one: below 2
+                        low[h][r][k] *= alpha[h][r];
+                        const float both = e_alpha > 0 && e_both > 0 ? __uint_as_float((__float_as_uint(alpha[h][r]) & 0x7fffffu) | static_cast<uint32_t>(e_both) << 23) : 0.f;
+                        seconds[h][r][k] *= both;
+#pragma unroll
+                        for (int j = k * (S::MT / S::NG); j < (k + 1) * (S::MT / S::NG); ++j) {
+                            o[h][j][r] *= both;
+                            o[h][j][2 + r] *= both;
+                        }
                     }
                 }
+            weights();
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int k = 0; k < S::NG; ++k) vmul[r][k] *= inv_unit;
-        // ---- P^T times the scales as the second operand: tokens in pairs per lane, heads over lane / 4
-        uint32_t pb[NH][S::NG][2], pl[NH][S::NG][2];
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            const float p0 = exp2f(s[h][0] - m_use[h][0]), p1 = exp2f(s[h][1] - m_use[h][1]);
-            const float p2 = exp2f(s[h][2] - m_use[h][0]), p3 = exp2f(s[h][3] - m_use[h][1]);
-            l_run[h][0] += p0 + p2;
-            l_run[h][1] += p1 + p3;
-#pragma unroll
-            for (int k = 0; k < S::NG; ++k) {
+            for (int r = 0; r < 2; ++r) {
+                l_run[h][r] += pair[h][r];
                 if (BITS == 4) {
-                    low[h][0][k] += p0 * vleast[0][k] + p2 * vleast[1][k];
-                    low[h][1][k] += p1 * vleast[0][k] + p3 * vleast[1][k];
-                }
-                const float w0 = p0 * vmul[0][k], w1 = p1 * vmul[0][k], w2 = p2 * vmul[1][k], w3 = p3 * vmul[1][k];
-                const uint32_t a = pack_f16x2(w0, w1), bb = pack_f16x2(w2, w3);
-                pb[h][k][0] = movmatrix_trans(a);
-                pb[h][k][1] = movmatrix_trans(bb);
-                if (FINE) {
-                    const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&a)), rb = __half22float2(*reinterpret_cast<const __half2*>(&bb));
-                    const float l0 = w0 - ra.x, l1 = w1 - ra.y, l2 = w2 - rb.x, l3 = w3 - rb.y;
-                    pl[h][k][0] = movmatrix_trans(pack_f16x2(l0, l1));
-                    pl[h][k][1] = movmatrix_trans(pack_f16x2(l2, l3));
-                    if (BITS == 4) {   // their codes' offset
-                        low[h][0][k] -= 8.f * unit * (l0 + l2);
-                        low[h][1][k] -= 8.f * unit * (l1 + l3);
+#pragma unroll
+                    for (int k = 0; k < S::NG; ++k) {
+                        low[h][r][k] += pr[h][r] * vleast[0][k] + pr[h][2 + r] * vleast[1][k];
+                        if (FINE) seconds[h][r][k] += rest[h][r][k];
                     }
                 }
             }
-        }
         // ---- O^T += V^T P^T: row g of MMA m is dimension 2 m of the lane's, row g + 8 the one after it
-        Words<S::VW> vw[4][S::VC];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
         if (BITS == 4) {
 #pragma unroll
             for (int h = 0; h < NH; ++h)
@@ -811,12 +839,10 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
     turn = (turn + x.i1 - x.i0) % WARPS;
 
     // ---- the warps' sums, in the values' units
-    float m_run[NH][2];
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            m_run[h][r] = limit[h][r] == -CUDART_INF_F ? -CUDART_INF_F : m_use[h][r];
             l_run[h][r] += __shfl_xor_sync(0xffffffffu, l_run[h][r], 4);
             l_run[h][r] += __shfl_xor_sync(0xffffffffu, l_run[h][r], 8);
             l_run[h][r] += __shfl_xor_sync(0xffffffffu, l_run[h][r], 16);
@@ -825,6 +851,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                 float add = 0.f;
                 if (BITS == 4) {
                     add = low[h][r][min(j, S::NG - 1)];
+                    if (FINE) add -= 8.f * one_over(inv_unit[h][r][min(j, S::NG - 1)]) * seconds[h][r][min(j, S::NG - 1)];   // the offset of the codes that they were multiplied by
                     add += __shfl_xor_sync(0xffffffffu, add, 4);
                     add += __shfl_xor_sync(0xffffffffu, add, 8);
                     add += __shfl_xor_sync(0xffffffffu, add, 16);
@@ -832,6 +859,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
                 for (int k = 0; k < S::VD / 2; ++k) {
                     const int m = j * (S::VD / 2) + k;
+                    const float unit = one_over(inv_unit[h][r][m / (S::MT / S::NG)]);
                     if (BITS == 4) {
                         o[h][m][r] *= 16777216.f;   // 2^24
                         o[h][m][2 + r] *= 1048576.f;
@@ -866,8 +894,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
             for (int r = 0; r < 2; ++r) {
                 const int head = 8 * h + 2 * c + r;
                 if (head >= heads) continue;
-                const float m_other = m_s[buf][head], m = fmaxf(m_run[h][r], m_other), mu = m == -CUDART_INF_F ? 0.f : m;
-                const float fa = exp2f(m_run[h][r] - mu), fb = exp2f(m_other - mu);
+                const float m_other = m_s[buf][head], m = fmaxf(m_run[h][r], m_other);
+                const float fa = exp2f(m_run[h][r] - m), fb = exp2f(m_other - m);
                 l_run[h][r] = l_run[h][r] * fa + l_s[buf][head] * fb;
                 m_run[h][r] = m;
                 const float* src = sums_s + (buf * HEADS + head) * OP + g * S::VD;
@@ -924,12 +952,11 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         const int base = split * slice, mine = min(slice, total - base);
         for (int idx = static_cast<int>(threadIdx.x) * 2; idx < mine; idx += THREADS * 2) {   // (D and slices are even)
             const int head = (base + idx) / D;
-            float m = -CUDART_INF_F;
+            float m = kNoScore;
             for (int s2 = 0; s2 < p.splits; ++s2) m = fmaxf(m, part_m[s2][head]);
-            const float mu = m == -CUDART_INF_F ? 0.f : m;
             float l = 0.f, a0 = 0.f, a1 = 0.f;
             for (int s2 = 0; s2 < p.splits; ++s2) {
-                const float f = exp2f(part_m[s2][head] - mu);
+                const float f = exp2f(part_m[s2][head] - m);
                 l += part_l[s2][head] * f;
                 const float2 v = *reinterpret_cast<const float2*>(slice_s + s2 * slice + idx);
                 a0 += v.x * f;
