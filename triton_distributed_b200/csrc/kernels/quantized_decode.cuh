@@ -922,6 +922,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         if (warp == 2 || warp == 3) give(warp - 2);
         __syncthreads();
         if (warp < 2) take(warp);
+        __syncwarp();   // warp 1: all lanes have read what its first ones overwrite
     }
     if (warp == 1) give(1);
     __syncthreads();
