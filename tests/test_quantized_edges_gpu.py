@@ -4,7 +4,7 @@ Bound per element, with p the weights relative to the largest, l their sum, A = 
 * half a step of the result's type, of itself (fp16: or half of its least step, 2^-25; results beyond its largest are infinite)
 * a weight times its value's scale (a group's step) is rounded to fp16: 2^-11 of itself, or 2^-25 of a unit that is at most 2^-5 of the largest such product of
   that group; codes reach 127 (8): per key 2^-30 max_j(p_j scale_j) 127 / l (4 bits: 8 step for 127 scale)
-* scores move weights and their sum: the query's share 2^-15 max|q| sum |k_d| scale, 2^-23 (D / 16 + 6) of sum |q_d k_d| scale, the exponential 2^-20; sums of n / 16 fp32 steps
+* scores move weights and their sum: the query's share max|q| / 32640 sum |k_d| scale, 2^-23 (D / 16 + 6) of sum |q_d k_d| scale, the exponential 2^-20; sums of n / 16 fp32 steps
 """
 import math
 
@@ -42,7 +42,7 @@ def _rows(cache, table, n, i):
     return (c * step + least).flatten(-2), (c * step + least.abs()).flatten(-2), (8.0 * step).expand_as(c).flatten(-2)
 
 
-def _check(q, cache, table, n, scale=None, **kw):
+def _check(q, cache, table, n, scale=None, query=1 / 32640, **kw):
     got = tdist.gqa_fwd_quantized_decode(q.cuda(), tdist.QuantizedKVCache(*(t.cuda() for t in cache)), torch.tensor([n], dtype=torch.int32).cuda(), table.cuda(),
                                          scale=scale, **kw).cpu()
     D, Hkv = q.shape[2], cache.k.shape[2]
@@ -54,7 +54,7 @@ def _check(q, cache, table, n, scale=None, **kw):
     l = p.sum(-1, keepdim=True)
     ref, A = p @ v / l, p @ va / l
     # a score's error counts with the key's weight: what weighs nothing may be off by much
-    off = 2.0 ** -15 * qq.abs().amax(-1, keepdim=True) * ka.sum(-1).unsqueeze(1) * abs(scale) + (D / 16 + 6) * 2.0 ** -23 * (qq.abs() @ ka.transpose(1, 2)) * abs(scale)
+    off = query * qq.abs().amax(-1, keepdim=True) * ka.sum(-1).unsqueeze(1) * abs(scale) + (D / 16 + 6) * 2.0 ** -23 * (qq.abs() @ ka.transpose(1, 2)) * abs(scale)
     moved = (p * torch.expm1(off + 2.0 ** -20)) @ va / l + (p * torch.expm1(off + 2.0 ** -20)).sum(-1, keepdim=True) / l * A
     least = torch.stack([(p[..., None] * size.unsqueeze(1)[..., d:d + 64]).amax(2) for d in range(0, D, 64)], 2).flatten(2) * n * 2.0 ** -30 / l
     tol = HALF[q.dtype] * ref.abs() + 1.01 * ((2.0 ** -11 + n / 16 * 2.0 ** -23) * A + moved + least) + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -120)
@@ -130,3 +130,31 @@ def test_a_long_tail_of_small_weights(bits, dtype):
     v = 1.0 + 0.01 * v
     v[100] = 2.0 ** -20
     _check(q.to(dtype).contiguous(), *_cache(k.bfloat16(), v.bfloat16(), bits), n, scale=1.0 / D, kv_split=8)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_queries_whose_elements_are_exact(bits, dtype):
+    """No element more than 2^6 (bf16, 8 significant bits) or 2^3 (fp16, 11) below the largest, whatever its leading bits: nothing is rounded."""
+    n, D, G = 300, 128, 4
+    g = torch.Generator().manual_seed(20)
+    most = 64.0 if dtype == torch.bfloat16 else 8.0
+    for lead in (1.0, 1.5, 255 / 128):
+        q = ((1 + torch.rand(1, G, D, generator=g)) * torch.where(torch.rand(1, G, D, generator=g) < 0.5, -1.0, 1.0)).clamp(-1.9, 1.9)
+        q[:, :, 5] = most * lead
+        k, v = (torch.randn(n, 1, D, generator=g) for _ in range(2))
+        k = 8 * k
+        k[:, :, 5] *= 0.01
+        _check(q.to(dtype), *_cache(k.bfloat16(), v.bfloat16(), bits), n, query=0.0)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size,scale", [(2.0 ** 124, 2.0 ** -126), (2.0 ** 125, 2.0 ** -126), (2.0 ** -95, 2.0 ** 90)])
+def test_queries_near_the_ends_of_bf16(bits, size, scale):
+    """Elements above 2^126, and tiny ones, with a scale that makes scores of ordinary size."""
+    n, D = 200, 64
+    g = torch.Generator().manual_seed(21)
+    q = torch.randn(1, 4, D, generator=g)
+    q = (q / q.abs().amax() * 3.98 * size).to(torch.bfloat16)
+    k, v = (torch.randn(n, 1, D, generator=g) for _ in range(2))
+    _check(q, *_cache(k.bfloat16(), v.bfloat16(), bits), n, scale=scale)

@@ -7,15 +7,16 @@
 // least_jg times the sum of q over the group is added), and to the weight p_j vs_j, with the sum of p_j least_jg kept beside the product.
 //
 // K. Codes are 8-bit operands of the integer MMA (m16n8k32, u8 x s8) as they lie in memory, 4-bit ones after two logic instructions
-// per eight. A query is brought to 16 bits for it, rint(q 32512 / max |q|), as a high and a low byte with a product each: the sums are exact, the second
-// continues from 256 times the first, and 128 times the sum of q takes the codes' offset off. (As fp16 operands the codes of a tile cost 64
+// per eight. A query is brought to 16 bits for it, times the power of two that takes its largest element to 2^14 and above, as a high and a low byte
+// with a product each: the sums are exact, the second continues from 256 times the first, and 128 times the sum of q takes the codes' offset off. (As fp16 operands the codes of a tile cost 64
 // instructions, and the kernel was bound by its issue slots: 567 per tile of 16 x 128, 32 x 16384 keys of 8 kv heads 148 us.)
-// A score is off by up to 2^-16 max |q| sum |k_d| scale: a 16-bit query against bf16's 8 bits.
+// Elements down to 2^-6 of the largest are exact in bf16 (2^-3 in fp16), smaller ones off by up to max |q| / 32640, and a score by that times the sum of
+// their |k_d| scale. (With 32512 / max |q| every element was rounded, and above 2^126, where a fast quotient is zero, the query was lost.)
 //
 // V. Codes become fp16, exactly, two tokens per register. The weights p_j vs_j of a head (4 bits: p_j step_jg of a head and group) are held in units of a power of two
 // that follows the largest of them so far: 2^-5 of it or less where it is set, down again as the maximum of the scores rises. So they stay below 2^15 whatever the values' magnitude, and
 // rounded to fp16 one is off by 2^-11 of itself, or by 2^-25 of a unit, 2^-30 of the largest (one below 2^-126 is zero). In units of the largest scale, which may be one
-// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights costs 16 x 16384 keys in 4 bits 1 %, heads of 256 5 %.
+// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights costs heads of 256 4 %, and heads of 128 in 4 bits nothing.
 // For fp16 results what that rounding left is a second weight (without it errors of 3.0e-4 of a result where its own rounding is 2.1e-4). 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
@@ -520,14 +521,15 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
         for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
         top = __reduce_max_sync(0xffffffffu, top);
-        // magnitudes below 2^-100 count as that; a query with a NaN or an infinity has a factor of NaN, and so has its result
+        // magnitudes below 2^-100 count as that; a query with a NaN or an infinity has a factor of NaN, and so has its result. The power of two by
+        // which the largest element comes to 2^14 .. 32639 (two signed bytes' largest): from 32640, whose upper eight bits are ones, half of it
         const bool good = top < 0x7f800000u;
-        const float most = fmaxf(good ? __uint_as_float(top) : 1.f, 7.888609052210118e-31f);
-        const float mul = there && good ? 32512.f / most : 0.f;
+        const uint32_t e_most = (max(good ? top : 0u, 27u << 23) + 0x10000u) >> 23;
+        const float mul = there && good ? __uint_as_float((268u - e_most) << 23) : 0.f;
         int sum = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int v = max(-32512, min(32512, __float2int_rn(f[e] * mul)));
+            const int v = __float2int_rn(f[e] * mul);
             const int hi = (v + 128) >> 8, d = lane * E + e;
             const int at = BITS == 8 ? d : (d & ~7) + (d & 1) * 4 + ((d >> 1) & 3);
             q_s[head * D + at] = static_cast<uint8_t>(hi);
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         if (lane % PER == 0) qsum_s[head][lane / PER] = static_cast<float>(sum);
         if (lane == 0) {
             bias_s[head] = BITS == 8 ? sum * -128 : 0;
-            factor_s[head] = (good ? most * (1.f / 32512.f) * p.scale : __uint_as_float(0x7fffffffu)) * (p.soft_cap > 0.f ? 1.f : kLog2e);
+            factor_s[head] = (good ? __uint_as_float((e_most - 14u) << 23) * p.scale : __uint_as_float(0x7fffffffu)) * (p.soft_cap > 0.f ? 1.f : kLog2e);
         }
     }
     __syncthreads();
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                     const float w0 = pr[h][0] * vmul[0][k] * inv_unit[h][0][k], w1 = pr[h][1] * vmul[0][k] * inv_unit[h][1][k];
                     const float w2 = pr[h][2] * vmul[1][k] * inv_unit[h][0][k], w3 = pr[h][3] * vmul[1][k] * inv_unit[h][1][k];
                     const uint32_t a = pack_f16x2(w0, w1), bb = pack_f16x2(w2, w3);
-                    all = __hadd2(all, __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bb)));
+                    all = __hadd2(__hadd2(all, *reinterpret_cast<const __half2*>(&a)), *reinterpret_cast<const __half2*>(&bb));
                     pb[h][k][0] = movmatrix_trans(a);
                     pb[h][k][1] = movmatrix_trans(bb);
                     if (FINE) {
