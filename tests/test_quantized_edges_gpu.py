@@ -158,3 +158,21 @@ def test_queries_near_the_ends_of_bf16(bits, size, scale):
     q = (q / q.abs().amax() * 3.98 * size).to(torch.bfloat16)
     k, v = (torch.randn(n, 1, D, generator=g) for _ in range(2))
     _check(q, *_cache(k.bfloat16(), v.bfloat16(), bits), n, scale=scale)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size,keys,scale", [(1.0, 2.0 ** 122, 2.0 ** -125), (2.0 ** -8, 2.0 ** 122, 2.0 ** -117), (2.0 ** 8, 2.0 ** 110, 2.0 ** -121), (2.0 ** 8, 2.0 ** -80, 2.0 ** 69),
+                                             (2.0 ** -80, 2.0 ** 77, None), (2.0 ** 77, 2.0 ** -80, None), (2.0 ** 121, 2.0 ** -90, 2.0 ** -34), (2.0 ** -90, 2.0 ** 122, 2.0 ** -35),
+                                             (2.0 ** -70, 2.0 ** -70, 2.0 ** 127), (2.0 ** 60, 2.0 ** 62, 2.0 ** -125)])
+def test_scores_of_ordinary_size_from_far_apart(bits, dtype, size, keys, scale):
+    """What is large and what is small come together only in the score."""
+    if dtype == torch.float16 and not 2.0 ** -9 < size < 2.0 ** 9:
+        size, scale = 2.0 ** -8, (64 ** -0.5 if scale is None else scale) * size * 2.0 ** 8
+        if not 2.0 ** -126 <= scale < 2.0 ** 127:
+            pytest.skip("fp16 queries of that size need a scale that fp32 does not have")
+    n, D = 200, 64
+    g = torch.Generator().manual_seed(22)
+    q = torch.randn(1, 4, D, generator=g) * size
+    k, v = (torch.randn(n, 1, D, generator=g) for _ in range(2))
+    _check(q.to(dtype), *_cache((k * keys).bfloat16(), v.bfloat16(), bits), n, scale=scale)

@@ -16,7 +16,7 @@
 // V. Codes become fp16, exactly, two tokens per register. The weights p_j vs_j of a head (4 bits: p_j step_jg of a head and group) are held in units of a power of two
 // that follows the largest of them so far: 2^-5 of it or less where it is set, down again as the maximum of the scores rises. So they stay below 2^15 whatever the values' magnitude, and
 // rounded to fp16 one is off by 2^-11 of itself, or by 2^-25 of a unit, 2^-30 of the largest (one below 2^-126 is zero). In units of the largest scale, which may be one
-// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights costs heads of 256 4 %, and heads of 128 in 4 bits nothing.
+// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights and factors costs heads of 256 5 %, 4 bits with fp16 results 2 %.
 // For fp16 results what that rounding left is a second weight (without it errors of 3.0e-4 of a result where its own rounding is 2.1e-4). 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
@@ -65,6 +65,9 @@ constexpr int MAX_CLUSTER = 8;
 // where every higher score raises it). Before the first score it is fp32's lowest number.
 constexpr float kMostPair = 256.f, kNoScore = -3.4028234663852886e38f;
 constexpr float kLog2e = 1.4426950408889634f;
+// A product of codes is multiplied by the query's factor before the key's scale, so that a huge key beside a small query stays in fp32; a factor outside 2^-60 .. 2^60
+// is taken in two steps, the other one behind the key's scale.
+constexpr float kFactor = 1152921504606846976.f;
 // Units of weights: powers of two from 2^-110, far below the least scale there is, to 2^123, as biased exponents. A new one is at least 2^-5 and more
 // than 2^-6 of the largest weighted scale, which is looked for among products with 2^-20.
 constexpr int kLeastExponent = 17, kMostExponent = 250, kTopExponent = 20 - 5;
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
     uint8_t* q_s = smem + WARPS * STAGES * S::STAGE + sums_bytes(D, NH, SMALL);
     uint8_t* last_s = q_s + 2 * HEADS * D;
     __shared__ float m_s[BUFS][HEADS], l_s[BUFS][HEADS];
-    __shared__ float factor_s[HEADS], qsum_s[HEADS][S::NG];
+    __shared__ float factor_s[HEADS], far_s[HEADS], qsum_s[HEADS][S::NG];
     __shared__ int bias_s[HEADS];
     __shared__ float part_m[MAX_CLUSTER][HEADS], part_l[MAX_CLUSTER][HEADS];
     __shared__ uint32_t scan_s[WARPS];
@@ -542,16 +545,22 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         if (lane % PER == 0) qsum_s[head][lane / PER] = static_cast<float>(sum);
         if (lane == 0) {
             bias_s[head] = BITS == 8 ? sum * -128 : 0;
-            factor_s[head] = (good ? __uint_as_float((e_most - 14u) << 23) * p.scale : __uint_as_float(0x7fffffffu)) * (p.soft_cap > 0.f ? 1.f : kLog2e);
+            // the factor, or as much of it as lies in kFactor's range, and the rest
+            const float power = __uint_as_float((e_most - 14u) << 23), scale = p.scale * (p.soft_cap > 0.f ? 1.f : kLog2e), both = power * scale;
+            const bool near = fabsf(both) >= 1.f / kFactor && fabsf(both) <= kFactor;
+            const float part = fminf(fmaxf(power, 1.f / kFactor), kFactor);
+            factor_s[head] = !good ? __uint_as_float(0x7fffffffu) : (near ? both : part);
+            far_s[head] = near ? 1.f : power / part * scale;
         }
     }
     __syncthreads();
 
     // ---- q as the second operand: column g of the MMA is head 8 h + g
     uint32_t qf[NH][S::KC][4][2];  // high and low bytes of four dimensions
-    float factor[NH][2];           // of heads 8 h + 2 c + {0, 1}: what turns a product of codes into a score in units of log2
+    float factor[NH][2];           // of heads 8 h + 2 c + {0, 1}: what turns a product of codes, times the key's scale, into a score in units of log2
+    bool more = p.soft_cap > 0.f;  // whether that is not all
     int bias[NH][2];               // 8 bits: -128 times the sum of the 16-bit q
-    float qsum[NH][2][S::NG];      // 4 bits: that sum over a group
+    float qsum[NH][2][S::NG];      // 4 bits: that sum over a group, times the factor
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
 #pragma unroll
@@ -569,7 +578,8 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
             factor[h][r] = factor_s[8 * h + 2 * c + r];
             bias[h][r] = bias_s[8 * h + 2 * c + r];
 #pragma unroll
-            for (int k = 0; k < S::NG; ++k) qsum[h][r][k] = qsum_s[8 * h + 2 * c + r][k];
+            for (int k = 0; k < S::NG; ++k) qsum[h][r][k] = qsum_s[8 * h + 2 * c + r][k] * factor[h][r];
+            more |= far_s[8 * h + 2 * c + r] != 1.f;
         }
     }
 
@@ -647,21 +657,23 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = e >> 1;
-                float v = 0.f;
                 if (BITS == 8) {
-                    v = static_cast<float>(acc[h][0][e]) * __uint_as_float(kscale[r].w[0]);
+                    s[h][e] = static_cast<float>(acc[h][0][e]) * factor[h][e & 1] * __uint_as_float(kscale[r].w[0]);
                 } else {
+                    s[h][e] = 0.f;
 #pragma unroll
                     for (int k = 0; k < S::NG; ++k)
-                        v += __uint_as_float(kscale[r].w[k] << 16) * static_cast<float>(acc[h][k][e]) + __uint_as_float(kscale[r].w[k] & 0xffff0000u) * qsum[h][e & 1][k];
+                        s[h][e] += __uint_as_float(kscale[r].w[k] << 16) * (static_cast<float>(acc[h][k][e]) * factor[h][e & 1]) + __uint_as_float(kscale[r].w[k] & 0xffff0000u) * qsum[h][e & 1][k];
                 }
-                s[h][e] = v * factor[h][e & 1];
             }
-        if (p.soft_cap > 0.f) {
+        if (more) {
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[h][e] = soft_cap(s[h][e] * kLog2e, s[h][e] * cap_inv, p.soft_cap * kLog2e);
+                for (int e = 0; e < 4; ++e) {
+                    s[h][e] *= far_s[8 * h + 2 * c + (e & 1)];
+                    if (p.soft_cap > 0.f) s[h][e] = soft_cap(s[h][e] * kLog2e, s[h][e] * cap_inv, p.soft_cap * kLog2e);
+                }
         }
         // ---- the values' scales
         float vmul[2][S::NG], vleast[2][S::NG];
@@ -687,12 +699,6 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                 vmul[r][k] = __uint_as_float(BITS == 8 ? vscale[r].w[k] : vscale[r].w[k] << 16);
                 if (BITS == 4) vleast[r][k] = fmaf(8.f, vmul[r][k], __uint_as_float(vscale[r].w[k] & 0xffff0000u));
             }
-        // the values' codes, on their way while the weights are made
-        Words<S::VW> vw[4][S::VC];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
         // ---- P^T times the scales, in units, as the second operand: tokens in pairs per lane, heads over lane / 4
         float pr[NH][4], pair[NH][2], rest[NH][2][S::NG];
         uint32_t pb[NH][S::NG][2], pl[NH][S::NG][2];
@@ -725,6 +731,11 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
             }
         };
         weights();
+        Words<S::VW> vw[4][S::VC];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
         bool again = !__hblt2(all, __half2half2(__ushort_as_half(0x7800)));   // 2^15 and above, infinities and NaN
 #pragma unroll
         for (int h = 0; h < NH; ++h)
