@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import triton_distributed_b200 as tdist
+from test_quantized_edges_cpu import wide_rows
 
 pytestmark = pytest.mark.gpu
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
@@ -176,3 +177,15 @@ def test_scores_of_ordinary_size_from_far_apart(bits, dtype, size, keys, scale):
     q = torch.randn(1, 4, D, generator=g) * size
     k, v = (torch.randn(n, 1, D, generator=g) for _ in range(2))
     _check(q.to(dtype), *_cache((k * keys).bfloat16(), v.bfloat16(), bits), n, scale=scale)
+
+
+# ---------------------------------------------------------------------------- writing
+@pytest.mark.parametrize("heads", [1, 3])
+def test_groups_whose_range_is_beyond_fp32_are_the_statement_bit_for_bit(heads):
+    x = torch.cat([wide_rows(), wide_rows().flip(0), torch.randn(8, 1, 64).to(torch.bfloat16)], 1)[:, :heads].contiguous()
+    cpu = tdist.create_quantized_kv_cache(1, 8, heads, 64, 4, "cpu")
+    gpu = tdist.QuantizedKVCache(*(t.cuda() for t in cpu))
+    tdist.kv_cache_write(cpu, x, x, torch.arange(8))
+    tdist.kv_cache_write(gpu, x.cuda(), x.cuda(), torch.arange(8).cuda())
+    for a, b in zip(cpu, gpu):
+        assert torch.equal(a.view(torch.uint8), b.cpu().view(torch.uint8))

@@ -149,16 +149,26 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
             const float lo = fminf(P::low(lo2), P::high(lo2)), hi = fmaxf(P::low(hi2), P::high(hi2));
             const uint32_t least = bf16_down(lo);
             const float base = __uint_as_float(least << 16);
-            const float wide = fmaxf(__fdiv_rn(__fsub_rn(hi, base), 15.f), kLeast);
-            const uint32_t step = bf16_down(-wide) & 0x7fffu;   // up: down of the negative (a range beyond fp32's: infinite)
+            const float range = __fsub_rn(hi, base);
+            const bool halved = range > 3.4028234663852886e38f;   // a range beyond fp32's largest: differences of halves
+            const float wide = halved ? 2.f * __fdiv_rn(__fsub_rn(0.5f * hi, 0.5f * base), 15.f) : fmaxf(__fdiv_rn(range, 15.f), kLeast);
+            const uint32_t step = bf16_down(-wide) & 0x7fffu;   // up: down of the negative
             const float inv = __fdiv_rn(1.f, __uint_as_float(step << 16));
             uint32_t o[2] = {0u, 0u};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                // (a NaN, from a range beyond fp32's, gives 0)
                 const float c0 = fminf(15.f, fmaxf(0.f, __fmul_rn(__fsub_rn(P::low(w[i][j]), base), inv))), c1 = fminf(15.f, fmaxf(0.f, __fmul_rn(__fsub_rn(P::high(w[i][j]), base), inv)));
                 const uint32_t pair = (__float_as_uint(__fadd_rn(c0, 12582912.f)) & 15u) | (__float_as_uint(__fadd_rn(c1, 12582912.f)) & 15u) << 4;
                 o[j >> 2] |= pair << (8 * (j & 3));
+            }
+            if (halved && good) {
+                o[0] = o[1] = 0u;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float c0 = fminf(15.f, __fmul_rn(__fsub_rn(0.5f * P::low(w[i][j]), 0.5f * base), 2.f * inv)), c1 = fminf(15.f, __fmul_rn(__fsub_rn(0.5f * P::high(w[i][j]), 0.5f * base), 2.f * inv));
+                    const uint32_t pair = (__float_as_uint(__fadd_rn(c0, 12582912.f)) & 15u) | (__float_as_uint(__fadd_rn(c1, 12582912.f)) & 15u) << 4;
+                    o[j >> 2] |= pair << (8 * (j & 3));
+                }
             }
             if (kept) {
                 *reinterpret_cast<uint2*>(dst + l * 8) = good ? make_uint2(o[0], o[1]) : make_uint2(0u, 0u);

@@ -97,9 +97,10 @@ def ref_quantize_rows(x: torch.Tensor, bits: int) -> Tuple[torch.Tensor, torch.T
     g = x.unflatten(-1, (-1, GROUP))
     good = g.abs().amax(-1, keepdim=True) < math.inf
     g = torch.where(good, g, 0.0)
-    least = _bf16_down(g.amin(-1, keepdim=True))
-    step = -_bf16_down(-quotient(g.amax(-1, keepdim=True) - least, 15.0).clamp_min(LEAST))
-    code = torch.round((g - least) * quotient(1.0, step)).nan_to_num(0.0).clamp(0.0, 15.0).to(torch.uint8).flatten(-2)
+    least, most = _bf16_down(g.amin(-1, keepdim=True)), g.amax(-1, keepdim=True)
+    half = torch.where((most - least).isinf(), 0.5, 1.0)   # of a range beyond fp32's largest: differences of halves
+    step = -_bf16_down(-(quotient(most * half - least * half, 15.0) / half).clamp_min(LEAST))
+    code = torch.round((g * half - least * half) * (quotient(1.0, step) / half)).clamp(0.0, 15.0).to(torch.uint8).flatten(-2)
     pairs = torch.where(good, torch.cat([step, least], -1), math.nan)
     return code[..., 0::2] | (code[..., 1::2] << 4), pairs.to(torch.bfloat16)
 
