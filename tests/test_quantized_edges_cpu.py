@@ -33,3 +33,45 @@ def test_groups_whose_range_is_beyond_fp32():
     assert bool((step <= ((y.amax(-1)[..., None] - least) / 15) * (1 + 2.0 ** -7)).all())
     c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).double()
     assert bool(((c * step + least - y).abs() <= step * (0.5 + 2.0 ** -18)).all())
+
+
+def largest_rows(dtype):
+    """Groups that reach the type's largest numbers, of either sign, and beyond (8: read in a narrower type)."""
+    most = torch.finfo(dtype).max
+    x = torch.randn(9, 1, 64, generator=torch.Generator().manual_seed(2)).clamp(-4, 4) / 4 * most
+    x[0, 0, ::2], x[0, 0, 1::2] = most, 0.0
+    x[1, 0, ::2], x[1, 0, 1::2] = -most, 0.0
+    x[2], x[2, 0, 5], x[2, 0, 6] = most / 2, most, -most
+    x[3] = -most
+    x[4], x[4, 0, 7] = most * 0.997, -most * 0.998
+    x[5] = x[5].abs()
+    x[6] = -x[6].abs()
+    x[7] = 1.0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_finite_rows_read_as_finite(bits, dtype):
+    """And no further off than half a step, which saturating only lessens; a type's rounding in 8 bits, where half a step is 2^-8 of the largest."""
+    x = torch.cat([largest_rows(dtype), wide_rows()]) if dtype == torch.bfloat16 else largest_rows(dtype)
+    n = x.shape[0]
+    cache = tdist.create_quantized_kv_cache(1, n, 1, 64, bits, "cpu")
+    tdist.kv_cache_write(cache, x, x, torch.arange(n))
+    k, v = tdist.kv_cache_read(cache, torch.tensor([0, n]), torch.tensor([n]), torch.tensor([[0]]), n, dtype)
+    assert torch.equal(k, v) and bool(k.isfinite().all())
+    most = x.double().abs().amax(-1, keepdim=True)
+    half = most / 254 if bits == 8 else cache.k_scales.double()[0, 0, :, :, 0].unsqueeze(1) / 2
+    assert bool(((k.double() - x.double()).abs() <= half * (1 + 2.0 ** -16) + most * torch.finfo(dtype).eps / 2).all())
+
+
+def test_what_does_not_fit_a_narrower_type_is_infinite():
+    """Numbers of bf16 read as fp16: 10^6 lies beyond by more than half a step of its group, 65536 by less."""
+    x = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    x[0, 0, :2] = torch.tensor([1e6, -1e6])
+    x[1] = 65536.0
+    x[1, 0, 0] = 60000.0
+    cache = tdist.create_quantized_kv_cache(1, 2, 1, 64, 4, "cpu")
+    tdist.kv_cache_write(cache, x, x, torch.arange(2))
+    k, _ = tdist.kv_cache_read(cache, torch.tensor([0, 2]), torch.tensor([2]), torch.tensor([[0]]), 2, torch.float16)
+    assert k[0, 0, 0] == math.inf and k[0, 0, 1] == -math.inf and bool(k[0, 0, 2:].isfinite().all()) and bool(k[1].isfinite().all())

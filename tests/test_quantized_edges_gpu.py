@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import triton_distributed_b200 as tdist
-from test_quantized_edges_cpu import wide_rows
+from test_quantized_edges_cpu import largest_rows, wide_rows
 
 pytestmark = pytest.mark.gpu
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
@@ -189,3 +189,20 @@ def test_groups_whose_range_is_beyond_fp32_are_the_statement_bit_for_bit(heads):
     tdist.kv_cache_write(gpu, x.cuda(), x.cuda(), torch.arange(8).cuda())
     for a, b in zip(cpu, gpu):
         assert torch.equal(a.view(torch.uint8), b.cpu().view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------- reading
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("into", [torch.bfloat16, torch.float16])
+def test_largest_numbers_are_read_as_the_statement_has_them(bits, dtype, into):
+    x = torch.cat([largest_rows(dtype), wide_rows().to(dtype).clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max)])
+    x[-1, 0, 3], x[-2, 0, 4] = math.nan, math.inf
+    n = x.shape[0]
+    cpu = tdist.create_quantized_kv_cache(1, n, 1, 64, bits, "cpu")
+    tdist.kv_cache_write(cpu, x, x.flip(0), torch.arange(n))
+    gpu = tdist.QuantizedKVCache(*(t.cuda() for t in cpu))
+    args = torch.tensor([0, n]), torch.tensor([n]), torch.tensor([[0]])
+    for a, b in zip(tdist.kv_cache_read(cpu, *args, n, into), tdist.kv_cache_read(gpu, *(t.cuda() for t in args), n, into)):
+        b = b.cpu()
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.0, math.inf, -math.inf), b.nan_to_num(0.0, math.inf, -math.inf))

@@ -189,9 +189,21 @@ __device__ __forceinline__ void values16(const uint4& codes, float scale, float 
     }
 }
 
+// 4 bits: a value beyond the largest number of the type by no more than half a step, as rounding to a code and the pair's rounding outwards leave it of one that was not
+// beyond, is that number: stored once more, over the infinity. In halves: 15 steps above the least value may lie beyond fp32.
+__device__ __forceinline__ void store_within(uint16_t* dst, uint32_t w0, uint32_t w1, float scale, float least, bool is_f16) {
+    const float most = is_f16 ? 32752.f : 1.69476569462576775e38f;
+    if (!(fmaxf(fmaf(7.5f, scale, 0.5f * least), -0.5f * least) > most)) return;   // (NaN too)
+#pragma unroll 1
+    for (int j = 0; j < 16; ++j) {
+        const float half = fmaf(static_cast<float>(((j < 8 ? w0 : w1) >> (4 * (j & 7))) & 15u), 0.5f * scale, 0.5f * least);
+        if (fabsf(half) > most && fabsf(half) - 0.25f * scale <= most) dst[j] = static_cast<uint16_t>((is_f16 ? 0x7bffu : 0x7f7fu) | (half < 0.f ? 0x8000u : 0u));
+    }
+}
+
 // A CTA takes `rows_per_cta` rows of the output: first a thread per row looks its place up, then LANES lanes read a (row, head)'s k and v.
 template <int BITS, int D>
-__global__ void __launch_bounds__(THREADS) read_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, 4) read_kernel(const Params p) {
     constexpr int LANES = D / 16;
     __shared__ int page_s[MAX_ROWS], row_s[MAX_ROWS];
     pdl_wait_and_release();
@@ -272,6 +284,7 @@ __global__ void __launch_bounds__(THREADS) read_kernel(const Params p) {
                 uint4* dst = reinterpret_cast<uint4*>(p.out[i] + ((r0 + r[u]) * p.Hkv + h[u]) * (D * 2ll) + l * 32);
                 dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
                 dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+                if (BITS == 4 && there[u]) store_within(reinterpret_cast<uint16_t*>(dst), codes[u][i].x, codes[u][i].y, scale[u][i], least[u][i], p.is_f16);
             }
         }
     }

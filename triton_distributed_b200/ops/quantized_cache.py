@@ -14,7 +14,8 @@ The format, per row of D values (one token's key or value of one head):
   ``code = rint((x - least) (1 / step))`` in 0..15; value ``least + step code``. Two codes per byte, the even index in the low half.
 
 So a key and value of 128 dimensions take 264 and 144 bytes where bf16 takes 512. A row (64 values) that holds a NaN or an infinity is
-stored with a scale of NaN: it reads as NaN, and so does the result of every query that sees it. Codes are exact in every product; a result
+stored with a scale of NaN: it reads as NaN, and so does the result of every query that sees it. A finite row reads as finite in the type that it was written in: what 4 bits put
+beyond the type's largest number by up to half a step reads as that number. Codes are exact in every product; a result
 differs from attention over the rows read back only by the roundings of the query to 16 bits, of the weights and of the result.
 
 Slots must differ, as a server's pages do: of two tokens with one slot either's codes may stay beside the other's scale. Tokens whose slot is
@@ -105,13 +106,16 @@ def ref_quantize_rows(x: torch.Tensor, bits: int) -> Tuple[torch.Tensor, torch.T
     return code[..., 0::2] | (code[..., 1::2] << 4), pairs.to(torch.bfloat16)
 
 
-def ref_dequantize_rows(codes: torch.Tensor, scales: torch.Tensor, bits: int) -> torch.Tensor:
-    """fp32 rows of codes and scales."""
+def ref_dequantize_rows(codes: torch.Tensor, scales: torch.Tensor, bits: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Rows of codes and scales. 4 bits: a value beyond the type's largest number by no more than half a step is that number (a number that
+    was not beyond may come to lie there by its rounding to a code and the pair's rounding outwards)."""
     if bits == 8:
-        return (codes.float() - 128.0) * scales.unsqueeze(-1)
-    c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).float().unflatten(-1, (-1, GROUP))
-    p = scales.float()
-    return (c * p[..., 0:1] + p[..., 1:2]).flatten(-2)
+        return ((codes.float() - 128.0) * scales.unsqueeze(-1)).to(dtype)
+    c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).double().unflatten(-1, (-1, GROUP))
+    step, least = scales.double()[..., 0:1], scales.double()[..., 1:2]
+    v, most = c * step + least, torch.finfo(dtype).max
+    near = (v.abs() > most) & (v.abs() - step / 2 <= most)
+    return torch.where(near, most * v.sign(), v).float().to(dtype).flatten(-2)
 
 
 def ref_kv_cache_write(cache: QuantizedKVCache, k, v, slots) -> None:
@@ -124,15 +128,15 @@ def ref_kv_cache_write(cache: QuantizedKVCache, k, v, slots) -> None:
         scales.transpose(1, 2)[at // page, at % page] = s
 
 
-def _rows_of(cache: QuantizedKVCache, table, at):
-    """fp32 k and v of the positions ``at`` of one sequence; zeros for pages that the cache does not have."""
+def _rows_of(cache: QuantizedKVCache, table, at, dtype=torch.float32):
+    """k and v of the positions ``at`` of one sequence; zeros for pages that the cache does not have."""
     blocks, page = cache.k.shape[:2]
     pages, rows = table[at // page].long(), at % page
     there = (pages >= 0) & (pages < blocks)
     pages = torch.where(there, pages, 0)
     out = []
     for codes, scales in ((cache.k, cache.k_scales), (cache.v, cache.v_scales)):
-        x = ref_dequantize_rows(codes[pages, rows], scales.transpose(1, 2)[pages, rows], cache.bits)
+        x = ref_dequantize_rows(codes[pages, rows], scales.transpose(1, 2)[pages, rows], cache.bits, dtype)
         out.append(torch.where(there.view(-1, 1, 1), x, 0.0))
     return out
 
@@ -149,8 +153,8 @@ def ref_kv_cache_read(cache: QuantizedKVCache, starts, kv_lens, block_table, row
         r0 = int(starts[b])
         n = min(n, int(starts[b + 1]) - r0, rows - r0)
         if n > 0 and r0 >= 0:
-            for o, x in zip(out, _rows_of(cache, block_table[b], torch.arange(n, device=cache.k.device))):
-                o[r0:r0 + n] = x.to(dtype)
+            for o, x in zip(out, _rows_of(cache, block_table[b], torch.arange(n, device=cache.k.device), dtype)):
+                o[r0:r0 + n] = x
     return out[0], out[1]
 
 
