@@ -206,3 +206,18 @@ def test_largest_numbers_are_read_as_the_statement_has_them(bits, dtype, into):
     for a, b in zip(tdist.kv_cache_read(cpu, *args, n, into), tdist.kv_cache_read(gpu, *(t.cuda() for t in args), n, into)):
         b = b.cpu()
         assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.0, math.inf, -math.inf), b.nan_to_num(0.0, math.inf, -math.inf))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("first", [-5, -(1 << 31), -(1 << 40)])
+def test_sequences_that_start_before_row_0_are_not_read(bits, first):
+    """As in the statement; with pages of one token and the lowest start a row's distance from it would pass 31 bits."""
+    x = torch.randn(40, 2, 64, generator=torch.Generator().manual_seed(30)).to(torch.bfloat16)
+    cpu = tdist.create_quantized_kv_cache(40, 1, 2, 64, bits, "cpu")
+    tdist.kv_cache_write(cpu, x, x, torch.arange(40))
+    gpu = tdist.QuantizedKVCache(*(t.cuda() for t in cpu))
+    for starts in ([first, 7, 20], [first, first + 3, 12], [first, first, first]):
+        args = torch.tensor(starts), torch.tensor([(1 << 31) - 1, 9]), torch.arange(40).view(2, 20)
+        want, got = tdist.kv_cache_read(cpu, *args, 24), tdist.kv_cache_read(gpu, *(t.cuda() for t in args), 24)
+        for a, b in zip(want, got):
+            assert torch.equal(a, b.cpu())

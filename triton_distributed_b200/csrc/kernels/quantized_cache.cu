@@ -219,8 +219,10 @@ __global__ void __launch_bounds__(THREADS, 4) read_kernel(const Params p) {
             else b = m;
         }
         int page = -1, row = 0;
-        if (a > 0 && r < p.starts[a]) {
-            const int j = r - p.starts[a - 1];
+        // (a sequence that starts before row 0 has none: rows count from 0, and r less its start might pass 31 bits)
+        const int start = a > 0 ? p.starts[a - 1] : -1;
+        if (start >= 0 && r < p.starts[a]) {
+            const int j = r - start;
             const int in_table = static_cast<int>(quotient(static_cast<uint32_t>(j), p.page_mul, p.page_shift));
             if (j < p.lens[a - 1] && in_table < p.max_blocks) {
                 page = p.table[static_cast<long long>(a - 1) * p.max_blocks + in_table];

@@ -315,7 +315,7 @@ def _int32(t):
 def kv_cache_read(cache: QuantizedKVCache, starts: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor, rows: int,
                   dtype: torch.dtype = torch.bfloat16, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a batch as rows of ``dtype`` (bf16 or fp16): sequence b's first ``kv_lens[b]`` keys from row ``starts[b]`` on, at most
-    up to ``starts[b + 1]`` (``starts`` must not decrease). Returns ``(k, v)``, each ``[rows, Hkv, D]`` (``out``, if given); rows of no
+    up to ``starts[b + 1]`` (``starts`` must not decrease; a sequence with a negative one is not read). Returns ``(k, v)``, each ``[rows, Hkv, D]`` (``out``, if given); rows of no
     sequence are zeros."""
     rows = int(rows)
     given = () if out is None else tuple(out)
