@@ -75,3 +75,24 @@ def test_what_does_not_fit_a_narrower_type_is_infinite():
     tdist.kv_cache_write(cache, x, x, torch.arange(2))
     k, _ = tdist.kv_cache_read(cache, torch.tensor([0, 2]), torch.tensor([2]), torch.tensor([[0]]), 2, torch.float16)
     assert k[0, 0, 0] == math.inf and k[0, 0, 1] == -math.inf and bool(k[0, 0, 2:].isfinite().all()) and bool(k[1].isfinite().all())
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Views of one element; the native arguments are 32 bits wide and would be cut."""
+    many = 1 << 32
+    one = lambda dtype, *shape: torch.zeros((1,) * len(shape), dtype=dtype).expand(*shape)   # noqa: E731
+    for shape in ((1, many + 16), (1, 1 << 31), (1 << 31, 16)):
+        with pytest.raises(ValueError, match="31 bits"):
+            tdist.quantize_int8_rowwise(one(torch.bfloat16, *shape))
+    a, b, sa, sb = one(torch.int8, 4, 16), one(torch.int8, 8, 16), torch.ones(4), torch.ones(8)
+    for m in (many + 4, (1 << 31) - 256):
+        with pytest.raises(ValueError, match="at most"):
+            tdist.gemm_int8(one(torch.int8, m, 16), one(torch.float32, m), b, sb)
+        with pytest.raises(ValueError, match="at most"):
+            tdist.gemm_int8(a, sa, one(torch.int8, m, 16), one(torch.float32, m))
+    cache = tdist.create_quantized_kv_cache(2, 4, 1, 64, 8, "cpu")
+    lens, wide = torch.tensor([3]), one(torch.int32, 1, many + 1)
+    with pytest.raises(ValueError, match="31 bits"):
+        tdist.gqa_fwd_quantized_decode(torch.zeros(1, 2, 64), cache, lens, wide)
+    with pytest.raises(ValueError, match="31 bits"):
+        tdist.kv_cache_read(cache, torch.tensor([0, 3]), lens, wide, 3)

@@ -24,6 +24,7 @@ from .quantized_cache import LEAST, quotient
 
 launch_count = 0
 MAX_K = 131071   # 128 x 128 x K stays below 2^31
+MAX_ROWS = (1 << 31) - 512   # of either operand: rows are counted in 32 bits, whole tiles of them
 _OUT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _ROWS = {**_OUT, torch.float32: _lib.DT_F32}
 
@@ -72,6 +73,8 @@ def quantize_int8_rowwise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if plan is None:
         if x.dim() != 2 or x.shape[1] % 16 or x.shape[1] < 16:
             raise ValueError(f"expected [M, K] with K a multiple of 16, got {tuple(x.shape)}")
+        if x.shape[0] >= 1 << 31 or x.shape[1] >= 1 << 31:
+            raise ValueError("rows and their values are counted in 31 bits")
         if x.dtype not in _ROWS:
             raise TypeError("rows must be bf16, fp16 or fp32")
         if x.device.type != "cuda":
@@ -95,6 +98,8 @@ def _check(a, sa, b, sb, out_dtype, out):
         raise ValueError(f"expected a[M,K], b[N,K] with K a multiple of 16, got {tuple(a.shape)} and {tuple(b.shape)}")
     if a.shape[1] > MAX_K:
         raise ValueError(f"K must be at most {MAX_K // 16 * 16}: longer sums may leave 32 bits")
+    if a.shape[0] > MAX_ROWS or b.shape[0] > MAX_ROWS:
+        raise ValueError(f"M and N must be at most {MAX_ROWS}")
     if b.shape[0] % 8:
         raise ValueError("N must be a multiple of 8")
     if a.dtype != torch.int8 or b.dtype != torch.int8:
@@ -116,7 +121,7 @@ def _check(a, sa, b, sb, out_dtype, out):
 @nvtx_range("tdist.gemm_int8")
 def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``a [M, K]``, ``b [N, K]`` int8, ``sa [M]``, ``sb [N]`` fp32 -> ``[M, N]`` bf16 or fp16. K a multiple of 16, N of 8."""
+    """``a [M, K]``, ``b [N, K]`` int8, ``sa [M]``, ``sb [N]`` fp32 -> ``[M, N]`` bf16 or fp16. K a multiple of 16, N of 8; M and N at most 2^31 - 512."""
     global launch_count
     index = a.get_device()
     key = (a.shape, b.shape, sa.shape, sb.shape, a.dtype, b.dtype, sa.dtype, sb.dtype, index, b.get_device(), sa.get_device(), sb.get_device(),

@@ -217,6 +217,8 @@ def _check_ints(device, ints):
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {['any' if s is None else s for s in shape]}")
         if t.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"{name} must hold integers (int32 or int64)")
+        if any(n >= 1 << 31 for n in t.shape):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}: sizes are counted in 31 bits")
         if t.device != device:
             raise ValueError(f"{name} must be on the cache's device")
 
