@@ -29,11 +29,10 @@ def _cache(k, v, bits, page=16):
     return cache, table
 
 
-def _rows(cache, table, n, i):
-    """What is stored, in 64 bits: [Hkv, n, D]; |step c| + |least| of each; the product's size per unit of weight [Hkv, n, D]."""
+def _rows(cache, table, at, i):
+    """What is stored at the positions of a sequence, in 64 bits: [Hkv, n, D]; |step c| + |least| of each; the product's size per unit of weight [Hkv, n, D]."""
     page = cache.k.shape[1]
-    at = torch.arange(n)
-    pages, rows = table[0].long()[at // page], at % page
+    pages, rows = table[at // page].long(), at % page
     c, s = cache[i][pages, rows].transpose(0, 1), cache[2 + i].transpose(1, 2)[pages, rows].double().transpose(0, 1)
     if cache.bits == 8:
         v = (c.double() - 128.0) * s.unsqueeze(-1)
@@ -44,28 +43,36 @@ def _rows(cache, table, n, i):
 
 
 def _check(q, cache, table, n, scale=None, query=1 / 32640, **kw):
-    got = tdist.gqa_fwd_quantized_decode(q.cuda(), tdist.QuantizedKVCache(*(t.cuda() for t in cache)), torch.tensor([n], dtype=torch.int32).cuda(), table.cuda(),
-                                         scale=scale, **kw).cpu()
+    """A sequence of n keys."""
+    gpu = q.cuda(), tdist.QuantizedKVCache(*(t.cuda() for t in cache)), torch.tensor([n], dtype=torch.int32).cuda(), table.cuda()
+    _compare(tdist.gqa_fwd_quantized_decode(*gpu, scale=scale, **kw).cpu(), q, cache, table, [n], scale, query)
+
+
+def _compare(got, q, cache, table, lens, scale=None, query=1 / 32640, window=None, sinks=0):
     D, Hkv = q.shape[2], cache.k.shape[2]
     scale = D ** -0.5 if scale is None else scale
-    (k, ka, _), (v, va, size) = _rows(cache, table, n, 0), _rows(cache, table, n, 1)
-    qq = q[0].double().view(Hkv, -1, D)
-    t = qq @ k.transpose(1, 2) * scale
-    p = torch.exp(t - t.amax(-1, keepdim=True))
-    l = p.sum(-1, keepdim=True)
-    ref, A = p @ v / l, p @ va / l
-    # a score's error counts with the key's weight: what weighs nothing may be off by much
-    off = query * qq.abs().amax(-1, keepdim=True) * ka.sum(-1).unsqueeze(1) * abs(scale) + (D / 16 + 6) * 2.0 ** -23 * (qq.abs() @ ka.transpose(1, 2)) * abs(scale)
-    moved = (p * torch.expm1(off + 2.0 ** -20)) @ va / l + (p * torch.expm1(off + 2.0 ** -20)).sum(-1, keepdim=True) / l * A
-    least = torch.stack([(p[..., None] * size.unsqueeze(1)[..., d:d + 64]).amax(2) for d in range(0, D, 64)], 2).flatten(2) * n * 2.0 ** -30 / l
-    tol = HALF[q.dtype] * ref.abs() + 1.01 * ((2.0 ** -11 + n / 16 * 2.0 ** -23) * A + moved + least) + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -120)
-    out = got[0].double().view(Hkv, -1, D)
-    most = torch.finfo(q.dtype).max
-    inf = out.abs() == math.inf                   # where the bound reaches beyond the type's range, and has to where it lies beyond
-    assert bool((out == ref.sign() * math.inf)[inf].all()) and bool((ref.abs() + tol > most)[inf].all()) and bool(inf[ref.abs() - tol > most].all())
-    err = (out - ref).abs().masked_fill(inf, 0.0)
-    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
-    return got
+    for b, n in enumerate(lens):
+        lo = 0 if window is None else max(0, n - window)
+        at = torch.cat([torch.arange(0, min(sinks, lo)), torch.arange(lo, n)])
+        if at.numel() == 0:
+            assert (got[b] == 0).all()
+            continue
+        (k, ka, _), (v, va, size) = _rows(cache, table[b], at, 0), _rows(cache, table[b], at, 1)
+        qq = q[b].double().view(Hkv, -1, D)
+        t = qq @ k.transpose(1, 2) * scale
+        p = torch.exp(t - t.amax(-1, keepdim=True))
+        l = p.sum(-1, keepdim=True)
+        ref, A = p @ v / l, p @ va / l
+        # a score's error counts with the key's weight: what weighs nothing may be off by much
+        off = query * qq.abs().amax(-1, keepdim=True) * ka.sum(-1).unsqueeze(1) * abs(scale) + (D / 16 + 6) * 2.0 ** -23 * (qq.abs() @ ka.transpose(1, 2)) * abs(scale)
+        moved = (p * torch.expm1(off + 2.0 ** -20)) @ va / l + (p * torch.expm1(off + 2.0 ** -20)).sum(-1, keepdim=True) / l * A
+        least = torch.stack([(p * size[..., d].unsqueeze(1)).amax(2, keepdim=True).expand(-1, -1, 64) for d in range(0, D, 64)], 2).flatten(2) * at.numel() * 2.0 ** -30 / l
+        tol = HALF[q.dtype] * ref.abs() + 1.01 * ((2.0 ** -11 + at.numel() / 16 * 2.0 ** -23) * A + moved + least) + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -120)
+        out, most = got[b].double().view(Hkv, -1, D), torch.finfo(q.dtype).max
+        inf = out.abs() == math.inf               # where the bound reaches beyond the type's range, and has to where it lies beyond
+        assert bool((out == ref.sign() * math.inf)[inf].all()) and bool((ref.abs() + tol > most)[inf].all()) and bool(inf[ref.abs() - tol > most].all())
+        err = (out - ref).abs().masked_fill(inf, 0.0)
+        assert bool((err <= tol).all()), (b, n, float(err.max()), float((err / tol).max()))
 
 
 def _keys(n, G, D, scores, seed):
@@ -221,3 +228,56 @@ def test_sequences_that_start_before_row_0_are_not_read(bits, first):
         want, got = tdist.kv_cache_read(cpu, *args, 24), tdist.kv_cache_read(gpu, *(t.cuda() for t in args), 24)
         for a, b in zip(want, got):
             assert torch.equal(a, b.cpu())
+
+
+# ---------------------------------------------------------------------------- as it is chosen
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,most,window,sinks", [
+    (70, 8, 2, 128, 16, 9000, None, 0),       # equal shares of many ragged sequences
+    (1, 16, 8, 64, 16, 150000, None, 0),      # of a long one
+    (3, 10, 1, 256, 7, 40000, None, 0),       # heads of 256, pages that tiles straddle
+    (513, 2, 1, 64, 16, 3001, None, 0),       # more sequences than shares take
+    (300, 4, 1, 128, 1, 2500, 700, 5),        # windows
+    (40, 32, 2, 128, 64, 6000, None, 0)])     # two tiles of heads
+def test_ways_that_are_chosen_by_sizes(bits, dtype, B, Hq, Hkv, D, page, most, window, sinks):
+    """Ragged sequences of a cache whose pages they share, some of them empty; two calls give the same bits."""
+    g = torch.Generator().manual_seed(B + D)
+    x = [(torch.randn(most, Hkv, D, generator=g) * torch.where(torch.rand(Hkv, D, generator=g) < 0.05, 6.0, 1.0)).to(dtype) for _ in range(2)]
+    cache, table = _cache(*x, bits, page)
+    table = torch.stack([table[0][torch.randperm(table.shape[1], generator=g)] for _ in range(B)])
+    lens = [most] if B == 1 else [most * (i + 1) // B if i % 9 else 0 for i in torch.randperm(B, generator=g).tolist()]
+    few = list(range(B)) if B <= 3 else [0, 1, B // 2, B - 2, B - 1] + [lens.index(max(lens)), lens.index(0)]
+    q = torch.randn(B, Hq, D, generator=g).to(dtype)
+    gpu = q.cuda(), tdist.QuantizedKVCache(*(t.cuda() for t in cache)), torch.tensor(lens, dtype=torch.int32).cuda(), table.cuda()
+    got = [tdist.gqa_fwd_quantized_decode(*gpu, window=window, sinks=sinks).cpu() for _ in range(2)]
+    assert torch.equal(*got)
+    _compare(got[0][few], q[few], cache, table[few], [lens[b] for b in few], window=window, sinks=sinks)
+
+
+def test_two_threads_at_once():
+    """Calls of the same sizes, each thread on a stream of its own."""
+    import threading
+    x, w = torch.randn(600, 1024, device="cuda").bfloat16(), torch.randn(2048, 1024, device="cuda")
+    k = torch.randn(300, 2, 128, device="cuda").bfloat16()
+    q, lens, table = torch.randn(2, 8, 128, device="cuda").bfloat16(), torch.tensor([300, 150]).cuda(), torch.arange(38, device="cuda").view(2, 19)
+    torch.cuda.synchronize()
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            cache = tdist.create_quantized_kv_cache(38, 16, 2, 128, 4)
+            tdist.kv_cache_write(cache, k, k, torch.arange(300, device="cuda"))
+            a, b = tdist.quantize_int8_rowwise(x), tdist.quantize_int8_rowwise(w)
+            out = [tdist.gemm_int8(*a, *b) for _ in range(20)] + [tdist.gqa_fwd_quantized_decode(q, cache, lens, table) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+            return out
+
+    got = [None] * 4
+    threads = [threading.Thread(target=lambda i=i: got.__setitem__(i, work())) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, got[0]))
+        assert all(torch.equal(out[i], out[0]) for i in range(20)) and all(torch.equal(out[i], out[20]) for i in range(20, 40))

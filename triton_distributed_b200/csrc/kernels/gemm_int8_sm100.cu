@@ -20,6 +20,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "../device/ptx.cuh"
@@ -294,15 +295,15 @@ const void* kernel_of(bool wide) {
 // CTAs of the pair kernel that are resident at once on the current device; opts in to its shared memory. Cached per device.
 int resident(bool wide) {
     using namespace tdist::int8;
-    static int cache[64][2] = {};
+    static std::atomic<int> cache[64][2];   // (threads that ask at once find the same)
     int dev = 0;
     const int nominal = tdist_host::sm_count() & ~1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
         cudaGetLastError();
         return nominal;
     }
-    int& slot = cache[dev][wide];
-    if (slot > 0) return slot;
+    std::atomic<int>& slot = cache[dev][wide];
+    if (const int kept = slot) return kept;
     int clusters = 0;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
