@@ -37,7 +37,7 @@ NVCC_FLAGS = [
 
 
 # Sources whose results are defined bit by bit: IEEE division, CUDA's expf and logf, no flush of subnormals.
-PRECISE = {"sampling.cu", "quantized_cache.cu", "quantize_int8.cu"}
+PRECISE = {"sampling.cu", "quantized_cache.cu", "quantize_int8.cu", "gemm_int8_sm100.cu", "gemm_int8_skinny_sm100.cu"}
 
 
 def _flags(src: Path) -> list[str]:
