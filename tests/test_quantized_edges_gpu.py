@@ -186,6 +186,22 @@ def test_scores_of_ordinary_size_from_far_apart(bits, dtype, size, keys, scale):
     _check(q.to(dtype), *_cache((k * keys).bfloat16(), v.bfloat16(), bits), n, scale=scale)
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("cap", [1e-10, 2.0 ** -61, 1e-38, 1e-39, 1e-44, 1e30, 2.0 ** 127])
+def test_caps_of_any_size(bits, cap):
+    """A tiny cap (subnormal ones too): the mean of the values. A huge one: as none, up to the cap's own arithmetic."""
+    n, D = 300, 64
+    g = torch.Generator().manual_seed(23)
+    q, (k, v) = torch.randn(1, 4, D, generator=g).to(torch.bfloat16), (torch.randn(n, 1, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    cache, table = _cache(k, v, bits)
+    gpu = q.cuda(), tdist.QuantizedKVCache(*(t.cuda() for t in cache)), torch.tensor([n], dtype=torch.int32).cuda(), table.cuda()
+    got = tdist.gqa_fwd_quantized_decode(*gpu, soft_cap=cap).cpu()
+    if cap > 1.0:
+        _compare(got, q, cache, table, [n])
+    else:
+        _compare(got, torch.zeros_like(q), cache, table, [n])
+
+
 # ---------------------------------------------------------------------------- writing
 @pytest.mark.parametrize("heads", [1, 3])
 def test_groups_whose_range_is_beyond_fp32_are_the_statement_bit_for_bit(heads):

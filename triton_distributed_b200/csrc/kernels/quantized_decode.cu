@@ -128,7 +128,8 @@ extern "C" int tdist_quant_decode(const TdistQuantDecodeArgs* a) {
     p.table_keys = static_cast<int>(keys < 0x7fffffc0ll ? keys : 0x7fffffc0ll);
     const bool f16 = c.dtype == TDIST_F16;
     p.scale = a->scale;
-    p.soft_cap = a->soft_cap;
+    // a cap below 2^-60 makes all weights alike as 2^-60 does, whose inverse fp32 has
+    p.soft_cap = a->soft_cap > 0.f && a->soft_cap < 8.673617379884035e-19f ? 8.673617379884035e-19f : a->soft_cap;
     const long long segments = static_cast<long long>(c.B) * c.Hkv * p.head_tiles, grid = p.shares > 0 ? static_cast<long long>(p.shares) * c.Hkv * p.head_tiles : segments * p.splits;
     if (grid > 0x7fffffffll) return fail(TDIST_EINVAL, "quantised decode: too many sequences");
     if (p.shares > 0) {
