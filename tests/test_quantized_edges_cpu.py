@@ -96,3 +96,10 @@ def test_sizes_beyond_32_bits_are_refused():
         tdist.gqa_fwd_quantized_decode(torch.zeros(1, 2, 64), cache, lens, wide)
     with pytest.raises(ValueError, match="31 bits"):
         tdist.kv_cache_read(cache, torch.tensor([0, 3]), lens, wide, 3)
+
+
+def test_lengths_end_with_what_is_counted():
+    cache = tdist.create_quantized_kv_cache(1, 1 << 20, 1, 64, 8, "cpu")
+    table = torch.zeros((1, 1), dtype=torch.int32).expand(1, 1 << 11)
+    assert QC._limits(cache, table, torch.tensor([(1 << 31) - 1])) == [(1 << 31) - 64] and QC._limits(cache, table, torch.tensor([77])) == [77]
+    assert QC._limits(cache, table[:, :3], torch.tensor([1 << 40])) == [3 << 20]

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 4) read_kernel(const Params p) {
         if (start >= 0 && r < p.starts[a]) {
             const int j = r - start;
             const int in_table = static_cast<int>(quotient(static_cast<uint32_t>(j), p.page_mul, p.page_shift));
-            if (j < p.lens[a - 1] && in_table < p.max_blocks) {
+            if (j < min(p.lens[a - 1], 0x7fffffc0) && in_table < p.max_blocks) {
                 page = p.table[static_cast<long long>(a - 1) * p.max_blocks + in_table];
                 row = j - in_table * p.page_size;
                 if (page < 0 || page >= p.blocks) page = -1;

@@ -19,7 +19,7 @@ beyond the type's largest number by up to half a step reads as that number. Code
 differs from attention over the rows read back only by the roundings of the query to 16 bits, of the weights and of the result.
 
 Slots must differ, as a server's pages do: of two tokens with one slot either's codes may stay beside the other's scale. Tokens whose slot is
-no place of the cache (a negative one: padding) are left out. Lengths are cut to what the table has room for, and a page that the cache does not
+no place of the cache (a negative one: padding) are left out. Lengths are cut to what the table has room for (at most 2^31 - 64 keys), and a page that the cache does not
 have reads as zeros: nothing outside the tensors is touched.
 
 CUDA tensors run ``csrc/kernels/quantized_cache.cu`` and ``quantized_decode.cu``, CPU tensors the plain statements. No call keeps
@@ -41,6 +41,7 @@ from . import paged_attention as PA
 launch_count = 0
 GROUP = 64            # values that share a pair of 4-bit scales
 LEAST = 2.0 ** -100   # magnitudes below it count as it
+MOST_KEYS = (1 << 31) - 64   # of a sequence: whole tiles of them are counted in 31 bits
 _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
@@ -142,8 +143,8 @@ def _rows_of(cache: QuantizedKVCache, table, at, dtype=torch.float32):
 
 
 def _limits(cache, block_table, kv_lens):
-    """Lengths on the host, cut to the table."""
-    room = block_table.shape[1] * cache.k.shape[1] if cache.k.shape[0] else 0
+    """Lengths on the host, cut to the table and to what the kernels count."""
+    room = min(block_table.shape[1] * cache.k.shape[1], MOST_KEYS) if cache.k.shape[0] else 0
     return [min(max(int(n), 0), room) for n in kv_lens]
 
 
