@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
     const int page = slot < 0 ? 0 : static_cast<int>(quotient(static_cast<uint32_t>(slot), p.page_mul, p.page_shift));
     const int row = slot - page * p.page_size;
     const bool kept = slot >= 0 && page < p.blocks;
+    bool again[2] = {false, false};
+    float bases[2], invs[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         uint32_t top = 0, lo2 = w[i][0], hi2 = w[i][0];
@@ -150,8 +152,8 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
             const uint32_t least = bf16_down(lo);
             const float base = __uint_as_float(least << 16);
             const float range = __fsub_rn(hi, base);
-            const bool halved = range > 3.4028234663852886e38f;   // a range beyond fp32's largest: differences of halves
-            const float wide = halved ? 2.f * __fdiv_rn(__fsub_rn(0.5f * hi, 0.5f * base), 15.f) : fmaxf(__fdiv_rn(range, 15.f), kLeast);
+            const bool halved = !F16 && range > 3.4028234663852886e38f;   // a range beyond fp32's largest: differences of halves
+            const float part = __fdiv_rn(halved ? __fsub_rn(0.5f * hi, 0.5f * base) : range, 15.f), wide = halved ? 2.f * part : fmaxf(part, kLeast);
             const uint32_t step = bf16_down(-wide) & 0x7fffu;   // up: down of the negative
             const float inv = __fdiv_rn(1.f, __uint_as_float(step << 16));
             uint32_t o[2] = {0u, 0u};
@@ -161,18 +163,25 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const Params p) {
                 const uint32_t pair = (__float_as_uint(__fadd_rn(c0, 12582912.f)) & 15u) | (__float_as_uint(__fadd_rn(c1, 12582912.f)) & 15u) << 4;
                 o[j >> 2] |= pair << (8 * (j & 3));
             }
-            if (halved && good) {
-                o[0] = o[1] = 0u;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float c0 = fminf(15.f, __fmul_rn(__fsub_rn(0.5f * P::low(w[i][j]), 0.5f * base), 2.f * inv)), c1 = fminf(15.f, __fmul_rn(__fsub_rn(0.5f * P::high(w[i][j]), 0.5f * base), 2.f * inv));
-                    const uint32_t pair = (__float_as_uint(__fadd_rn(c0, 12582912.f)) & 15u) | (__float_as_uint(__fadd_rn(c1, 12582912.f)) & 15u) << 4;
-                    o[j >> 2] |= pair << (8 * (j & 3));
-                }
-            }
             if (kept) {
                 *reinterpret_cast<uint2*>(dst + l * 8) = good ? make_uint2(o[0], o[1]) : make_uint2(0u, 0u);
                 if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(sdst + (l >> 2) * 4) = good ? step | (least << 16) : 0x7fff7fffu;
+                again[i] = halved && good;
+                bases[i] = base;
+                invs[i] = inv;
+            }
+        }
+    }
+    if (BITS == 4 && (again[0] || again[1])) {   // the codes once more, from the values as they were read: a rare case, behind both rows so that their work stays side by side
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (!again[i]) continue;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.x[i] + t * p.x_token[i] + h * p.x_head[i] + l * 32);
+            uint8_t* dst = p.codes[i] + page * p.code_block + row * p.code_token + h * p.code_head + l * 8;
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+                const float c0 = fminf(15.f, __fmul_rn(__fsub_rn(0.5f * P::low(src[j]), 0.5f * bases[i]), 2.f * invs[i])), c1 = fminf(15.f, __fmul_rn(__fsub_rn(0.5f * P::high(src[j]), 0.5f * bases[i]), 2.f * invs[i]));
+                dst[j] = static_cast<uint8_t>((__float_as_uint(__fadd_rn(c0, 12582912.f)) & 15u) | (__float_as_uint(__fadd_rn(c1, 12582912.f)) & 15u) << 4);
             }
         }
     }
