@@ -16,7 +16,7 @@
 // V. Codes become fp16, exactly, two tokens per register. The weights p_j vs_j of a head (4 bits: p_j step_jg of a head and group) are held in units of a power of two
 // that follows the largest of them so far: 2^-5 of it or less where it is set, down again as the maximum of the scores rises. So they stay below 2^15 whatever the values' magnitude, and
 // rounded to fp16 one is off by 2^-11 of itself, or by 2^-25 of a unit, 2^-30 of the largest (one below 2^-126 is zero). In units of the largest scale, which may be one
-// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights and factors costs heads of 256 5 %, 4 bits with fp16 results 2 %.
+// of a key that weighs nothing, a value 2^25 times the others took the others' weights away; looking at weights and factors costs heads of 256 2 %, 4 bits with fp16 results 2 %.
 // For fp16 results what that rounding left is a second weight (without it errors of 3.0e-4 of a result where its own rounding is 2.1e-4). 4-bit codes are taken as c - 8 with least + 8 step, so that the sums stay small.
 //
 // As in the plain decode tokens are the 16 rows of the MMA and query heads its 8 columns (two tiles of them above 8 heads per kv head):
@@ -732,10 +732,13 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
         };
         weights();
         Words<S::VW> vw[4][S::VC];
+        auto load_values = [&]() {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
+                for (int j = 0; j < S::VC; ++j) vw[r][j] = lds_words<S::VW>(stage + v_at[r & 1][j] + (r >> 1) * (8 * S::BOX));
+        };
+        if (D != 256) load_values();   // (heads of 256 have no registers to hold them over the branch: 64 x 8000 keys in 4 bits 54.4 us, 52.3 behind it)
         bool again = !__hblt2(all, __half2half2(__ushort_as_half(0x7800)));   // 2^15 and above, infinities and NaN
 #pragma unroll
         for (int h = 0; h < NH; ++h)
@@ -796,6 +799,7 @@ __global__ void __launch_bounds__(32 * warps_of(D, NH, SMALL), ctas_per_sm(D, NH
                     }
                 }
             }
+        if (D == 256) load_values();
         // ---- O^T += V^T P^T: row g of MMA m is dimension 2 m of the lane's, row g + 8 the one after it
         if (BITS == 4) {
 #pragma unroll
