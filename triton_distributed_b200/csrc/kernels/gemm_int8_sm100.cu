@@ -12,8 +12,8 @@
 // What follows the product differs: an epilogue thread owns a row, so SA is one number per thread, and SB of a tile's columns is
 // fetched into shared memory while the product is made (from L1 and L2 as it was needed: 2048 x 14336 x 256 56 us).
 //
-// Measured, quantised inputs: 8192 x 14336 x 16384 1159 - 1196 us with the clock, 3.2 - 3.3 POP/s, twice the bf16 GEMM's measured rate; 8192 x 14336 x 4096
-// 330 us, 4096^3 51. Below that rounds bound it: 1000 x 5504 x 4096 24 us, 14 of them MMAs at their full rate: one round of 60 items of 256 x 384 on 74
+// Measured, quantised inputs (at twice the measured bf16 rate, 3.28 POP/s): 8192 x 14336 x 16384 1159 - 1196 us with the clock (1174); 8192 x 14336 x 4096
+// 325 us (293), 4096^3 50 (42). Below that rounds bound it: 1000 x 5504 x 4096 24 us, 14 of them MMAs at their full rate: one round of 60 items of 256 x 384 on 74
 // pairs, its prologue and its exposed epilogue.
 //
 // Warps (192 threads): 0 = TMA producer, 1 = MMA issuer and TMEM owner, 2..5 = epilogue (TMEM -> scale -> swizzled smem -> TMA store).

@@ -12,9 +12,10 @@
 // four loads of each lane under way at once. Quotients of places by heads and page sizes go by a multiplication, rounding by
 // the addition of 1.5 2^23, whose low byte is the code. (8 values a lane when writing: 24 us for 16.8 below.)
 //
-// Measured, 8 kv heads of 128, bf16 (at HBM's copy rate): 16384 tokens written in 8 bits 16.8 us (15.5), in 4 21.4 (13.1); 131072 keys read
-// back from 8 bits 135 us (124), from 4 138 (105). 4 bits are bound by instructions: a minimum and a maximum per 64 values, four shuffles, and per
-// code a subtraction, a product and its half of a byte; reading, a conversion and a multiply-add per value.
+// Measured, 8 kv heads of 128, bf16 (at HBM's copy rate): 16384 tokens written in 8 bits 16.9 us (15.5), in 4 22.1 (13.1); 131072 keys read
+// back from 8 bits 131 us (124), from 4 122 (105). Writing 4 bits is bound by instructions (issue slots 81 % busy, the integer pipe 73 %): a largest magnitude, a minimum and a
+// maximum per 64 values, each with two shuffles, and per code a subtraction, a product and its half of a byte. Reading 4 bits waits for memory (7 of 14 stalls per
+// instruction; issue slots 61 %), some thousand keys for a chain of latencies: search, length, page, codes.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

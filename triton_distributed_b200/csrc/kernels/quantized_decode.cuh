@@ -36,9 +36,10 @@
 // read from HBM twice, and 16 x 16384 keys took 107 us in 8 bits.) The copies run on from one piece to the next: while a piece's sums meet,
 // the next one's first tiles are under way. No counters: nothing has to be zero before a call, and calls share nothing.
 //
-// Measured, heads of 128, 8 of kv, 4 query heads each, 16 x 16384 keys: 8 bits 93 us, 5.95 TB/s of codes and scales, HBM. 4 bits 95 us where HBM would take
-// 46: issue slots and the integer pipe, 413 instructions per tile of 16 tokens (nibbles 72, scales 16). One
-// sequence of 4096 keys, 8 bits: 9.8 us, a chain of latencies: length, page, codes, merge.
+// Measured, heads of 128, 8 of kv, 4 query heads each, 16 x 16384 keys: 8 bits 92 us, 6.0 TB/s of codes and scales, HBM. 4 bits 91 us where HBM would take
+// 46: a chain of dependent steps per tile (loads from shared memory, unpacking, integer MMAs, scales, exponentials, transposes, fp16 MMAs) in three warps per scheduler. No unit is full:
+// 426 instructions per tile of 16 tokens, issue slots 61 % busy, the integer pipe 53 %, the tensor pipe 27 %, 1.2 warps ready per cycle at 1.77 GHz. One
+// sequence of 4096 keys, 8 bits: 9.7 us (10.5 where L2 has lost the inputs), a chain of latencies: length, page, codes, merge.
 
 #pragma once
 
@@ -61,8 +62,8 @@ namespace qdecode {
 
 constexpr int TOK = 16;          // tokens of a tile
 constexpr int MAX_CLUSTER = 8;
-// The maximum that weights are relative to is raised, and the sums scaled, when two weights of a lane come to more than 2^8 (4 bits, 16 x 16384 keys 94.7 us, 97.6
-// where every higher score raises it). Before the first score it is fp32's lowest number.
+// The maximum that weights are relative to is raised, and the sums scaled, when two weights of a lane come to more than 2^8 (4 bits, 524288 keys 162.7 us, 166.4
+// where more than 2 raises it). Before the first score it is fp32's lowest number.
 constexpr float kMostPair = 256.f, kNoScore = -3.4028234663852886e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 // A product of codes is multiplied by the query's factor before the key's scale, so that a huge key beside a small query stays in fp32; a factor outside 2^-60 .. 2^60
@@ -111,7 +112,7 @@ __device__ __forceinline__ void mma_u8s8_from(int (&d)[4], int c0, int c1, uint3
 }
 // Codes as operands of the fp16 MMA, exactly. A byte n under the exponent of 1024 is 1024 + n, from which 1152 is taken. A nibble n alone is the subnormal n 2^-24,
 // and in the upper nibble of a byte n 2^-20: rows of the MMA that take those are off by 16 until the end, and the offset of 8 is taken off by a product of its
-// own with the same weights, one MMA for four subtractions (64 ragged sequences to 16384 keys of 8 kv heads 193 us, 210 with subtractions; 8 bits, whose
+// own with the same weights, one MMA for four subtractions (when it was brought in: 64 ragged sequences to 16384 keys of 8 kv heads 193 us, 210 with subtractions; 8 bits, whose
 // weights are two numbers in fp16 and would need two such products, 16 x 16384 keys 98 and 94). The sums stay small either way; with the offset
 // in them until the end, their roundings come to 1.5e-3 of a flat result over 524288 keys.
 constexpr uint32_t kMagic = 0x64006400u;

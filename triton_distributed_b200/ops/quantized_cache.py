@@ -16,7 +16,9 @@ The format, per row of D values (one token's key or value of one head):
 So a key and value of 128 dimensions take 264 and 144 bytes where bf16 takes 512. A row (64 values) that holds a NaN or an infinity is
 stored with a scale of NaN: it reads as NaN, and so does the result of every query that sees it. A finite row reads as finite in the type that it was written in: what 4 bits put
 beyond the type's largest number by up to half a step reads as that number. Codes are exact in every product; a result
-differs from attention over the rows read back only by the roundings of the query to 16 bits, of the weights and of the result.
+differs from attention over the rows read back only by roundings: of the query to 16 bits (elements below 2^-6 of its largest in bf16, 2^-3 in fp16, by up to
+1 / 32640 of the largest), of each key's weight times its value's scale to fp16 (2^-11 of itself, or 2^-30 of the largest such product of the head; fp16 results: a second number for
+what is left), and of the result.
 
 Slots must differ, as a server's pages do: of two tokens with one slot either's codes may stay beside the other's scale. Tokens whose slot is
 no place of the cache (a negative one: padding) are left out. Lengths are cut to what the table has room for (at most 2^31 - 64 keys), and a page that the cache does not
@@ -368,10 +370,11 @@ def _decode_parts(B: int, per_b: int, most: int, table_keys: int, asked: int, sl
     has room for ``slots`` large CTAs (``wide``: one per SM, otherwise two). CTAs per segment; or 0 and the CTAs that take equal shares of
     all sequences; or 0, 0: a small CTA per segment.
 
-    Small CTAs leave room for three (wide: two) times as many: a short segment is mostly latency and the meeting of its warps' sums (8 bits, heads
-    of 128, 8 of kv: 256 sequences of 512 keys 74.2 us with large CTAs, 58.8 with small ones, of 128 keys 42.6 and 22.2; 24 sequences
-    of 512 keys 10.3 and 10.9; wide, heads of 256, 500 sequences of 1024 keys 75.0 and 59.8, of 8192 ones 403 and 416). A cluster's 8
-    parts merge without a second kernel (one sequence, 4096 keys 10.3 us and 12.8 as shares, 8192 keys 14.4 and 13.7)."""
+    Small CTAs leave room for three (wide: two) times as many: a short segment is mostly latency and the meeting of its warps' sums (8 bits, 4 query
+    heads on each of 8 kv heads of 128: 256 sequences of 512 keys 75.4 us with large CTAs, 58.2 with small ones, of 128 keys 43.1 and 22.7; 24 sequences
+    of 512 keys 10.3 and 11.5; wide, 6 query heads on one of 256, 500 sequences of 1024 keys 66.7 and 51.7, of 4096 ones 188 and 165, as shares 178; 16 on
+    one of 128, 300 of 1024 keys 49.3 and 40.0, as shares 40.6, of 4096 ones 104 and 107, as shares 81). A cluster's 8
+    parts merge without a second kernel (one sequence, 4096 keys 10.4 us and 12.7 as shares, 8192 keys 13.4 and 13.7)."""
     may_share = B <= MOST_SHARED and B * (-(-table_keys // 16) + 2) < 1 << 31
     segments = B * per_b
     if asked == 0:
